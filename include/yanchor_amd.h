@@ -804,6 +804,115 @@ int yh_ring_fill(const void* k, int64_t k_stride, const void* v, int64_t v_strid
                  void* ring_k, void* ring_v, int32_t* ring_pos, int64_t G, int64_t D, int64_t window, int dtype,
                  yh_stream_t stream);
 
+/* ---- drafted trees over the caches ----------------------------------------
+ *
+ * A draft is a tree of nodes a request, verified in one pass.  The nodes of all
+ * requests are packed rows: request r owns [cu_seqlens[r], cu_seqlens[r + 1]),
+ * cu_seqlens int32 [n_seqs + 1] non-decreasing from 0, at most 64 nodes a
+ * request.  parents int32 [total]: the request's own earlier node that a node
+ * follows, anything else the request's context; NULL: every node follows the
+ * one before it (a single token is a chain of one).  A node's depth is the
+ * number of nodes above it, its position lengths[r] + depth.  Outputs of rows
+ * behind the last request are zeros, those of nodes past max_nodes (1 to 64)
+ * not-a-numbers.  Nothing is read back to the host, and offsets, parents,
+ * tables and slots that lead outside their tensors lead to no access.
+ *
+ * A block cache holds keys / values [blocks, G, block, D]: position p of
+ * request r is row p % block of block tables[r][p / block % columns], tables
+ * int32 [n_seqs, columns], entries below 0 none.  slot = id * block + row.
+ * The SWA ring [rows, G, window, D] is such a cache of one column.
+ */
+
+/* Bytes of the `plan` of the two calls below (4-byte aligned). */
+int64_t yh_block_plan_bytes(int64_t n_seqs);
+
+/*
+ * Blocks for cu_seqlens[r + 1] - cu_seqlens[r] tokens behind the lengths[r]
+ * (int64) that request r has, from the top of the stack free_blocks[0 ..
+ * *free_count) (int32 ids; *free_count int32, updated), and the slot of each of
+ * the tokens (int64 [total], -1: none).  In the order of requests, then of
+ * columns, the call's block i is free_blocks[*free_count - 1 - i].  A request
+ * takes all of its blocks or none: served[r] is 0 where its table has too few
+ * columns, or the stack too few blocks for it and the requests before it.
+ * wrap: a table's columns are a ring, and once all are in use no more are taken.
+ */
+int yh_extend_block_tables(const int64_t* lengths, const int32_t* cu_seqlens, int32_t* tables,
+                           const int32_t* free_blocks, int32_t* free_count, int64_t* slots, uint8_t* served,
+                           void* plan, int64_t n_seqs, int64_t columns, int64_t n_free, int64_t total, int64_t block,
+                           int wrap, yh_stream_t stream);
+
+/*
+ * The blocks that request r uses at lengths[r] but not at kept[r] (int64) back
+ * onto the stack, their table entries -1: in the order of requests, then of
+ * columns, the call's block i ends where an extension takes its block i.
+ */
+int yh_trim_block_tables(const int64_t* lengths, const int64_t* kept, int32_t* tables, int32_t* free_blocks,
+                         int32_t* free_count, void* plan, int64_t n_seqs, int64_t columns, int64_t n_free,
+                         int64_t block, int wrap, yh_stream_t stream);
+
+/*
+ * Slots (int64 [total], -1: none) of the packed nodes: of all, or, with last
+ * (int32 [n_seqs], each request's last accepted node, anything else none), of
+ * the nodes on the path to it.  kept int64 [n_seqs]: the length of the request
+ * with those nodes.  Chains (parents NULL) may be of any length.
+ */
+int yh_slot_map(const int32_t* cu_seqlens, const int64_t* lengths, const int32_t* tables, const int32_t* parents,
+                const int32_t* last, int64_t* slots, int64_t* kept, int64_t n_seqs, int64_t columns, int64_t total,
+                int64_t block, yh_stream_t stream);
+
+/*
+ * keys / values [blocks, G, block, D] at slots[n] (int64 [N]; outside the cache:
+ * not written) <- k[n], v[n] (rows k_stride / v_stride elements apart, [G, D]
+ * dense, 16-byte aligned; f32, bf16 or f16), and, where given, cache_pos int32
+ * [blocks, G, block] <- positions[n] (int64 [N]).  Slots must be distinct.
+ */
+int yh_cache_write(const void* k, int64_t k_stride, const void* v, int64_t v_stride, const int64_t* slots, void* keys,
+                   void* values, const int64_t* positions, int32_t* cache_pos, int64_t N, int64_t blocks, int64_t G,
+                   int64_t D, int64_t block, int dtype, yh_stream_t stream);
+
+/*
+ * Attention of the nodes: node i sees the cached positions and its own
+ * ancestors, itself included, that lie less than `window` (0: no window) before
+ * it: out = softmax(scale q k^T) v (* sigmoid(gate)), [total, H, D].
+ *   q [total, H, D], k, v [total, G, D] (bf16 / f16, token strides in elements,
+ *   16-byte aligned rows of dense heads), gate NULL or [total, H, D] with token
+ *   and head strides; keys / values / tables the block cache, lengths int64
+ *   [n_seqs] the positions in it, of which the last columns * block are read.
+ * H % G == 0, D 64 or 128.
+ */
+int yh_tree_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                      int64_t v_stride, const int32_t* parents, const int32_t* cu_seqlens, const int64_t* lengths,
+                      const void* keys, const void* values, const int32_t* tables, const void* gate,
+                      int64_t gate_token_stride, int64_t gate_head_stride, void* out, int64_t n_seqs, int64_t total,
+                      int64_t blocks, int64_t columns, int64_t H, int64_t G, int64_t D, int64_t block, int64_t window,
+                      int64_t max_nodes, float scale, int dtype, yh_stream_t stream);
+
+/*
+ * The gated delta rule of the nodes: each node's state is its parent's (the
+ * request's, for a node that follows the context) under yh_gdn_recurrent's
+ * step; o [total, HV, V] is its output.  No state is written.
+ *   q, k [total, H, K], v [total, HV, V] (qkv_dtype), g, beta [total, HV],
+ *   state [n_state_rows, HV, K, V] (f32 or f16), state_indices NULL (row r) or
+ *   int32 [n_seqs]: a row outside the state stands for no request, its nodes'
+ *   outputs are zeros.
+ * HV % H == 0; K, V in {64, 128}.
+ */
+int yh_tree_gated_delta_rule(const void* q, const void* k, const void* v, const void* g, const void* beta,
+                             const int32_t* parents, const int32_t* cu_seqlens, const void* state, int state_dtype,
+                             const int32_t* state_indices, void* o, int64_t n_seqs, int64_t total, int64_t H,
+                             int64_t HV, int64_t K, int64_t V, int64_t n_state_rows, int64_t max_nodes, float scale,
+                             int use_qk_l2norm, int qkv_dtype, int g_dtype, int beta_dtype, yh_stream_t stream);
+
+/*
+ * yh_conv_prefill's conv + SiLU of the nodes, each continuing its own path:
+ * proj [total, proj_stride] bf16 (conv inputs in the first `channels`
+ * columns), window [n_seqs, 3, channels] the inputs before the nodes (not
+ * changed), conv_w [channels, 4], out [planes, total, channels / planes].
+ */
+int yh_conv_tree(const void* proj, int64_t proj_stride, const void* window, const void* conv_w,
+                 const int32_t* parents, const int32_t* cu_seqlens, int64_t n_seqs, int64_t total, int64_t channels,
+                 int64_t planes, void* out, int dtype, yh_stream_t stream);
+
 /*
  * HBM calibration stream (no counterpart in the reference: the measuring stick
  * for the HBM-bound kernels, whose roofline fractions are quoted against the

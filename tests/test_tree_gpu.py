@@ -1,0 +1,360 @@
+"""Drafted trees over the caches on the GPU, against float64 request by request.
+
+Tolerances, from the roundings that each kernel makes (e = half a step of the
+output's type, torch.finfo(t).eps / 2):
+* attention: the output is rounded once (e |o|) and every weight of the value
+  product once (e sum p |v|); scores, exponentials and sums are float32, whose
+  error in the exponent (below 2^-24 x 128 terms x the largest score) leaves
+  2^-12 sum p |v|.
+* delta rule: the output once (e |o|); everything else is float32 or a pair of
+  16-bit values (2^-16): 2^-12 of the size of the terms.
+* conv: the output once, the four products and the SiLU in float32 (2^-18 of
+  the products' size).
+* tables, slots and copies are exact.
+"""
+import pytest
+import torch
+
+from oracle import tree as ref
+from yanchor_amd import gdn, layers
+from yanchor_amd import independent_memory as im
+from yanchor_amd import inference_kernels as ik
+
+pytestmark = pytest.mark.gpu
+
+NAN = float("nan")
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def within(x, want, bound, what=""):
+    """|x - want| <= bound everywhere; the worst ratio is told."""
+    x = x.detach().double().cpu()
+    assert x.shape == want.shape
+    bad = (x - want).abs() > bound + 1e-30
+    bad |= ~torch.isfinite(x) & torch.isfinite(want)
+    ratio = ((x - want).abs() / (bound + 1e-30)).max().item() if x.numel() else 0
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {x.numel()} off, {ratio:.2f} times the bound, first at {bad.nonzero()[0].tolist()}"
+
+
+def trees(counts, seed, back=4):
+    """(cu list, parents list) of packed random trees."""
+    gen = torch.Generator().manual_seed(seed)
+    cu, parents = [0], []
+    for n in counts:
+        for i in range(n):
+            parents.append(max(-1, i - int(torch.randint(1, back + 1, (), generator=gen))))
+        cu.append(cu[-1] + n)
+    return cu, parents
+
+
+def rnd(*shape, seed, dtype=torch.bfloat16, std=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype)
+
+
+def i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+# --- attention ------------------------------------------------------------------
+
+def attention_case(dev, lengths, counts, *, h=8, g=2, d=128, block=16, columns=None, window=None, gate=None,
+                   dtype=torch.bfloat16, chain=False, pad=0, seed=0, max_nodes=None, bad=None, fill=NAN, scale=None,
+                   std=1.0, max_length=None):
+    cu, parents = trees(counts, seed)
+    n = cu[-1]
+    if chain:
+        parents = None
+    columns = columns or max(1, max(-(-x // block) for x in lengths))
+    blocks = len(lengths) * columns + 2
+    order = torch.randperm(blocks, generator=torch.Generator().manual_seed(seed)).tolist()
+    keys, values = (rnd(blocks, g, block, d, seed=seed + s, dtype=dtype) for s in (1, 2))
+    tables = torch.full((len(lengths), columns), -1, dtype=torch.int32)
+    live = torch.zeros(blocks, block, dtype=torch.bool)
+    for r, x in enumerate(lengths):
+        for p in range(max(0, x - columns * block), x):
+            c = p // block % columns
+            tables[r, c] = order[r * columns + c]
+            live[tables[r, c], p % block] = True
+    dead = ~live[:, None, :, None].expand_as(keys)    # what no position holds may be anything
+    keys[dead] = fill
+    values[dead] = fill
+    for r, c, x in bad or []:
+        tables[r, c] = x
+    q = rnd(n + pad, h, d, seed=seed + 3, dtype=dtype, std=1.5 * std)
+    k, v = (rnd(n + pad, g, d, seed=seed + s, dtype=dtype) for s in (4, 5))
+    gt = None
+    if gate == "dense":
+        gt = rnd(n + pad, h, d, seed=seed + 6, dtype=dtype)
+    elif gate == "odd":      # heads interleaved with something else, rows off 8-byte alignment
+        gt = rnd(n + pad, h, 2 * d + 1, seed=seed + 6, dtype=dtype)[:, :, d:2 * d]
+    for t in (q, k, v):
+        t[n:] = NAN
+    to = dict(device=dev)
+    got = layers.tree_attention(q.to(**to), k.to(**to), v.to(**to), None if parents is None else i32(parents + [7] * pad, dev),
+                                i32(cu, dev), torch.tensor(lengths, device=dev), keys.to(**to), values.to(**to),
+                                tables.to(**to), window=window, scale=scale, max_nodes=max_nodes, max_length=max_length,
+                                gate=None if gt is None else torch.empty_strided(gt.shape, gt.stride(), dtype=dtype, device=dev).copy_(gt))
+    args = (parents, cu, lengths, keys)
+    want = ref.attention(q[:n], k[:n], v[:n], *args, values, tables, window, None if gt is None else gt[:n], scale)
+    size = ref.attention(q[:n], k[:n], v[:n].abs(), *args, values.abs(), tables, window, None, scale)
+    if gt is not None:
+        size = size * torch.sigmoid(gt[:n].double())
+    torch.cuda.synchronize()
+    assert torch.equal(got[n:].cpu(), torch.zeros(pad, h, d, dtype=dtype))
+    within(got[:n], want, half_step(dtype) * (want.abs() + size) + 2.0 ** -12 * size)
+    return got
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 128), (torch.bfloat16, 64),
+                                     (torch.float16, 64)])
+def test_attention_lengths_and_node_counts(gpu, dtype, d):
+    attention_case(gpu, [0, 1, 63, 64, 65, 150, 7, 128], [1, 0, 5, 64, 17, 3, 33, 2], d=d, dtype=dtype, seed=1)
+
+
+@pytest.mark.parametrize("h,g,block", [(1, 1, 16), (6, 2, 24), (5, 1, 1), (16, 2, 64), (8, 8, 7), (12, 1, 100)])
+def test_attention_heads_and_blocks(gpu, h, g, block):
+    attention_case(gpu, [70, 5, 131], [9, 64, 1], h=h, g=g, block=block, seed=2)
+
+
+@pytest.mark.parametrize("window,block,columns", [(40, 40, 1), (64, 64, 1), (1, 16, None), (3, 16, None),
+                                                  (100, 16, 8), (50, 24, 3)])
+def test_attention_windows_and_rings(gpu, window, block, columns):
+    """Rings of one block, rings of blocks, and windows over a whole cache; some not yet full."""
+    attention_case(gpu, [0, 39, 40, 41, 300, 1000, 64], [4, 12, 1, 20, 64, 7, 2], window=window, block=block,
+                   columns=columns, seed=3)
+
+
+def test_attention_reads_the_last_positions_that_are_there(gpu):
+    attention_case(gpu, [100, 48, 49], [3, 3, 3], block=16, columns=3, seed=4)
+
+
+@pytest.mark.parametrize("gate", ["dense", "odd"])
+def test_attention_gate_padding_and_chains(gpu, gate):
+    attention_case(gpu, [33, 90], [6, 11], gate=gate, chain=True, pad=5, seed=5)
+    attention_case(gpu, [33, 90], [6, 11], gate=gate, pad=70, seed=6)
+
+
+def test_attention_of_single_tokens(gpu):
+    attention_case(gpu, [513, 0, 1024, 77], [1, 1, 1, 1], chain=True, max_nodes=1, h=32, g=8, seed=7)
+
+
+def test_attention_holes_in_a_table_are_not_seen(gpu):
+    attention_case(gpu, [200, 130], [8, 8], bad=[(0, 3, -1), (0, 7, 1 << 30), (1, 0, 10 ** 6), (1, 8, -5)], seed=8)
+
+
+def test_attention_scale_and_large_scores(gpu):
+    """Scores of several hundred: the softmax is nearly one key."""
+    attention_case(gpu, [150], [16], scale=1.0, seed=9)
+    for scale in (0.0, -1.0, float("inf"), NAN):     # the scores' order is what the masks count on
+        with pytest.raises(ValueError, match="positive"):
+            attention_case(gpu, [150], [16], scale=scale, seed=10)
+
+
+def test_attention_equal_keys_and_infinite_keys(gpu):
+    """A key of infinities takes all of the weight, or none."""
+    dev = gpu
+    q = torch.ones(2, 1, 128, dtype=torch.bfloat16, device=dev)
+    k = torch.zeros(2, 1, 128, dtype=torch.bfloat16, device=dev)
+    v = torch.full((2, 1, 128), 3.0, dtype=torch.bfloat16, device=dev)
+    keys = torch.zeros(1, 1, 16, 128, dtype=torch.bfloat16, device=dev)
+    values = torch.arange(16, device=dev, dtype=torch.bfloat16)[None, None, :, None].expand(1, 1, 16, 128).contiguous()
+    keys[0, 0, 5] = -float("inf")
+    out = layers.tree_attention(q, k, v, None, i32([0, 2], dev), torch.tensor([8], device=dev), keys, values,
+                                i32([[0]], dev))
+    want = torch.tensor([(sum(range(8)) - 5 + 3) / 8, (sum(range(8)) - 5 + 6) / 9], dtype=torch.float64)
+    within(out[:, 0, 0], want, want * 2.0 ** -7)
+
+
+def test_attention_counts_past_max_nodes(gpu):
+    """Nodes past the most are not-a-number, the others as ever."""
+    q, k, v = (rnd(80, 2, 64, seed=s).to(gpu) for s in (1, 2, 3))
+    cache = rnd(1, 2, 16, 64, seed=4).to(gpu)
+    args = (torch.tensor([5, 9], device=gpu), cache, cache, i32([[0], [0]], gpu))
+    out = layers.tree_attention(q, k, v, None, i32([0, 70, 80], gpu), *args)
+    assert out[64:70].isnan().all() and not out[:64].isnan().any() and not out[70:].isnan().any()
+    few = layers.tree_attention(q, k, v, None, i32([0, 70, 80], gpu), *args, max_nodes=8)
+    assert torch.equal(few[:8], out[:8]) and few[8:70].isnan().all() and torch.equal(few[70:78], out[70:78])
+
+
+def test_attention_empty_calls(gpu):
+    z = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=gpu)
+    cache = torch.zeros(0, 4, 16, 64, dtype=torch.bfloat16, device=gpu)
+    none = torch.zeros(0, dtype=torch.int64, device=gpu)
+    out = layers.tree_attention(z, z, z, None, i32([0], gpu), none, cache, cache, torch.zeros(0, 1, dtype=torch.int32, device=gpu))
+    assert out.shape == (0, 4, 64)
+    three = torch.ones(3, 4, 64, dtype=torch.bfloat16, device=gpu)   # rows, but no request
+    out = layers.tree_attention(three, three, three, None, i32([0], gpu), none, cache, cache,
+                                torch.zeros(0, 1, dtype=torch.int32, device=gpu))
+    assert torch.equal(out, torch.zeros_like(three))
+
+
+# --- gated delta rule -------------------------------------------------------------
+
+def delta_case(dev, counts, *, h=2, hv=4, kd=128, vd=128, dtype=torch.bfloat16, state=torch.float32, rows=None, pad=0,
+               l2=True, scale=None, gates=(torch.float32, torch.float32), chain=False, seed=0, max_nodes=None,
+               decay=1.0):
+    cu, parents = trees(counts, seed)
+    if chain:
+        parents = None
+    n = cu[-1]
+    pool = len(counts) + 2
+    q, k = (rnd(1, n + pad, h, kd, seed=seed + s, dtype=dtype, std=1.0 if l2 else kd ** -0.5) for s in (1, 2))
+    v = rnd(1, n + pad, hv, vd, seed=seed + 3, dtype=dtype)
+    g = (-decay * torch.rand(1, n + pad, hv, generator=torch.Generator().manual_seed(seed + 4))).to(gates[0])
+    beta = torch.sigmoid(rnd(1, n + pad, hv, seed=seed + 5, dtype=torch.float32)).to(gates[1])
+    s0 = rnd(pool, hv, kd, vd, seed=seed + 6, dtype=state, std=0.3)
+    for t in (q, k, v, g, beta):
+        t[:, n:] = NAN
+    on = [x.to(dev) for x in (q, k, v, g, beta)]
+    got = gdn.tree_gated_delta_rule(*on, None if parents is None else i32(parents + [3] * pad, dev), i32(cu, dev), s0.to(dev),
+                                    state_indices=None if rows is None else i32(rows, dev), scale=scale,
+                                    use_qk_l2norm_in_kernel=l2, max_nodes=max_nodes)
+    want, size = ref.delta_rule(q[0, :n], k[0, :n], v[0, :n], g[0, :n], beta[0, :n], parents, cu, s0, rows, scale, l2)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0, n:].cpu(), torch.zeros(pad, hv, vd, dtype=dtype))
+    within(got[0, :n], want, half_step(dtype) * want.abs() + 2.0 ** -12 * size)
+
+
+@pytest.mark.parametrize("vd,state", [(128, torch.float32), (64, torch.float32), (128, torch.float16),
+                                      (64, torch.float16)])
+def test_delta_rule_node_counts(gpu, vd, state):
+    delta_case(gpu, [1, 0, 5, 16, 17, 33, 48, 64, 63], vd=vd, state=state, seed=11)
+
+
+@pytest.mark.parametrize("counts,most", [([1, 1, 1], 1), ([7, 2], 7), ([16, 3], 16), ([17, 1], 17), ([32, 9], 32)])
+def test_delta_rule_small_trees(gpu, counts, most):
+    delta_case(gpu, counts, max_nodes=most, seed=12)
+
+
+@pytest.mark.parametrize("kd,vd,dtype", [(64, 64, torch.bfloat16), (64, 128, torch.float32), (128, 128, torch.float16),
+                                         (128, 64, torch.float32)])
+def test_delta_rule_other_types(gpu, kd, vd, dtype):
+    delta_case(gpu, [3, 20, 64], kd=kd, vd=vd, dtype=dtype, gates=(dtype, torch.float32), seed=13)
+
+
+def test_delta_rule_rows_padding_and_options(gpu):
+    delta_case(gpu, [4, 9, 2, 6], rows=[5, -1, 0, 3], pad=6, seed=14)
+    delta_case(gpu, [4, 9], rows=[1, 1], pad=70, chain=True, seed=15)          # one state, two drafts
+    delta_case(gpu, [20, 9], l2=False, scale=0.7, h=4, gates=(torch.bfloat16, torch.float16), seed=16)
+    delta_case(gpu, [30, 64], decay=40.0, seed=17)     # decays that underflow along a path
+    delta_case(gpu, [30, 64], decay=0.0, chain=True, seed=18)
+
+
+def test_delta_rule_counts_past_max_nodes(gpu):
+    x, v = rnd(1, 80, 2, 128, seed=1).to(gpu), rnd(1, 80, 2, 128, seed=2).to(gpu)
+    g, b, s = torch.zeros(1, 80, 2, device=gpu), torch.ones(1, 80, 2, device=gpu), torch.zeros(2, 2, 128, 128, device=gpu)
+    o = gdn.tree_gated_delta_rule(x, x, v, g, b, None, i32([0, 70, 80], gpu), s)
+    assert o[0, 64:70].isnan().all() and not o[0, :64].isnan().any() and not o[0, 70:].isnan().any()
+
+
+# --- conv ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("channels,planes,extra,chain", [(24, 3, 8, False), (4096, 1, 0, False), (30, 3, 1, False),
+                                                         (6144, 3, 4160, True), (9, 1, 2, True)])
+def test_conv(gpu, channels, planes, extra, chain):
+    counts = [1, 0, 2, 3, 64, 17]
+    cu, parents = trees(counts, 21)
+    n, pad = cu[-1], 3
+    proj = rnd(n + pad, channels + extra, seed=22)
+    window, w = rnd(len(counts), 3, channels, seed=23), rnd(channels, 4, seed=24, std=0.5)
+    got = layers.conv_tree(proj.to(gpu), window.to(gpu), w.to(gpu), None if chain else i32(parents + [0] * pad, gpu), i32(cu, gpu),
+                           channels, planes=planes)
+    if planes > 1:
+        got = got.transpose(0, 1).reshape(n + pad, channels)
+    x = proj[:n, :channels]
+    want = ref.conv(x, window, w, None if chain else parents, cu)
+    one = torch.ones(1, dtype=torch.float64)
+    a = torch.zeros_like(want)
+    for r in range(len(counts)):   # the size of the four products
+        for i, path in enumerate(ref.paths(None if chain else parents[cu[r]:cu[r + 1]], counts[r])):
+            taps = torch.cat((window[r], x[[cu[r] + j for j in path]])).double()[-4:]
+            a[cu[r] + i] = (taps * w.double().T).abs().sum(0) * one
+    assert not got[n:].any()
+    within(got[:n], want, 2.0 ** -8 * want.abs() + 2.0 ** -18 * a)
+
+
+# --- tables, slots, write -----------------------------------------------------------
+
+@pytest.mark.parametrize("n,block,columns,wrap,most", [(1, 16, 4, False, 20), (5, 16, 5, False, 30), (40, 1, 60, False, 20),
+                                                       (300, 7, 8, True, 60), (1500, 16, 9, False, 60),
+                                                       (70, 64, 1000, False, 3000)])
+def test_extend_and_trim(gpu, n, block, columns, wrap, most):
+    gen = torch.Generator().manual_seed(n)
+    lengths = torch.randint(0, most, (n,), generator=gen).tolist()
+    added = torch.randint(0, most, (n,), generator=gen).tolist()
+    pad = 9
+    for share in (1.0, 0.4):      # enough blocks, and a stack that runs dry
+        tables = [[-1] * columns for _ in range(n)]
+        big = list(range(10 ** 6, 10 ** 6 + sum(ref._used(x, block, columns, wrap) for x in lengths)))
+        ok = ref.extend([0] * n, lengths, tables, big, len(big), block, sum(lengths), wrap)[1]
+        need = sum(ref._used(a + b, block, columns, wrap) - ref._used(a, block, columns, wrap)
+                   for a, b in zip(lengths, added))
+        free = torch.randperm(int(need * share) + 3, generator=gen).tolist() + [-1] * 5
+        count = len(free) - 5
+        cu = torch.tensor([0] + added).cumsum(0)
+        total = int(cu[-1]) + pad
+        t_dev, f_dev = i32(tables, gpu), i32(free, gpu)
+        c_dev = i32([count], gpu)
+        start = (t_dev.clone(), f_dev[:count].clone())
+        slots, served = ik.extend_block_tables(torch.tensor(lengths, device=gpu), cu.to(gpu), t_dev, f_dev, c_dev, block,
+                                               total, wrap=wrap)
+        want, serve, left = ref.extend(lengths, added, tables, free, count, block, total, wrap)
+        assert served.tolist() == serve and slots.tolist() == want
+        assert c_dev.tolist() == [left] and t_dev.tolist() == tables
+        longer = [a + b for a, b in zip(lengths, added)]
+        ik.trim_block_tables(torch.tensor(longer, device=gpu), torch.tensor(lengths, device=gpu), t_dev, f_dev, c_dev, block,
+                             wrap=wrap)
+        assert ref.trim(longer, lengths, tables, free, left, block, wrap) == c_dev.item() == count
+        assert torch.equal(t_dev, start[0]) and torch.equal(f_dev[:count], start[1])
+        assert all(ok) or not wrap
+        ik.trim_block_tables(torch.tensor(lengths, device=gpu), torch.zeros(n, dtype=torch.int64, device=gpu), t_dev, f_dev,
+                             c_dev, block, wrap=wrap)
+        assert (t_dev == -1).all()       # the stack may be too small for them all; nothing is written behind it
+
+
+@pytest.mark.parametrize("tree", [True, False])
+def test_slot_map(gpu, tree):
+    counts = [5, 0, 64, 1, 17] if tree else [5, 0, 200, 1, 17]
+    cu, parents = trees(counts, 31)
+    lengths, block, columns = [3, 8, 100, 0, 61], 16, 21
+    tables = torch.randperm(len(counts) * columns, generator=torch.Generator().manual_seed(1)).view(-1, columns).to(torch.int32)
+    tables[4, 4] = -1           # position 64 on: not served
+    par = parents if tree else None
+    pad = 6
+    args = (i32(cu, gpu), torch.tensor(lengths, device=gpu), tables.to(gpu), block, cu[-1] + pad)
+    dev_par = None if par is None else i32(par + [0] * pad, gpu)
+    for last in (None, [4, -1, 40, 0, 16], [-1, 0, 63, 5, 3]):
+        slots, kept = ik.slot_map(*args, parents=dev_par, last=None if last is None else i32(last, gpu))
+        got, want = slots.tolist(), ref.slot_map(cu, lengths, tables.tolist(), block, cu[-1] + pad, par,
+                                                 None if last is None else [min(x, c - 1) if not tree else x for x, c in zip(last, counts)])
+        assert kept.tolist() == want[1]
+        assert got == [-1 if x < 0 else x for x in want[0]]
+
+
+@pytest.mark.parametrize("dtype,g,d,block", [(torch.bfloat16, 8, 128, 16), (torch.float16, 5, 64, 1),
+                                             (torch.float32, 3, 12, 7), (torch.bfloat16, 1, 8, 1024)])
+def test_cache_write(gpu, dtype, g, d, block):
+    for n in (1, 3, 300):
+        blocks = -(-n // block) + 2
+        gen = torch.Generator().manual_seed(n)
+        slots = torch.randperm(blocks * block, generator=gen)[:n]
+        slots[torch.rand(n, generator=gen) < 0.3] = -1
+        if n > 1:
+            slots[0] = blocks * block     # past the cache
+        wide = rnd(n, 3 * g * d, seed=n, dtype=dtype)
+        k, v = wide[:, :g * d].view(n, g, d), wide[:, 2 * g * d:].view(n, g, d)
+        keys, values = (torch.full((blocks, g, block, d), NAN, dtype=dtype) for _ in range(2))
+        pos, cpos = torch.arange(n) + 7, torch.full((blocks, g, block), -1, dtype=torch.int32)
+        dk, dv, dp = keys.to(gpu), values.to(gpu), cpos.to(gpu)
+        w = wide.to(gpu)
+        layers.cache_write(w[:, :g * d].view(n, g, d), w[:, 2 * g * d:].view(n, g, d), slots.to(gpu), dk, dv,
+                           positions=pos.to(gpu), cache_positions=dp)
+        for i, s in enumerate(slots.tolist()):
+            if 0 <= s < blocks * block:
+                keys[s // block, :, s % block], values[s // block, :, s % block] = k[i], v[i]
+                cpos[s // block, :, s % block] = pos[i]
+        assert torch.equal(dk.cpu().nan_to_num(9.5), keys.nan_to_num(9.5))
+        assert torch.equal(dv.cpu().nan_to_num(9.5), values.nan_to_num(9.5)) and torch.equal(dp.cpu(), cpos)

@@ -15,8 +15,9 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libyanchor_amd.so"
 # yh_abi_version() of the library these signatures describe (103: yh_rmsnorm_partials takes
 # out2_stride; 104: yh_linear_pack lays K blocks outermost; 105: yh_rmsnorm_partials takes part2;
 # 106: yh_gdn_decode_fused takes the state dtype; 107: the yh_anchor_tokens_* calls are added,
-# yh_gdn_chunk_varlen uses its workspace, yh_conv_prefill's dtype may hold a number of planes)
-ABI_VERSION = 107
+# yh_gdn_chunk_varlen uses its workspace, yh_conv_prefill's dtype may hold a number of planes;
+# 108: the calls for drafted trees and block tables are added)
+ABI_VERSION = 108
 
 F32, BF16, F16, I32, I64, U8 = 0, 1, 2, 3, 4, 5
 DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16,
@@ -88,11 +89,19 @@ SIGNATURES: dict[str, list] = {
     "yh_gated_rmsnorm": [_p, _p, _i64, _p, _p, _i64, _i64, _i64, _f32, _p],
     "yh_silu_mul": [_p, _i64, _p, _i64, _i64, _p],
     "yh_head_norm_rope": [_p, _i64, _i64, _p, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _f32, _p],
+    "yh_extend_block_tables": [_p] * 8 + [_i64] * 5 + [_i32, _p],
+    "yh_trim_block_tables": [_p] * 6 + [_i64] * 4 + [_i32, _p],
+    "yh_slot_map": [_p] * 7 + [_i64] * 4 + [_p],
+    "yh_cache_write": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _p],
+    "yh_tree_attention": [_p, _i64, _p, _i64, _p, _i64] + [_p] * 7 + [_i64, _i64, _p] + [_i64] * 10 + [_f32, _i32, _p],
+    "yh_tree_gated_delta_rule": [_p] * 8 + [_i32, _p, _p] + [_i64] * 8 + [_f32, _i32, _i32, _i32, _i32, _p],
+    "yh_conv_tree": [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i32, _p],
     "yh_hbm_stream": [_i32, _i32, _p, _p, _i64, _i32, _p],
 }
 
 # entry points that do not return a status
 PLAIN: dict[str, tuple] = {
+    "yh_block_plan_bytes": (_i64, [_i64]),
     "yh_topk_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "yh_linear_split": (_i32, [_i64, _i64, _i64]),
     "yh_linear_packed_split": (_i32, [_i64, _i64, _i64]),
@@ -145,6 +154,15 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib().yh_last_error().decode(errors="replace")
         raise NativeError(f"{name} failed ({rc}): {msg}")
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with ``device`` current, as a launch on its streams needs."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

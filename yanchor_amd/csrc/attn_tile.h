@@ -124,23 +124,24 @@ __device__ __forceinline__ void load_rows(Rows& t, CopyFn copy) {
 
 // FRESH: LDS addresses are formed in every tile instead of staying in registers
 // over the tile loop, where a kernel's own invariants leave no room for them (a
-// spilled one is reloaded behind the copies in flight).
-template <int DT, bool FRESH = false>
+// spilled one is reloaded behind the copies in flight).  D: head dim, 64 or
+// 128; the pieces of a shorter row lie at the same places of a 16-piece row.
+template <int DT, bool FRESH = false, int D = kD>
 struct State {
   static __device__ __forceinline__ int lane_id() {
     int lane = threadIdx.x & 63;
     if constexpr (FRESH) asm volatile("" : "+v"(lane));
     return lane;
   }
-  typename Mfma<DT>::vec q[8];  // Q^T: dims 16 s + 8 half .. + 7 of the lane's query
-  f32x16 acc[4];                // O^T: dim 32 t + 8 (i / 4) + 4 half + i % 4
+  typename Mfma<DT>::vec q[D / 16];  // Q^T: dims 16 s + 8 half .. + 7 of the lane's query
+  f32x16 acc[D / 32];           // O^T: dim 32 t + 8 (i / 4) + 4 half + i % 4
   float base;                   // running maximum, log2 units
   float den;                    // this half's share of the denominator
 
   // sink: a logit 0 with value 0 takes part in the softmax
   __device__ __forceinline__ void init(bool sink) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < D / 32; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
     base = sink ? 0.f : -3.0e38f;
@@ -149,7 +150,7 @@ struct State {
   __device__ __forceinline__ void load_q(const uint16_t* row, bool valid) {
     const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
+    for (int s = 0; s < D / 16; ++s) {
       uint4 x = make_uint4(0, 0, 0, 0);
       if (valid) x = *reinterpret_cast<const uint4*>(row + s * 16 + half * 8);
       q[s] = __builtin_bit_cast(typename Mfma<DT>::vec, x);
@@ -174,10 +175,10 @@ struct State {
       for (int i = 0; i < 16; ++i) c[kt][i] = 0.f;
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int n = 0; n < 16; ++n) {
+    for (int n = 0; n < D / 8; ++n) {
       __builtin_amdgcn_sched_barrier(0);
       c[n & 1] = M::run(kf[n % kAhead], q[n >> 1], c[n & 1]);
-      if (n + kAhead < 16) kf[n % kAhead] = read_k(n + kAhead);
+      if (n + kAhead < D / 8) kf[n % kAhead] = read_k(n + kAhead);
     }
     __builtin_amdgcn_s_setprio(0);
   }
@@ -212,8 +213,9 @@ struct State {
     // 4 m .. + 3 (of the group's 16) of row 16 ks + 8 u + 4 half + j
     const int j = (lane & 15) >> 2, m = lane & 3, gi = (lane >> 4) & 1;
     const int low = 2 * gi + (m >> 1);
-    auto read_v = [&](int n) {   // n = 4 ks + d
-      const int d = n & 3, ks = n >> 2;
+    constexpr int kDims = D / 32;
+    auto read_v = [&](int n) {   // n = kDims ks + d
+      const int d = n % kDims, ks = n / kDims;
       s16x4v x[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -257,9 +259,9 @@ struct State {
     for (int e = 0; e < 4; ++e) quarter(0, e);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int n = 0; n < 16; ++n) {
+    for (int n = 0; n < 4 * kDims; ++n) {
       __builtin_amdgcn_sched_barrier(0);
-      const int d = n & 3, ks = n >> 2;
+      const int d = n % kDims, ks = n / kDims;
       const uint32_t* h = ph[ks & 1];
       if (ks == 0) acc[d] *= alpha;
       if constexpr (EDGE) {
@@ -273,8 +275,11 @@ struct State {
         const uint32_t* l = pl[ks & 1];
         acc[d] = M::run(vf[n % kAhead], __builtin_bit_cast(vec, make_uint4(l[0], l[1], l[2], l[3])), acc[d]);
       }
-      if (n + kAhead < 16) vf[n % kAhead] = read_v(n + kAhead);
-      if (ks < 3) quarter(ks + 1, d);
+      if (n + kAhead < 4 * kDims) vf[n % kAhead] = read_v(n + kAhead);
+      if (ks < 3) {
+#pragma unroll
+        for (int e = d * (4 / kDims); e < (d + 1) * (4 / kDims); ++e) quarter(ks + 1, e);
+      }
     }
     __builtin_amdgcn_s_setprio(0);
   }

@@ -1,0 +1,82 @@
+// Drafted trees: the packed nodes of a request, their ancestors, and division
+// by a run-time constant, shared by the kernels that work on them.
+#pragma once
+#include "common.h"
+
+namespace yh {
+namespace tree {
+
+constexpr int kNodes = 64;   // most nodes of a request: one wave, one 64-bit set
+
+// The packed rows [first, first + count) of request r: offsets are clamped to
+// the rows that exist, so no offset leads outside them.
+struct Span {
+  int64_t first;
+  int64_t count;
+};
+__device__ __forceinline__ Span span_of(const int32_t* cu, int64_t r, int64_t total) {
+  int64_t s = cu[r], e = cu[r + 1];
+  s = s < 0 ? 0 : s > total ? total : s;
+  e = e < s ? s : e > total ? total : e;
+  return {s, e - s};
+}
+
+// Lane i's node i of n (one wave, all lanes active): the set of its ancestors,
+// itself included, by doubling -- after step k, `set` holds the nodes less than
+// 2^k steps up and `up` the node 2^k steps up (-1: the context).  A parent that
+// is not an earlier node counts as the context.  parents null: a chain.
+// sum(up node's value) of `x` along the path is formed with it.
+__device__ __forceinline__ uint64_t ancestors(const int32_t* parents, int n, float* x = nullptr) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int up = -1;
+  if (lane < n) up = parents ? parents[lane] : lane - 1;
+  if (up >= lane || up < 0) up = -1;
+  uint64_t set = 1ull << lane;
+  float v = x ? *x : 0.f;
+#pragma unroll
+  for (int step = 0; step < 6; ++step) {
+    const int from = up < 0 ? lane : up;
+    const uint64_t other = __shfl(set, from, kWave);
+    const float ov = x ? __shfl(v, from, kWave) : 0.f;
+    const int next = __shfl(up, from, kWave);
+    if (up >= 0) {
+      set |= other;
+      v += ov;
+      up = next;
+    }
+  }
+  if (x) *x = v;
+  return set;
+}
+
+// n / d for 0 <= n < 2^31 by a multiplication: m = ceil(2^(31 + l) / d) with
+// l = ceil(log2 d) is below 2^32, and its error e = m d - 2^(31 + l) < d <= 2^l
+// keeps n e below 2^(31 + l).
+struct Div {
+  uint32_t m, d;
+  int s;
+  __device__ __forceinline__ uint32_t quot(uint32_t n) const {
+    return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> s);
+  }
+};
+inline Div make_div(uint32_t d) {
+  int l = 0;
+  while ((1ull << l) < d) ++l;
+  const unsigned __int128 p = static_cast<unsigned __int128>(1) << (31 + l);
+  return {static_cast<uint32_t>((p + d - 1) / d), d, 31 + l};
+}
+
+// Request of packed row t among r in [lo, hi]: the last with cu[r] <= t.
+__device__ __forceinline__ int request_of(const int32_t* cu, int lo, int hi, int64_t t) {
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cu[mid] <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace tree
+}  // namespace yh

@@ -1,0 +1,274 @@
+// A GDN layer over drafted trees: the causal conv and the gated delta rule of
+// every node, each continuing its own path from the request's window and state.
+// Neither is written: which path stays is known only after the verification.
+//
+// Delta rule, with G_i the sum of the log decays g along the path to node i
+// (itself included), S the request's state and every token's u_j the rank-one
+// update that it leaves, S_i = e^{G_i} S + sum over the path e^{G_i - G_j} k_j u_j^T:
+//   u_i = beta_i (v_i - e^{G_i} k_i S - sum_{j above i} e^{G_i - G_j} (k_i . k_j) u_j)
+//   o_i = e^{G_i} q_i S + sum_{j above i, and i} e^{G_i - G_j} (q_i . k_j) u_j
+// which is the chunk form of the rule with the ancestor sets in place of the
+// causal triangle: the state is read once for all nodes and no state of a node
+// is ever formed.
+#include "conv_chan.h"
+#include "tree.h"
+
+namespace yh {
+namespace {
+
+struct GdnArgs {
+  const void* q;           // [N, H, K]
+  const void* k;
+  const void* v;           // [N, HV, V]
+  const void* g;           // [N, HV]
+  const void* beta;
+  const int32_t* parents;  // [N] or null: chains
+  const int32_t* cu;       // [R + 1]
+  const void* state;       // [rows, HV, K, V]
+  const int32_t* rows;     // [R] or null; < 0: no request
+  void* o;                 // [N, HV, V]
+  int64_t total, n_rows;
+  int R, H, HV, max_nodes, l2, dt, g_dt, beta_dt, state_dt;
+  float scale;
+};
+
+__device__ __forceinline__ void fill(void* p, int64_t from, int64_t to, int dt, float x, int threads) {
+  for (int64_t i = from + threadIdx.x; i < to; i += threads) store_any(p, i, dt, x);
+}
+
+// Any of the types: fp32 arithmetic on the vector unit, a workgroup a request
+// and value head.
+template <int K, int V>
+__global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
+  constexpr int kN = tree::kNodes;
+  __shared__ float s_q[kN][K + 1], s_k[kN][K + 1], s_low[kN][kN], s_att[kN][kN], s_u[kN][V];
+  __shared__ float s_g[kN], s_beta[kN];
+  __shared__ uint64_t s_set[kN];
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(a.R) * a.HV) {   // rows of no request
+    const int64_t end = a.R ? a.cu[a.R] : 0, row = static_cast<int64_t>(a.HV) * V;
+    fill(a.o, (end < 0 ? 0 : end) * row, a.total * row, a.dt, 0.f, 256);
+    return;
+  }
+  const int hv = blockIdx.x % a.HV, r = blockIdx.x / a.HV, h = hv / (a.HV / a.H);
+  const tree::Span span = tree::span_of(a.cu, r, a.total);
+  const int64_t srow = a.rows ? a.rows[r] : r;
+  const bool none = srow < 0 || srow >= a.n_rows;
+  const int n = none ? 0 : static_cast<int>(span.count < a.max_nodes ? span.count : a.max_nodes);
+  for (int64_t i = n; i < span.count; ++i)   // no request: zeros; nodes past the most that the call takes: not a number
+    for (int c = tid; c < V; c += 256) store_any(a.o, ((span.first + i) * a.HV + hv) * V + c, a.dt, none ? 0.f : NAN);
+  if (n == 0) return;
+
+  if (tid < 64) {
+    const int64_t i = (span.first + (lane < n ? lane : 0)) * a.HV + hv;
+    float gate = lane < n ? load_any(a.g, i, a.g_dt) : 0.f;
+    const uint64_t set = tree::ancestors(a.parents ? a.parents + span.first : nullptr, n, &gate);
+    s_set[lane] = set;
+    s_g[lane] = gate;
+    s_beta[lane] = load_any(a.beta, i, a.beta_dt);
+  }
+  for (int i = tid >> 6; i < n; i += 4) {   // a wave a row: load, normalise
+    const int64_t at = ((span.first + i) * a.H + h) * K;
+    float x[K / 64], y[K / 64], sx = 0.f, sy = 0.f;
+#pragma unroll
+    for (int c = 0; c < K / 64; ++c) {
+      x[c] = load_any(a.q, at + c * 64 + lane, a.dt);
+      y[c] = load_any(a.k, at + c * 64 + lane, a.dt);
+      sx += x[c] * x[c];
+      sy += y[c] * y[c];
+    }
+    const float rx = a.scale * (a.l2 ? rsqrtf(wave_sum(sx) + 1e-6f) : 1.f), ry = a.l2 ? rsqrtf(wave_sum(sy) + 1e-6f) : 1.f;
+#pragma unroll
+    for (int c = 0; c < K / 64; ++c) {
+      s_q[i][c * 64 + lane] = x[c] * rx;
+      s_k[i][c * 64 + lane] = y[c] * ry;
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e < n * n; e += 256) {
+    const int i = e / n, j = e % n;
+    float low = 0.f, att = 0.f;
+    if ((s_set[i] >> j) & 1) {
+      for (int c = 0; c < K; ++c) {
+        low = fmaf(s_k[i][c], s_k[j][c], low);
+        att = fmaf(s_q[i][c], s_k[j][c], att);
+      }
+      const float decay = expf(s_g[i] - s_g[j]);
+      low = i == j ? 0.f : low * decay * s_beta[i];
+      att *= decay;
+    }
+    s_low[i][j] = low;
+    s_att[i][j] = att;
+  }
+  __syncthreads();
+  for (int c = tid; c < V; c += 256) {   // a thread a column
+    float s[K];
+    const int64_t at = (srow * a.HV + hv) * K * V + c;
+#pragma unroll
+    for (int d = 0; d < K; ++d) s[d] = load_any(a.state, at + d * V, a.state_dt);
+    for (int i = 0; i < n; ++i) {
+      float ks = 0.f, qs = 0.f;
+#pragma unroll
+      for (int d = 0; d < K; ++d) {
+        ks = fmaf(s_k[i][d], s[d], ks);
+        qs = fmaf(s_q[i][d], s[d], qs);
+      }
+      const float eg = expf(s_g[i]);
+      const int64_t row = ((span.first + i) * a.HV + hv) * V + c;
+      float u = s_beta[i] * (load_any(a.v, row, a.dt) - eg * ks), o = eg * qs;
+      for (int j = 0; j < i; ++j)
+        if ((s_set[i] >> j) & 1) {
+          u = fmaf(-s_low[i][j], s_u[j][c], u);
+          o = fmaf(s_att[i][j], s_u[j][c], o);
+        }
+      s_u[i][c] = u;
+      store_any(a.o, row, a.dt, fmaf(s_att[i][i], u, o));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+struct ConvTreeArgs {
+  const uint16_t* proj;     // [N, P], the first C columns
+  int64_t P;
+  const uint16_t* window;   // [R, 3, C], oldest first
+  const uint16_t* w;        // [C, 4]
+  const int32_t* parents;   // [N] or null: chains
+  const int32_t* cu;
+  uint16_t* y;              // [C / Cp, N, Cp]
+  int64_t C, Cp, total;
+  int R, run;
+};
+
+// y_i = silu(sum_j w_j x(3 - j steps up the path of node i)): a thread takes VEC
+// channels of `run` nodes of a request.
+template <int VEC>
+__global__ void __launch_bounds__(256) conv_tree_kernel(ConvTreeArgs a) {
+  using Ch = Chan<VEC>;
+  typedef typename Ch::T T;
+  __shared__ int s_up[3][tree::kNodes];   // the rows 1, 2 and 3 steps up: a node, or -1 .. -3 in the window from its end
+  const int lane = threadIdx.x & 63, r = blockIdx.x;
+  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * VEC;
+  const int64_t plane = c / a.Cp;
+  T* dst = reinterpret_cast<T*>(a.y + plane * a.total * a.Cp + (c - plane * a.Cp));
+  const int64_t yc = a.Cp / VEC;
+  if (r == a.R) {   // rows of no request
+    const int64_t end = a.R ? a.cu[a.R] : 0;
+    if (c < a.C)
+      for (int64_t i = (end < 0 ? 0 : end) + blockIdx.z; i < a.total; i += gridDim.z) dst[i * yc] = T{};
+    return;
+  }
+  const tree::Span span = tree::span_of(a.cu, r, a.total);
+  const int n = static_cast<int>(span.count < tree::kNodes ? span.count : tree::kNodes);
+  const int i0 = blockIdx.z * a.run, i1 = i0 + a.run < n ? i0 + a.run : n;
+  if (blockIdx.z == 0 && c < a.C) {   // nodes past the most: not a number
+    float nan[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) nan[v] = NAN;
+    for (int64_t i = n; i < span.count; ++i) dst[(span.first + i) * yc] = Ch::pack(nan);
+  }
+  if (i0 >= n) return;
+  if (threadIdx.x < 64) {
+    int up = -1;
+    if (lane < n) up = a.parents ? a.parents[span.first + lane] : lane - 1;
+    if (up >= lane || up < 0) up = -1;
+    int two = __shfl(up, up < 0 ? 0 : up, 64);
+    if (up < 0) two = up - 1;
+    int three = __shfl(up, two < 0 ? 0 : two, 64);
+    if (two < 0) three = two - 1;
+    s_up[0][lane] = up;
+    s_up[1][lane] = two;
+    s_up[2][lane] = three;
+  }
+  __syncthreads();
+  if (c >= a.C) return;
+  float wt[4][VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) wt[j][i] = bf16_to_f32(a.w[(c + i) * 4 + j]);
+  const T* src = reinterpret_cast<const T*>(a.proj + span.first * a.P + c);
+  const T* win = reinterpret_cast<const T*>(a.window + static_cast<int64_t>(r) * 3 * a.C + c);
+  const int64_t sp = a.P / VEC, sc = a.C / VEC;
+#pragma unroll 2
+  for (int i = i0; i < i1; ++i) {
+    T x[4];
+    x[3] = src[i * sp];
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const int u = s_up[j][i];
+      x[2 - j] = u >= 0 ? src[u * sp] : win[(3 + u) * sc];
+    }
+    float y[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      float acc = Ch::f32(x[0], v) * wt[0][v];
+#pragma unroll
+      for (int j = 1; j < 4; ++j) acc = fmaf(Ch::f32(x[j], v), wt[j][v], acc);
+      y[v] = silu(acc);
+    }
+    dst[(span.first + i) * yc] = Ch::pack(y);
+  }
+}
+
+}  // namespace
+}  // namespace yh
+
+extern "C" int yh_tree_gated_delta_rule(const void* q, const void* k, const void* v, const void* g, const void* beta,
+                                        const int32_t* parents, const int32_t* cu_seqlens, const void* state,
+                                        int state_dtype, const int32_t* state_indices, void* o, int64_t n_seqs,
+                                        int64_t total, int64_t H, int64_t HV, int64_t K, int64_t V,
+                                        int64_t n_state_rows, int64_t max_nodes, float scale, int use_qk_l2norm,
+                                        int qkv_dtype, int g_dtype, int beta_dtype, yh_stream_t stream) {
+  using namespace yh;
+  YH_CHECK_ARG(n_seqs >= 0 && total >= 0 && n_state_rows >= 0 && H > 0 && HV > 0, "tree_gated_delta_rule: bad sizes");
+  YH_CHECK_ARG(HV % H == 0, "tree_gated_delta_rule: HV must be a multiple of H");
+  YH_CHECK_ARG((K == 64 || K == 128) && (V == 64 || V == 128), "tree_gated_delta_rule: K and V must be 64 or 128");
+  YH_CHECK_ARG(max_nodes > 0 && max_nodes <= tree::kNodes, "tree_gated_delta_rule: max_nodes must be 1 to %d",
+               tree::kNodes);
+  YH_CHECK_ARG(is_float_dtype(qkv_dtype) && is_float_dtype(g_dtype) && is_float_dtype(beta_dtype),
+               "tree_gated_delta_rule: dtypes must be f32, bf16 or f16");
+  YH_CHECK_ARG(state_dtype == YH_F32 || state_dtype == YH_F16, "tree_gated_delta_rule: state must be f32 or f16");
+  if (total == 0) return YH_OK;
+  YH_CHECK_ARG(q && k && v && g && beta && o && (cu_seqlens || n_seqs == 0) && (state || n_state_rows == 0),
+               "tree_gated_delta_rule: null pointer");
+  YH_CHECK_ARG(state_indices || n_state_rows >= n_seqs, "tree_gated_delta_rule: fewer state rows than requests");
+  YH_CHECK_ARG(total < (1ll << 31) && HV < (1ll << 20) && n_seqs * HV < (1ll << 23),
+               "tree_gated_delta_rule: sizes too large");
+  GdnArgs a{q, k, v, g, beta, parents, cu_seqlens, state, state_indices, o, total, n_state_rows, (int)n_seqs, (int)H,
+            (int)HV, (int)max_nodes, use_qk_l2norm ? 1 : 0, qkv_dtype, g_dtype, beta_dtype, state_dtype, scale};
+  const unsigned grid = static_cast<unsigned>(n_seqs * HV + 1);   // the last clears the rows of no request
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (K == 128 && V == 128) hipLaunchKernelGGL((tree_gdn_any_kernel<128, 128>), dim3(grid), dim3(256), 0, st, a);
+  else if (K == 128) hipLaunchKernelGGL((tree_gdn_any_kernel<128, 64>), dim3(grid), dim3(256), 0, st, a);
+  else if (V == 128) hipLaunchKernelGGL((tree_gdn_any_kernel<64, 128>), dim3(grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((tree_gdn_any_kernel<64, 64>), dim3(grid), dim3(256), 0, st, a);
+  YH_CHECK_LAUNCH("tree_gated_delta_rule");
+  return YH_OK;
+}
+
+extern "C" int yh_conv_tree(const void* proj, int64_t proj_stride, const void* window, const void* conv_w,
+                            const int32_t* parents, const int32_t* cu_seqlens, int64_t n_seqs, int64_t total,
+                            int64_t channels, int64_t planes, void* out, int dtype, yh_stream_t stream) {
+  using namespace yh;
+  YH_CHECK_ARG(n_seqs >= 0 && total >= 0 && channels > 0 && proj_stride >= channels, "conv_tree: bad sizes");
+  YH_CHECK_ARG(dtype == YH_BF16, "conv_tree: activations must be bfloat16");
+  YH_CHECK_ARG(planes > 0 && channels % planes == 0, "conv_tree: planes must divide the channels");
+  if (total == 0) return YH_OK;
+  YH_CHECK_ARG(proj && out && conv_w && ((window && cu_seqlens) || n_seqs == 0), "conv_tree: null pointer");
+  YH_CHECK_ARG(total < (1ll << 31) && n_seqs < (1ll << 20) && channels < (1ll << 24), "conv_tree: sizes too large");
+  const bool vec = channels / planes % 8 == 0 && proj_stride % 8 == 0 && tree::aligned16(proj) &&
+                   tree::aligned16(window) && tree::aligned16(out);
+  const int64_t per_block = 256 * (vec ? 8 : 1), cb = (channels + per_block - 1) / per_block;
+  // a request's nodes in one workgroup, or four nodes a workgroup where the requests leave the chip empty
+  const int run = n_seqs * cb >= 1024 ? tree::kNodes : 4;
+  ConvTreeArgs a{static_cast<const uint16_t*>(proj), proj_stride, static_cast<const uint16_t*>(window),
+                 static_cast<const uint16_t*>(conv_w), parents, cu_seqlens, static_cast<uint16_t*>(out), channels,
+                 channels / planes, total, (int)n_seqs, run};
+  const dim3 grid(static_cast<unsigned>(n_seqs + 1), static_cast<unsigned>(cb), tree::kNodes / run);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (vec) hipLaunchKernelGGL(conv_tree_kernel<8>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(conv_tree_kernel<1>, grid, dim3(256), 0, st, a);
+  YH_CHECK_LAUNCH("conv_tree");
+  return YH_OK;
+}

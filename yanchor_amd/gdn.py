@@ -13,6 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
+from . import _tree
 
 
 def _contig(x: torch.Tensor) -> torch.Tensor:
@@ -191,3 +192,49 @@ def chunk_gated_delta_rule(query, key, value, g=None, beta=None, scale=None, ini
            state.data_ptr(), None, cu.data_ptr(), o.data_ptr(), n, h, hv, kd, vd, n, sc,
            int(bool(use_qk_l2norm_in_kernel)), N.code(q), N.code(g_), N.code(be), N.stream_of(q))
     return o, (state if output_final_state else None)
+
+
+def tree_gated_delta_rule(query, key, value, g, beta, parents, cu_seqlens, initial_state, *, state_indices=None,
+                          scale=None, use_qk_l2norm_in_kernel=True, max_nodes=None):
+    """Gated delta rule of the packed nodes of drafted trees: query / key ``[1,
+    N, H, K]``, value ``[1, N, HV, V]``, g / beta ``[1, N, HV]``; request r owns
+    the nodes ``cu_seqlens[r]`` .. ``cu_seqlens[r + 1] - 1`` (at most 64), and
+    ``parents`` (int32 ``[N]``) names the request's own earlier node that each
+    node follows, -1 its context (None: chains).  Each node continues its
+    parent's state, a node that follows the context the request's row of
+    ``initial_state`` ``[rows, HV, K, V]`` (float32 or float16): row r, or
+    ``state_indices[r]`` (int ``[R]``; a row outside the state, as -1: no
+    request, zeros).  Returns o ``[1, N, HV, V]``; rows behind the last request
+    are zeros.  The state is NOT updated: run the accepted path through
+    ``chunk_gated_delta_rule`` or ``recurrent_gated_delta_rule`` once it is
+    known.  ``max_nodes``: the most nodes of any request (default 64); a node
+    past it comes back as not-a-number."""
+    if query.ndim != 4 or key.shape != query.shape or value.ndim != 4 or query.shape[0] != 1:
+        raise ValueError("query/key must be [1, N, H, K] and value [1, N, HV, V]")
+    _, n, h, kd = key.shape
+    hv, vd = value.shape[2], value.shape[3]
+    if value.shape[:2] != (1, n) or g.shape != (1, n, hv) or beta.shape != (1, n, hv):
+        raise ValueError("value/g/beta shapes do not match the packed query/key")
+    if query.dtype != key.dtype or value.dtype != key.dtype:
+        raise ValueError("query, key and value must share one dtype")
+    if h < 1 or hv < 1 or hv % h or kd not in (64, 128) or vd not in (64, 128):
+        raise ValueError("HV must be a multiple of H, and K and V 64 or 128")
+    dev = N.require_device(query, key, value, g, beta, initial_state)
+    if initial_state.dtype not in (torch.float32, torch.float16) or initial_state.ndim != 4 or \
+            tuple(initial_state.shape[1:]) != (hv, kd, vd) or not initial_state.is_contiguous():
+        raise ValueError(f"initial_state must be contiguous float32 or float16 [rows, {hv}, {kd}, {vd}]")
+    parents, cu, most = _tree.nodes(parents, cu_seqlens, max_nodes, n, dev)
+    r = cu.shape[0] - 1
+    idx = None
+    if state_indices is not None:
+        idx = _tree.ints(state_indices, torch.int32, dev, "state_indices", r)
+    elif initial_state.shape[0] < r:
+        raise ValueError("state pool has fewer rows than requests")
+    q, k, v, g_, be = (_contig(x) for x in (query, key, value, g, beta))
+    o = torch.empty(1, n, hv, vd, device=dev, dtype=value.dtype)
+    sc = float(kd ** -0.5 if scale is None else scale)
+    N.call_on(dev, "yh_tree_gated_delta_rule", q.data_ptr(), k.data_ptr(), v.data_ptr(), g_.data_ptr(), be.data_ptr(),
+              N.ptr(parents), cu.data_ptr(), initial_state.data_ptr(), N.code(initial_state), N.ptr(idx), o.data_ptr(),
+              r, n, h, hv, kd, vd, initial_state.shape[0], most, sc, int(bool(use_qk_l2norm_in_kernel)), N.code(q),
+              N.code(g_), N.code(be), N.stream_of(q))
+    return o

@@ -21,6 +21,7 @@ import ctypes
 import torch
 
 from . import _native as N
+from . import _tree
 
 COUNTER_SAMPLING_REVISION = "counter_cdf_v2"
 SAMPLE_FUSED, SAMPLE_TORCH = 0, 1
@@ -296,3 +297,111 @@ def gather_rows(pairs, src_index=None, dst_index=None, n=None):
            ctypes.cast(dstp, ctypes.c_void_p).value, ctypes.cast(rb, ctypes.c_void_p).value,
            ctypes.cast(sr, ctypes.c_void_p).value, ctypes.cast(dr, ctypes.c_void_p).value, N.ptr(si),
            N.ptr(di), int(n), N.stream_of(pairs[0][0]))
+
+
+# ---------------------------------------------------------------------------
+# Block tables of a block cache (keys / values [blocks, G, block, D]) and the
+# slots of tokens and drafted nodes in it, for ``layers.cache_write`` and
+# ``layers.tree_attention``.
+
+def _tables(block_tables, block, device, n):
+    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or not block_tables.is_contiguous():
+        raise ValueError("block_tables must be contiguous int32 [R, columns]")
+    if block_tables.shape[0] != n or block_tables.shape[1] < 1:
+        raise ValueError(f"block_tables must hold at least one column for each of the {n} requests")
+    if int(block) < 1:
+        raise ValueError("block must be at least 1")
+    return block_tables
+
+
+def _free_stack(free, free_count):
+    if free.dtype != torch.int32 or free.ndim != 1 or not free.is_contiguous():
+        raise ValueError("free must be a contiguous int32 vector of block ids")
+    if free_count.dtype != torch.int32 or free_count.numel() != 1:
+        raise ValueError("free_count must be one int32")
+
+
+def extend_block_tables(lengths, cu_seqlens, block_tables, free, free_count, block, total, *, wrap=False):
+    """Blocks and cache slots for the new tokens of every request, in order:
+    request r has ``lengths[r]`` tokens and gets ``cu_seqlens[r + 1] -
+    cu_seqlens[r]`` more.  ``block_tables`` int32 [R, columns] (-1: none),
+    ``free`` int32 [F], a stack of free block ids of which ``free_count``
+    (int32 [1]) are there, are updated IN PLACE.  Returns (slots int64 [total],
+    served bool [R]): token t's slot is block id * ``block`` + position %
+    ``block``, -1 behind the last request and for the tokens of a request that
+    is not served.  A request is served whole or not at all: not where its
+    table has too few columns, nor where the stack holds too few blocks for it
+    and the requests before it.  ``wrap``: a table's columns are a ring
+    (position p in column p // block % columns), for caches that keep a window.
+    Block i of the call, requests first, then columns, is
+    ``free[free_count - 1 - i]``.  Stays on the device."""
+    dev = N.require_device(block_tables, free, free_count)
+    total = int(total)
+    if total < 0:
+        raise ValueError("total must not be negative")
+    cu = _tree.offsets(cu_seqlens, total, dev)
+    n = cu.shape[0] - 1
+    lens = _tree.ints(lengths, torch.int64, dev, "lengths", n)
+    _tables(block_tables, block, dev, n)
+    _free_stack(free, free_count)
+    slots = torch.empty(total, dtype=torch.int64, device=dev)
+    served = torch.empty(n, dtype=torch.bool, device=dev)
+    if n == 0:
+        return slots.fill_(-1), served
+    plan = torch.empty(n + 1, dtype=torch.int32, device=dev)
+    N.call_on(dev, "yh_extend_block_tables", lens.data_ptr(), cu.data_ptr(), block_tables.data_ptr(), free.data_ptr(),
+              free_count.data_ptr(), slots.data_ptr(), served.data_ptr(), plan.data_ptr(), n, block_tables.shape[1],
+              free.shape[0], total, int(block), int(bool(wrap)), N.stream_of(block_tables))
+    return slots, served
+
+
+def trim_block_tables(lengths, kept, block_tables, free, free_count, block, *, wrap=False):
+    """The blocks that the requests use at ``lengths`` but not at ``kept``
+    (int [R], fewer tokens: a rejected draft, or 0 for a finished request) go
+    back onto the stack ``free`` / ``free_count``, and their entries in
+    ``block_tables`` become -1, all IN PLACE.  Entries below 0 (requests that
+    were not served) are passed over.  Trimming what an
+    ``extend_block_tables`` added restores the stack as it was."""
+    dev = N.require_device(block_tables, free, free_count)
+    n = block_tables.shape[0] if block_tables.ndim == 2 else -1
+    lens = _tree.ints(lengths, torch.int64, dev, "lengths", n)
+    keep = _tree.ints(kept, torch.int64, dev, "kept", n)
+    _tables(block_tables, block, dev, n)
+    _free_stack(free, free_count)
+    if n == 0:
+        return
+    plan = torch.empty(n + 1, dtype=torch.int32, device=dev)
+    N.call_on(dev, "yh_trim_block_tables", lens.data_ptr(), keep.data_ptr(), block_tables.data_ptr(), free.data_ptr(),
+              free_count.data_ptr(), plan.data_ptr(), n, block_tables.shape[1], free.shape[0], int(block),
+              int(bool(wrap)), N.stream_of(block_tables))
+
+
+def slot_map(cu_seqlens, lengths, block_tables, block, total, *, parents=None, last=None):
+    """Cache slots of the packed nodes of drafted trees: (slots int64 [total],
+    kept int64 [R]).  Node i of request r is at position lengths[r] + its depth
+    in the tree of ``parents`` (int32 [total], each the request's own earlier
+    node, -1: the context; None: chains, of any length).  With ``last`` (int [R],
+    the last accepted node of each request, -1: none) only the nodes on the path
+    to it get slots and the others -1, which ``layers.cache_write`` passes over;
+    ``kept`` is the request's length with them.  Without ``last`` all nodes get
+    one, siblings the same.  Trees of more than 64 nodes: -1 for the others."""
+    dev = N.require_device(block_tables)
+    total = int(total)
+    if total < 0:
+        raise ValueError("total must not be negative")
+    cu = _tree.offsets(cu_seqlens, total, dev, None if parents is None else _tree.MAX_NODES)
+    n = cu.shape[0] - 1
+    lens = _tree.ints(lengths, torch.int64, dev, "lengths", n)
+    _tables(block_tables, block, dev, n)
+    if parents is not None:
+        parents = _tree.ints(parents, torch.int32, dev, "parents", total)
+    if last is not None:
+        last = _tree.ints(last, torch.int32, dev, "last", n)
+    slots = torch.empty(total, dtype=torch.int64, device=dev)
+    kept = torch.empty(n, dtype=torch.int64, device=dev)
+    if n == 0:
+        return slots.fill_(-1), kept
+    N.call_on(dev, "yh_slot_map", cu.data_ptr(), lens.data_ptr(), block_tables.data_ptr(), N.ptr(parents), N.ptr(last),
+              slots.data_ptr(), kept.data_ptr(), n, block_tables.shape[1], total, int(block),
+              N.stream_of(block_tables))
+    return slots, kept

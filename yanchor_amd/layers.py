@@ -13,6 +13,7 @@ import ctypes
 import torch
 
 from . import _native as N
+from . import _tree
 
 
 def _bf16(*ts):
@@ -615,3 +616,147 @@ def ring_fill(k, v, cu_seqlens, starts, ring_rows, ring_k, ring_v, ring_pos):
     N.call("yh_ring_fill", k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), rr.data_ptr(), st.data_ptr(),
            cu.data_ptr(), r, n, ring_k.data_ptr(), ring_v.data_ptr(), ring_pos.data_ptr(), g, d, ring_k.shape[2],
            N.code(k), N.stream_of(k))
+
+
+# ---------------------------------------------------------------------------
+# Drafted trees over the caches: the nodes of all requests packed
+# (cu_seqlens), at most 64 a request; ``parents`` int32 [N] names the request's
+# own earlier node that each node follows, -1 the context (None: chains).
+# Nothing is read back to the host, so these calls can be captured.
+
+def _heads(x):
+    """(x, its token stride) of x [N, heads, D] with dense heads and 16-byte
+    aligned rows (a column view of a projection qualifies), of a copy otherwise."""
+    n, h, d = x.shape
+    if x.is_contiguous():   # a stride of a single row says nothing
+        return (x if x.data_ptr() % 16 == 0 else x.clone()), h * d
+    if x.stride(2) != 1 or (h > 1 and x.stride(1) != d) or x.stride(0) % 8 or x.stride(0) < h * d or \
+            x.data_ptr() % 16:
+        return x.contiguous(), h * d
+    return x, x.stride(0)
+
+
+def _cache(keys, values, g, d, dtype):
+    if keys.ndim != 4 or keys.shape[1] != g or keys.shape[3] != d or values.shape != keys.shape or \
+            keys.shape[2] < 1 or keys.dtype != dtype or values.dtype != dtype or not keys.is_contiguous() or \
+            not values.is_contiguous():
+        raise ValueError(f"keys / values must be contiguous [blocks, {g}, block, {d}] in {dtype}")
+
+
+def cache_write(k, v, slots, keys, values, *, positions=None, cache_positions=None):
+    """Key and value rows into a block cache IN PLACE: keys / values [blocks, G,
+    block, D] (the SWA ring [rows, G, window, D] is one) at slot
+    ``slots[n]`` = block id * block + row take k[n], v[n] [N, G, D] (any token
+    stride).  A slot below 0 or past the cache is passed over; the others must
+    be distinct.  With ``positions`` (int [N]) they go into
+    ``cache_positions`` int32 [blocks, G, block], as the ring's."""
+    if k.ndim != 3 or v.shape != k.shape or k.dtype != v.dtype or \
+            k.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError("cache_write takes bf16 / fp16 / fp32 k and v [N, G, D]")
+    n, g, d = k.shape
+    if d * k.element_size() % 16 or d == 0 or g == 0:
+        raise ValueError("a head's row must be a multiple of 16 bytes")
+    _cache(keys, values, g, d, k.dtype)
+    dev = N.require_device(k, v, keys, values, cache_positions)
+    slots = _tree.ints(slots, torch.int64, dev, "slots", n)
+    if (positions is None) != (cache_positions is None):
+        raise ValueError("positions and cache_positions come together")
+    if positions is not None:
+        positions = _tree.ints(positions, torch.int64, dev, "positions", n)
+        if cache_positions.dtype != torch.int32 or cache_positions.shape != keys.shape[:3] or \
+                not cache_positions.is_contiguous():
+            raise ValueError("cache_positions must be contiguous int32 [blocks, G, block]")
+    (k, ks), (v, vs) = _heads(k), _heads(v)
+    N.call_on(dev, "yh_cache_write", k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(),
+              keys.data_ptr(), values.data_ptr(), N.ptr(positions), N.ptr(cache_positions), n, keys.shape[0], g, d,
+              keys.shape[2], N.code(k), N.stream_of(k))
+
+
+def tree_attention(q, k, v, parents, cu_seqlens, lengths, keys, values, block_tables, *, window=None, gate=None,
+                   scale=None, max_nodes=None, max_length=None):
+    """Attention of the packed nodes of drafted trees over a block cache.  Node
+    i of request r is at position lengths[r] + its depth and sees, as far as
+    they lie less than ``window`` before it (None: all), the ``lengths[r]``
+    cached positions and its own ancestors among the nodes, itself included.
+    q [N, H, D], k, v [N, G, D] (the nodes', normed and rotated, any token
+    stride; D 64 or 128, bf16 / fp16); keys / values [blocks, G, block, D]:
+    position p is row p % block of block ``block_tables[r, p // block %
+    columns]`` (int32 [R, columns]), of which the last columns * block
+    positions are there.  The SWA ring is such a cache: keys = ring_k, values =
+    ring_v, block_tables = ring rows [R, 1], window = the ring's.  gate None or
+    [N, H, D] (unit last stride): the result is read * sigmoid(gate).  A chain
+    (parents None) of one node a request is decode attention.  Returns [N, H,
+    D]; rows behind the last request are zeros.  ``max_nodes``: the most nodes
+    of any request (default 64); a node past it comes back as not-a-number.
+    The nodes' keys and values are not written to the cache (``cache_write``
+    writes those of the accepted path)."""
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("tree_attention takes bf16 / fp16 q, k, v of one dtype")
+    if q.ndim != 3 or k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or v.shape != k.shape or \
+            k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError("tree_attention needs q [N, H, D] and k / v [N, G, D] with G dividing the query heads")
+    n, h, d = q.shape
+    g = k.shape[1]
+    if d not in (64, 128):
+        raise ValueError("head dim must be 64 or 128")
+    _cache(keys, values, g, d, q.dtype)
+    dev = N.require_device(q, k, v, keys, values, block_tables, gate)
+    parents, cu, most = _tree.nodes(parents, cu_seqlens, max_nodes, n, dev)
+    r = cu.shape[0] - 1
+    lens = _tree.ints(lengths, torch.int64, dev, "lengths", r)
+    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.shape[0] != r or \
+            block_tables.shape[1] < 1:
+        raise ValueError("block_tables must be int32 [R, columns]")
+    tables = block_tables if block_tables.is_contiguous() else block_tables.contiguous()
+    if window is not None and int(window) < 1:
+        raise ValueError("window must be at least 1")
+    sc = float(d ** -0.5 if scale is None else scale)
+    if not 0 < sc < float("inf"):   # the masks count on scores that keep their order
+        raise ValueError("scale must be positive")
+    (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k), _heads(v)
+    gp, gts, ghs = None, 0, 0
+    if gate is not None:
+        if gate.shape != (n, h, d) or gate.dtype != q.dtype:
+            raise ValueError("gate must be [N, H, D] in the query dtype")
+        if gate.stride(2) != 1 or gate.stride(1) < d or gate.stride(0) < h * gate.stride(1):   # not rows of heads
+            gate = gate.contiguous()
+        gp = gate.data_ptr()
+        gts, ghs = (h * d, d) if gate.is_contiguous() else (gate.stride(0), gate.stride(1))
+    out = torch.empty(n, h, d, dtype=q.dtype, device=dev)
+    N.call_on(dev, "yh_tree_attention", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+              N.ptr(parents), cu.data_ptr(), lens.data_ptr(), keys.data_ptr(), values.data_ptr(),
+              tables.data_ptr(), gp, gts, ghs, out.data_ptr(), r, n, keys.shape[0], tables.shape[1], h, g, d,
+              keys.shape[2], 0 if window is None else int(window), most, sc,
+              N.code(q), N.stream_of(q))
+    return out
+
+
+def conv_tree(proj, window, conv_w, parents, cu_seqlens, channels, planes=1):
+    """``conv_prefill``'s causal conv1d + SiLU for the packed nodes of drafted
+    trees, each over its own path: proj [N, >= channels] bf16 (the conv inputs
+    are its first ``channels`` columns, any row stride), window [R, 3,
+    channels] bf16 the inputs before the nodes, NOT updated (which path stays
+    is not known yet); conv_w [channels, 4].  Returns [N, channels], or with
+    ``planes`` > 1 [planes, N, channels / planes]; rows behind the last request
+    are zeros."""
+    _bf16(proj, window, conv_w)
+    dev = N.require_device(proj, window, conv_w)
+    channels, planes = int(channels), int(planes)
+    if proj.ndim != 2 or channels < 1 or proj.shape[1] < channels:
+        raise ValueError("proj must be [N, >= channels]")
+    if planes < 1 or channels % planes:
+        raise ValueError("planes must divide the channels")
+    n = proj.shape[0]
+    parents, cu, _ = _tree.nodes(parents, cu_seqlens, None, n, dev)
+    r = cu.shape[0] - 1
+    if window.shape != (r, 3, channels) or not window.is_contiguous():
+        raise ValueError(f"window must be contiguous [{r}, 3, {channels}]")
+    if conv_w.shape != (channels, 4) or not conv_w.is_contiguous():
+        raise ValueError("conv_w must be contiguous [channels, 4]")
+    if proj.stride(1) != 1 or (n > 1 and proj.stride(0) < channels):
+        proj = proj.contiguous()
+    out = torch.empty((n, channels) if planes == 1 else (planes, n, channels // planes), dtype=proj.dtype, device=dev)
+    N.call_on(dev, "yh_conv_tree", proj.data_ptr(), max(proj.stride(0), channels), window.data_ptr(),
+              conv_w.data_ptr(), N.ptr(parents), cu.data_ptr(), r, n, channels, planes, out.data_ptr(), N.BF16,
+              N.stream_of(proj))
+    return out
