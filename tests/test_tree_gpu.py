@@ -250,6 +250,30 @@ def test_delta_rule_counts_past_max_nodes(gpu):
     assert o[0, 64:70].isnan().all() and not o[0, :64].isnan().any() and not o[0, 70:].isnan().any()
 
 
+@pytest.mark.parametrize("which", ["q", "k", "v", "g", "beta"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_delta_rule_keeps_what_is_not_finite_on_its_path(gpu, which, dtype):
+    cu, parents = trees([40, 20], 41)
+    n = cu[-1]
+    x = dict(q=rnd(1, n, 2, 128, seed=1, dtype=dtype), k=rnd(1, n, 2, 128, seed=2, dtype=dtype),
+             v=rnd(1, n, 2, 128, seed=3, dtype=dtype), g=-torch.rand(1, n, 2), beta=torch.rand(1, n, 2))
+    s0 = rnd(2, 2, 128, 128, seed=4, dtype=torch.float32)
+    call = lambda: gdn.tree_gated_delta_rule(*(x[t].to(gpu) for t in ("q", "k", "v", "g", "beta")), i32(parents, gpu),  # noqa: E731
+                                             i32(cu, gpu), s0.to(gpu))[0].cpu()
+    clean = call()
+    for at, value in ((7, NAN), (45, float("inf"))):
+        x[which][0, at] = value
+    got = call()
+    for r in range(2):
+        for i, path in enumerate(ref.paths(parents[cu[r]:cu[r + 1]], cu[r + 1] - cu[r])):
+            row = cu[r] + i
+            if 7 - cu[r] in path or 45 - cu[r] in path:
+                if which != "q" or row in (7, 45):     # a query is its own node's alone
+                    assert not torch.isfinite(got[row]).all()
+                    continue
+            assert torch.equal(got[row], clean[row]), row
+
+
 # --- conv ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("channels,planes,extra,chain", [(24, 3, 8, False), (4096, 1, 0, False), (30, 3, 1, False),

@@ -128,6 +128,328 @@ __global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// bf16 q / k / v with K = 128 on MFMA: a workgroup a request and value head, its
+// four waves a quarter of the value columns each.
+//
+// In the masks' order (a node's ancestors come before it) everything above is
+// a lower triangular product over 16-node tiles, as in a chunk of a prompt:
+//   low_ij = beta_i e^{G_i - G_j} (k_i . k_j), att_ij = e^{G_i - G_j} (q_i . k_j)
+// where j is above i, 0 elsewhere; w_i = beta_i (v_i - e^{G_i} k_i S); then tile by
+// tile u_b = (I + low_bb)^-1 (w_b - sum_{a < b} low_ba u_a), with the inverses of
+// the diagonal tiles by forward substitution.
+//
+// q and k are exact bf16 operands, their norms and the decays go into the
+// factors; float32 operands (S, low, att, w, u) enter the products as pairs hi +
+// lo of bf16, which leaves 2^-16 of each product.  S is read straight into the
+// operand layout: a lane holds rows 32 s + 8 (lane / 16) + 0..7 of V / 64
+// neighbouring columns.
+//
+// What is not finite in one node may reach its own descendants only, but a
+// product of a 0 in the mask with it would spread it: such elements enter the
+// products as 0 and their bits (`bad`) turn the descendants' outputs into NaN.
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+typedef float f32x2v __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x4v mma32(bf16x8_t a, bf16x8_t b, f32x4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4v mma16(uint2 a, uint2 b, f32x4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, a), __builtin_bit_cast(s16x4_t, b), c, 0,
+                                                   0, 0);
+}
+// Two values as bf16 hi (to nearest) and lo = bf16(x - hi), packed in pairs.
+__device__ __forceinline__ void pair2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v){x, y}, bf16x2_t));
+  lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v){x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u)}, bf16x2_t));
+}
+// One value as a word hi << 16 | lo, and back.
+__device__ __forceinline__ uint32_t split1(float x) {
+  const uint16_t hi = f32_to_bf16(x);
+  return static_cast<uint32_t>(hi) << 16 | f32_to_bf16(x - bf16_to_f32(hi));
+}
+__device__ __forceinline__ float join1(uint32_t w) { return __uint_as_float(w & 0xffff0000u) + __uint_as_float(w << 16); }
+// Four such words as the hi and the lo operand.
+__device__ __forceinline__ void unzip4(uint4 w, uint2& hi, uint2& lo) {
+  hi = make_uint2(__builtin_amdgcn_perm(w.y, w.x, 0x07060302), __builtin_amdgcn_perm(w.w, w.z, 0x07060302));
+  lo = make_uint2(__builtin_amdgcn_perm(w.y, w.x, 0x05040100), __builtin_amdgcn_perm(w.w, w.z, 0x05040100));
+}
+__device__ __forceinline__ f32x4v mma16x3(uint4 a, uint2 bhi, uint2 blo, f32x4v c) {
+  uint2 hi, lo;
+  unzip4(a, hi, lo);
+  c = mma16(lo, bhi, c);
+  c = mma16(hi, blo, c);
+  return mma16(hi, bhi, c);
+}
+
+template <int ST, int V, int T>
+__global__ void __launch_bounds__(256, T == 4 ? 2 : 4) tree_gdn_mfma_kernel(GdnArgs a) {
+  constexpr int kN = 16 * T, K = 128, CT = V / 64, SF = kN + 4;   // CT columns a lane
+  __shared__ uint4 s_q[kN * 16], s_k[kN * 16];     // rows of 16 pieces, piece p of row r at p ^ (r % 16)
+  __shared__ uint32_t s_low[kN][SF], s_att[kN][SF], s_inv[kN][20];   // split1 words; -low
+  __shared__ float s_g[64], s_beta[64], s_rk[kN], s_rq[kN];
+  __shared__ uint64_t s_set[64];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n16 = lane & 15, quad = lane >> 4;
+  uint16_t* out = static_cast<uint16_t*>(a.o);
+  if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(a.R) * a.HV) {   // rows of no request
+    const int64_t end = a.R ? a.cu[a.R] : 0, row = static_cast<int64_t>(a.HV) * V;
+    for (int64_t i = (end < 0 ? 0 : end) * row + tid; i < a.total * row; i += 256) out[i] = 0;
+    return;
+  }
+  const int hv = blockIdx.x % a.HV, r = blockIdx.x / a.HV, h = hv / (a.HV / a.H);
+  const tree::Span span = tree::span_of(a.cu, r, a.total);
+  const int64_t srow = a.rows ? a.rows[r] : r;
+  const bool none = srow < 0 || srow >= a.n_rows;
+  const int most = a.max_nodes < kN ? a.max_nodes : kN;
+  const int n = none ? 0 : static_cast<int>(span.count < most ? span.count : most);
+  for (int64_t i = n; i < span.count; ++i)   // no request: zeros; nodes past the most that the call takes: not a number
+    for (int c = tid; c < V; c += 256) out[((span.first + i) * a.HV + hv) * V + c] = none ? 0 : 0x7fc0;
+  if (n == 0) return;
+  const int nt = (n + 15) >> 4;
+
+  // q and k rows (a thread a piece of every 16th row), then the state, which arrives behind them
+  uint4 rq[T], rk[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int i = 16 * t + (tid >> 4);
+    const int64_t at = ((span.first + (i < n ? i : 0)) * a.H + h) * K + (tid & 15) * 8;
+    rq[t] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at);
+    rk[t] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.k) + at);
+    if (i >= n) rq[t] = rk[t] = make_uint4(0, 0, 0, 0);
+  }
+  const int64_t gat = (span.first + (lane < n ? lane : 0)) * a.HV + hv;
+  float gate = 0.f, beta = 0.f;
+  if (w == 0) {
+    gate = lane < n ? load_any(a.g, gat, a.g_dt) : 0.f;
+    beta = lane < n ? load_any(a.beta, gat, a.beta_dt) : 0.f;
+  }
+  const int col = w * 16 * CT + n16 * CT;
+  float sv[4][8][CT];
+  const int64_t sat = (srow * a.HV + hv) * K * V + col;
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t at = sat + (32 * s + 8 * quad + j) * V;
+      if constexpr (ST == YH_F32) {
+        typedef float ldv __attribute__((ext_vector_type(CT)));
+        const ldv x = __builtin_nontemporal_load(reinterpret_cast<const ldv*>(static_cast<const float*>(a.state) + at));
+#pragma unroll
+        for (int c = 0; c < CT; ++c) sv[s][j][c] = x[c];
+      } else {
+        typedef _Float16 ldv __attribute__((ext_vector_type(CT)));
+        const ldv x = __builtin_nontemporal_load(reinterpret_cast<const ldv*>(static_cast<const _Float16*>(a.state) + at));
+#pragma unroll
+        for (int c = 0; c < CT; ++c) sv[s][j][c] = static_cast<float>(x[c]);
+      }
+    }
+  if (w == 0) {
+    const uint64_t set = tree::ancestors(a.parents ? a.parents + span.first : nullptr, n, &gate);
+    s_set[lane] = set;
+    s_g[lane] = gate;
+    s_beta[lane] = beta;
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int i = 16 * t + (tid >> 4), p = i * 16 + ((tid & 15) ^ (i & 15));
+    s_q[p] = rq[t];
+    s_k[p] = rk[t];
+    float sums[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const uint4 y = x ? rk[t] : rq[t];
+      const uint32_t word[4] = {y.x, y.y, y.z, y.w};
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float lo = __uint_as_float(word[e] << 16), hi = __uint_as_float(word[e] & 0xffff0000u);
+        sum = fmaf(lo, lo, fmaf(hi, hi, sum));
+      }
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+      sums[x] = a.l2 ? rsqrtf(sum + 1e-6f) : 1.f;
+    }
+    if ((tid & 15) == 0) {
+      s_rq[i] = a.scale * sums[0];
+      s_rk[i] = sums[1];
+    }
+  }
+  __syncthreads();
+
+  auto operand = [&](const uint4* m, int t, int s) {   // rows of tile t, columns 32 s + 8 quad ..
+    return __builtin_bit_cast(bf16x8_t, m[(16 * t + n16) * 16 + ((4 * s + quad) ^ n16)]);
+  };
+  // low and att, a wave every fourth pair of tiles
+  {
+    int pair = 0;
+#pragma unroll 1
+    for (int ta = 0; ta < nt; ++ta)
+#pragma unroll 1
+      for (int tb = 0; tb <= ta; ++tb, ++pair) {
+        if ((pair & 3) != w) continue;
+        f32x4v kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const bf16x8_t b = operand(s_k, tb, s);
+          kk = mma32(operand(s_k, ta, s), b, kk);
+          qk = mma32(operand(s_q, ta, s), b, qk);
+        }
+        const int j = 16 * tb + n16;
+        const float rkj = s_rk[j], gj = s_g[j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 16 * ta + 4 * quad + e;
+          const bool above = (s_set[i] >> j) & 1;
+          const float f = above ? __expf(s_g[i] - gj) * rkj : 0.f;
+          s_low[i][j] = above && i != j ? split1(-s_beta[i] * s_rk[i] * f * kk[e]) : 0u;
+          s_att[i][j] = above ? split1(s_rq[i] * f * qk[e]) : 0u;
+        }
+      }
+  }
+  __syncthreads();
+  if (w == 0) {   // the diagonal tiles' inverses: a lane a column
+    const int b = 16 * quad;
+    if (quad < nt) {
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float acc = i == n16 ? 1.f : 0.f;
+#pragma unroll
+        for (int m = 0; m < i; ++m) {
+          const uint32_t l = s_low[b + i][b + m];
+          acc = l ? fmaf(join1(l), x[m], acc) : acc;
+        }
+        x[i] = acc;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s_inv[b + i][n16] = split1(x[i]);
+    }
+  }
+  // k S and q S
+  f32x4v ks[T][CT], qs[T][CT];
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int c = 0; c < CT; ++c) ks[t][c] = qs[t][c] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    bf16x8_t hi[CT], lo[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      uint32_t x[4], y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pair2(sv[s][2 * j][c], sv[s][2 * j + 1][c], x[j], y[j]);
+      hi[c] = __builtin_bit_cast(bf16x8_t, make_uint4(x[0], x[1], x[2], x[3]));
+      lo[c] = __builtin_bit_cast(bf16x8_t, make_uint4(y[0], y[1], y[2], y[3]));
+    }
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      if (t >= nt) break;
+      const bf16x8_t k8 = operand(s_k, t, s), q8 = operand(s_q, t, s);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        ks[t][c] = mma32(k8, lo[c], ks[t][c]);
+        ks[t][c] = mma32(k8, hi[c], ks[t][c]);
+        qs[t][c] = mma32(q8, lo[c], qs[t][c]);
+        qs[t][c] = mma32(q8, hi[c], qs[t][c]);
+      }
+    }
+  }
+  __syncthreads();
+
+  uint2 uhi[T][CT], ulo[T][CT];
+  uint64_t bad[CT] = {};
+#pragma unroll
+  for (int b = 0; b < T; ++b) {
+    if (b >= nt) break;
+    float ge[4], bt[4];
+    f32x4v x[CT];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 16 * b + 4 * quad + e;
+      ge[e] = __expf(s_g[i]);
+      bt[e] = s_beta[i];
+      const uint16_t* v = static_cast<const uint16_t*>(a.v) + ((span.first + (i < n ? i : 0)) * a.HV + hv) * V + col;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const float y = bt[e] * (bf16_to_f32(v[c]) - ge[e] * s_rk[i] * ks[b][c][e]);
+        x[c][e] = i < n ? y : 0.f;
+      }
+    }
+#pragma unroll
+    for (int ta = 0; ta < b; ++ta) {
+      const uint4 l = *reinterpret_cast<const uint4*>(&s_low[16 * b + n16][16 * ta + 4 * quad]);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) x[c] = mma16x3(l, uhi[ta][c], ulo[ta][c], x[c]);
+    }
+    // elements that are not finite: 0, and their bit
+    auto pack = [&](f32x4v& y, int c, uint2& hi, uint2& lo) {
+      uint32_t off = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (!(fabsf(y[e]) < INFINITY)) {
+          off |= 1u << e;
+          y[e] = 0.f;
+        }
+      bad[c] |= static_cast<uint64_t>(off) << (16 * b + 4 * quad);
+      pair2(y[0], y[1], hi.x, lo.x);
+      pair2(y[2], y[3], hi.y, lo.y);
+    };
+    const uint4 inv = *reinterpret_cast<const uint4*>(&s_inv[16 * b + n16][4 * quad]);
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      uint2 hi, lo;
+      pack(x[c], c, hi, lo);
+      f32x4v u = mma16x3(inv, hi, lo, f32x4v{0.f, 0.f, 0.f, 0.f});
+      pack(u, c, uhi[b][c], ulo[b][c]);
+    }
+    f32x4v o[CT];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int c = 0; c < CT; ++c) o[c][e] = ge[e] * s_rq[16 * b + 4 * quad + e] * qs[b][c][e];
+#pragma unroll
+    for (int ta = 0; ta <= b; ++ta) {
+      const uint4 l = *reinterpret_cast<const uint4*>(&s_att[16 * b + n16][16 * ta + 4 * quad]);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) o[c] = mma16x3(l, uhi[ta][c], ulo[ta][c], o[c]);
+    }
+    uint64_t any = bad[0];
+    if constexpr (CT == 2) any |= bad[1];
+    if (__any(any != 0)) {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        bad[c] |= __shfl_xor(bad[c], 16, 64);
+        bad[c] |= __shfl_xor(bad[c], 32, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (bad[c] & s_set[16 * b + 4 * quad + e]) o[c][e] = NAN;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 16 * b + 4 * quad + e;
+      if (i >= n) continue;
+      uint16_t* to = out + ((span.first + i) * a.HV + hv) * V + col;
+      if constexpr (CT == 2)
+        *reinterpret_cast<uint32_t*>(to) = attn::Mfma<YH_BF16>::round2(o[0][e], o[1][e]);
+      else
+        *to = f32_to_bf16(o[0][e]);
+    }
+  }
+}
+
+template <int ST, int V>
+void launch_mfma(const GdnArgs& a, unsigned grid, hipStream_t st) {
+  if (a.max_nodes <= 16) hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 1>), dim3(grid), dim3(256), 0, st, a);
+  else if (a.max_nodes <= 32) hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 2>), dim3(grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 4>), dim3(grid), dim3(256), 0, st, a);
+}
+
+// ---------------------------------------------------------------------------
 struct ConvTreeArgs {
   const uint16_t* proj;     // [N, P], the first C columns
   int64_t P;
@@ -239,7 +561,13 @@ extern "C" int yh_tree_gated_delta_rule(const void* q, const void* k, const void
             (int)HV, (int)max_nodes, use_qk_l2norm ? 1 : 0, qkv_dtype, g_dtype, beta_dtype, state_dtype, scale};
   const unsigned grid = static_cast<unsigned>(n_seqs * HV + 1);   // the last clears the rows of no request
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (K == 128 && V == 128) hipLaunchKernelGGL((tree_gdn_any_kernel<128, 128>), dim3(grid), dim3(256), 0, st, a);
+  const bool mfma = K == 128 && qkv_dtype == YH_BF16 && tree::aligned16(q) && tree::aligned16(k) &&
+                    tree::aligned16(state) && (reinterpret_cast<uintptr_t>(o) & 3) == 0;
+  if (mfma && state_dtype == YH_F32 && V == 128) launch_mfma<YH_F32, 128>(a, grid, st);
+  else if (mfma && state_dtype == YH_F32) launch_mfma<YH_F32, 64>(a, grid, st);
+  else if (mfma && V == 128) launch_mfma<YH_F16, 128>(a, grid, st);
+  else if (mfma) launch_mfma<YH_F16, 64>(a, grid, st);
+  else if (K == 128 && V == 128) hipLaunchKernelGGL((tree_gdn_any_kernel<128, 128>), dim3(grid), dim3(256), 0, st, a);
   else if (K == 128) hipLaunchKernelGGL((tree_gdn_any_kernel<128, 64>), dim3(grid), dim3(256), 0, st, a);
   else if (V == 128) hipLaunchKernelGGL((tree_gdn_any_kernel<64, 128>), dim3(grid), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((tree_gdn_any_kernel<64, 64>), dim3(grid), dim3(256), 0, st, a);
