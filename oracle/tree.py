@@ -87,14 +87,13 @@ def attention(q, k, v, parents, cu, lengths, keys, values, tables, window=None, 
             pos = length + len(path) - 1
             oldest = max(0, length - columns * block, pos - window + 1 if window else 0)
             at = [p for p in range(oldest, length) if 0 <= int(tables[r, p // block % columns]) < keys.shape[0]]
-            rows = [(int(tables[r, p // block % columns]), p % block) for p in at]
+            ids, rows = [int(tables[r, p // block % columns]) for p in at], [p % block for p in at]
             near = [j for e, j in enumerate(path) if not window or len(path) - 1 - e < window]
             for head in range(h):
                 kv = head // (h // g)
-                ks = [keys[x, kv, y] for x, y in rows] + [k[a + j, kv] for j in near]
-                vs = [values[x, kv, y] for x, y in rows] + [v[a + j, kv] for j in near]
-                s = torch.stack(ks).to(F64) @ q[a + i, head].to(F64) * scale
-                out[a + i, head] = torch.softmax(s, 0) @ torch.stack(vs).to(F64)
+                ks = torch.cat((keys[ids, kv, rows], k[[a + j for j in near], kv])).to(F64)
+                vs = torch.cat((values[ids, kv, rows], v[[a + j for j in near], kv])).to(F64)
+                out[a + i, head] = torch.softmax(ks @ q[a + i, head].to(F64) * scale, 0) @ vs
     return out if gate is None else out * torch.sigmoid(gate.to(F64))
 
 

@@ -141,6 +141,21 @@ def test_attention_of_single_tokens(gpu):
     attention_case(gpu, [513, 0, 1024, 77], [1, 1, 1, 1], chain=True, max_nodes=1, h=32, g=8, seed=7)
 
 
+def test_attention_long_caches_in_parts(gpu):
+    attention_case(gpu, [3000, 70, 900, 4097], [2, 40, 17, 1], h=4, g=2, seed=51)
+    attention_case(gpu, [2500, 1300], [64, 3], h=8, g=1, block=64, gate="dense", seed=52)    # 512 rows a head
+    attention_case(gpu, [5000], [1], h=2, g=1, d=64, chain=True, max_nodes=1, dtype=torch.float16, seed=53)
+
+
+def test_attention_of_many_requests(gpu):
+    """More requests than a workgroup has threads, some of one token and some of none."""
+    gen = torch.Generator().manual_seed(1)
+    lengths = torch.randint(0, 90, (700,), generator=gen).tolist()
+    lengths[3], lengths[600] = 2000, 1500
+    counts = torch.randint(0, 3, (700,), generator=gen).tolist()
+    attention_case(gpu, lengths, counts, h=2, g=1, seed=54, window=1200)
+
+
 def test_attention_holes_in_a_table_are_not_seen(gpu):
     attention_case(gpu, [200, 130], [8, 8], bad=[(0, 3, -1), (0, 7, 1 << 30), (1, 0, 10 ** 6), (1, 8, -5)], seed=8)
 

@@ -8,10 +8,16 @@
 // tables[r][p / block % columns], so the last columns * block positions are
 // there; a ring is a table of one column whose block is the ring.
 //
-// A workgroup takes a request, a KV head and 128 of the rows (node, query head
-// of the group): four waves of 32 rows share 64-key tiles (attn_tile.h) that
-// begin at multiples of 64 positions; the nodes themselves are the last tile,
-// its mask the ancestor sets.
+// A workgroup of NW waves (4, or 8 for more than 128 rows) takes a request, a KV
+// head and 32 NW of the rows (node, query head of the group): the waves, 32 rows
+// each, share 64-key tiles (attn_tile.h) that begin at multiples of 64
+// positions; the nodes themselves are the last tile, its mask the ancestor sets.
+//
+// Requests are few or of very different lengths, so the tiles of an item
+// (request, rows, head) are cut into parts of about one size (`chunk`, about
+// kParts parts a workgroup that fits the chip): every workgroup finds its part
+// from the lengths by itself, parts of a cut item leave their unnormalised sums
+// with their maximum, and a second launch joins them in order.
 #include <type_traits>
 
 #include "attn_tile.h"
@@ -41,38 +47,179 @@ struct TreeArgs {
   int R, H, G, NB, max_nodes, mtiles;
   int gate8;               // gate rows keep 8-byte alignment
   float scale;
+  // the cut: parts aimed at, and for requests [0, R] the first part, the first partial sum
+  int target, slot_rows;
+  int32_t* first;          // [R + 1]
+  int32_t* slot;           // [R + 1]
+  float* part;             // [slots, slot_rows, D]
+  float2* stat;            // [slots, slot_rows]: maximum (log2), denominator
 };
 
-constexpr int kNW = 4;                       // waves a workgroup
-constexpr int kM = kNW * attn::kRows;        // rows a workgroup
+constexpr int kMinChunk = 4;   // tiles a part at least (but for short items)
 
-template <int DT, int D>
-__global__ void __launch_bounds__(kNW * 64, 2) tree_attention_kernel(TreeArgs a) {
+// What a request asks for: rows, and the positions [lo, L) of its cache that
+// some node sees, in tiles from `base`.
+struct Geometry {
+  tree::Span span;
+  int64_t length;
+  int n, lo, L, base, ctx;
+};
+__device__ __forceinline__ Geometry geometry(const TreeArgs& a, int64_t r) {
+  Geometry q;
+  q.span = tree::span_of(a.cu, r, a.total);
+  q.n = static_cast<int>(q.span.count < a.max_nodes ? q.span.count : a.max_nodes);
+  q.length = a.lengths[r] < 0 ? 0 : a.lengths[r];
+  const int64_t room = static_cast<int64_t>(a.columns.d) * a.block.d;
+  int64_t oldest = q.length - room;
+  if (a.window && q.length - a.window + 1 > oldest) oldest = q.length - a.window + 1;
+  oldest = oldest < 0 ? 0 : oldest > q.length ? q.length : oldest;
+  constexpr int64_t kEnd = (1ll << 31) - 1;
+  q.lo = static_cast<int>(oldest < kEnd ? oldest : kEnd);
+  q.L = static_cast<int>(q.length < kEnd ? q.length : kEnd);
+  q.base = q.lo & ~(attn::kTile - 1);
+  q.ctx = q.L > q.lo ? (q.L - q.base + attn::kTile - 1) / attn::kTile : 0;
+  return q;
+}
+
+// A part: tiles [t0, t1) of an item, its partial sum's place (-1: the item is whole).
+struct Part {
+  int r, mt, g, t0, t1, slot;
+};
+
+template <int TH>
+__device__ __forceinline__ int64_t block_sum(int64_t x, int64_t* before) {   // total, and the sum of earlier threads
+  __shared__ int64_t sums[TH / 64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int64_t incl = x;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t y = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += y;
+  }
+  if (lane == 63) sums[w] = incl;
+  __syncthreads();
+  int64_t all = 0, early = 0;
+#pragma unroll
+  for (int i = 0; i < TH / 64; ++i) {
+    early += i < w ? sums[i] : 0;
+    all += sums[i];
+  }
+  __syncthreads();
+  *before = early + incl - x;
+  return all;
+}
+
+// Part `id` of the call, false if there are not so many.  An item of T tiles is
+// cut into the T / chunk parts to the nearest whole, so only items of 1.5 chunks
+// and more are: at most 4/3 target parts leave partial sums.
+template <int NW>
+__device__ __forceinline__ bool find_part(const TreeArgs& a, int64_t id, Part* out) {
+  constexpr int TH = NW * 64, kM = NW * attn::kRows;
+  __shared__ int found[6];
+  const int tid = threadIdx.x;
+  auto shape = [&](int64_t r, int64_t* items, int* tiles) {
+    *items = 0;
+    *tiles = 1;
+    if (r >= a.R) return;
+    const Geometry q = geometry(a, r);
+    *items = static_cast<int64_t>((q.n * static_cast<int>(a.rep.d) + kM - 1) / kM) * a.G;
+    *tiles = q.ctx + 1;
+  };
+  int64_t units = 0, before;
+  for (int64_t r = tid; r - tid < a.R; r += TH) {
+    int64_t items;
+    int tiles;
+    shape(r, &items, &tiles);
+    units += block_sum<TH>(items * tiles, &before);
+  }
+  int64_t chunk = (units + a.target - 1) / a.target;
+  chunk = chunk < kMinChunk ? kMinChunk : chunk;
+  int64_t parts = 0, cut = 0;
+  if (tid == 0) found[0] = -1;
+  for (int64_t r = tid; r - tid < a.R; r += TH) {
+    int64_t items, first, slot;
+    int tiles;
+    shape(r, &items, &tiles);
+    const int64_t p = tiles * 2ll < 3 * chunk ? 1 : (2ll * tiles + chunk) / (2 * chunk), mine = items * p;
+    const int64_t all = block_sum<TH>(mine, &first), all_cut = block_sum<TH>(p > 1 ? mine : 0, &slot);
+    first += parts;
+    slot += cut;
+    if (r < a.R) {
+      if (id == 0) {
+        a.first[r] = static_cast<int32_t>(first);
+        a.slot[r] = static_cast<int32_t>(slot);
+        if (r == a.R - 1) a.first[a.R] = static_cast<int32_t>(first + mine);
+      }
+      if (id >= first && id < first + mine) {
+        const int64_t in = id - first, item = in / p, j = in - item * p;
+        found[0] = static_cast<int>(r);
+        found[1] = static_cast<int>(item / a.G);
+        found[2] = static_cast<int>(item % a.G);
+        found[3] = static_cast<int>(j * tiles / p);
+        found[4] = static_cast<int>((j + 1) * tiles / p);
+        found[5] = p > 1 ? static_cast<int>(slot + in) : -1;
+      }
+    }
+    parts += all;
+    cut += all_cut;
+  }
+  __syncthreads();
+  *out = Part{found[0], found[1], found[2], found[3], found[4], found[5]};
+  return found[0] >= 0;
+}
+
+// read * sigmoid(gate) and the rounding to 16 bits of 4 outputs of dims dim .. dim + 3
+template <int DT>
+__device__ __forceinline__ void put4(const TreeArgs& a, int64_t row, int head, int dim, int D, float4 o) {
   using M = attn::Mfma<DT>;
+  if (a.gate) {
+    const uint16_t* gate = a.gate + row * a.g_ts + head * a.g_hs + dim;
+    uint16_t x[4];
+    if (a.gate8) {
+      const uint2 y = *reinterpret_cast<const uint2*>(gate);
+      x[0] = y.x & 0xffff;
+      x[1] = y.x >> 16;
+      x[2] = y.y & 0xffff;
+      x[3] = y.y >> 16;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = gate[e];
+    }
+    o.x *= 1.f / (1.f + __expf(-M::widen(x[0])));
+    o.y *= 1.f / (1.f + __expf(-M::widen(x[1])));
+    o.z *= 1.f / (1.f + __expf(-M::widen(x[2])));
+    o.w *= 1.f / (1.f + __expf(-M::widen(x[3])));
+  }
+  *reinterpret_cast<uint2*>(a.out + (row * a.H + head) * D + dim) = make_uint2(M::round2(o.x, o.y), M::round2(o.z, o.w));
+}
+
+template <int DT, int D, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) {
+  constexpr int kM = NW * attn::kRows;   // rows of the workgroup
   __shared__ attn::Rows stage[4];   // two buffers of key rows, two of value rows
   __shared__ uint64_t s_set[tree::kNodes];
   __shared__ int s_deep;
   attn::Rows *ktile = stage, *vtile = stage + 2;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  const int64_t work = static_cast<int64_t>(a.R) * a.G * a.mtiles;
-  if (static_cast<int64_t>(blockIdx.x) >= work) {   // rows of no request
+  if (blockIdx.x == gridDim.x - 1) {   // rows of no request
     const int64_t end = a.R ? a.cu[a.R] : 0, row = static_cast<int64_t>(a.H) * D;
-    for (int64_t i = (end < 0 ? 0 : end) * row + threadIdx.x; i < a.total * row; i += kNW * 64) a.out[i] = 0;
+    for (int64_t i = (end < 0 ? 0 : end) * row + threadIdx.x; i < a.total * row; i += NW * 64) a.out[i] = 0;
     return;
   }
-  const int g = blockIdx.x % a.G, mt = blockIdx.x / a.G % a.mtiles, r = blockIdx.x / a.G / a.mtiles;
-  const tree::Span span = tree::span_of(a.cu, r, a.total);
-  const int n = static_cast<int>(span.count < a.max_nodes ? span.count : a.max_nodes);
-  const int rep = a.rep.d;
-  if (mt == 0) {   // nodes past the most that the call takes: not a number
+  Part part;
+  if (!find_part<NW>(a, blockIdx.x, &part)) return;
+  const int g = part.g, mt = part.mt, r = part.r;
+  const Geometry geo = geometry(a, r);
+  const tree::Span span = geo.span;
+  const int n = geo.n, rep = a.rep.d;
+  if (mt == 0 && part.t0 == 0) {   // nodes past the most that the call takes: not a number
     const int64_t first = span.first + n, row = static_cast<int64_t>(a.H) * D;
-    for (int64_t i = threadIdx.x; i < (span.count - n) * rep * D; i += kNW * 64) {
+    for (int64_t i = threadIdx.x; i < (span.count - n) * rep * D; i += NW * 64) {
       const int64_t t = i / (rep * D);
       a.out[(first + t) * row + static_cast<int64_t>(g) * rep * D + (i - t * rep * D)] = DT == YH_BF16 ? 0x7fc0 : 0x7e00;
     }
   }
-  if (mt * kM >= n * rep) return;
 
   if (w == 0) {
     const uint64_t set = tree::ancestors(a.parents ? a.parents + span.first : nullptr, n);
@@ -92,15 +239,10 @@ __global__ void __launch_bounds__(kNW * 64, 2) tree_attention_kernel(TreeArgs a)
   const int node = mine ? a.rep.quot(m) : 0, head = g * rep + (mine ? m - node * rep : 0);
   uint64_t see = mine ? s_set[node] : 0;
   const int depth = mine ? __popcll(see) - 1 : 0;
-  const int64_t length = a.lengths[r] < 0 ? 0 : a.lengths[r];
+  const int64_t length = geo.length;
   const int64_t W = a.window ? a.window : (1ll << 40);
   for (int far = depth + 1; far > W; --far) see &= see - 1;   // ancestors past the window: the earliest nodes of the path
-  // positions that are there and that some node sees
-  const int64_t room = static_cast<int64_t>(a.columns.d) * a.block.d;
-  const int64_t oldest = max(max(length - room, length - W + 1), static_cast<int64_t>(0));
-  const int lo = static_cast<int>(min(oldest, length)), L = static_cast<int>(min(length, (1ll << 31) - 1));
-  const int base = lo & ~(attn::kTile - 1);
-  const int ctx = L > lo ? (L - base + attn::kTile - 1) / attn::kTile : 0, tiles = ctx + 1;
+  const int lo = geo.lo, L = geo.L, base = geo.base, ctx = geo.ctx, tiles = part.t1;
   // the first position that this lane's query sees, and the wave's rows' earliest
   const int from = static_cast<int>(min(max(length + depth - W + 1, static_cast<int64_t>(0)), (1ll << 31) - 1));
   int wfrom = mine ? from : 0x7fffffff;
@@ -141,7 +283,7 @@ __global__ void __launch_bounds__(kNW * 64, 2) tree_attention_kernel(TreeArgs a)
                                     : (which ? a.v + span.first * a.v_ts : a.k + span.first * a.k_ts) +
                                           static_cast<int64_t>(g) * D;
       const int64_t stride = t < ctx ? D : which ? a.v_ts : a.k_ts;
-      attn::load_rows<kNW>(which ? vtile[buf] : ktile[buf], [&](int rr, int e, const void* l) {
+      attn::load_rows<NW>(which ? vtile[buf] : ktile[buf], [&](int rr, int e, const void* l) {
         const int x = __shfl(row, rr, 64);
         const uint16_t* p = x < 0 ? reinterpret_cast<const uint16_t*>(attn::zero_row) : src + x * stride;
         if (D == attn::kD || e < D) attn::copy16(p + e, l);
@@ -149,9 +291,9 @@ __global__ void __launch_bounds__(kNW * 64, 2) tree_attention_kernel(TreeArgs a)
     }
   };
 
-  int t = 0, buf = 0, id = fetch(0);
-  issue(0, 0, id);
-  id = fetch(1);
+  int t = part.t0, buf = 0, id = fetch(t);
+  issue(t, 0, id);
+  id = fetch(t + 1);
   auto inner = [&]() { return t < ctx && have == ~0ull && base + t * attn::kTile >= allfrom; };
   auto tile = [&](auto edge) {
     const uint64_t there = have;
@@ -193,47 +335,89 @@ __global__ void __launch_bounds__(kNW * 64, 2) tree_attention_kernel(TreeArgs a)
   }
   if (!mine) return;
 
-  const float inv = 1.f / (st.den + __shfl_xor(st.den, 32, 64));
+  const float den = st.den + __shfl_xor(st.den, 32, 64), inv = 1.f / den;
   const int64_t row = span.first + node;
-  uint16_t* out = a.out + (row * a.H + head) * D + 4 * (lane >> 5);
-  const uint16_t* gate = a.gate ? a.gate + row * a.g_ts + head * a.g_hs + 4 * (lane >> 5) : nullptr;
+  const int at = w * attn::kRows + (lane & 31), half4 = 4 * (lane >> 5);
+  const int64_t slot = static_cast<int64_t>(part.slot) * a.slot_rows + at;
+  if (part.slot >= 0 && lane < 32) a.stat[slot] = make_float2(st.base, den);
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int rr = 0; rr < 4; ++rr) {
-      const int dim = 32 * d + 8 * rr;
-      float o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = st.acc[d][4 * rr + e] * inv;
-      if (gate) {
-        uint16_t x[4];
-        if (a.gate8) {
-          const uint2 y = *reinterpret_cast<const uint2*>(gate + dim);
-          x[0] = y.x & 0xffff;
-          x[1] = y.x >> 16;
-          x[2] = y.y & 0xffff;
-          x[3] = y.y >> 16;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = gate[dim + e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] *= 1.f / (1.f + __expf(-M::widen(x[e])));
-      }
-      *reinterpret_cast<uint2*>(out + dim) = make_uint2(M::round2(o[0], o[1]), M::round2(o[2], o[3]));
+      const int dim = 32 * d + 8 * rr + half4;
+      const float4 o = make_float4(st.acc[d][4 * rr], st.acc[d][4 * rr + 1], st.acc[d][4 * rr + 2], st.acc[d][4 * rr + 3]);
+      if (part.slot >= 0) *reinterpret_cast<float4*>(a.part + slot * D + dim) = o;
+      else put4<DT>(a, row, head, dim, D, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
 }
 
-template <int DT>
-void launch(const TreeArgs& a, int64_t D, unsigned grid, hipStream_t st) {
-  if (D == 128)
-    hipLaunchKernelGGL((tree_attention_kernel<DT, 128>), dim3(grid), dim3(kNW * 64), 0, st, a);
+// The parts of the cut items joined in order, D / 4 lanes a row: the largest of
+// their maxima, then the sums at its scale.
+template <int DT, int D>
+__global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int rows) {
+  constexpr int kLanes = D / 4;
+  const int g = blockIdx.x % a.G, mt = blockIdx.x / a.G % a.mtiles, r = blockIdx.x / a.G / a.mtiles;
+  const tree::Span span = tree::span_of(a.cu, r, a.total);
+  const int n = static_cast<int>(span.count < a.max_nodes ? span.count : a.max_nodes), rep = a.rep.d;
+  const int at = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes, m = mt * rows + at;
+  if (at >= rows || m >= n * rep) return;
+  const int items = (n * rep + rows - 1) / rows * a.G, all = a.first[r + 1] - a.first[r];
+  if (all == items) return;   // not cut
+  const int p = all / items;
+  const int64_t slot = (static_cast<int64_t>(a.slot[r]) + static_cast<int64_t>(mt * a.G + g) * p) * a.slot_rows + at;
+  float top = -3.0e38f;
+  for (int j = 0; j < p; ++j) top = fmaxf(top, a.stat[slot + static_cast<int64_t>(j) * a.slot_rows].x);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float den = 0.f;
+  const int dim = 4 * (threadIdx.x % kLanes);
+#pragma unroll 4
+  for (int j = 0; j < p; ++j) {
+    const int64_t s = slot + static_cast<int64_t>(j) * a.slot_rows;
+    const float2 st = a.stat[s];
+    const float4 x = *reinterpret_cast<const float4*>(a.part + s * D + dim);
+    const float f = __builtin_amdgcn_exp2f(st.x - top);
+    den = fmaf(st.y, f, den);
+    o.x = fmaf(x.x, f, o.x);
+    o.y = fmaf(x.y, f, o.y);
+    o.z = fmaf(x.z, f, o.z);
+    o.w = fmaf(x.w, f, o.w);
+  }
+  const float inv = 1.f / den;
+  const int node = a.rep.quot(m);
+  put4<DT>(a, span.first + node, g * rep + (m - node * rep), dim, D, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+}
+
+// Workgroups that fit the chip, and parts a workgroup aimed at.
+constexpr int kChip = 512, kParts = 2;
+
+int rows_of(int64_t max_nodes, int64_t rep) { return max_nodes * rep > 4 * attn::kRows ? 8 * attn::kRows : 4 * attn::kRows; }
+int target_of(int rows) { return kChip * 4 * attn::kRows / rows * kParts; }
+int64_t plan_bytes(int64_t n_seqs) { return (2 * (n_seqs + 1) * 4 + 255) / 256 * 256; }
+
+template <int DT, int D>
+void launch(const TreeArgs& a, int rows, unsigned grid, hipStream_t st) {
+  if (rows == 8 * attn::kRows)
+    hipLaunchKernelGGL((tree_attention_kernel<DT, D, 8>), dim3(grid), dim3(512), 0, st, a);
   else
-    hipLaunchKernelGGL((tree_attention_kernel<DT, 64>), dim3(grid), dim3(kNW * 64), 0, st, a);
+    hipLaunchKernelGGL((tree_attention_kernel<DT, D, 4>), dim3(grid), dim3(256), 0, st, a);
+  const int most = static_cast<int>(a.max_nodes * a.rep.d < static_cast<uint32_t>(rows) ? a.max_nodes * a.rep.d : rows);
+  if (a.R == 0) return;
+  const int per = 256 / (D / 4);
+  hipLaunchKernelGGL((tree_join_kernel<DT, D>), dim3(a.R * a.G * a.mtiles, (most + per - 1) / per), dim3(256), 0, st, a,
+                     rows);
 }
 
 }  // namespace
 }  // namespace yh
+
+extern "C" int64_t yh_tree_attention_workspace_bytes(int64_t n_seqs, int64_t H, int64_t G, int64_t D,
+                                                     int64_t max_nodes) {
+  using namespace yh;
+  if (n_seqs < 0 || H <= 0 || G <= 0 || D <= 0 || max_nodes <= 0 || max_nodes > tree::kNodes) return 0;
+  const int64_t rep = H / G, rows = rows_of(max_nodes, rep), used = max_nodes * rep < rows ? max_nodes * rep : rows;
+  const int64_t slots = target_of(static_cast<int>(rows)) * 4 / 3 + 1;
+  return plan_bytes(n_seqs) + slots * used * (D * 4 + 8);
+}
 
 extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                                  int64_t v_stride, const int32_t* parents, const int32_t* cu_seqlens,
@@ -241,7 +425,7 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
                                  const void* gate, int64_t gate_token_stride, int64_t gate_head_stride, void* out,
                                  int64_t n_seqs, int64_t total, int64_t blocks, int64_t columns, int64_t H, int64_t G,
                                  int64_t D, int64_t block, int64_t window, int64_t max_nodes, float scale, int dtype,
-                                 yh_stream_t stream) {
+                                 void* workspace, int64_t workspace_bytes, yh_stream_t stream) {
   using namespace yh;
   YH_CHECK_ARG(n_seqs >= 0 && total >= 0 && blocks >= 0 && columns > 0 && H > 0 && G > 0 && H % G == 0 && block > 0 &&
                    window >= 0,
@@ -268,8 +452,12 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
   YH_CHECK_ARG(total < (1ll << 31) && columns < (1ll << 31) && block < (1ll << 31) &&
                    H < (1ll << 20) && blocks < (1ll << 31) && block * G < (1ll << 31) && blocks * (G * block) < (1ll << 31),
                "tree_attention: sizes too large");
-  const int64_t rep = H / G, mtiles = (max_nodes * rep + kM - 1) / kM, work = n_seqs * G * mtiles;
-  YH_CHECK_ARG(work < (1ll << 23), "tree_attention: sizes too large");
+  const int64_t rep = H / G, rows = rows_of(max_nodes, rep), mtiles = (max_nodes * rep + rows - 1) / rows;
+  const int64_t items = n_seqs * G * mtiles, target = target_of(static_cast<int>(rows));
+  YH_CHECK_ARG(items < (1ll << 22), "tree_attention: sizes too large");
+  YH_CHECK_ARG(workspace && tree::aligned16(workspace) &&
+                   workspace_bytes >= yh_tree_attention_workspace_bytes(n_seqs, H, G, D, max_nodes),
+               "tree_attention: workspace too small");
   const bool gate8 = gate && (reinterpret_cast<uintptr_t>(gate) & 7) == 0 && gate_token_stride % 4 == 0 &&
                      gate_head_stride % 4 == 0;
   TreeArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
@@ -278,10 +466,20 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
              gate_head_stride, static_cast<uint16_t*>(out), total, window,
              tree::make_div(static_cast<uint32_t>(block)), tree::make_div(static_cast<uint32_t>(columns)),
              tree::make_div(static_cast<uint32_t>(rep)), (int)n_seqs, (int)H, (int)G, (int)blocks, (int)max_nodes,
-             (int)mtiles, gate8 ? 1 : 0, scale};
-  const unsigned grid = static_cast<unsigned>(work + 1);   // the last clears the rows of no request
-  if (dtype == YH_BF16) launch<YH_BF16>(a, D, grid, static_cast<hipStream_t>(stream));
-  else launch<YH_F16>(a, D, grid, static_cast<hipStream_t>(stream));
+             (int)mtiles, gate8 ? 1 : 0, scale, (int)target, (int)(max_nodes * rep < rows ? max_nodes * rep : rows),
+             static_cast<int32_t*>(workspace), static_cast<int32_t*>(workspace) + n_seqs + 1, nullptr, nullptr};
+  char* sums = static_cast<char*>(workspace) + plan_bytes(n_seqs);
+  a.part = reinterpret_cast<float*>(sums);
+  a.stat = reinterpret_cast<float2*>(sums + (target * 4 / 3 + 1) * a.slot_rows * D * 4);
+  const unsigned grid = static_cast<unsigned>(target + items + 1);   // the last clears the rows of no request
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == YH_BF16) {
+    if (D == 128) launch<YH_BF16, 128>(a, (int)rows, grid, st);
+    else launch<YH_BF16, 64>(a, (int)rows, grid, st);
+  } else {
+    if (D == 128) launch<YH_F16, 128>(a, (int)rows, grid, st);
+    else launch<YH_F16, 64>(a, (int)rows, grid, st);
+  }
   YH_CHECK_LAUNCH("tree_attention");
   return YH_OK;
 }

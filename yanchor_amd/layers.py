@@ -723,11 +723,14 @@ def tree_attention(q, k, v, parents, cu_seqlens, lengths, keys, values, block_ta
         gp = gate.data_ptr()
         gts, ghs = (h * d, d) if gate.is_contiguous() else (gate.stride(0), gate.stride(1))
     out = torch.empty(n, h, d, dtype=q.dtype, device=dev)
+    # scratch of the call: concurrent calls on different streams are independent
+    need = N.lib().yh_tree_attention_workspace_bytes(r, h, g, d, most)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
     N.call_on(dev, "yh_tree_attention", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
               N.ptr(parents), cu.data_ptr(), lens.data_ptr(), keys.data_ptr(), values.data_ptr(),
               tables.data_ptr(), gp, gts, ghs, out.data_ptr(), r, n, keys.shape[0], tables.shape[1], h, g, d,
               keys.shape[2], 0 if window is None else int(window), most, sc,
-              N.code(q), N.stream_of(q))
+              N.code(q), ws.data_ptr(), need, N.stream_of(q))
     return out
 
 
