@@ -194,8 +194,10 @@ struct State {
   // The softmax of a tile's scores c and its value product.  HILO: P enters the
   // product as a hi + lo pair.  k2 = scale * log2(e).  EDGE: keep (wave-uniform)
   // has a bit for each key of the tile; the others' values count as zeros, since
-  // a weight of 0 does not take out a value that is not finite.
-  template <bool HILO, bool EDGE>
+  // a weight of 0 does not take out a value that is not finite.  LAZY: the sums
+  // are rescaled in a branch of their own, where some row's maximum moved (the
+  // same bits: a factor of 1 changes nothing).
+  template <bool HILO, bool EDGE, bool LAZY = false>
   __device__ __forceinline__ void step(const f32x16 (&c)[2], const Rows& v, float k2, uint64_t keep = ~0ull) {
     using M = Mfma<DT>;
     using vec = typename M::vec;
@@ -207,8 +209,16 @@ struct State {
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     const float nb = fmaxf(base, mx);
     const float alpha = __builtin_amdgcn_exp2f(base - nb);
+    if constexpr (LAZY) {
+      if (__any(nb != base)) {
+        den *= alpha;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] *= alpha;
+      }
+    } else {
+      den *= alpha;
+    }
     base = nb;
-    den *= alpha;
     // V operands: lane 4 j + m of a 16-lane group reads the 8 bytes at columns
     // 4 m .. + 3 (of the group's 16) of row 16 ks + 8 u + 4 half + j
     const int j = (lane & 15) >> 2, m = lane & 3, gi = (lane >> 4) & 1;
@@ -263,7 +273,7 @@ struct State {
       __builtin_amdgcn_sched_barrier(0);
       const int d = n % kDims, ks = n / kDims;
       const uint32_t* h = ph[ks & 1];
-      if (ks == 0) acc[d] *= alpha;
+      if (!LAZY && ks == 0) acc[d] *= alpha;
       if constexpr (EDGE) {
         if (d == 0) find_kept(ks);
         const uint4 x = __builtin_bit_cast(uint4, vf[n % kAhead]);

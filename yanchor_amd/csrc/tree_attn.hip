@@ -45,6 +45,7 @@ struct TreeArgs {
   int64_t total, window;   // window 0: none
   Div block, columns, rep;
   int R, H, G, NB, max_nodes, mtiles;
+  int runs;                // blocks hold whole fours of rows
   int gate8;               // gate rows keep 8-byte alignment
   float scale;
   // the cut: parts aimed at, and for requests [0, R] the first part, the first partial sum
@@ -79,6 +80,14 @@ __device__ __forceinline__ Geometry geometry(const TreeArgs& a, int64_t r) {
   q.base = q.lo & ~(attn::kTile - 1);
   q.ctx = q.L > q.lo ? (q.L - q.base + attn::kTile - 1) / attn::kTile : 0;
   return q;
+}
+
+// attn::copy16 from a scalar address plus a lane's offset, past the caches: a
+// cache row is read once.
+__device__ __forceinline__ void copy_run(const uint16_t* src, int voff, const void* lds) {
+  const unsigned m0v = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(reinterpret_cast<uintptr_t>(lds)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(m0v), "v"(voff), "s"(src)
+               : "memory", "m0");
 }
 
 // A part: tiles [t0, t1) of an item, its partial sum's place (-1: the item is whole).
@@ -267,6 +276,8 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
     const uint32_t qd = a.block.quot(p);
     return table[qd - a.columns.quot(qd) * a.columns.d];
   };
+  // the lane's piece of the four rows of a copy (load_rows' order), and its offset from the first
+  const int piece = (lane & 15) ^ attn::swz(4 * w + (lane >> 4)), voff = ((lane >> 4) * D + piece * 8) * 2;
   uint64_t have = 0;   // rows of the tile that exist
   auto issue = [&](int t, int buf, int id) {
     int row = -1;   // in the cache, or the node
@@ -277,6 +288,18 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
       row = lane;
     }
     have = __ballot(row >= 0);
+    if (t < ctx && have == ~0ull && a.runs) {
+      // every four rows that an instruction copies lie together: one scalar address
+#pragma unroll
+      for (int it = 0; it < 16 / NW; ++it) {
+        const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(row, 4 * (it * NW + w))) * D;
+        if (D == attn::kD || piece < D / 8) {
+          copy_run(a.keys + at, voff, &ktile[buf][64 * (it * NW + w)]);
+          copy_run(a.values + at, voff, &vtile[buf][64 * (it * NW + w)]);
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       const uint16_t* src = t < ctx ? (which ? a.values : a.keys)
@@ -319,7 +342,7 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
         const uint64_t sh = live >> (4 * (lane >> 5));
         st.mask(c, [&](int key, int) { return ((key < 32 ? static_cast<uint32_t>(sh) >> key : static_cast<uint32_t>(sh >> 32) >> (key - 32)) & 1) != 0; });
       }
-      st.template step<false, edge.value>(c, vtile[buf], k2, keep);
+      st.template step<false, edge.value, true>(c, vtile[buf], k2, keep);
     }
     ++t;
     buf ^= 1;
@@ -466,7 +489,7 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
              gate_head_stride, static_cast<uint16_t*>(out), total, window,
              tree::make_div(static_cast<uint32_t>(block)), tree::make_div(static_cast<uint32_t>(columns)),
              tree::make_div(static_cast<uint32_t>(rep)), (int)n_seqs, (int)H, (int)G, (int)blocks, (int)max_nodes,
-             (int)mtiles, gate8 ? 1 : 0, scale, (int)target, (int)(max_nodes * rep < rows ? max_nodes * rep : rows),
+             (int)mtiles, block % 4 == 0 ? 1 : 0, gate8 ? 1 : 0, scale, (int)target, (int)(max_nodes * rep < rows ? max_nodes * rep : rows),
              static_cast<int32_t*>(workspace), static_cast<int32_t*>(workspace) + n_seqs + 1, nullptr, nullptr};
   char* sums = static_cast<char*>(workspace) + plan_bytes(n_seqs);
   a.part = reinterpret_cast<float*>(sums);
