@@ -8,7 +8,7 @@
 // tables[r][p / block % columns], so the last columns * block positions are
 // there; a ring is a table of one column whose block is the ring.
 //
-// A workgroup of NW waves (4, or 8 for more than 128 rows) takes a request, a KV
+// A workgroup of NW waves (2, 4 or 8, as the rows need) takes a request, a KV
 // head and 32 NW of the rows (node, query head of the group): the waves, 32 rows
 // each, share 64-key tiles (attn_tile.h) that begin at multiples of 64
 // positions; the nodes themselves are the last tile, its mask the ancestor sets.
@@ -202,13 +202,39 @@ __device__ __forceinline__ void put4(const TreeArgs& a, int64_t row, int head, i
   *reinterpret_cast<uint2*>(a.out + (row * a.H + head) * D + dim) = make_uint2(M::round2(o.x, o.y), M::round2(o.z, o.w));
 }
 
+// The pipeline: keys and values of tile after tile pass through S slots of LDS,
+// one barrier a slot: at step q (the keys, then the values of a tile) slot q has
+// arrived, q - 1 is consumed, and its place is filled again, so that S - 2 to
+// S - 1 slots are in flight.  S fills the LDS that the workgroups of a CU leave:
+// 2 waves 3 slots (three workgroups), 4 waves 4 (two), 8 waves 8 (one).  The
+// block ids of a tile come the same way, kAhead tiles before its keys: a load
+// into registers would have its wait drain the copies.
+template <int NW>
+struct Pipe {
+  static constexpr int S = NW == 8 ? 8 : NW == 4 ? 4 : 3;
+  static constexpr int kAhead = S / 2, kIds = S == 3 ? 2 : S;
+  static constexpr int kCopies = 16 / NW;                               // a wave's copies of a slot
+  static constexpr int kWaitK = (S - 2) * kCopies + (S - 2) / 2;        // younger than tile t's keys
+  static constexpr int kWaitV = (S - 2) * kCopies + (S - 1) / 2;        // and its values (ids go with keys)
+};
+template <int N>
+__device__ __forceinline__ void copies_left() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void copy4(const int32_t* src, const void* lds) {   // 4 bytes a lane
+  const unsigned m0v = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(reinterpret_cast<uintptr_t>(lds)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(m0v), "v"(src) : "memory", "m0");
+}
+
 template <int DT, int D, int NW>
 __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) {
   constexpr int kM = NW * attn::kRows;   // rows of the workgroup
-  __shared__ attn::Rows stage[4];   // two buffers of key rows, two of value rows
+  using P = Pipe<NW>;
+  constexpr int S = P::S;
+  __shared__ attn::Rows stage[S];
+  __shared__ int32_t ids[P::kIds][NW][64];
   __shared__ uint64_t s_set[tree::kNodes];
   __shared__ int s_deep;
-  attn::Rows *ktile = stage, *vtile = stage + 2;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   if (blockIdx.x == gridDim.x - 1) {   // rows of no request
@@ -268,88 +294,110 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
   const float k2 = a.scale * 1.4426950408889634f;
 
   const int32_t* table = a.tables + static_cast<int64_t>(r) * a.columns.d;
-  // Lane l stands for the tile's row l: its block id is loaded a tile ahead of
-  // the copies, which take the row from the lane.
+  // Lane l stands for the tile's row l: it brings its block id, and the copies take the row from it.
   auto fetch = [&](int t) {
     const int p = base + t * attn::kTile + lane;
-    if (t >= ctx || p < lo || p >= L) return -1;
-    const uint32_t qd = a.block.quot(p);
-    return table[qd - a.columns.quot(qd) * a.columns.d];
+    const uint32_t qd = a.block.quot(t < ctx && p >= lo && p < L ? p : lo);
+    copy4(table + (qd - a.columns.quot(qd) * a.columns.d), ids[t % P::kIds][w]);
   };
-  // the lane's piece of the four rows of a copy (load_rows' order), and its offset from the first
-  const int piece = (lane & 15) ^ attn::swz(4 * w + (lane >> 4)), voff = ((lane >> 4) * D + piece * 8) * 2;
-  uint64_t have = 0;   // rows of the tile that exist
-  auto issue = [&](int t, int buf, int id) {
-    int row = -1;   // in the cache, or the node
+  // the lane's piece of the four rows of copy `it` (load_rows' order), and its offset from the first
+  auto piece_of = [&](int it) { return (lane & 15) ^ (((lane >> 4) << 2) | ((it * NW + w) & 3)); };
+  auto voff_of = [&](int it) { return ((lane >> 4) * D + piece_of(it) * 8) * 2; };
+  int row = -1;          // the lane's row of the tile being copied: in the cache, or the node
+  uint64_t have[P::kAhead + 1];   // rows that exist, of this tile and the next ones
+  auto issue_keys = [&](int t) {   // -> the rows that exist
+    row = -1;
     if (t < ctx) {
-      const int p = base + t * attn::kTile + lane;
-      if (id >= 0 && id < a.NB) row = (id * a.G + g) * a.block.d + (p - a.block.quot(p) * a.block.d);
+      const int p = base + t * attn::kTile + lane, id = ids[t % P::kIds][w][lane];
+      if (p >= lo && p < L && id >= 0 && id < a.NB) row = (id * a.G + g) * a.block.d + (p - a.block.quot(p) * a.block.d);
     } else if (lane < n) {
       row = lane;
     }
-    have = __ballot(row >= 0);
-    if (t < ctx && have == ~0ull && a.runs) {
+    fetch(t + P::kAhead);
+    return static_cast<uint64_t>(__ballot(row >= 0));
+  };
+  auto copy_slot = [&](int t, int slot, bool values) {
+    attn::Rows& to = stage[slot];
+    if (t < ctx && a.runs && __ballot(row >= 0) == ~0ull) {
       // every four rows that an instruction copies lie together: one scalar address
+      const uint16_t* src = values ? a.values : a.keys;
 #pragma unroll
       for (int it = 0; it < 16 / NW; ++it) {
         const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(row, 4 * (it * NW + w))) * D;
-        if (D == attn::kD || piece < D / 8) {
-          copy_run(a.keys + at, voff, &ktile[buf][64 * (it * NW + w)]);
-          copy_run(a.values + at, voff, &vtile[buf][64 * (it * NW + w)]);
-        }
+        if (D == attn::kD || piece_of(it) < D / 8) copy_run(src + at, voff_of(it), &to[64 * (it * NW + w)]);
       }
       return;
     }
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const uint16_t* src = t < ctx ? (which ? a.values : a.keys)
-                                    : (which ? a.v + span.first * a.v_ts : a.k + span.first * a.k_ts) +
-                                          static_cast<int64_t>(g) * D;
-      const int64_t stride = t < ctx ? D : which ? a.v_ts : a.k_ts;
-      attn::load_rows<NW>(which ? vtile[buf] : ktile[buf], [&](int rr, int e, const void* l) {
-        const int x = __shfl(row, rr, 64);
-        const uint16_t* p = x < 0 ? reinterpret_cast<const uint16_t*>(attn::zero_row) : src + x * stride;
-        if (D == attn::kD || e < D) attn::copy16(p + e, l);
-      });
-    }
+    const uint16_t* src = t < ctx ? (values ? a.values : a.keys)
+                                  : (values ? a.v + span.first * a.v_ts : a.k + span.first * a.k_ts) +
+                                        static_cast<int64_t>(g) * D;
+    const int64_t stride = t < ctx ? D : values ? a.v_ts : a.k_ts;
+    attn::load_rows<NW>(to, [&](int rr, int e, const void* l) {
+      const int x = __shfl(row, rr, 64);
+      const uint16_t* p = x < 0 ? reinterpret_cast<const uint16_t*>(attn::zero_row) : src + x * stride;
+      if (D == attn::kD || e < D) attn::copy16(p + e, l);
+    });
   };
 
-  int t = part.t0, buf = 0, id = fetch(t);
-  issue(t, 0, id);
-  id = fetch(t + 1);
-  auto inner = [&]() { return t < ctx && have == ~0ull && base + t * attn::kTile >= allfrom; };
+  // slot q: the keys (even q) or the values of tile part.t0 + q / 2
+  const int t0 = part.t0, slots = 2 * (tiles - t0);
+  auto issue = [&](int q, int ahead) {   // ahead: its tile from the current one
+    if (q >= slots) return;
+    const int t = t0 + (q >> 1);
+    if ((q & 1) == 0) {
+      const uint64_t rows = issue_keys(t);
+#pragma unroll
+      for (int i = 0; i <= P::kAhead; ++i)
+        if (i == ahead) have[i] = rows;
+    }
+    copy_slot(t, q % S, (q & 1) != 0);
+  };
+#pragma unroll
+  for (int i = 0; i < P::kAhead; ++i) fetch(t0 + i);
+  // as a builtin, so that the compiler counts the queries as loaded too and waits for none in the loop
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int q = 0; q < S - 1; ++q) issue(q, q >> 1);
+  int t = t0, q = 0;
+  auto inner = [&]() { return t < ctx && have[0] == ~0ull && base + t * attn::kTile >= allfrom; };
   auto tile = [&](auto edge) {
-    const uint64_t there = have;
-    attn::copy_wait();      // this wave's part of the tile has arrived
-    attn::tile_barrier();   // everyone's has, and the other buffers are consumed
-    if (t + 1 < tiles) issue(t + 1, buf ^ 1, id);
-    id = fetch(t + 2);
+    const uint64_t there = have[0];
+    attn::f32x16 c[2];
+    if (q + S - 2 < slots) copies_left<P::kWaitK>();   // this wave's part of the keys has arrived
+    else copies_left<0>();
+    attn::tile_barrier();   // everyone's has, and the slot before is consumed
+    issue(q + S - 1, (S - 1) / 2);
     if (active) {
-      attn::f32x16 c[2];
-      st.scores(ktile[buf], c);
-      uint64_t keep = ~0ull;
+      st.scores(stage[q % S], c);
       if constexpr (edge.value) {
-        uint64_t live;   // the tile's keys that the lane's query sees
-        if (t < ctx) {
-          const int p0 = base + t * attn::kTile;
-          const int skip = min(max(from - p0, 0), 64), wskip = min(max(wfrom - p0, 0), 64);
-          live = skip > 63 ? 0 : there & (~0ull << skip);
-          keep = wskip > 63 ? 0 : there & (~0ull << wskip);
-        } else {
-          live = see;
-          keep = wsee;
-        }
+        const int p0 = base + t * attn::kTile, skip = min(max(from - p0, 0), 64);
+        const uint64_t live = t < ctx ? (skip > 63 ? 0 : there & (~0ull << skip)) : see;   // keys that the lane's query sees
         const uint64_t sh = live >> (4 * (lane >> 5));
         st.mask(c, [&](int key, int) { return ((key < 32 ? static_cast<uint32_t>(sh) >> key : static_cast<uint32_t>(sh >> 32) >> (key - 32)) & 1) != 0; });
       }
-      st.template step<false, edge.value, true>(c, vtile[buf], k2, keep);
     }
+    ++q;
+    if (q + S - 2 < slots) copies_left<P::kWaitV>();
+    else copies_left<0>();
+    attn::tile_barrier();
+    issue(q + S - 1, S / 2);
+    if (active) {
+      uint64_t keep = ~0ull;
+      if constexpr (edge.value) {
+        const int p0 = base + t * attn::kTile, wskip = min(max(wfrom - p0, 0), 64);
+        keep = t < ctx ? (wskip > 63 ? 0 : there & (~0ull << wskip)) : wsee;
+      }
+      st.template step<false, edge.value, true>(c, stage[q % S], k2, keep);
+    }
+    ++q;
     ++t;
-    buf ^= 1;
+#pragma unroll
+    for (int i = 0; i < P::kAhead; ++i) have[i] = have[i + 1];
   };
   // Tiles whose keys all rows see and the others take a loop each: as branches
   // of one loop they spill (the waves' conditions may differ: both loops pass
-  // one barrier a tile).
+  // two barriers a tile).
   while (t < tiles) {
 #pragma unroll 1
     while (t < tiles && inner()) tile(std::false_type{});
@@ -359,7 +407,7 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
   if (!mine) return;
 
   const float den = st.den + __shfl_xor(st.den, 32, 64), inv = 1.f / den;
-  const int64_t row = span.first + node;
+  const int64_t token = span.first + node;
   const int at = w * attn::kRows + (lane & 31), half4 = 4 * (lane >> 5);
   const int64_t slot = static_cast<int64_t>(part.slot) * a.slot_rows + at;
   if (part.slot >= 0 && lane < 32) a.stat[slot] = make_float2(st.base, den);
@@ -370,7 +418,7 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
       const int dim = 32 * d + 8 * rr + half4;
       const float4 o = make_float4(st.acc[d][4 * rr], st.acc[d][4 * rr + 1], st.acc[d][4 * rr + 2], st.acc[d][4 * rr + 3]);
       if (part.slot >= 0) *reinterpret_cast<float4*>(a.part + slot * D + dim) = o;
-      else put4<DT>(a, row, head, dim, D, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+      else put4<DT>(a, token, head, dim, D, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
 }
 
@@ -410,19 +458,18 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int rows) {
   put4<DT>(a, span.first + node, g * rep + (m - node * rep), dim, D, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
-// Workgroups that fit the chip, and parts a workgroup aimed at.
-constexpr int kChip = 512, kParts = 2;
-
-int rows_of(int64_t max_nodes, int64_t rep) { return max_nodes * rep > 4 * attn::kRows ? 8 * attn::kRows : 4 * attn::kRows; }
-int target_of(int rows) { return kChip * 4 * attn::kRows / rows * kParts; }
+// Rows of a workgroup: 64 (two waves), 128 or 256.
+int rows_of(int64_t max_nodes, int64_t rep) { return max_nodes * rep > 128 ? 256 : max_nodes * rep > 64 ? 128 : 64; }
+// Parts aimed at: kParts for every workgroup that fits the chip (3, 2 or 1 a CU).
+constexpr int kParts = 2;
+int target_of(int rows) { return (rows == 64 ? 768 : rows == 128 ? 512 : 256) * kParts; }
 int64_t plan_bytes(int64_t n_seqs) { return (2 * (n_seqs + 1) * 4 + 255) / 256 * 256; }
 
 template <int DT, int D>
 void launch(const TreeArgs& a, int rows, unsigned grid, hipStream_t st) {
-  if (rows == 8 * attn::kRows)
-    hipLaunchKernelGGL((tree_attention_kernel<DT, D, 8>), dim3(grid), dim3(512), 0, st, a);
-  else
-    hipLaunchKernelGGL((tree_attention_kernel<DT, D, 4>), dim3(grid), dim3(256), 0, st, a);
+  if (rows == 256) hipLaunchKernelGGL((tree_attention_kernel<DT, D, 8>), dim3(grid), dim3(512), 0, st, a);
+  else if (rows == 128) hipLaunchKernelGGL((tree_attention_kernel<DT, D, 4>), dim3(grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((tree_attention_kernel<DT, D, 2>), dim3(grid), dim3(128), 0, st, a);
   const int most = static_cast<int>(a.max_nodes * a.rep.d < static_cast<uint32_t>(rows) ? a.max_nodes * a.rep.d : rows);
   if (a.R == 0) return;
   const int per = 256 / (D / 4);
