@@ -21,15 +21,13 @@ __device__ __forceinline__ Span span_of(const int32_t* cu, int64_t r, int64_t to
   return {s, e - s};
 }
 
-// Lane i's node i of n (one wave, all lanes active): the set of its ancestors,
-// itself included, by doubling -- after step k, `set` holds the nodes less than
-// 2^k steps up and `up` the node 2^k steps up (-1: the context).  A parent that
-// is not an earlier node counts as the context.  parents null: a chain.
-// sum(up node's value) of `x` along the path is formed with it.
-__device__ __forceinline__ uint64_t ancestors(const int32_t* parents, int n, float* x = nullptr) {
+// Lane i's node i (one wave, all lanes active), `up` its parent: the set of its
+// ancestors, itself included, by doubling -- after step k, `set` holds the nodes
+// less than 2^k steps up and `up` the node 2^k steps up (-1: the context).  A
+// parent that is not an earlier node counts as the context.  The sum of `x` along
+// the path is formed with it.
+__device__ __forceinline__ uint64_t ancestors_of(int up, float* x = nullptr) {
   const int lane = threadIdx.x & (kWave - 1);
-  int up = -1;
-  if (lane < n) up = parents ? parents[lane] : lane - 1;
   if (up >= lane || up < 0) up = -1;
   uint64_t set = 1ull << lane;
   float v = x ? *x : 0.f;
@@ -47,6 +45,11 @@ __device__ __forceinline__ uint64_t ancestors(const int32_t* parents, int n, flo
   }
   if (x) *x = v;
   return set;
+}
+// The same for the n nodes whose parents are at `parents` (null: a chain).
+__device__ __forceinline__ uint64_t ancestors(const int32_t* parents, int n, float* x = nullptr) {
+  const int lane = threadIdx.x & (kWave - 1);
+  return ancestors_of(lane >= n ? -1 : parents ? parents[lane] : lane - 1, x);
 }
 
 // n / d for 0 <= n < 2^31 by a multiplication: m = ceil(2^(31 + l) / d) with

@@ -65,11 +65,11 @@ struct Geometry {
   int64_t length;
   int n, lo, L, base, ctx;
 };
-__device__ __forceinline__ Geometry geometry(const TreeArgs& a, int64_t r) {
+__device__ __forceinline__ Geometry geometry(const TreeArgs& a, const tree::Span& span, int64_t length) {
   Geometry q;
-  q.span = tree::span_of(a.cu, r, a.total);
-  q.n = static_cast<int>(q.span.count < a.max_nodes ? q.span.count : a.max_nodes);
-  q.length = a.lengths[r] < 0 ? 0 : a.lengths[r];
+  q.span = span;
+  q.n = static_cast<int>(span.count < a.max_nodes ? span.count : a.max_nodes);
+  q.length = length < 0 ? 0 : length;
   const int64_t room = static_cast<int64_t>(a.columns.d) * a.block.d;
   int64_t oldest = q.length - room;
   if (a.window && q.length - a.window + 1 > oldest) oldest = q.length - a.window + 1;
@@ -92,6 +92,7 @@ __device__ __forceinline__ void copy_run(const uint16_t* src, int voff, const vo
 
 // A part: tiles [t0, t1) of an item, its partial sum's place (-1: the item is whole).
 struct Part {
+  int64_t first, count, length;
   int r, mt, g, t0, t1, slot;
 };
 
@@ -124,32 +125,31 @@ __device__ __forceinline__ int64_t block_sum(int64_t x, int64_t* before) {   // 
 template <int NW>
 __device__ __forceinline__ bool find_part(const TreeArgs& a, int64_t id, Part* out) {
   constexpr int TH = NW * 64, kM = NW * attn::kRows;
-  __shared__ int found[6];
+  __shared__ Part found;
   const int tid = threadIdx.x;
+  Geometry geo{};
   auto shape = [&](int64_t r, int64_t* items, int* tiles) {
     *items = 0;
     *tiles = 1;
     if (r >= a.R) return;
-    const Geometry q = geometry(a, r);
-    *items = static_cast<int64_t>((q.n * static_cast<int>(a.rep.d) + kM - 1) / kM) * a.G;
-    *tiles = q.ctx + 1;
+    geo = geometry(a, tree::span_of(a.cu, r, a.total), a.lengths[r]);
+    *items = static_cast<int64_t>((geo.n * static_cast<int>(a.rep.d) + kM - 1) / kM) * a.G;
+    *tiles = geo.ctx + 1;
   };
-  int64_t units = 0, before;
+  int64_t units = 0, before, items = 0;
+  int tiles = 1;
   for (int64_t r = tid; r - tid < a.R; r += TH) {
-    int64_t items;
-    int tiles;
     shape(r, &items, &tiles);
     units += block_sum<TH>(items * tiles, &before);
   }
   int64_t chunk = (units + a.target - 1) / a.target;
   chunk = chunk < kMinChunk ? kMinChunk : chunk;
   int64_t parts = 0, cut = 0;
-  if (tid == 0) found[0] = -1;
+  if (tid == 0) found.r = -1;
   for (int64_t r = tid; r - tid < a.R; r += TH) {
-    int64_t items, first, slot;
-    int tiles;
-    shape(r, &items, &tiles);
+    if (a.R > TH) shape(r, &items, &tiles);   // otherwise the first loop's
     const int64_t p = tiles * 2ll < 3 * chunk ? 1 : (2ll * tiles + chunk) / (2 * chunk), mine = items * p;
+    int64_t first, slot;
     const int64_t all = block_sum<TH>(mine, &first), all_cut = block_sum<TH>(p > 1 ? mine : 0, &slot);
     first += parts;
     slot += cut;
@@ -161,20 +161,17 @@ __device__ __forceinline__ bool find_part(const TreeArgs& a, int64_t id, Part* o
       }
       if (id >= first && id < first + mine) {
         const int64_t in = id - first, item = in / p, j = in - item * p;
-        found[0] = static_cast<int>(r);
-        found[1] = static_cast<int>(item / a.G);
-        found[2] = static_cast<int>(item % a.G);
-        found[3] = static_cast<int>(j * tiles / p);
-        found[4] = static_cast<int>((j + 1) * tiles / p);
-        found[5] = p > 1 ? static_cast<int>(slot + in) : -1;
+        found = Part{geo.span.first, geo.span.count, geo.length, static_cast<int>(r), static_cast<int>(item / a.G),
+                     static_cast<int>(item % a.G), static_cast<int>(j * tiles / p), static_cast<int>((j + 1) * tiles / p),
+                     p > 1 ? static_cast<int>(slot + in) : -1};
       }
     }
     parts += all;
     cut += all_cut;
   }
   __syncthreads();
-  *out = Part{found[0], found[1], found[2], found[3], found[4], found[5]};
-  return found[0] >= 0;
+  *out = found;
+  return found.r >= 0;
 }
 
 // read * sigmoid(gate) and the rounding to 16 bits of 4 outputs of dims dim .. dim + 3
@@ -206,13 +203,14 @@ __device__ __forceinline__ void put4(const TreeArgs& a, int64_t row, int head, i
 // one barrier a slot: at step q (the keys, then the values of a tile) slot q has
 // arrived, q - 1 is consumed, and its place is filled again, so that S - 2 to
 // S - 1 slots are in flight.  S fills the LDS that the workgroups of a CU leave:
-// 2 waves 3 slots (three workgroups), 4 waves 4 (two), 8 waves 8 (one).  The
+// 2 waves 2 slots (four workgroups), 4 waves 4 (two), 8 waves 8 (one).  (2 waves
+// with 3 slots, three workgroups a CU: 134 us for 122 in the 128 rings.)  The
 // block ids of a tile come the same way, kAhead tiles before its keys: a load
 // into registers would have its wait drain the copies.
 template <int NW>
 struct Pipe {
-  static constexpr int S = NW == 8 ? 8 : NW == 4 ? 4 : 3;
-  static constexpr int kAhead = S / 2, kIds = S == 3 ? 2 : S;
+  static constexpr int S = NW == 8 ? 8 : NW == 4 ? 4 : 2;
+  static constexpr int kAhead = S / 2, kIds = S;
   static constexpr int kCopies = 16 / NW;                               // a wave's copies of a slot
   static constexpr int kWaitK = (S - 2) * kCopies + (S - 2) / 2;        // younger than tile t's keys
   static constexpr int kWaitV = (S - 2) * kCopies + (S - 1) / 2;        // and its values (ids go with keys)
@@ -244,10 +242,12 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
   }
   Part part;
   if (!find_part<NW>(a, blockIdx.x, &part)) return;
-  const int g = part.g, mt = part.mt, r = part.r;
-  const Geometry geo = geometry(a, r);
+  const int g = __builtin_amdgcn_readfirstlane(part.g), mt = __builtin_amdgcn_readfirstlane(part.mt),
+            r = __builtin_amdgcn_readfirstlane(part.r);
+  const Geometry geo = geometry(a, tree::Span{part.first, part.count}, part.length);
   const tree::Span span = geo.span;
   const int n = geo.n, rep = a.rep.d;
+  const int lo = geo.lo, L = geo.L, base = geo.base, ctx = geo.ctx, tiles = part.t1;
   if (mt == 0 && part.t0 == 0) {   // nodes past the most that the call takes: not a number
     const int64_t first = span.first + n, row = static_cast<int64_t>(a.H) * D;
     for (int64_t i = threadIdx.x; i < (span.count - n) * rep * D; i += NW * 64) {
@@ -256,43 +256,13 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
     }
   }
 
-  if (w == 0) {
-    const uint64_t set = tree::ancestors(a.parents ? a.parents + span.first : nullptr, n);
-    s_set[lane] = set;
-    int d = lane < n ? __popcll(set) - 1 : 0;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) d = max(d, __shfl_xor(d, off, 64));
-    if (lane == 0) s_deep = d;
-  }
-  __syncthreads();
-  const int deep = s_deep;
-
   // this lane's query: row m of the request's (node, head of the group) rows
   const int m = mt * kM + w * attn::kRows + (lane & 31);
   const bool active = mt * kM + w * attn::kRows < n * rep;   // of the wave
   const bool mine = m < n * rep;
   const int node = mine ? a.rep.quot(m) : 0, head = g * rep + (mine ? m - node * rep : 0);
-  uint64_t see = mine ? s_set[node] : 0;
-  const int depth = mine ? __popcll(see) - 1 : 0;
-  const int64_t length = geo.length;
   const int64_t W = a.window ? a.window : (1ll << 40);
-  for (int far = depth + 1; far > W; --far) see &= see - 1;   // ancestors past the window: the earliest nodes of the path
-  const int lo = geo.lo, L = geo.L, base = geo.base, ctx = geo.ctx, tiles = part.t1;
-  // the first position that this lane's query sees, and the wave's rows' earliest
-  const int from = static_cast<int>(min(max(length + depth - W + 1, static_cast<int64_t>(0)), (1ll << 31) - 1));
-  int wfrom = mine ? from : 0x7fffffff;
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) wfrom = min(wfrom, __shfl_xor(wfrom, off, 64));
-  uint64_t wsee = see;
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) wsee |= __shfl_xor(wsee, off, 64);
-  const int64_t allfrom = length + deep - W + 1;   // from here on every node sees
-
-  attn::State<DT, false, D> st;
-  st.init(false);
-  st.load_q(a.q + (span.first + node) * a.q_ts + static_cast<int64_t>(head) * D, mine);
   const float k2 = a.scale * 1.4426950408889634f;
-
   const int32_t* table = a.tables + static_cast<int64_t>(r) * a.columns.d;
   // Lane l stands for the tile's row l: it brings its block id, and the copies take the row from it.
   auto fetch = [&](int t) {
@@ -352,13 +322,43 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
     }
     copy_slot(t, q % S, (q & 1) != 0);
   };
+  // The block ids, the queries and the parents together, then the first slots;
+  // the masks are formed while they arrive.
 #pragma unroll
   for (int i = 0; i < P::kAhead; ++i) fetch(t0 + i);
+  attn::State<DT, false, D> st;
+  st.init(false);
+  st.load_q(a.q + (span.first + node) * a.q_ts + static_cast<int64_t>(head) * D, mine);
+  int up = -1;
+  if (w == 0 && lane < n) up = a.parents ? a.parents[span.first + lane] : lane - 1;
   // as a builtin, so that the compiler counts the queries as loaded too and waits for none in the loop
   __builtin_amdgcn_s_waitcnt(0x0F70);
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int q = 0; q < S - 1; ++q) issue(q, q >> 1);
+  if (w == 0) {
+    const uint64_t set = tree::ancestors_of(up);
+    s_set[lane] = set;
+    int d = lane < n ? __popcll(set) - 1 : 0;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) d = max(d, __shfl_xor(d, off, 64));
+    if (lane == 0) s_deep = d;
+  }
+  attn::tile_barrier();
+  const int deep = s_deep;
+  uint64_t see = mine ? s_set[node] : 0;
+  const int depth = mine ? __popcll(see) - 1 : 0;
+  for (int far = depth + 1; far > W; --far) see &= see - 1;   // ancestors past the window: the earliest nodes of the path
+  // the first position that this lane's query sees, and the wave's rows' earliest
+  const int from = static_cast<int>(min(max(geo.length + depth - W + 1, static_cast<int64_t>(0)), (1ll << 31) - 1));
+  int wfrom = mine ? from : 0x7fffffff;
+  uint64_t wsee = see;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    wfrom = min(wfrom, __shfl_xor(wfrom, off, 64));
+    wsee |= __shfl_xor(wsee, off, 64);
+  }
+  const int64_t allfrom = geo.length + deep - W + 1;   // from here on every node sees
   int t = t0, q = 0;
   auto inner = [&]() { return t < ctx && have[0] == ~0ull && base + t * attn::kTile >= allfrom; };
   auto tile = [&](auto edge) {
@@ -460,9 +460,9 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int rows) {
 
 // Rows of a workgroup: 64 (two waves), 128 or 256.
 int rows_of(int64_t max_nodes, int64_t rep) { return max_nodes * rep > 128 ? 256 : max_nodes * rep > 64 ? 128 : 64; }
-// Parts aimed at: kParts for every workgroup that fits the chip (3, 2 or 1 a CU).
-constexpr int kParts = 2;
-int target_of(int rows) { return (rows == 64 ? 768 : rows == 128 ? 512 : 256) * kParts; }
+// Parts aimed at: kParts for every workgroup that fits the chip (4, 2 or 1 a CU).
+constexpr int kParts = 1;
+int target_of(int rows) { return (rows == 64 ? 1024 : rows == 128 ? 512 : 256) * kParts; }
 int64_t plan_bytes(int64_t n_seqs) { return (2 * (n_seqs + 1) * 4 + 255) / 256 * 256; }
 
 template <int DT, int D>
