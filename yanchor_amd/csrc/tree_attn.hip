@@ -45,7 +45,6 @@ struct TreeArgs {
   int64_t total, window;   // window 0: none
   Div block, columns, rep;
   int R, H, G, NB, max_nodes, mtiles;
-  int runs;                // blocks hold whole fours of rows
   int gate8;               // gate rows keep 8-byte alignment
   float scale;
   // the cut: parts aimed at, and for requests [0, R] the first part, the first partial sum
@@ -81,6 +80,9 @@ __device__ __forceinline__ Geometry geometry(const TreeArgs& a, const tree::Span
   q.ctx = q.L > q.lo ? (q.L - q.base + attn::kTile - 1) / attn::kTile : 0;
   return q;
 }
+
+// Four rows of zeros for those that do not exist.
+__device__ const uint4 zero_rows[4 * attn::kD / 8] = {};
 
 // attn::copy16 from a scalar address plus a lane's offset, past the caches: a
 // cache row is read once.
@@ -204,16 +206,19 @@ __device__ __forceinline__ void put4(const TreeArgs& a, int64_t row, int head, i
 // arrived, q - 1 is consumed, and its place is filled again, so that S - 2 to
 // S - 1 slots are in flight.  S fills the LDS that the workgroups of a CU leave:
 // 2 waves 2 slots (four workgroups), 4 waves 4 (two), 8 waves 8 (one).  (2 waves
-// with 3 slots, three workgroups a CU: 134 us for 122 in the 128 rings.)  The
-// block ids of a tile come the same way, kAhead tiles before its keys: a load
-// into registers would have its wait drain the copies.
+// with 3 slots, three workgroups a CU: 134 us for 122 in the 128 rings.)
+//
+// With blocks of whole fours of rows (RUNS) the addresses are scalars: lane l
+// holds where the rows 4 l .. 4 l + 3 of a window of four tiles lie, from block
+// ids that come through LDS as the copies do, a window ahead (a load into
+// registers would have its wait drain the copies).  Resolved for every row of
+// every tile, they cost a step 1000 cycles, more than its products.
 template <int NW>
 struct Pipe {
   static constexpr int S = NW == 8 ? 8 : NW == 4 ? 4 : 2;
-  static constexpr int kAhead = S / 2, kIds = S;
-  static constexpr int kCopies = 16 / NW;                               // a wave's copies of a slot
-  static constexpr int kWaitK = (S - 2) * kCopies + (S - 2) / 2;        // younger than tile t's keys
-  static constexpr int kWaitV = (S - 2) * kCopies + (S - 1) / 2;        // and its values (ids go with keys)
+  static constexpr int kCopies = 16 / NW;                // a wave's copies of a slot
+  static constexpr int kWait = (S - 2) * kCopies;        // younger than slot q's at step q, at least
+  static constexpr bool kEarly = S <= 4;                 // refill before the products: few slots
 };
 template <int N>
 __device__ __forceinline__ void copies_left() {
@@ -224,13 +229,13 @@ __device__ __forceinline__ void copy4(const int32_t* src, const void* lds) {   /
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(m0v), "v"(src) : "memory", "m0");
 }
 
-template <int DT, int D, int NW>
+template <int DT, int D, int NW, bool RUNS>
 __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) {
   constexpr int kM = NW * attn::kRows;   // rows of the workgroup
   using P = Pipe<NW>;
   constexpr int S = P::S;
   __shared__ attn::Rows stage[S];
-  __shared__ int32_t ids[P::kIds][NW][64];
+  __shared__ int32_t ids[2][NW][64];
   __shared__ uint64_t s_set[tree::kNodes];
   __shared__ int s_deep;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -264,68 +269,94 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
   const int64_t W = a.window ? a.window : (1ll << 40);
   const float k2 = a.scale * 1.4426950408889634f;
   const int32_t* table = a.tables + static_cast<int64_t>(r) * a.columns.d;
-  // Lane l stands for the tile's row l: it brings its block id, and the copies take the row from it.
-  auto fetch = [&](int t) {
-    const int p = base + t * attn::kTile + lane;
-    const uint32_t qd = a.block.quot(t < ctx && p >= lo && p < L ? p : lo);
-    copy4(table + (qd - a.columns.quot(qd) * a.columns.d), ids[t % P::kIds][w]);
+  // where position p is in the cache, -1: nowhere (the id may be a row's of a window that is not all there)
+  auto entry = [&](int p) {
+    const uint32_t qd = a.block.quot(p >= lo && p < L ? p : lo);
+    return table + (qd - a.columns.quot(qd) * a.columns.d);
   };
-  // the lane's piece of the four rows of copy `it` (load_rows' order), and its offset from the first
-  auto piece_of = [&](int it) { return (lane & 15) ^ (((lane >> 4) << 2) | ((it * NW + w) & 3)); };
-  auto voff_of = [&](int it) { return ((lane >> 4) * D + piece_of(it) * 8) * 2; };
-  int row = -1;          // the lane's row of the tile being copied: in the cache, or the node
-  uint64_t have[P::kAhead + 1];   // rows that exist, of this tile and the next ones
-  auto issue_keys = [&](int t) {   // -> the rows that exist
-    row = -1;
-    if (t < ctx) {
-      const int p = base + t * attn::kTile + lane, id = ids[t % P::kIds][w][lane];
-      if (p >= lo && p < L && id >= 0 && id < a.NB) row = (id * a.G + g) * a.block.d + (p - a.block.quot(p) * a.block.d);
-    } else if (lane < n) {
-      row = lane;
+  auto row_at = [&](int p, int id) {
+    const int in = p - static_cast<int>(a.block.quot(p) * a.block.d);
+    return id >= 0 && id < a.NB ? (id * a.G + g) * static_cast<int>(a.block.d) + in : -1;
+  };
+  // RUNS: window j holds tiles 4 j .. 4 j + 3 from `base`; a four is there if its
+  // block is (rows of it outside [lo, L) are copied too, and masked)
+  auto four = [&](int j) { return base + 256 * j + 4 * lane; };
+  auto fetch = [&](int j) {
+    if constexpr (RUNS) {   // any of the four's positions in [lo, L) names the block
+      const int p = four(j);
+      copy4(entry(p < lo ? p + 3 : p), ids[j & 1][w]);
     }
-    fetch(t + P::kAhead);
-    return static_cast<uint64_t>(__ballot(row >= 0));
+  };
+  int fours = -1;                       // the lane's four of the window being copied
+  uint64_t there_now = 0, there_next = 0;   // the fours that are there, of the window at hand and of the next
+  auto open_window = [&](int j) {       // its ids have arrived
+    const int p = four(j);
+    fours = p + 3 >= lo && p < L ? row_at(p, ids[j & 1][w][lane]) : -1;
+    there_next = __ballot(fours >= 0);
   };
   auto copy_slot = [&](int t, int slot, bool values) {
     attn::Rows& to = stage[slot];
-    if (t < ctx && a.runs && __ballot(row >= 0) == ~0ull) {
-      // every four rows that an instruction copies lie together: one scalar address
-      const uint16_t* src = values ? a.values : a.keys;
-#pragma unroll
-      for (int it = 0; it < 16 / NW; ++it) {
-        const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(row, 4 * (it * NW + w))) * D;
-        if (D == attn::kD || piece_of(it) < D / 8) copy_run(src + at, voff_of(it), &to[64 * (it * NW + w)]);
-      }
+    if (t >= ctx) {   // the nodes; rows past them repeat the last and are masked
+      const int64_t ts = values ? a.v_ts : a.k_ts;
+      const uint16_t* src = (values ? a.v : a.k) + span.first * ts + static_cast<int64_t>(g) * D;
+      attn::load_rows<NW>(to, [&](int rr, int e, const void* l) {
+        if (D == attn::kD || e < D) attn::copy16(src + min(rr, n - 1) * ts + e, l);
+      });
       return;
     }
-    const uint16_t* src = t < ctx ? (values ? a.values : a.keys)
-                                  : (values ? a.v + span.first * a.v_ts : a.k + span.first * a.k_ts) +
-                                        static_cast<int64_t>(g) * D;
-    const int64_t stride = t < ctx ? D : values ? a.v_ts : a.k_ts;
-    attn::load_rows<NW>(to, [&](int rr, int e, const void* l) {
-      const int x = __shfl(row, rr, 64);
-      const uint16_t* p = x < 0 ? reinterpret_cast<const uint16_t*>(attn::zero_row) : src + x * stride;
-      if (D == attn::kD || e < D) attn::copy16(p + e, l);
-    });
+    const uint16_t* src = values ? a.values : a.keys;
+    if constexpr (RUNS) {
+#pragma unroll
+      for (int it = 0; it < 16 / NW; ++it) {
+        const int row = __builtin_amdgcn_readlane(fours, 16 * (t & 3) + it * NW + w);
+        const uint16_t* from = row < 0 ? reinterpret_cast<const uint16_t*>(zero_rows) : src + static_cast<int64_t>(row) * D;
+        // the lane's piece of the four rows (load_rows' order)
+        const int piece = (lane & 15) ^ (((lane >> 4) << 2) | ((it * NW + w) & 3));
+        if (D == attn::kD || piece < D / 8) copy_run(from, ((lane >> 4) * D + piece * 8) * 2, &to[64 * (it * NW + w)]);
+      }
+    } else {
+      const int p0 = base + t * attn::kTile;
+      attn::load_rows<NW>(to, [&](int rr, int e, const void* l) {
+        const int p = p0 + rr, row = p >= lo && p < L ? row_at(p, *entry(p)) : -1;
+        const uint16_t* from = row < 0 ? reinterpret_cast<const uint16_t*>(zero_rows) : src + static_cast<int64_t>(row) * D;
+        if (D == attn::kD || e < D) attn::copy16(from + e, l);
+      });
+    }
   };
 
   // slot q: the keys (even q) or the values of tile part.t0 + q / 2
   const int t0 = part.t0, slots = 2 * (tiles - t0);
-  auto issue = [&](int q, int ahead) {   // ahead: its tile from the current one
+  auto issue = [&](int q) {
     if (q >= slots) return;
     const int t = t0 + (q >> 1);
-    if ((q & 1) == 0) {
-      const uint64_t rows = issue_keys(t);
-#pragma unroll
-      for (int i = 0; i <= P::kAhead; ++i)
-        if (i == ahead) have[i] = rows;
-    }
+    if constexpr (RUNS)
+      if ((q & 1) == 0 && t < ctx && ((t & 3) == 0 || q == 0)) {
+        open_window(t >> 2);
+        if (q) fetch((t >> 2) + 1);   // arrives with the keys of tile t, 8 slots before it is opened
+      }
     copy_slot(t, q % S, (q & 1) != 0);
+  };
+  // the keys of tile t that are there, a bit a row
+  auto rows_there = [&](int t) -> uint64_t {
+    const int p0 = base + t * attn::kTile;
+    if constexpr (RUNS) {
+      uint64_t m = (there_now >> (16 * (t & 3))) & 0xffffull;   // every bit to four
+      m = (m | m << 24) & 0x000000ff000000ffull;
+      m = (m | m << 12) & 0x000f000f000f000full;
+      m = (m | m << 6) & 0x0303030303030303ull;
+      m = (m | m << 3) & 0x1111111111111111ull;
+      m *= 15;
+      const int head = min(max(lo - p0, 0), 63), tail = min(max(p0 + 63 - (L - 1), 0), 63);
+      return m & (~0ull << head) & (~0ull >> tail);
+    } else {
+      const int p = p0 + lane;
+      return __ballot(p >= lo && p < L && row_at(p, *entry(p)) >= 0);
+    }
   };
   // The block ids, the queries and the parents together, then the first slots;
   // the masks are formed while they arrive.
-#pragma unroll
-  for (int i = 0; i < P::kAhead; ++i) fetch(t0 + i);
+  fetch(t0 >> 2);
+  fetch((t0 >> 2) + 1);   // the first window may be short
   attn::State<DT, false, D> st;
   st.init(false);
   st.load_q(a.q + (span.first + node) * a.q_ts + static_cast<int64_t>(head) * D, mine);
@@ -334,8 +365,10 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
   // as a builtin, so that the compiler counts the queries as loaded too and waits for none in the loop
   __builtin_amdgcn_s_waitcnt(0x0F70);
   asm volatile("" ::: "memory");
+  issue(0);
+  there_now = there_next;
 #pragma unroll
-  for (int q = 0; q < S - 1; ++q) issue(q, q >> 1);
+  for (int q = 1; q < S - 1; ++q) issue(q);
   if (w == 0) {
     const uint64_t set = tree::ancestors_of(up);
     s_set[lane] = set;
@@ -360,40 +393,49 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
   }
   const int64_t allfrom = geo.length + deep - W + 1;   // from here on every node sees
   int t = t0, q = 0;
-  auto inner = [&]() { return t < ctx && have[0] == ~0ull && base + t * attn::kTile >= allfrom; };
-  auto tile = [&](auto edge) {
-    const uint64_t there = have[0];
-    attn::f32x16 c[2];
-    if (q + S - 2 < slots) copies_left<P::kWaitK>();   // this wave's part of the keys has arrived
+  auto arrive = [&]() {   // slot q is there for all waves, and q - 1 consumed by them
+    if (q + S - 2 < slots) copies_left<P::kWait>();
     else copies_left<0>();
-    attn::tile_barrier();   // everyone's has, and the slot before is consumed
-    issue(q + S - 1, (S - 1) / 2);
-    if (active) {
-      st.scores(stage[q % S], c);
-      if constexpr (edge.value) {
-        const int p0 = base + t * attn::kTile, skip = min(max(from - p0, 0), 64);
+    attn::tile_barrier();
+    if constexpr (P::kEarly) issue(q + S - 1);
+  };
+  auto inner = [&]() {
+    const int p0 = base + t * attn::kTile;
+    if constexpr (RUNS)
+      return t < ctx && p0 >= lo && p0 + attn::kTile <= L && p0 >= allfrom && ((there_now >> (16 * (t & 3))) & 0xffff) == 0xffff;
+    else
+      return false;
+  };
+  auto tile = [&](auto edge) {
+    attn::f32x16 c[2];
+    uint64_t there = 0;
+    arrive();
+    if (active) st.scores(stage[q % S], c);
+    if constexpr (!P::kEarly) issue(q + S - 1);
+    const int p0 = base + t * attn::kTile;
+    if constexpr (edge.value) {
+      there = t < ctx ? rows_there(t) : 0;
+      if (active) {
+        const int skip = min(max(from - p0, 0), 64);
         const uint64_t live = t < ctx ? (skip > 63 ? 0 : there & (~0ull << skip)) : see;   // keys that the lane's query sees
         const uint64_t sh = live >> (4 * (lane >> 5));
         st.mask(c, [&](int key, int) { return ((key < 32 ? static_cast<uint32_t>(sh) >> key : static_cast<uint32_t>(sh >> 32) >> (key - 32)) & 1) != 0; });
       }
     }
     ++q;
-    if (q + S - 2 < slots) copies_left<P::kWaitV>();
-    else copies_left<0>();
-    attn::tile_barrier();
-    issue(q + S - 1, S / 2);
+    arrive();
     if (active) {
       uint64_t keep = ~0ull;
       if constexpr (edge.value) {
-        const int p0 = base + t * attn::kTile, wskip = min(max(wfrom - p0, 0), 64);
+        const int wskip = min(max(wfrom - p0, 0), 64);
         keep = t < ctx ? (wskip > 63 ? 0 : there & (~0ull << wskip)) : wsee;
       }
       st.template step<false, edge.value, true>(c, stage[q % S], k2, keep);
     }
+    if constexpr (!P::kEarly) issue(q + S - 1);
     ++q;
     ++t;
-#pragma unroll
-    for (int i = 0; i < P::kAhead; ++i) have[i] = have[i + 1];
+    if ((t & 3) == 0) there_now = there_next;
   };
   // Tiles whose keys all rows see and the others take a loop each: as branches
   // of one loop they spill (the waves' conditions may differ: both loops pass
@@ -430,32 +472,36 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeArgs a, int rows) {
   const int g = blockIdx.x % a.G, mt = blockIdx.x / a.G % a.mtiles, r = blockIdx.x / a.G / a.mtiles;
   const tree::Span span = tree::span_of(a.cu, r, a.total);
   const int n = static_cast<int>(span.count < a.max_nodes ? span.count : a.max_nodes), rep = a.rep.d;
-  const int at = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes, m = mt * rows + at;
-  if (at >= rows || m >= n * rep) return;
   const int items = (n * rep + rows - 1) / rows * a.G, all = a.first[r + 1] - a.first[r];
   if (all == items) return;   // not cut
-  const int p = all / items;
-  const int64_t slot = (static_cast<int64_t>(a.slot[r]) + static_cast<int64_t>(mt * a.G + g) * p) * a.slot_rows + at;
-  float top = -3.0e38f;
-  for (int j = 0; j < p; ++j) top = fmaxf(top, a.stat[slot + static_cast<int64_t>(j) * a.slot_rows].x);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float den = 0.f;
-  const int dim = 4 * (threadIdx.x % kLanes);
+  const int p = all / items, dim = 4 * (threadIdx.x % kLanes);
+  const int64_t first = (static_cast<int64_t>(a.slot[r]) + static_cast<int64_t>(mt * a.G + g) * p) * a.slot_rows;
+  for (int at = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes; at < rows; at += gridDim.y * (256 / kLanes)) {
+    const int m = mt * rows + at;
+    if (m >= n * rep) return;
+    const int64_t slot = first + at;
+    float top = -3.0e38f;
 #pragma unroll 4
-  for (int j = 0; j < p; ++j) {
-    const int64_t s = slot + static_cast<int64_t>(j) * a.slot_rows;
-    const float2 st = a.stat[s];
-    const float4 x = *reinterpret_cast<const float4*>(a.part + s * D + dim);
-    const float f = __builtin_amdgcn_exp2f(st.x - top);
-    den = fmaf(st.y, f, den);
-    o.x = fmaf(x.x, f, o.x);
-    o.y = fmaf(x.y, f, o.y);
-    o.z = fmaf(x.z, f, o.z);
-    o.w = fmaf(x.w, f, o.w);
+    for (int j = 0; j < p; ++j) top = fmaxf(top, a.stat[slot + static_cast<int64_t>(j) * a.slot_rows].x);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < p; ++j) {
+      const int64_t s = slot + static_cast<int64_t>(j) * a.slot_rows;
+      const float2 st = a.stat[s];
+      const float4 x = *reinterpret_cast<const float4*>(a.part + s * D + dim);
+      const float f = __builtin_amdgcn_exp2f(st.x - top);
+      den = fmaf(st.y, f, den);
+      o.x = fmaf(x.x, f, o.x);
+      o.y = fmaf(x.y, f, o.y);
+      o.z = fmaf(x.z, f, o.z);
+      o.w = fmaf(x.w, f, o.w);
+    }
+    const float inv = 1.f / den;
+    const int node = a.rep.quot(m);
+    put4<DT>(a, span.first + node, g * rep + (m - node * rep), dim, D,
+             make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
   }
-  const float inv = 1.f / den;
-  const int node = a.rep.quot(m);
-  put4<DT>(a, span.first + node, g * rep + (m - node * rep), dim, D, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
 // Rows of a workgroup: 64 (two waves), 128 or 256.
@@ -465,15 +511,22 @@ constexpr int kParts = 1;
 int target_of(int rows) { return (rows == 64 ? 1024 : rows == 128 ? 512 : 256) * kParts; }
 int64_t plan_bytes(int64_t n_seqs) { return (2 * (n_seqs + 1) * 4 + 255) / 256 * 256; }
 
+template <int DT, int D, bool RUNS>
+void launch_rows(const TreeArgs& a, int rows, unsigned grid, hipStream_t st) {
+  if (rows == 256) hipLaunchKernelGGL((tree_attention_kernel<DT, D, 8, RUNS>), dim3(grid), dim3(512), 0, st, a);
+  else if (rows == 128) hipLaunchKernelGGL((tree_attention_kernel<DT, D, 4, RUNS>), dim3(grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((tree_attention_kernel<DT, D, 2, RUNS>), dim3(grid), dim3(128), 0, st, a);
+}
+
 template <int DT, int D>
 void launch(const TreeArgs& a, int rows, unsigned grid, hipStream_t st) {
-  if (rows == 256) hipLaunchKernelGGL((tree_attention_kernel<DT, D, 8>), dim3(grid), dim3(512), 0, st, a);
-  else if (rows == 128) hipLaunchKernelGGL((tree_attention_kernel<DT, D, 4>), dim3(grid), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((tree_attention_kernel<DT, D, 2>), dim3(grid), dim3(128), 0, st, a);
+  if (a.block.d % 4 == 0) launch_rows<DT, D, true>(a, rows, grid, st);
+  else launch_rows<DT, D, false>(a, rows, grid, st);
   const int most = static_cast<int>(a.max_nodes * a.rep.d < static_cast<uint32_t>(rows) ? a.max_nodes * a.rep.d : rows);
   if (a.R == 0) return;
-  const int per = 256 / (D / 4);
-  hipLaunchKernelGGL((tree_join_kernel<DT, D>), dim3(a.R * a.G * a.mtiles, (most + per - 1) / per), dim3(256), 0, st, a,
+  // rows of an item: as many workgroups as 1024 of them need
+  const int items = a.R * a.G * a.mtiles, per = 256 / (D / 4), all = (most + per - 1) / per, some = 1024 / items;
+  hipLaunchKernelGGL((tree_join_kernel<DT, D>), dim3(items, all < some ? all : some < 1 ? 1 : some), dim3(256), 0, st, a,
                      rows);
 }
 
@@ -536,7 +589,7 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
              gate_head_stride, static_cast<uint16_t*>(out), total, window,
              tree::make_div(static_cast<uint32_t>(block)), tree::make_div(static_cast<uint32_t>(columns)),
              tree::make_div(static_cast<uint32_t>(rep)), (int)n_seqs, (int)H, (int)G, (int)blocks, (int)max_nodes,
-             (int)mtiles, block % 4 == 0 ? 1 : 0, gate8 ? 1 : 0, scale, (int)target, (int)(max_nodes * rep < rows ? max_nodes * rep : rows),
+             (int)mtiles, gate8 ? 1 : 0, scale, (int)target, (int)(max_nodes * rep < rows ? max_nodes * rep : rows),
              static_cast<int32_t*>(workspace), static_cast<int32_t*>(workspace) + n_seqs + 1, nullptr, nullptr};
   char* sums = static_cast<char*>(workspace) + plan_bytes(n_seqs);
   a.part = reinterpret_cast<float*>(sums);
