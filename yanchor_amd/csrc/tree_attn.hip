@@ -122,8 +122,9 @@ __device__ __forceinline__ int64_t block_sum(int64_t x, int64_t* before) {   // 
 }
 
 // Part `id` of the call, false if there are not so many.  An item of T tiles is
-// cut into the T / chunk parts to the nearest whole, so only items of 1.5 chunks
-// and more are: at most 4/3 target parts leave partial sums.
+// cut into ceil(T / chunk) parts; chunk is at least the mean (all tiles / target),
+// so there are at most target + items parts, and, two and more being at most
+// 2 T / chunk, at most 2 target that leave partial sums.
 template <int NW>
 __device__ __forceinline__ bool find_part(const TreeArgs& a, int64_t id, Part* out) {
   constexpr int TH = NW * 64, kM = NW * attn::kRows;
@@ -144,13 +145,38 @@ __device__ __forceinline__ bool find_part(const TreeArgs& a, int64_t id, Part* o
     shape(r, &items, &tiles);
     units += block_sum<TH>(items * tiles, &before);
   }
-  int64_t chunk = (units + a.target - 1) / a.target;
-  chunk = chunk < kMinChunk ? kMinChunk : chunk;
+  // The longest part decides: of sizes from the mean on, the first that gives at
+  // most `target` parts (more items than that: 1.5 times the mean).
+  constexpr int kSizes = 8;
+  constexpr float kSize[kSizes] = {1.f, 1.06f, 1.12f, 1.2f, 1.28f, 1.36f, 1.45f, 1.5f};
+  const float mean = fmaxf(static_cast<float>(units) / a.target, kMinChunk);
+  float guess[kSizes] = {};
+  for (int64_t r = tid; r - tid < a.R; r += TH) {
+    if (a.R > TH) shape(r, &items, &tiles);   // otherwise the first loop's
+#pragma unroll
+    for (int i = 0; i < kSizes; ++i) guess[i] += items * ceilf(tiles / ceilf(mean * kSize[i]));
+  }
+  int pick = kSizes - 1;
+#pragma unroll
+  for (int i = 0; i < kSizes; ++i) guess[i] = wave_sum(guess[i]);
+  __shared__ float guesses[NW][kSizes];
+  if ((tid & 63) == 0)
+#pragma unroll
+    for (int i = 0; i < kSizes; ++i) guesses[tid >> 6][i] = guess[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = kSizes - 1; i >= 0; --i) {
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) all += guesses[w][i];
+    if (all <= a.target) pick = i;
+  }
+  const int64_t chunk = static_cast<int64_t>(ceilf(mean * kSize[pick]));
   int64_t parts = 0, cut = 0;
   if (tid == 0) found.r = -1;
   for (int64_t r = tid; r - tid < a.R; r += TH) {
-    if (a.R > TH) shape(r, &items, &tiles);   // otherwise the first loop's
-    const int64_t p = tiles * 2ll < 3 * chunk ? 1 : (2ll * tiles + chunk) / (2 * chunk), mine = items * p;
+    if (a.R > TH) shape(r, &items, &tiles);
+    const int64_t p = (tiles + chunk - 1) / chunk, mine = items * p;
     int64_t first, slot;
     const int64_t all = block_sum<TH>(mine, &first), all_cut = block_sum<TH>(p > 1 ? mine : 0, &slot);
     first += parts;
@@ -538,7 +564,7 @@ extern "C" int64_t yh_tree_attention_workspace_bytes(int64_t n_seqs, int64_t H, 
   using namespace yh;
   if (n_seqs < 0 || H <= 0 || G <= 0 || D <= 0 || max_nodes <= 0 || max_nodes > tree::kNodes) return 0;
   const int64_t rep = H / G, rows = rows_of(max_nodes, rep), used = max_nodes * rep < rows ? max_nodes * rep : rows;
-  const int64_t slots = target_of(static_cast<int>(rows)) * 4 / 3 + 1;
+  const int64_t slots = target_of(static_cast<int>(rows)) * 2;
   return plan_bytes(n_seqs) + slots * used * (D * 4 + 8);
 }
 
@@ -593,7 +619,7 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
              static_cast<int32_t*>(workspace), static_cast<int32_t*>(workspace) + n_seqs + 1, nullptr, nullptr};
   char* sums = static_cast<char*>(workspace) + plan_bytes(n_seqs);
   a.part = reinterpret_cast<float*>(sums);
-  a.stat = reinterpret_cast<float2*>(sums + (target * 4 / 3 + 1) * a.slot_rows * D * 4);
+  a.stat = reinterpret_cast<float2*>(sums + target * 2 * a.slot_rows * D * 4);
   const unsigned grid = static_cast<unsigned>(target + items + 1);   // the last clears the rows of no request
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == YH_BF16) {
