@@ -185,10 +185,21 @@ __device__ __forceinline__ f32x4v mma16x3(uint4 a, uint2 bhi, uint2 blo, f32x4v 
 }
 
 template <int ST, int V, int T>
-__global__ void __launch_bounds__(256, T == 4 ? 2 : 4) tree_gdn_mfma_kernel(GdnArgs a) {
+__global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnArgs a) {
   constexpr int kN = 16 * T, K = 128, CT = V / 64, SF = kN + 4;   // CT columns a lane
-  __shared__ uint4 s_q[kN * 16], s_k[kN * 16];     // rows of 16 pieces, piece p of row r at p ^ (r % 16)
-  __shared__ uint32_t s_low[kN][SF], s_att[kN][SF], s_inv[kN][20];   // split1 words; -low
+  // q and k: rows of 16 pieces, piece p of row r at p ^ (r % 16).  Once every wave
+  // has its products of them, split1 words of -low (its diagonal tiles then
+  // replaced by their inverses) and att: 36 KB for 64 nodes, three workgroups a CU.
+  __shared__ union {
+    uint4 qk[2][kN * 16];
+    struct {
+      uint32_t low[kN][SF], att[kN][SF];
+    };
+  } s_m;
+  auto& s_q = s_m.qk[0];
+  auto& s_k = s_m.qk[1];
+  auto& s_low = s_m.low;
+  auto& s_att = s_m.att;
   __shared__ float s_g[64], s_beta[64], s_rk[kN], s_rq[kN];
   __shared__ uint64_t s_set[64];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -222,7 +233,9 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 4) tree_gdn_mfma_kernel(GdnA
   }
   const int64_t gat = (span.first + (lane < n ? lane : 0)) * a.HV + hv;
   float gate = 0.f, beta = 0.f;
+  int up = -1;
   if (w == 0) {
+    if (lane < n) up = a.parents ? a.parents[span.first + lane] : lane - 1;
     gate = lane < n ? load_any(a.g, gat, a.g_dt) : 0.f;
     beta = lane < n ? load_any(a.beta, gat, a.beta_dt) : 0.f;
   }
@@ -246,8 +259,17 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 4) tree_gdn_mfma_kernel(GdnA
         for (int c = 0; c < CT; ++c) sv[s][j][c] = static_cast<float>(x[c]);
       }
     }
+  typedef uint16_t vcol __attribute__((ext_vector_type(CT)));
+  vcol vv[T][4];   // the lane's values
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 16 * t + 4 * quad + e;
+      vv[t][e] = *reinterpret_cast<const vcol*>(static_cast<const uint16_t*>(a.v) + ((span.first + (i < n ? i : 0)) * a.HV + hv) * V + col);
+    }
   if (w == 0) {
-    const uint64_t set = tree::ancestors(a.parents ? a.parents + span.first : nullptr, n, &gate);
+    const uint64_t set = tree::ancestors_of(up, &gate);
     s_set[lane] = set;
     s_g[lane] = gate;
     s_beta[lane] = beta;
@@ -282,52 +304,6 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 4) tree_gdn_mfma_kernel(GdnA
   auto operand = [&](const uint4* m, int t, int s) {   // rows of tile t, columns 32 s + 8 quad ..
     return __builtin_bit_cast(bf16x8_t, m[(16 * t + n16) * 16 + ((4 * s + quad) ^ n16)]);
   };
-  // low and att, a wave every fourth pair of tiles
-  {
-    int pair = 0;
-#pragma unroll 1
-    for (int ta = 0; ta < nt; ++ta)
-#pragma unroll 1
-      for (int tb = 0; tb <= ta; ++tb, ++pair) {
-        if ((pair & 3) != w) continue;
-        f32x4v kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const bf16x8_t b = operand(s_k, tb, s);
-          kk = mma32(operand(s_k, ta, s), b, kk);
-          qk = mma32(operand(s_q, ta, s), b, qk);
-        }
-        const int j = 16 * tb + n16;
-        const float rkj = s_rk[j], gj = s_g[j];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 16 * ta + 4 * quad + e;
-          const bool above = (s_set[i] >> j) & 1;
-          const float f = above ? __expf(s_g[i] - gj) * rkj : 0.f;
-          s_low[i][j] = above && i != j ? split1(-s_beta[i] * s_rk[i] * f * kk[e]) : 0u;
-          s_att[i][j] = above ? split1(s_rq[i] * f * qk[e]) : 0u;
-        }
-      }
-  }
-  __syncthreads();
-  if (w == 0) {   // the diagonal tiles' inverses: a lane a column
-    const int b = 16 * quad;
-    if (quad < nt) {
-      float x[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float acc = i == n16 ? 1.f : 0.f;
-#pragma unroll
-        for (int m = 0; m < i; ++m) {
-          const uint32_t l = s_low[b + i][b + m];
-          acc = l ? fmaf(join1(l), x[m], acc) : acc;
-        }
-        x[i] = acc;
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s_inv[b + i][n16] = split1(x[i]);
-    }
-  }
   // k S and q S
   f32x4v ks[T][CT], qs[T][CT];
 #pragma unroll
@@ -358,6 +334,55 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 4) tree_gdn_mfma_kernel(GdnA
       }
     }
   }
+  // k k^T and q k^T, a wave every fourth pair of tiles
+  constexpr int kPairs = T * (T + 1) / 2, kMine = (kPairs + 3) / 4;
+  f32x4v kk[kMine], qk[kMine];
+  auto tile_a = [](int pair) { return (pair >= 1) + (pair >= 3) + (pair >= 6); };
+#pragma unroll
+  for (int x = 0; x < kMine; ++x) {
+    const int pair = 4 * x + w, ta = tile_a(pair), tb = pair - ta * (ta + 1) / 2;
+    kk[x] = qk[x] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    if (pair >= kPairs || ta >= nt) continue;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const bf16x8_t b = operand(s_k, tb, s);
+      kk[x] = mma32(operand(s_k, ta, s), b, kk[x]);
+      qk[x] = mma32(operand(s_q, ta, s), b, qk[x]);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < kMine; ++x) {
+    const int pair = 4 * x + w, ta = tile_a(pair), tb = pair - ta * (ta + 1) / 2;
+    if (pair >= kPairs || ta >= nt) continue;
+    const int j = 16 * tb + n16;
+    const float rkj = s_rk[j], gj = s_g[j];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 16 * ta + 4 * quad + e;
+      const bool above = (s_set[i] >> j) & 1;
+      const float f = above ? __expf(s_g[i] - gj) * rkj : 0.f;
+      s_low[i][j] = above && i != j ? split1(-s_beta[i] * s_rk[i] * f * kk[x][e]) : 0u;
+      s_att[i][j] = above ? split1(s_rq[i] * f * qk[x][e]) : 0u;
+    }
+  }
+  __syncthreads();
+  if (w == 0 && quad < nt) {   // the diagonal tiles' inverses, in their places: a lane a column
+    const int b = 16 * quad;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float acc = i == n16 ? 1.f : 0.f;
+#pragma unroll
+      for (int m = 0; m < i; ++m) {
+        const uint32_t l = s_low[b + i][b + m];
+        acc = l ? fmaf(join1(l), x[m], acc) : acc;
+      }
+      x[i] = acc;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s_low[b + i][b + n16] = split1(x[i]);
+  }
   __syncthreads();
 
   uint2 uhi[T][CT], ulo[T][CT];
@@ -372,10 +397,9 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 4) tree_gdn_mfma_kernel(GdnA
       const int i = 16 * b + 4 * quad + e;
       ge[e] = __expf(s_g[i]);
       bt[e] = s_beta[i];
-      const uint16_t* v = static_cast<const uint16_t*>(a.v) + ((span.first + (i < n ? i : 0)) * a.HV + hv) * V + col;
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        const float y = bt[e] * (bf16_to_f32(v[c]) - ge[e] * s_rk[i] * ks[b][c][e]);
+        const float y = bt[e] * (bf16_to_f32(vv[b][e][c]) - ge[e] * s_rk[i] * ks[b][c][e]);
         x[c][e] = i < n ? y : 0.f;
       }
     }
@@ -398,7 +422,7 @@ __global__ void __launch_bounds__(256, T == 4 ? 2 : 4) tree_gdn_mfma_kernel(GdnA
       pair2(y[0], y[1], hi.x, lo.x);
       pair2(y[2], y[3], hi.y, lo.y);
     };
-    const uint4 inv = *reinterpret_cast<const uint4*>(&s_inv[16 * b + n16][4 * quad]);
+    const uint4 inv = *reinterpret_cast<const uint4*>(&s_low[16 * b + n16][16 * b + 4 * quad]);
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       uint2 hi, lo;
@@ -562,7 +586,7 @@ extern "C" int yh_tree_gated_delta_rule(const void* q, const void* k, const void
   const unsigned grid = static_cast<unsigned>(n_seqs * HV + 1);   // the last clears the rows of no request
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool mfma = K == 128 && qkv_dtype == YH_BF16 && tree::aligned16(q) && tree::aligned16(k) &&
-                    tree::aligned16(state) && (reinterpret_cast<uintptr_t>(o) & 3) == 0;
+                    tree::aligned16(state) && ((reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o)) & 3) == 0;
   if (mfma && state_dtype == YH_F32 && V == 128) launch_mfma<YH_F32, 128>(a, grid, st);
   else if (mfma && state_dtype == YH_F32) launch_mfma<YH_F32, 64>(a, grid, st);
   else if (mfma && V == 128) launch_mfma<YH_F16, 128>(a, grid, st);
