@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
 
 // ---------------------------------------------------------------------------
 // bf16 q / k / v with K = 128 on MFMA: a workgroup a request and value head, its
-// four waves a quarter of the value columns each.
+// W waves 1 / W of the value columns each.
 //
 // In the masks' order (a node's ancestors come before it) everything above is
 // a lower triangular product over 16-node tiles, as in a chunk of a prompt:
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
 // q and k are exact bf16 operands, their norms and the decays go into the
 // factors; float32 operands (S, low, att, w, u) enter the products as pairs hi +
 // lo of bf16, which leaves 2^-16 of each product.  S is read straight into the
-// operand layout: a lane holds rows 32 s + 8 (lane / 16) + 0..7 of V / 64
+// operand layout: a lane holds rows 32 s + 8 (lane / 16) + 0..7 of CT
 // neighbouring columns.
 //
 // What is not finite in one node may reach its own descendants only, but a
@@ -184,12 +184,12 @@ __device__ __forceinline__ f32x4v mma16x3(uint4 a, uint2 bhi, uint2 blo, f32x4v 
   return mma16(hi, bhi, c);
 }
 
-template <int ST, int V, int T>
-__global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnArgs a) {
-  constexpr int kN = 16 * T, K = 128, CT = V / 64, SF = kN + 4;   // CT columns a lane
+template <int ST, int V, int T, int W>
+__global__ void __launch_bounds__(64 * W, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnArgs a) {
+  constexpr int kN = 16 * T, K = 128, CT = V / (16 * W), SF = kN + 4, TH = 64 * W;   // CT columns a lane
   // q and k: rows of 16 pieces, piece p of row r at p ^ (r % 16).  Once every wave
-  // has its products of them, split1 words of -low (its diagonal tiles then
-  // replaced by their inverses) and att: 36 KB for 64 nodes, three workgroups a CU.
+  // has its products of them, split1 words of -low (below the diagonal tiles) and
+  // att: 41 KB in all for 64 nodes, three workgroups a CU.
   __shared__ union {
     uint4 qk[2][kN * 16];
     struct {
@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnA
   auto& s_k = s_m.qk[1];
   auto& s_low = s_m.low;
   auto& s_att = s_m.att;
+  __shared__ float s_diag[kN][20];   // -low's diagonal tiles transposed, then their inverses as split1 words
   __shared__ float s_g[64], s_beta[64], s_rk[kN], s_rq[kN];
   __shared__ uint64_t s_set[64];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnA
   uint16_t* out = static_cast<uint16_t*>(a.o);
   if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(a.R) * a.HV) {   // rows of no request
     const int64_t end = a.R ? a.cu[a.R] : 0, row = static_cast<int64_t>(a.HV) * V;
-    for (int64_t i = (end < 0 ? 0 : end) * row + tid; i < a.total * row; i += 256) out[i] = 0;
+    for (int64_t i = (end < 0 ? 0 : end) * row + tid; i < a.total * row; i += TH) out[i] = 0;
     return;
   }
   const int hv = blockIdx.x % a.HV, r = blockIdx.x / a.HV, h = hv / (a.HV / a.H);
@@ -217,15 +218,16 @@ __global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnA
   const int most = a.max_nodes < kN ? a.max_nodes : kN;
   const int n = none ? 0 : static_cast<int>(span.count < most ? span.count : most);
   for (int64_t i = n; i < span.count; ++i)   // no request: zeros; nodes past the most that the call takes: not a number
-    for (int c = tid; c < V; c += 256) out[((span.first + i) * a.HV + hv) * V + c] = none ? 0 : 0x7fc0;
+    for (int c = tid; c < V; c += TH) out[((span.first + i) * a.HV + hv) * V + c] = none ? 0 : 0x7fc0;
   if (n == 0) return;
   const int nt = (n + 15) >> 4;
 
-  // q and k rows (a thread a piece of every 16th row), then the state, which arrives behind them
-  uint4 rq[T], rk[T];
+  // q and k rows (a thread a piece of a row), then the state, which arrives behind them
+  constexpr int kRows = TH / 16, kLoads = (kN + kRows - 1) / kRows;
+  uint4 rq[kLoads], rk[kLoads];
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int i = 16 * t + (tid >> 4);
+  for (int t = 0; t < kLoads; ++t) {
+    const int i = kRows * t + (tid >> 4);
     const int64_t at = ((span.first + (i < n ? i : 0)) * a.H + h) * K + (tid & 15) * 8;
     rq[t] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at);
     rk[t] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.k) + at);
@@ -275,8 +277,9 @@ __global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnA
     s_beta[lane] = beta;
   }
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int i = 16 * t + (tid >> 4), p = i * 16 + ((tid & 15) ^ (i & 15));
+  for (int t = 0; t < kLoads; ++t) {
+    const int i = kRows * t + (tid >> 4), p = i * 16 + ((tid & 15) ^ (i & 15));
+    if (kN % kRows && i >= kN) break;
     s_q[p] = rq[t];
     s_k[p] = rk[t];
     float sums[2];
@@ -334,13 +337,20 @@ __global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnA
       }
     }
   }
-  // k k^T and q k^T, a wave every fourth pair of tiles
-  constexpr int kPairs = T * (T + 1) / 2, kMine = (kPairs + 3) / 4;
+  // The branches above end right behind matrix instructions, and where they meet the
+  // compiler (LLVM 22) misses the wait for their results: nothing reads them before this.
+  asm volatile("s_nop 7\n\ts_nop 7");
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int c = 0; c < CT; ++c) asm volatile("" : "+v"(ks[t][c]), "+v"(qs[t][c]));
+  // k k^T and q k^T, a wave every W-th pair of tiles
+  constexpr int kPairs = T * (T + 1) / 2, kMine = (kPairs + W - 1) / W;
   f32x4v kk[kMine], qk[kMine];
   auto tile_a = [](int pair) { return (pair >= 1) + (pair >= 3) + (pair >= 6); };
 #pragma unroll
   for (int x = 0; x < kMine; ++x) {
-    const int pair = 4 * x + w, ta = tile_a(pair), tb = pair - ta * (ta + 1) / 2;
+    const int pair = W * x + w, ta = tile_a(pair), tb = pair - ta * (ta + 1) / 2;
     kk[x] = qk[x] = f32x4v{0.f, 0.f, 0.f, 0.f};
     if (pair >= kPairs || ta >= nt) continue;
 #pragma unroll
@@ -353,7 +363,7 @@ __global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnA
   __syncthreads();
 #pragma unroll
   for (int x = 0; x < kMine; ++x) {
-    const int pair = 4 * x + w, ta = tile_a(pair), tb = pair - ta * (ta + 1) / 2;
+    const int pair = W * x + w, ta = tile_a(pair), tb = pair - ta * (ta + 1) / 2;
     if (pair >= kPairs || ta >= nt) continue;
     const int j = 16 * tb + n16;
     const float rkj = s_rk[j], gj = s_g[j];
@@ -362,26 +372,33 @@ __global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnA
       const int i = 16 * ta + 4 * quad + e;
       const bool above = (s_set[i] >> j) & 1;
       const float f = above ? __expf(s_g[i] - gj) * rkj : 0.f;
-      s_low[i][j] = above && i != j ? split1(-s_beta[i] * s_rk[i] * f * kk[x][e]) : 0u;
+      kk[x][e] = above && i != j ? -s_beta[i] * s_rk[i] * f * kk[x][e] : 0.f;
+      if (ta != tb) s_low[i][j] = split1(kk[x][e]);
       s_att[i][j] = above ? split1(s_rq[i] * f * qk[x][e]) : 0u;
     }
+    if (ta == tb) *reinterpret_cast<f32x4v*>(&s_diag[16 * ta + n16][4 * quad]) = kk[x];
   }
   __syncthreads();
-  if (w == 0 && quad < nt) {   // the diagonal tiles' inverses, in their places: a lane a column
+  if (w == 0 && quad < nt) {   // the diagonal tiles' inverses: a lane a column
     const int b = 16 * quad;
     float x[16];
+    f32x4v l[2][4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float acc = i == n16 ? 1.f : 0.f;
+    for (int i = 0; i < 16; ++i) x[i] = i == n16 ? 1.f : 0.f;
 #pragma unroll
-      for (int m = 0; m < i; ++m) {
-        const uint32_t l = s_low[b + i][b + m];
-        acc = l ? fmaf(join1(l), x[m], acc) : acc;
-      }
-      x[i] = acc;
+    for (int i = 0; i < 4; ++i) l[0][i] = *reinterpret_cast<const f32x4v*>(&s_diag[b][4 * i]);
+#pragma unroll
+    for (int m = 0; m < 15; ++m) {
+#pragma unroll
+      for (int i = (m + 2) / 4; i < 4; ++i) l[(m + 1) & 1][i] = *reinterpret_cast<const f32x4v*>(&s_diag[b + m + 1][4 * i]);
+      // what is not finite stays in its row, whose u then marks the descendants
+      const float f = fabsf(x[m]) < INFINITY ? x[m] : 0.f;
+#pragma unroll
+      for (int i = m + 1; i < 16; ++i) x[i] = fmaf(l[m & 1][i >> 2][i & 3], f, x[i]);
+      asm volatile("" ::: "memory");   // one column ahead, not all
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s_low[b + i][b + n16] = split1(x[i]);
+    for (int i = 0; i < 16; ++i) s_diag[b + i][n16] = __uint_as_float(split1(x[i]));
   }
   __syncthreads();
 
@@ -422,13 +439,25 @@ __global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnA
       pair2(y[0], y[1], hi.x, lo.x);
       pair2(y[2], y[3], hi.y, lo.y);
     };
-    const uint4 inv = *reinterpret_cast<const uint4*>(&s_low[16 * b + n16][16 * b + 4 * quad]);
+    const uint4 inv = *reinterpret_cast<const uint4*>(&s_diag[16 * b + n16][4 * quad]);
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       uint2 hi, lo;
       pack(x[c], c, hi, lo);
       f32x4v u = mma16x3(inv, hi, lo, f32x4v{0.f, 0.f, 0.f, 0.f});
       pack(u, c, uhi[b][c], ulo[b][c]);
+    }
+    uint64_t any = bad[0];
+    if constexpr (CT == 2) any |= bad[1];
+    bool lost[CT][4] = {};
+    if (__any(any != 0)) {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        bad[c] |= __shfl_xor(bad[c], 16, 64);
+        bad[c] |= __shfl_xor(bad[c], 32, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lost[c][e] = (bad[c] & s_set[16 * b + 4 * quad + e]) != 0;
+      }
     }
     f32x4v o[CT];
 #pragma unroll
@@ -441,18 +470,10 @@ __global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnA
 #pragma unroll
       for (int c = 0; c < CT; ++c) o[c] = mma16x3(l, uhi[ta][c], ulo[ta][c], o[c]);
     }
-    uint64_t any = bad[0];
-    if constexpr (CT == 2) any |= bad[1];
-    if (__any(any != 0)) {
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        bad[c] |= __shfl_xor(bad[c], 16, 64);
-        bad[c] |= __shfl_xor(bad[c], 32, 64);
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (bad[c] & s_set[16 * b + 4 * quad + e]) o[c][e] = NAN;
-      }
-    }
+      for (int e = 0; e < 4; ++e) o[c][e] = lost[c][e] ? NAN : o[c][e];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = 16 * b + 4 * quad + e;
@@ -468,9 +489,10 @@ __global__ void __launch_bounds__(256, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(GdnA
 
 template <int ST, int V>
 void launch_mfma(const GdnArgs& a, unsigned grid, hipStream_t st) {
-  if (a.max_nodes <= 16) hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 1>), dim3(grid), dim3(256), 0, st, a);
-  else if (a.max_nodes <= 32) hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 2>), dim3(grid), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 4>), dim3(grid), dim3(256), 0, st, a);
+  // up to 32 nodes a wave 16 columns; past them V / 4, whose registers then hold a workgroup less a CU but spill little
+  if (a.max_nodes <= 16) hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 1, V / 16>), dim3(grid), dim3(V * 4), 0, st, a);
+  else if (a.max_nodes <= 32) hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 2, V / 16>), dim3(grid), dim3(V * 4), 0, st, a);
+  else hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 4, 4>), dim3(grid), dim3(256), 0, st, a);
 }
 
 // ---------------------------------------------------------------------------
