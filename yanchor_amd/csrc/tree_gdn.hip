@@ -505,78 +505,95 @@ struct ConvTreeArgs {
   const int32_t* cu;
   uint16_t* y;              // [C / Cp, N, Cp]
   int64_t C, Cp, total;
-  int R, run;
+  int R;
 };
 
-// y_i = silu(sum_j w_j x(3 - j steps up the path of node i)): a thread takes VEC
-// channels of `run` nodes of a request.
+// y_i = silu(sum_j w_j x(3 - j steps up the path of node i)).  Bound by HBM: a
+// workgroup takes 32 VEC channels of a request, brings the window and the nodes'
+// inputs into LDS once (every row is read by up to four nodes: from L1 and L2
+// that took 73 us for 50 at 128 requests of 8 to 64 nodes x 12288 channels), and
+// each eighth of it a node at a time, a lane VEC channels.
 template <int VEC>
 __global__ void __launch_bounds__(256) conv_tree_kernel(ConvTreeArgs a) {
   using Ch = Chan<VEC>;
   typedef typename Ch::T T;
-  __shared__ int s_up[3][tree::kNodes];   // the rows 1, 2 and 3 steps up: a node, or -1 .. -3 in the window from its end
-  const int lane = threadIdx.x & 63, r = blockIdx.x;
-  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * VEC;
+  constexpr int kN = tree::kNodes, kGroups = 8;
+  __shared__ T s_x[kN + 3][32];      // the nodes, then the window
+  __shared__ int s_up[3][kN];        // rows of s_x 1, 2 and 3 steps up
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, r = blockIdx.y;
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * VEC;
+  const bool in = c < a.C;
   const int64_t plane = c / a.Cp;
   T* dst = reinterpret_cast<T*>(a.y + plane * a.total * a.Cp + (c - plane * a.Cp));
-  const int64_t yc = a.Cp / VEC;
+  const int64_t yc = a.Cp / VEC, sp = a.P / VEC, sc = a.C / VEC;
   if (r == a.R) {   // rows of no request
     const int64_t end = a.R ? a.cu[a.R] : 0;
-    if (c < a.C)
-      for (int64_t i = (end < 0 ? 0 : end) + blockIdx.z; i < a.total; i += gridDim.z) dst[i * yc] = T{};
+    if (in)
+      for (int64_t i = (end < 0 ? 0 : end) + grp; i < a.total; i += kGroups) dst[i * yc] = T{};
     return;
   }
   const tree::Span span = tree::span_of(a.cu, r, a.total);
-  const int n = static_cast<int>(span.count < tree::kNodes ? span.count : tree::kNodes);
-  const int i0 = blockIdx.z * a.run, i1 = i0 + a.run < n ? i0 + a.run : n;
-  if (blockIdx.z == 0 && c < a.C) {   // nodes past the most: not a number
-    float nan[VEC];
+  const int n = static_cast<int>(span.count < kN ? span.count : kN);
+  if (n == 0) return;
+  const T* src = reinterpret_cast<const T*>(a.proj + span.first * a.P + c);
+  T x[kN / kGroups];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) nan[v] = NAN;
-    for (int64_t i = n; i < span.count; ++i) dst[(span.first + i) * yc] = Ch::pack(nan);
-  }
-  if (i0 >= n) return;
+  for (int u = 0; u < kN / kGroups; ++u)
+    if (in && u * kGroups + grp < n) x[u] = src[(u * kGroups + grp) * sp];
+  if (in && grp < 3) s_x[kN + grp][lane] = reinterpret_cast<const T*>(a.window + static_cast<int64_t>(r) * 3 * a.C + c)[grp * sc];
   if (threadIdx.x < 64) {
+    const int node = threadIdx.x;
     int up = -1;
-    if (lane < n) up = a.parents ? a.parents[span.first + lane] : lane - 1;
-    if (up >= lane || up < 0) up = -1;
+    if (node < n) up = a.parents ? a.parents[span.first + node] : node - 1;
+    if (up >= node || up < 0) up = -1;
     int two = __shfl(up, up < 0 ? 0 : up, 64);
     if (up < 0) two = up - 1;
     int three = __shfl(up, two < 0 ? 0 : two, 64);
     if (two < 0) three = two - 1;
-    s_up[0][lane] = up;
-    s_up[1][lane] = two;
-    s_up[2][lane] = three;
+    s_up[0][node] = up < 0 ? kN + 3 + up : up;   // -1, -2, -3: the window from its end
+    s_up[1][node] = two < 0 ? kN + 3 + two : two;
+    s_up[2][node] = three < 0 ? kN + 3 + three : three;
   }
+  uint2 wr[VEC];
+  if (in)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) wr[i] = reinterpret_cast<const uint2*>(a.w)[c + i];
+#pragma unroll
+  for (int u = 0; u < kN / kGroups; ++u)
+    if (u * kGroups + grp < n) s_x[u * kGroups + grp][lane] = x[u];
   __syncthreads();
-  if (c >= a.C) return;
+  if (!in) return;
   float wt[4][VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i)
+  for (int i = 0; i < VEC; ++i) {
+    wt[0][i] = __uint_as_float(wr[i].x << 16);
+    wt[1][i] = __uint_as_float(wr[i].x & 0xffff0000u);
+    wt[2][i] = __uint_as_float(wr[i].y << 16);
+    wt[3][i] = __uint_as_float(wr[i].y & 0xffff0000u);
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) wt[j][i] = bf16_to_f32(a.w[(c + i) * 4 + j]);
-  const T* src = reinterpret_cast<const T*>(a.proj + span.first * a.P + c);
-  const T* win = reinterpret_cast<const T*>(a.window + static_cast<int64_t>(r) * 3 * a.C + c);
-  const int64_t sp = a.P / VEC, sc = a.C / VEC;
-#pragma unroll 2
-  for (int i = i0; i < i1; ++i) {
-    T x[4];
-    x[3] = src[i * sp];
-#pragma unroll
-    for (int j = 0; j < 3; ++j) {
-      const int u = s_up[j][i];
-      x[2 - j] = u >= 0 ? src[u * sp] : win[(3 + u) * sc];
-    }
+  for (int u = 0; u < kN / kGroups; ++u) {
+    const int i = u * kGroups + grp;
+    if (i >= n) break;
     float y[VEC];
+    T t[3];
+#pragma unroll
+    for (int j = 0; j < 3; ++j) t[j] = s_x[s_up[2 - j][i]][lane];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-      float acc = Ch::f32(x[0], v) * wt[0][v];
-#pragma unroll
-      for (int j = 1; j < 4; ++j) acc = fmaf(Ch::f32(x[j], v), wt[j][v], acc);
-      y[v] = silu(acc);
+      float acc = Ch::f32(t[0], v) * wt[0][v];
+      acc = fmaf(Ch::f32(t[1], v), wt[1][v], acc);
+      acc = fmaf(Ch::f32(t[2], v), wt[2][v], acc);
+      acc = fmaf(Ch::f32(x[u], v), wt[3][v], acc);
+      // silu on the hardware's exp2 and reciprocal (1 ulp each, far below the rounding to bf16)
+      y[v] = acc * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(acc * -1.4426950408889634f));
     }
     dst[(span.first + i) * yc] = Ch::pack(y);
   }
+  float nan[VEC];   // nodes past the most: not a number
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) nan[v] = NAN;
+  for (int64_t i = n + grp; i < span.count; i += kGroups) dst[(span.first + i) * yc] = Ch::pack(nan);
 }
 
 }  // namespace
@@ -630,16 +647,15 @@ extern "C" int yh_conv_tree(const void* proj, int64_t proj_stride, const void* w
   YH_CHECK_ARG(planes > 0 && channels % planes == 0, "conv_tree: planes must divide the channels");
   if (total == 0) return YH_OK;
   YH_CHECK_ARG(proj && out && conv_w && ((window && cu_seqlens) || n_seqs == 0), "conv_tree: null pointer");
-  YH_CHECK_ARG(total < (1ll << 31) && n_seqs < (1ll << 20) && channels < (1ll << 24), "conv_tree: sizes too large");
+  YH_CHECK_ARG(total < (1ll << 31) && n_seqs < 65535 && channels < (1ll << 24), "conv_tree: sizes too large");
+  YH_CHECK_ARG((reinterpret_cast<uintptr_t>(conv_w) & 7) == 0, "conv_tree: conv_w must be 8-byte aligned");
   const bool vec = channels / planes % 8 == 0 && proj_stride % 8 == 0 && tree::aligned16(proj) &&
                    tree::aligned16(window) && tree::aligned16(out);
-  const int64_t per_block = 256 * (vec ? 8 : 1), cb = (channels + per_block - 1) / per_block;
-  // a request's nodes in one workgroup, or four nodes a workgroup where the requests leave the chip empty
-  const int run = n_seqs * cb >= 1024 ? tree::kNodes : 4;
-  ConvTreeArgs a{static_cast<const uint16_t*>(proj), proj_stride, static_cast<const uint16_t*>(window),
+  const int64_t per_block = 32 * (vec ? 8 : 1), cb = (channels + per_block - 1) / per_block;
+    ConvTreeArgs a{static_cast<const uint16_t*>(proj), proj_stride, static_cast<const uint16_t*>(window),
                  static_cast<const uint16_t*>(conv_w), parents, cu_seqlens, static_cast<uint16_t*>(out), channels,
-                 channels / planes, total, (int)n_seqs, run};
-  const dim3 grid(static_cast<unsigned>(n_seqs + 1), static_cast<unsigned>(cb), tree::kNodes / run);
+                 channels / planes, total, (int)n_seqs};
+  const dim3 grid(static_cast<unsigned>(cb), static_cast<unsigned>(n_seqs + 1));   // neighbours read on in the same rows
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (vec) hipLaunchKernelGGL(conv_tree_kernel<8>, grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL(conv_tree_kernel<1>, grid, dim3(256), 0, st, a);

@@ -756,6 +756,8 @@ def conv_tree(proj, window, conv_w, parents, cu_seqlens, channels, planes=1):
         raise ValueError(f"window must be contiguous [{r}, 3, {channels}]")
     if conv_w.shape != (channels, 4) or not conv_w.is_contiguous():
         raise ValueError("conv_w must be contiguous [channels, 4]")
+    if conv_w.data_ptr() % 8:   # read 8 bytes at a time
+        conv_w = conv_w.clone()
     if proj.stride(1) != 1 or (n > 1 and proj.stride(0) < channels):
         proj = proj.contiguous()
     out = torch.empty((n, channels) if planes == 1 else (planes, n, channels // planes), dtype=proj.dtype, device=dev)
