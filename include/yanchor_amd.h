@@ -823,8 +823,9 @@ int yh_ring_fill(const void* k, int64_t k_stride, const void* v, int64_t v_strid
  * The SWA ring [rows, G, window, D] is such a cache of one column.
  */
 
-/* Bytes of the `plan` of the two calls below (4-byte aligned). */
-int64_t yh_block_plan_bytes(int64_t n_seqs);
+/* Bytes of the `plan` (4-byte aligned scratch) of the two calls below; 0: none, NULL will do. */
+int64_t yh_extend_plan_bytes(int64_t n_seqs, int64_t total);
+int64_t yh_trim_plan_bytes(int64_t n_seqs, int64_t columns);
 
 /*
  * Blocks for cu_seqlens[r + 1] - cu_seqlens[r] tokens behind the lengths[r]

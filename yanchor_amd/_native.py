@@ -101,7 +101,8 @@ SIGNATURES: dict[str, list] = {
 
 # entry points that do not return a status
 PLAIN: dict[str, tuple] = {
-    "yh_block_plan_bytes": (_i64, [_i64]),
+    "yh_extend_plan_bytes": (_i64, [_i64, _i64]),
+    "yh_trim_plan_bytes": (_i64, [_i64, _i64]),
     "yh_tree_attention_workspace_bytes": (_i64, [_i64] * 5),
     "yh_topk_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "yh_linear_split": (_i32, [_i64, _i64, _i64]),
@@ -158,12 +159,14 @@ def call(name: str, *args) -> None:
 
 
 def call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with ``device`` current, as a launch on its streams needs."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        call(name, *args)
+    """``call`` on the device's current stream (the last argument), with the
+    device current, as a launch on its streams needs."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream)
     else:
         with torch.cuda.device(device):
-            call(name, *args)
+            call(name, *args, stream)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -6,9 +6,22 @@ import torch
 MAX_NODES = 64
 
 
+def device_of(first, *rest):
+    """The ROCm device that all of the tensors (or None) share."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError(f"yanchor_amd kernels take ROCm device tensors (got a tensor on {dev})")
+    for t in rest:
+        if t is not None and t.device != dev:
+            if t.device.type != "cuda":
+                raise ValueError(f"yanchor_amd kernels take ROCm device tensors (got a tensor on {t.device})")
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    return dev
+
+
 def ints(t, dtype, device, name, size=None):
     """``t`` as a contiguous 1-D integer tensor of ``dtype`` on the device."""
-    if t.dtype not in (torch.int32, torch.int64) or t.ndim != 1:
+    if t.ndim != 1 or (t.dtype != dtype and t.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"{name} must be a 1-D integer tensor")
     if size is not None and t.shape[0] != size:
         raise ValueError(f"{name} must hold {size} entries, got {t.shape[0]}")
@@ -23,7 +36,7 @@ def offsets(cu_seqlens, total, device, most=None):
     to the packed rows."""
     if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must be a 1-D offset vector")
-    if cu_seqlens.device.type == "cpu":
+    if not cu_seqlens.is_cuda:
         h = cu_seqlens.tolist()
         if h[0] != 0 or h[-1] > total or any(b < a for a, b in zip(h, h[1:])):
             raise ValueError("cu_seqlens must be non-decreasing offsets from 0 within the packed rows")

@@ -159,8 +159,10 @@ __device__ __forceinline__ void row_range(const int32_t* cu, int R, int64_t t0, 
   *hi = tree::request_of(cu, *lo, R - 1, t1 - 1);
 }
 
+constexpr int kTokens = 512;   // of a workgroup
+
 __global__ void __launch_bounds__(256) extend_slots_kernel(ExtendArgs a) {
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * 1024, t1 = t0 + 1024 < a.total ? t0 + 1024 : a.total;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kTokens, t1 = t0 + kTokens < a.total ? t0 + kTokens : a.total;
   int lo, hi;
   row_range(a.cu, a.R, t0, t1, &lo, &hi);
   const int32_t top = a.plan[a.R];
@@ -181,7 +183,7 @@ struct TrimArgs {
   int32_t* tables;
   int32_t* free;
   int32_t* count;
-  int32_t* plan;            // [R + 1]: blocks that each request gives back, free blocks before
+  int32_t* plan;
   int64_t n_free;
   int block, columns, R, wrap;
 };
@@ -194,28 +196,44 @@ __device__ __forceinline__ void trim_range(const TrimArgs& a, int64_t r, int* lo
   *hi = static_cast<int>(to < a.columns ? to : a.columns);
 }
 
-// One wave: the blocks in columns [lo, hi) of a row; entries below 0 are none.
-__device__ __forceinline__ int count_blocks(const int32_t* row, int lo, int hi) {
+// One wave: its entries of the kDeep x 64 columns from c on; past hi none (-1).
+constexpr int kDeep = 4;   // loads in flight
+__device__ __forceinline__ void load_entries(const int32_t* row, int c, int hi, int32_t (&id)[kDeep]) {
   const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int u = 0; u < kDeep; ++u) {
+    const int at = c + u * kWave + lane;
+    id[u] = at < hi ? row[at] : -1;
+  }
+}
+// One wave: the blocks in columns [lo, hi) of a row.
+__device__ __forceinline__ int count_blocks(const int32_t* row, int lo, int hi) {
   int n = 0;
-  for (int c = lo; c < hi; c += kWave)
-    n += __popcll(__ballot(c + lane < hi && row[c + lane < hi ? c + lane : lo] >= 0));
+  for (int c = lo; c < hi; c += kDeep * kWave) {
+    int32_t id[kDeep];
+    load_entries(row, c, hi, id);
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) n += __popcll(__ballot(id[u] >= 0));
+  }
   return n;
 }
 // One wave: they become the blocks first, first + 1, ... of the call.
 __device__ __forceinline__ void give_back(const TrimArgs& a, int32_t* row, int lo, int hi, int64_t first,
                                           int64_t after) {
   const int lane = threadIdx.x & (kWave - 1);
-  for (int c = lo; c < hi; c += kWave) {
-    const bool in = c + lane < hi;
-    const int32_t id = in ? row[c + lane] : -1;
-    const uint64_t set = __ballot(id >= 0);
-    const int64_t at = after - 1 - (first + __popcll(set & ((1ull << lane) - 1)));
-    if (id >= 0) {
-      if (at >= 0 && at < a.n_free) a.free[at] = id;
-      row[c + lane] = -1;
+  for (int c = lo; c < hi; c += kDeep * kWave) {
+    int32_t id[kDeep];
+    load_entries(row, c, hi, id);
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      const uint64_t set = __ballot(id[u] >= 0);
+      const int64_t at = after - 1 - (first + __popcll(set & ((1ull << lane) - 1)));
+      if (id[u] >= 0) {
+        if (at >= 0 && at < a.n_free) a.free[at] = id[u];
+        row[c + u * kWave + lane] = -1;
+      }
+      first += __popcll(set);
     }
-    first += __popcll(set);
   }
 }
 
@@ -244,21 +262,43 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(TrimArgs a) {
   if (threadIdx.x == 0) *a.count = static_cast<int32_t>(top + all < a.n_free ? top + all : a.n_free);
 }
 
-__global__ void __launch_bounds__(kWave) trim_count_kernel(TrimArgs a) {
+// Large tables: kSplit waves a request, a share of its columns each.  plan: the
+// requests' counts, the waves', and the stack's height before.
+constexpr int kSplit = 8;
+__device__ __forceinline__ void wave_range(const TrimArgs& a, int64_t r, int* lo, int* hi) {
+  trim_range(a, r, lo, hi);
+  const int w = threadIdx.x / kWave, each = (max(*hi - *lo, 0) + kSplit - 1) / kSplit;
+  const int from = *lo + w * each;
+  *hi = min(*hi, from + each);
+  *lo = from;
+}
+
+__global__ void __launch_bounds__(kSplit * kWave) trim_count_kernel(TrimArgs a) {
+  __shared__ int s_n[kSplit];
   const int64_t r = blockIdx.x;
+  const int w = threadIdx.x / kWave;
   int lo, hi;
-  trim_range(a, r, &lo, &hi);
+  wave_range(a, r, &lo, &hi);
   const int n = count_blocks(a.tables + r * a.columns, lo, hi);
+  if ((threadIdx.x & (kWave - 1)) == 0) {
+    s_n[w] = n;
+    a.plan[a.R + r * kSplit + w] = n;
+  }
+  __syncthreads();
   if (threadIdx.x == 0) {
-    a.plan[r] = n;
-    if (r == 0) a.plan[a.R] = clamp_count(a.count, a.n_free);
+    int all = 0;
+    for (int i = 0; i < kSplit; ++i) all += s_n[i];
+    a.plan[r] = all;
+    if (r == 0) a.plan[static_cast<int64_t>(a.R) * (kSplit + 1)] = clamp_count(a.count, a.n_free);
   }
 }
 
-__global__ void __launch_bounds__(kWave) trim_move_kernel(TrimArgs a) {
+__global__ void __launch_bounds__(kSplit * kWave) trim_move_kernel(TrimArgs a) {
+  __shared__ int64_t s_before[kSplit], s_all[kSplit];
   const int64_t r = blockIdx.x;
+  const int w = threadIdx.x / kWave;
   int64_t before = 0, all = 0;
-  for (int64_t i = threadIdx.x; i < a.R; i += kWave) {
+  for (int64_t i = threadIdx.x; i < a.R; i += kSplit * kWave) {
     const int n = a.plan[i];
     all += n;
     before += i < r ? n : 0;
@@ -268,10 +308,21 @@ __global__ void __launch_bounds__(kWave) trim_move_kernel(TrimArgs a) {
     all += __shfl_xor(all, off, kWave);
     before += __shfl_xor(before, off, kWave);
   }
-  const int64_t after = a.plan[a.R] + all;
+  if ((threadIdx.x & (kWave - 1)) == 0) {
+    s_before[w] = before;
+    s_all[w] = all;
+  }
+  __syncthreads();
+  int64_t first = 0, after = a.plan[static_cast<int64_t>(a.R) * (kSplit + 1)];
+#pragma unroll
+  for (int i = 0; i < kSplit; ++i) {
+    first += s_before[i];
+    after += s_all[i];
+    if (i < w) first += a.plan[a.R + r * kSplit + i];
+  }
   int lo, hi;
-  trim_range(a, r, &lo, &hi);
-  if (a.plan[r]) give_back(a, a.tables + r * a.columns, lo, hi, before, after);
+  wave_range(a, r, &lo, &hi);
+  if (a.plan[r]) give_back(a, a.tables + r * a.columns, lo, hi, first, after);
   if (r == 0 && threadIdx.x == 0) *a.count = static_cast<int32_t>(after < a.n_free ? after : a.n_free);
 }
 
@@ -406,7 +457,22 @@ __global__ void __launch_bounds__(256) cache_write_kernel(WriteArgs a) {
 }  // namespace
 }  // namespace yh
 
-extern "C" int64_t yh_block_plan_bytes(int64_t n_seqs) { return n_seqs < 0 ? 0 : (n_seqs + 1) * 4; }
+namespace yh {
+namespace {
+// One launch where one workgroup can do it all: few tokens after the requests ...
+bool extend_in_one(int64_t n_seqs, int64_t total) { return n_seqs <= kThreads && total <= 4096; }
+// ... or tables of which one workgroup takes back all in about the second launch's time.  (128 tables
+// of 1000 columns: a few blocks each 13.9 us in one launch, 15.0 in two; all of them 86 and 21.)
+bool trim_in_one(int64_t n_seqs, int64_t columns) { return n_seqs <= kThreads && n_seqs * columns <= 16 * kThreads; }
+}  // namespace
+}  // namespace yh
+
+extern "C" int64_t yh_extend_plan_bytes(int64_t n_seqs, int64_t total) {
+  return n_seqs <= 0 || yh::extend_in_one(n_seqs, total) ? 0 : (n_seqs + 1) * 4;
+}
+extern "C" int64_t yh_trim_plan_bytes(int64_t n_seqs, int64_t columns) {
+  return n_seqs <= 0 || yh::trim_in_one(n_seqs, columns) ? 0 : (n_seqs * (yh::kSplit + 1) + 1) * 4;
+}
 
 extern "C" int yh_extend_block_tables(const int64_t* lengths, const int32_t* cu_seqlens, int32_t* tables,
                                       const int32_t* free_blocks, int32_t* free_count, int64_t* slots,
@@ -418,7 +484,7 @@ extern "C" int yh_extend_block_tables(const int64_t* lengths, const int32_t* cu_
                    n_free < (1ll << 31),
                "extend_block_tables: sizes too large");
   if (n_seqs == 0 && total == 0) return YH_OK;
-  YH_CHECK_ARG((lengths && cu_seqlens && tables && served && free_count && plan && (free_blocks || n_free == 0)) ||
+  YH_CHECK_ARG((lengths && cu_seqlens && tables && served && free_count && (plan || extend_in_one(n_seqs, total)) && (free_blocks || n_free == 0)) ||
                    n_seqs == 0,
                "extend_block_tables: null pointer");
   YH_CHECK_ARG(slots || total == 0, "extend_block_tables: null pointer");
@@ -427,14 +493,13 @@ extern "C" int yh_extend_block_tables(const int64_t* lengths, const int32_t* cu_
                static_cast<int>(n_seqs), wrap ? 1 : 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   YH_CHECK_ARG(n_seqs > 0, "extend_block_tables: tokens without requests");
-  // few tokens: one workgroup takes them after the requests, one launch
-  if (n_seqs <= kThreads && total <= 4096) {
+  if (extend_in_one(n_seqs, total)) {
     hipLaunchKernelGGL(extend_plan_kernel<true>, dim3(1), dim3(kThreads), 0, st, a);
   } else {
     hipLaunchKernelGGL(extend_plan_kernel<false>, dim3(1), dim3(kThreads), 0, st, a);
     YH_CHECK_LAUNCH("extend_block_tables plan");
     if (total)
-      hipLaunchKernelGGL(extend_slots_kernel, dim3(static_cast<unsigned>((total + 1023) / 1024)), dim3(256), 0, st, a);
+      hipLaunchKernelGGL(extend_slots_kernel, dim3(static_cast<unsigned>((total + kTokens - 1) / kTokens)), dim3(256), 0, st, a);
   }
   YH_CHECK_LAUNCH("extend_block_tables");
   return YH_OK;
@@ -445,21 +510,21 @@ extern "C" int yh_trim_block_tables(const int64_t* lengths, const int64_t* kept,
                                     int64_t columns, int64_t n_free, int64_t block, int wrap, yh_stream_t stream) {
   using namespace yh;
   YH_CHECK_ARG(n_seqs >= 0 && columns > 0 && n_free >= 0 && block > 0, "trim_block_tables: bad sizes");
-  YH_CHECK_ARG(n_seqs < (1ll << 31) && columns < (1ll << 31) && block < (1ll << 31) && n_free < (1ll << 31),
+  YH_CHECK_ARG(n_seqs < (1ll << 23) && columns < (1ll << 31) && block < (1ll << 31) && n_free < (1ll << 31),
                "trim_block_tables: sizes too large");
   if (n_seqs == 0) return YH_OK;
-  YH_CHECK_ARG(lengths && kept && tables && free_count && plan && (free_blocks || n_free == 0),
+  YH_CHECK_ARG(lengths && kept && tables && free_count && (plan || trim_in_one(n_seqs, columns)) &&
+                   (free_blocks || n_free == 0),
                "trim_block_tables: null pointer");
   TrimArgs a{lengths, kept, tables, free_blocks, free_count, static_cast<int32_t*>(plan), n_free,
              static_cast<int>(block), static_cast<int>(columns), static_cast<int>(n_seqs), wrap ? 1 : 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  // one workgroup where the tables are small: at most 64 rounds of its threads
-  if (n_seqs <= kThreads && n_seqs * columns <= 64 * kThreads) {
+  if (trim_in_one(n_seqs, columns)) {
     hipLaunchKernelGGL(trim_kernel, dim3(1), dim3(kThreads), 0, st, a);
   } else {
-    hipLaunchKernelGGL(trim_count_kernel, dim3(static_cast<unsigned>(n_seqs)), dim3(kWave), 0, st, a);
+    hipLaunchKernelGGL(trim_count_kernel, dim3(static_cast<unsigned>(n_seqs)), dim3(kSplit * kWave), 0, st, a);
     YH_CHECK_LAUNCH("trim_block_tables count");
-    hipLaunchKernelGGL(trim_move_kernel, dim3(static_cast<unsigned>(n_seqs)), dim3(kWave), 0, st, a);
+    hipLaunchKernelGGL(trim_move_kernel, dim3(static_cast<unsigned>(n_seqs)), dim3(kSplit * kWave), 0, st, a);
   }
   YH_CHECK_LAUNCH("trim_block_tables");
   return YH_OK;

@@ -219,7 +219,7 @@ def tree_gated_delta_rule(query, key, value, g, beta, parents, cu_seqlens, initi
         raise ValueError("query, key and value must share one dtype")
     if h < 1 or hv < 1 or hv % h or kd not in (64, 128) or vd not in (64, 128):
         raise ValueError("HV must be a multiple of H, and K and V 64 or 128")
-    dev = N.require_device(query, key, value, g, beta, initial_state)
+    dev = _tree.device_of(query, key, value, g, beta, initial_state)
     if initial_state.dtype not in (torch.float32, torch.float16) or initial_state.ndim != 4 or \
             tuple(initial_state.shape[1:]) != (hv, kd, vd) or not initial_state.is_contiguous():
         raise ValueError(f"initial_state must be contiguous float32 or float16 [rows, {hv}, {kd}, {vd}]")
@@ -236,5 +236,5 @@ def tree_gated_delta_rule(query, key, value, g, beta, parents, cu_seqlens, initi
     N.call_on(dev, "yh_tree_gated_delta_rule", q.data_ptr(), k.data_ptr(), v.data_ptr(), g_.data_ptr(), be.data_ptr(),
               N.ptr(parents), cu.data_ptr(), initial_state.data_ptr(), N.code(initial_state), N.ptr(idx), o.data_ptr(),
               r, n, h, hv, kd, vd, initial_state.shape[0], most, sc, int(bool(use_qk_l2norm_in_kernel)), N.code(q),
-              N.code(g_), N.code(be), N.stream_of(q))
+              N.code(g_), N.code(be))
     return o

@@ -335,7 +335,7 @@ def extend_block_tables(lengths, cu_seqlens, block_tables, free, free_count, blo
     (position p in column p // block % columns), for caches that keep a window.
     Block i of the call, requests first, then columns, is
     ``free[free_count - 1 - i]``.  Stays on the device."""
-    dev = N.require_device(block_tables, free, free_count)
+    dev = _tree.device_of(block_tables, free, free_count)
     total = int(total)
     if total < 0:
         raise ValueError("total must not be negative")
@@ -348,10 +348,11 @@ def extend_block_tables(lengths, cu_seqlens, block_tables, free, free_count, blo
     served = torch.empty(n, dtype=torch.bool, device=dev)
     if n == 0:
         return slots.fill_(-1), served
-    plan = torch.empty(n + 1, dtype=torch.int32, device=dev)
+    need = N.lib().yh_extend_plan_bytes(n, total)
+    plan = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     N.call_on(dev, "yh_extend_block_tables", lens.data_ptr(), cu.data_ptr(), block_tables.data_ptr(), free.data_ptr(),
-              free_count.data_ptr(), slots.data_ptr(), served.data_ptr(), plan.data_ptr(), n, block_tables.shape[1],
-              free.shape[0], total, int(block), int(bool(wrap)), N.stream_of(block_tables))
+              free_count.data_ptr(), slots.data_ptr(), served.data_ptr(), N.ptr(plan), n, block_tables.shape[1],
+              free.shape[0], total, int(block), int(bool(wrap)))
     return slots, served
 
 
@@ -362,7 +363,7 @@ def trim_block_tables(lengths, kept, block_tables, free, free_count, block, *, w
     ``block_tables`` become -1, all IN PLACE.  Entries below 0 (requests that
     were not served) are passed over.  Trimming what an
     ``extend_block_tables`` added restores the stack as it was."""
-    dev = N.require_device(block_tables, free, free_count)
+    dev = _tree.device_of(block_tables, free, free_count)
     n = block_tables.shape[0] if block_tables.ndim == 2 else -1
     lens = _tree.ints(lengths, torch.int64, dev, "lengths", n)
     keep = _tree.ints(kept, torch.int64, dev, "kept", n)
@@ -370,10 +371,11 @@ def trim_block_tables(lengths, kept, block_tables, free, free_count, block, *, w
     _free_stack(free, free_count)
     if n == 0:
         return
-    plan = torch.empty(n + 1, dtype=torch.int32, device=dev)
+    need = N.lib().yh_trim_plan_bytes(n, block_tables.shape[1])
+    plan = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     N.call_on(dev, "yh_trim_block_tables", lens.data_ptr(), keep.data_ptr(), block_tables.data_ptr(), free.data_ptr(),
-              free_count.data_ptr(), plan.data_ptr(), n, block_tables.shape[1], free.shape[0], int(block),
-              int(bool(wrap)), N.stream_of(block_tables))
+              free_count.data_ptr(), N.ptr(plan), n, block_tables.shape[1], free.shape[0], int(block),
+              int(bool(wrap)))
 
 
 def slot_map(cu_seqlens, lengths, block_tables, block, total, *, parents=None, last=None):
@@ -385,7 +387,7 @@ def slot_map(cu_seqlens, lengths, block_tables, block, total, *, parents=None, l
     to it get slots and the others -1, which ``layers.cache_write`` passes over;
     ``kept`` is the request's length with them.  Without ``last`` all nodes get
     one, siblings the same.  Trees of more than 64 nodes: -1 for the others."""
-    dev = N.require_device(block_tables)
+    dev = _tree.device_of(block_tables)
     total = int(total)
     if total < 0:
         raise ValueError("total must not be negative")
@@ -402,6 +404,5 @@ def slot_map(cu_seqlens, lengths, block_tables, block, total, *, parents=None, l
     if n == 0:
         return slots.fill_(-1), kept
     N.call_on(dev, "yh_slot_map", cu.data_ptr(), lens.data_ptr(), block_tables.data_ptr(), N.ptr(parents), N.ptr(last),
-              slots.data_ptr(), kept.data_ptr(), n, block_tables.shape[1], total, int(block),
-              N.stream_of(block_tables))
+              slots.data_ptr(), kept.data_ptr(), n, block_tables.shape[1], total, int(block))
     return slots, kept

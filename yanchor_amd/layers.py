@@ -657,7 +657,7 @@ def cache_write(k, v, slots, keys, values, *, positions=None, cache_positions=No
     if d * k.element_size() % 16 or d == 0 or g == 0:
         raise ValueError("a head's row must be a multiple of 16 bytes")
     _cache(keys, values, g, d, k.dtype)
-    dev = N.require_device(k, v, keys, values, cache_positions)
+    dev = _tree.device_of(k, v, keys, values, cache_positions)
     slots = _tree.ints(slots, torch.int64, dev, "slots", n)
     if (positions is None) != (cache_positions is None):
         raise ValueError("positions and cache_positions come together")
@@ -669,7 +669,7 @@ def cache_write(k, v, slots, keys, values, *, positions=None, cache_positions=No
     (k, ks), (v, vs) = _heads(k), _heads(v)
     N.call_on(dev, "yh_cache_write", k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(),
               keys.data_ptr(), values.data_ptr(), N.ptr(positions), N.ptr(cache_positions), n, keys.shape[0], g, d,
-              keys.shape[2], N.code(k), N.stream_of(k))
+              keys.shape[2], N.code(k))
 
 
 def tree_attention(q, k, v, parents, cu_seqlens, lengths, keys, values, block_tables, *, window=None, gate=None,
@@ -700,7 +700,7 @@ def tree_attention(q, k, v, parents, cu_seqlens, lengths, keys, values, block_ta
     if d not in (64, 128):
         raise ValueError("head dim must be 64 or 128")
     _cache(keys, values, g, d, q.dtype)
-    dev = N.require_device(q, k, v, keys, values, block_tables, gate)
+    dev = _tree.device_of(q, k, v, keys, values, block_tables, gate)
     parents, cu, most = _tree.nodes(parents, cu_seqlens, max_nodes, n, dev)
     r = cu.shape[0] - 1
     lens = _tree.ints(lengths, torch.int64, dev, "lengths", r)
@@ -730,7 +730,7 @@ def tree_attention(q, k, v, parents, cu_seqlens, lengths, keys, values, block_ta
               N.ptr(parents), cu.data_ptr(), lens.data_ptr(), keys.data_ptr(), values.data_ptr(),
               tables.data_ptr(), gp, gts, ghs, out.data_ptr(), r, n, keys.shape[0], tables.shape[1], h, g, d,
               keys.shape[2], 0 if window is None else int(window), most, sc,
-              N.code(q), ws.data_ptr(), need, N.stream_of(q))
+              N.code(q), ws.data_ptr(), need)
     return out
 
 
@@ -743,7 +743,7 @@ def conv_tree(proj, window, conv_w, parents, cu_seqlens, channels, planes=1):
     ``planes`` > 1 [planes, N, channels / planes]; rows behind the last request
     are zeros."""
     _bf16(proj, window, conv_w)
-    dev = N.require_device(proj, window, conv_w)
+    dev = _tree.device_of(proj, window, conv_w)
     channels, planes = int(channels), int(planes)
     if proj.ndim != 2 or channels < 1 or proj.shape[1] < channels:
         raise ValueError("proj must be [N, >= channels]")
@@ -762,6 +762,5 @@ def conv_tree(proj, window, conv_w, parents, cu_seqlens, channels, planes=1):
         proj = proj.contiguous()
     out = torch.empty((n, channels) if planes == 1 else (planes, n, channels // planes), dtype=proj.dtype, device=dev)
     N.call_on(dev, "yh_conv_tree", proj.data_ptr(), max(proj.stride(0), channels), window.data_ptr(),
-              conv_w.data_ptr(), N.ptr(parents), cu.data_ptr(), r, n, channels, planes, out.data_ptr(), N.BF16,
-              N.stream_of(proj))
+              conv_w.data_ptr(), N.ptr(parents), cu.data_ptr(), r, n, channels, planes, out.data_ptr(), N.BF16)
     return out
