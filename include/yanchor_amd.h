@@ -879,18 +879,20 @@ int yh_cache_write(const void* k, int64_t k_stride, const void* v, int64_t v_str
  *   16-byte aligned rows of dense heads), gate NULL or [total, H, D] with token
  *   and head strides; keys / values / tables the block cache, lengths int64
  *   [n_seqs] the positions in it, of which the last columns * block are read.
- * H % G == 0, D 64 or 128, scale > 0.  workspace: 16-byte aligned, of at least
- * yh_tree_attention_workspace_bytes bytes (the sums of parts of long caches); calls
- * that may overlap need one each.
+ * H % G == 0, D 64 or 128, scale > 0.  max_length: no request has more cached
+ * positions (< 0: unknown), which may save a launch.  workspace: 16-byte aligned,
+ * of at least yh_tree_attention_workspace_bytes bytes (the sums of parts of long
+ * caches; 0: none, NULL will do); calls that may overlap need one each.
  */
-int64_t yh_tree_attention_workspace_bytes(int64_t n_seqs, int64_t H, int64_t G, int64_t D, int64_t max_nodes);
+int64_t yh_tree_attention_workspace_bytes(int64_t n_seqs, int64_t H, int64_t G, int64_t D, int64_t block,
+                                          int64_t columns, int64_t window, int64_t max_nodes, int64_t max_length);
 int yh_tree_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                       int64_t v_stride, const int32_t* parents, const int32_t* cu_seqlens, const int64_t* lengths,
                       const void* keys, const void* values, const int32_t* tables, const void* gate,
                       int64_t gate_token_stride, int64_t gate_head_stride, void* out, int64_t n_seqs, int64_t total,
                       int64_t blocks, int64_t columns, int64_t H, int64_t G, int64_t D, int64_t block, int64_t window,
-                      int64_t max_nodes, float scale, int dtype, void* workspace, int64_t workspace_bytes,
-                      yh_stream_t stream);
+                      int64_t max_nodes, int64_t max_length, float scale, int dtype, void* workspace,
+                      int64_t workspace_bytes, yh_stream_t stream);
 
 /*
  * The gated delta rule of the nodes: each node's state is its parent's (the

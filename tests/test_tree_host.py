@@ -133,7 +133,7 @@ def test_c_calls_refuse_before_device_work(lib):
 
     def attn(q=p, d=128, block=16, max_nodes=64, qs=1024, cu=p, gate=None, ghs=0, dtype=1, blocks=2, total=4, ws=1 << 30):
         return lib.yh_tree_attention(q, qs, p, 256, p, 256, None, cu, p, p, p, p, gate, 1024, ghs, p, 1, total, blocks, 2,
-                                     8, 2, d, block, 0, max_nodes, 1.0, dtype, p, ws, None)
+                                     8, 2, d, block, 0, max_nodes, -1, 1.0, dtype, p, ws, None)
     refused(attn(d=96), b"64 or 128")
     refused(attn(block=0), b"bad sizes")
     refused(attn(max_nodes=65), b"max_nodes")
@@ -142,7 +142,7 @@ def test_c_calls_refuse_before_device_work(lib):
     refused(attn(qs=512), b"whole heads")
     refused(attn(gate=p, ghs=64), b"gate strides")
     refused(attn(blocks=1 << 28), b"too large")
-    refused(attn(ws=lib.yh_tree_attention_workspace_bytes(1, 8, 2, 128, 64) - 1), b"workspace")
+    refused(attn(ws=lib.yh_tree_attention_workspace_bytes(1, 8, 2, 128, 16, 2, 0, 64, -1) - 1), b"workspace")
     assert attn(dtype=0) == -3
     assert attn(total=0) == 0
 

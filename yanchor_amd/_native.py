@@ -93,7 +93,7 @@ SIGNATURES: dict[str, list] = {
     "yh_trim_block_tables": [_p] * 6 + [_i64] * 4 + [_i32, _p],
     "yh_slot_map": [_p] * 7 + [_i64] * 4 + [_p],
     "yh_cache_write": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _p],
-    "yh_tree_attention": [_p, _i64, _p, _i64, _p, _i64] + [_p] * 7 + [_i64, _i64, _p] + [_i64] * 10 + [_f32, _i32, _p, _i64, _p],
+    "yh_tree_attention": [_p, _i64, _p, _i64, _p, _i64] + [_p] * 7 + [_i64, _i64, _p] + [_i64] * 11 + [_f32, _i32, _p, _i64, _p],
     "yh_tree_gated_delta_rule": [_p] * 8 + [_i32, _p, _p] + [_i64] * 8 + [_f32, _i32, _i32, _i32, _i32, _p],
     "yh_conv_tree": [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i32, _p],
     "yh_hbm_stream": [_i32, _i32, _p, _p, _i64, _i32, _p],
@@ -103,7 +103,7 @@ SIGNATURES: dict[str, list] = {
 PLAIN: dict[str, tuple] = {
     "yh_extend_plan_bytes": (_i64, [_i64, _i64]),
     "yh_trim_plan_bytes": (_i64, [_i64, _i64]),
-    "yh_tree_attention_workspace_bytes": (_i64, [_i64] * 5),
+    "yh_tree_attention_workspace_bytes": (_i64, [_i64] * 9),
     "yh_topk_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "yh_linear_split": (_i32, [_i64, _i64, _i64]),
     "yh_linear_packed_split": (_i32, [_i64, _i64, _i64]),

@@ -48,14 +48,14 @@ struct TreeArgs {
   int gate8;               // gate rows keep 8-byte alignment
   float scale;
   // the cut: parts aimed at, and for requests [0, R] the first part, the first partial sum
-  int target, slot_rows;
+  int target, slot_rows;   // target 0: no item is cut
   int32_t* first;          // [R + 1]
   int32_t* slot;           // [R + 1]
   float* part;             // [slots, slot_rows, D]
   float2* stat;            // [slots, slot_rows]: maximum (log2), denominator
 };
 
-constexpr int kMinChunk = 4;   // tiles a part at least (but for short items)
+constexpr int kMinChunk = 2;   // tiles a part at least (but for short items)
 
 // What a request asks for: rows, and the positions [lo, L) of its cache that
 // some node sees, in tiles from `base`.
@@ -131,6 +131,13 @@ __device__ __forceinline__ bool find_part(const TreeArgs& a, int64_t id, Part* o
   __shared__ Part found;
   const int tid = threadIdx.x;
   Geometry geo{};
+  if (a.target == 0) {   // every item whole, one a workgroup
+    const int g = static_cast<int>(id % a.G), mt = static_cast<int>(id / a.G % a.mtiles), r = static_cast<int>(id / a.G / a.mtiles);
+    if (r >= a.R) return false;
+    geo = geometry(a, tree::span_of(a.cu, r, a.total), a.lengths[r]);
+    *out = Part{geo.span.first, geo.span.count, geo.length, r, mt, g, 0, geo.ctx + 1, -1};
+    return mt * kM < geo.n * static_cast<int>(a.rep.d);
+  }
   auto shape = [&](int64_t r, int64_t* items, int* tiles) {
     *items = 0;
     *tiles = 1;
@@ -549,23 +556,38 @@ void launch(const TreeArgs& a, int rows, unsigned grid, hipStream_t st) {
   if (a.block.d % 4 == 0) launch_rows<DT, D, true>(a, rows, grid, st);
   else launch_rows<DT, D, false>(a, rows, grid, st);
   const int most = static_cast<int>(a.max_nodes * a.rep.d < static_cast<uint32_t>(rows) ? a.max_nodes * a.rep.d : rows);
-  if (a.R == 0) return;
+  if (a.R == 0 || a.target == 0) return;
   // rows of an item: as many workgroups as 1024 of them need
   const int items = a.R * a.G * a.mtiles, per = 256 / (D / 4), all = (most + per - 1) / per, some = 1024 / items;
   hipLaunchKernelGGL((tree_join_kernel<DT, D>), dim3(items, all < some ? all : some < 1 ? 1 : some), dim3(256), 0, st, a,
                      rows);
 }
 
+// Parts aimed at, 0 where every item stays whole: as many of them as workgroups fit the chip, none longer than
+// 32 tiles.  (128 rings of 1024 slots, 8 groups: the second launch is 5 us of 97.)
+int64_t target_for(int64_t n_seqs, int64_t H, int64_t G, int64_t block, int64_t columns, int64_t window,
+                   int64_t max_nodes, int64_t max_length) {
+  const int rows = rows_of(max_nodes, H / G);
+  const int64_t items = n_seqs * G * ((max_nodes * (H / G) + rows - 1) / rows), target = target_of(rows);
+  int64_t most = columns * block;
+  if (window && window - 1 < most) most = window - 1;
+  if (max_length >= 0 && max_length < most) most = max_length;
+  return items >= target && most <= 30 * attn::kTile ? 0 : target;
+}
+
 }  // namespace
 }  // namespace yh
 
-extern "C" int64_t yh_tree_attention_workspace_bytes(int64_t n_seqs, int64_t H, int64_t G, int64_t D,
-                                                     int64_t max_nodes) {
+extern "C" int64_t yh_tree_attention_workspace_bytes(int64_t n_seqs, int64_t H, int64_t G, int64_t D, int64_t block,
+                                                     int64_t columns, int64_t window, int64_t max_nodes,
+                                                     int64_t max_length) {
   using namespace yh;
-  if (n_seqs < 0 || H <= 0 || G <= 0 || D <= 0 || max_nodes <= 0 || max_nodes > tree::kNodes) return 0;
+  if (n_seqs <= 0 || G <= 0 || H < G || D <= 0 || block <= 0 || columns <= 0 || columns >= (1ll << 31) ||
+      block >= (1ll << 31) || max_nodes <= 0 || max_nodes > tree::kNodes)
+    return 0;
   const int64_t rep = H / G, rows = rows_of(max_nodes, rep), used = max_nodes * rep < rows ? max_nodes * rep : rows;
-  const int64_t slots = target_of(static_cast<int>(rows)) * 2;
-  return plan_bytes(n_seqs) + slots * used * (D * 4 + 8);
+  const int64_t slots = target_for(n_seqs, H, G, block, columns, window, max_nodes, max_length) * 2;
+  return slots ? plan_bytes(n_seqs) + slots * used * (D * 4 + 8) : 0;
 }
 
 extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
@@ -573,8 +595,8 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
                                  const int64_t* lengths, const void* keys, const void* values, const int32_t* tables,
                                  const void* gate, int64_t gate_token_stride, int64_t gate_head_stride, void* out,
                                  int64_t n_seqs, int64_t total, int64_t blocks, int64_t columns, int64_t H, int64_t G,
-                                 int64_t D, int64_t block, int64_t window, int64_t max_nodes, float scale, int dtype,
-                                 void* workspace, int64_t workspace_bytes, yh_stream_t stream) {
+                                 int64_t D, int64_t block, int64_t window, int64_t max_nodes, int64_t max_length,
+                                 float scale, int dtype, void* workspace, int64_t workspace_bytes, yh_stream_t stream) {
   using namespace yh;
   YH_CHECK_ARG(n_seqs >= 0 && total >= 0 && blocks >= 0 && columns > 0 && H > 0 && G > 0 && H % G == 0 && block > 0 &&
                    window >= 0,
@@ -602,10 +624,11 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
                    H < (1ll << 20) && blocks < (1ll << 31) && block * G < (1ll << 31) && blocks * (G * block) < (1ll << 31),
                "tree_attention: sizes too large");
   const int64_t rep = H / G, rows = rows_of(max_nodes, rep), mtiles = (max_nodes * rep + rows - 1) / rows;
-  const int64_t items = n_seqs * G * mtiles, target = target_of(static_cast<int>(rows));
+  const int64_t items = n_seqs * G * mtiles;
+  const int64_t target = target_for(n_seqs, H, G, block, columns, window, max_nodes, max_length);
+  const int64_t need = yh_tree_attention_workspace_bytes(n_seqs, H, G, D, block, columns, window, max_nodes, max_length);
   YH_CHECK_ARG(items < (1ll << 22), "tree_attention: sizes too large");
-  YH_CHECK_ARG(workspace && tree::aligned16(workspace) &&
-                   workspace_bytes >= yh_tree_attention_workspace_bytes(n_seqs, H, G, D, max_nodes),
+  YH_CHECK_ARG(need == 0 || (workspace && tree::aligned16(workspace) && workspace_bytes >= need),
                "tree_attention: workspace too small");
   const bool gate8 = gate && (reinterpret_cast<uintptr_t>(gate) & 7) == 0 && gate_token_stride % 4 == 0 &&
                      gate_head_stride % 4 == 0;
@@ -616,10 +639,14 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
              tree::make_div(static_cast<uint32_t>(block)), tree::make_div(static_cast<uint32_t>(columns)),
              tree::make_div(static_cast<uint32_t>(rep)), (int)n_seqs, (int)H, (int)G, (int)blocks, (int)max_nodes,
              (int)mtiles, gate8 ? 1 : 0, scale, (int)target, (int)(max_nodes * rep < rows ? max_nodes * rep : rows),
-             static_cast<int32_t*>(workspace), static_cast<int32_t*>(workspace) + n_seqs + 1, nullptr, nullptr};
-  char* sums = static_cast<char*>(workspace) + plan_bytes(n_seqs);
-  a.part = reinterpret_cast<float*>(sums);
-  a.stat = reinterpret_cast<float2*>(sums + target * 2 * a.slot_rows * D * 4);
+             nullptr, nullptr, nullptr, nullptr};
+  if (need) {
+    char* sums = static_cast<char*>(workspace) + plan_bytes(n_seqs);
+    a.first = static_cast<int32_t*>(workspace);
+    a.slot = a.first + n_seqs + 1;
+    a.part = reinterpret_cast<float*>(sums);
+    a.stat = reinterpret_cast<float2*>(sums + target * 2 * a.slot_rows * D * 4);
+  }
   const unsigned grid = static_cast<unsigned>(target + items + 1);   // the last clears the rows of no request
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == YH_BF16) {

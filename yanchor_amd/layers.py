@@ -688,7 +688,8 @@ def tree_attention(q, k, v, parents, cu_seqlens, lengths, keys, values, block_ta
     (parents None) of one node a request is decode attention.  Returns [N, H,
     D]; rows behind the last request are zeros.  ``max_nodes``: the most nodes
     of any request (default 64); a node past it comes back as not-a-number.
-    The nodes' keys and values are not written to the cache (``cache_write``
+    ``max_length``: no request has more cached positions (a call of many short
+    ones then takes one launch).  The nodes' keys and values are not written to the cache (``cache_write``
     writes those of the accepted path)."""
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("tree_attention takes bf16 / fp16 q, k, v of one dtype")
@@ -723,14 +724,15 @@ def tree_attention(q, k, v, parents, cu_seqlens, lengths, keys, values, block_ta
         gp = gate.data_ptr()
         gts, ghs = (h * d, d) if gate.is_contiguous() else (gate.stride(0), gate.stride(1))
     out = torch.empty(n, h, d, dtype=q.dtype, device=dev)
+    block, columns, win = keys.shape[2], tables.shape[1], 0 if window is None else int(window)
+    longest = -1 if max_length is None else int(max_length)
     # scratch of the call: concurrent calls on different streams are independent
-    need = N.lib().yh_tree_attention_workspace_bytes(r, h, g, d, most)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    N.call_on(dev, "yh_tree_attention", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-              N.ptr(parents), cu.data_ptr(), lens.data_ptr(), keys.data_ptr(), values.data_ptr(),
-              tables.data_ptr(), gp, gts, ghs, out.data_ptr(), r, n, keys.shape[0], tables.shape[1], h, g, d,
-              keys.shape[2], 0 if window is None else int(window), most, sc,
-              N.code(q), ws.data_ptr(), need)
+    need = N.lib().yh_tree_attention_workspace_bytes(r, h, g, d, block, columns, win, most, longest)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    N.call_on(dev, "yh_tree_attention", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, N.ptr(parents),
+              cu.data_ptr(), lens.data_ptr(), keys.data_ptr(), values.data_ptr(), tables.data_ptr(), gp, gts, ghs,
+              out.data_ptr(), r, n, keys.shape[0], columns, h, g, d, block, win, most, longest, sc, N.code(q),
+              N.ptr(ws), need)
     return out
 
 
