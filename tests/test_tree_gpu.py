@@ -183,6 +183,44 @@ def test_attention_equal_keys_and_infinite_keys(gpu):
     within(out[:, 0, 0], want, want * 2.0 ** -7)
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("value", [NAN, float("inf")])
+def test_attention_keeps_what_is_not_finite_on_its_path(gpu, dtype, d, value):
+    """A node's key or value reaches its descendants, a cached one the nodes whose window holds it."""
+    cu, parents = trees([40, 20], 61)
+    n, lengths, window = cu[-1], [130, 90], 70
+    q, k, v = rnd(n, 8, d, seed=1, dtype=dtype), rnd(n, 2, d, seed=2, dtype=dtype), rnd(n, 2, d, seed=3, dtype=dtype)
+    keys, values = (rnd(20, 2, 16, d, seed=s, dtype=dtype) for s in (4, 5))
+    tables = torch.arange(20, dtype=torch.int32).view(2, 10)
+    call = lambda k, v, values: layers.tree_attention(  # noqa: E731
+        q.to(gpu), k.to(gpu), v.to(gpu), i32(parents, gpu), i32(cu, gpu), torch.tensor(lengths, device=gpu), keys.to(gpu),
+        values.to(gpu), tables.to(gpu), window=window).cpu()
+    args = (parents, cu, lengths, keys)
+    want = ref.attention(q, k, v, *args, values, tables, window)
+    size = ref.attention(q, k, v.abs(), *args, values.abs(), tables, window)
+    bound = half_step(dtype) * (want.abs() + size) + 2.0 ** -12 * size
+    p = 62                                       # request 0's position, at the edge of its nodes' windows
+    for which in ("k", "v", "cache"):
+        k2, v2, c2 = k.clone(), v.clone(), values.clone()
+        if which == "cache":
+            c2[tables[0, p // 16], :, p % 16, 3] = value
+        else:
+            (k2 if which == "k" else v2)[7, :, 3] = value
+            (k2 if which == "k" else v2)[45, :, 3] = value
+        got = call(k2, v2, c2)
+        for r in range(2):
+            for i, path in enumerate(ref.paths(parents[cu[r]:cu[r + 1]], cu[r + 1] - cu[r])):
+                row = cu[r] + i
+                if which == "cache":
+                    sees = r == 0 and lengths[0] + len(path) - 1 - p < window
+                else:
+                    sees = 7 - cu[r] in path or 45 - cu[r] in path
+                if sees and which != "k":
+                    assert not torch.isfinite(got[row, :, 3]).any(), (which, row)
+                elif not sees:
+                    within(got[row], want[row], bound[row], (which, row))
+
+
 def test_attention_counts_past_max_nodes(gpu):
     """Nodes past the most are not-a-number, the others as ever."""
     q, k, v = (rnd(80, 2, 64, seed=s).to(gpu) for s in (1, 2, 3))

@@ -417,11 +417,12 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
   for (int far = depth + 1; far > W; --far) see &= see - 1;   // ancestors past the window: the earliest nodes of the path
   // the first position that this lane's query sees, and the wave's rows' earliest
   const int from = static_cast<int>(min(max(geo.length + depth - W + 1, static_cast<int64_t>(0)), (1ll << 31) - 1));
-  int wfrom = mine ? from : 0x7fffffff;
+  int wfrom = mine ? from : 0x7fffffff, wto = mine ? from : 0;   // (and the latest such)
   uint64_t wsee = see;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     wfrom = min(wfrom, __shfl_xor(wfrom, off, 64));
+    wto = max(wto, __shfl_xor(wto, off, 64));
     wsee |= __shfl_xor(wsee, off, 64);
   }
   const int64_t allfrom = geo.length + deep - W + 1;   // from here on every node sees
@@ -478,6 +479,90 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
     while (t < tiles && inner()) tile(std::false_type{});
 #pragma unroll 1
     while (t < tiles && !inner()) tile(std::true_type{});
+  }
+  // A value that is not finite reaches, through its weights of 0, the queries of
+  // the wave that do not see it, where the part holds keys that only some of them
+  // see.  Then its rows are computed again one by one without such products, a
+  // lane a key for the scores: some 30 times slower.  (Taking such rows out of the
+  // tiles they are in would cost every call 4 %.)
+  float mark = st.den;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mark = fmaf(st.acc[d][i], 0.f, mark);
+  const bool mixed = (tiles > ctx && n > 1) ||
+                     (wto > wfrom && base + t0 * attn::kTile < wto && base + min(tiles, ctx) * attn::kTile > wfrom);
+  if (mixed && __any(mine && !(fabsf(mark) < INFINITY))) {
+    constexpr int kOwn = D / 64;   // dims of a lane
+    using M = attn::Mfma<DT>;
+    typedef uint16_t own_t __attribute__((ext_vector_type(kOwn)));
+#pragma unroll 1
+    for (int i = 0; i < attn::kRows; ++i) {
+      const int mi = mt * kM + w * attn::kRows + i;
+      if (mi >= n * rep) break;
+      const int nd = a.rep.quot(mi), hd = g * rep + (mi - nd * rep), first = __shfl(from, i, 64);
+      const uint64_t sees = __shfl(see, i, 64);
+      const uint4* qr = reinterpret_cast<const uint4*>(a.q + (span.first + nd) * a.q_ts + static_cast<int64_t>(hd) * D);
+      float top = -3.0e38f, den = 0.f, o[kOwn] = {};
+#pragma unroll 1
+      for (int u = t0; u < tiles; ++u) {
+        int64_t krow = -1, vrow = 0;   // the lane's key: elements from the start of its tensor
+        if (u < ctx) {
+          const int p = base + u * attn::kTile + lane;
+          if (p >= lo && p < L && p >= first) {
+            const int row = row_at(p, *entry(p));
+            krow = vrow = row < 0 ? -1 : static_cast<int64_t>(row) * D;
+          }
+        } else if ((sees >> lane) & 1) {
+          krow = (span.first + lane) * a.k_ts + static_cast<int64_t>(g) * D;
+          vrow = (span.first + lane) * a.v_ts + static_cast<int64_t>(g) * D;
+        }
+        uint64_t live = __ballot(krow >= 0);
+        if (live == 0) continue;
+        float x = -INFINITY;
+        if (krow >= 0) {
+          const uint4* kr = reinterpret_cast<const uint4*>((u < ctx ? a.keys : a.k) + krow);
+          x = 0.f;
+#pragma unroll 4
+          for (int e = 0; e < D / 8; ++e) {
+            const uint4 y = kr[e], z = qr[e];
+            const uint32_t ky[4] = {y.x, y.y, y.z, y.w}, qz[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              x = fmaf(M::widen(ky[j] & 0xffff), M::widen(qz[j] & 0xffff), fmaf(M::widen(ky[j] >> 16), M::widen(qz[j] >> 16), x));
+          }
+          x *= k2;
+        }
+        const float now = fmaxf(top, wave_max(x)), f = __builtin_amdgcn_exp2f(top - now);
+        const float pr = krow >= 0 ? __builtin_amdgcn_exp2f(x - now) : 0.f;
+        den = fmaf(den, f, wave_sum(pr));
+        top = now;
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) o[e] *= f;
+        const uint16_t* values = u < ctx ? a.values : a.v;
+        for (; live; live &= live - 1) {
+          const int key = __builtin_ctzll(live);
+          const own_t y = *reinterpret_cast<const own_t*>(values + __shfl(vrow, key, 64) + lane * kOwn);
+          const float pk = __shfl(pr, key, 64);
+#pragma unroll
+          for (int e = 0; e < kOwn; ++e) o[e] = fmaf(pk, M::widen(y[e]), o[e]);
+        }
+      }
+      const int64_t token = span.first + nd, slot = static_cast<int64_t>(part.slot) * a.slot_rows + w * attn::kRows + i;
+      if (part.slot >= 0 && lane == 0) a.stat[slot] = make_float2(top, den);
+#pragma unroll
+      for (int e = 0; e < kOwn; ++e) {
+        const int dim = lane * kOwn + e;
+        if (part.slot >= 0) {
+          a.part[slot * D + dim] = o[e];
+        } else {
+          float x = o[e] / den;
+          if (a.gate) x *= 1.f / (1.f + __expf(-M::widen(a.gate[token * a.g_ts + hd * a.g_hs + dim])));
+          a.out[(token * a.H + hd) * D + dim] = M::round(x);
+        }
+      }
+    }
+    return;
   }
   if (!mine) return;
 

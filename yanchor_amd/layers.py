@@ -689,8 +689,9 @@ def tree_attention(q, k, v, parents, cu_seqlens, lengths, keys, values, block_ta
     D]; rows behind the last request are zeros.  ``max_nodes``: the most nodes
     of any request (default 64); a node past it comes back as not-a-number.
     ``max_length``: no request has more cached positions (a call of many short
-    ones then takes one launch).  The nodes' keys and values are not written to the cache (``cache_write``
-    writes those of the accepted path)."""
+    ones then takes one launch).  The nodes' keys and values are not written to
+    the cache (``cache_write`` writes those of the accepted path).  What is not
+    finite in a key or value reaches the nodes that see it and no others."""
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("tree_attention takes bf16 / fp16 q, k, v of one dtype")
     if q.ndim != 3 or k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or v.shape != k.shape or \
