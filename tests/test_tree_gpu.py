@@ -435,3 +435,203 @@ def test_cache_write(gpu, dtype, g, d, block):
                 cpos[s // block, :, s % block] = pos[i]
         assert torch.equal(dk.cpu().nan_to_num(9.5), keys.nan_to_num(9.5))
         assert torch.equal(dv.cpu().nan_to_num(9.5), values.nan_to_num(9.5)) and torch.equal(dp.cpu(), cpos)
+
+
+# --- odd arguments, streams, graphs, and the operators together -------------------------
+
+def test_odd_parents_and_offsets(gpu):
+    """A parent that is not an earlier node is the context; offsets past the rows are clamped."""
+    n = 9
+    q, k, v = rnd(n, 4, 64, seed=1).to(gpu), rnd(n, 2, 64, seed=2).to(gpu), rnd(n, 2, 64, seed=3).to(gpu)
+    cache, tables = rnd(4, 2, 16, 64, seed=4).to(gpu), i32([[0, 1], [2, 3]], gpu)
+    lens = torch.tensor([20, 30], device=gpu)
+    call = lambda parents, cu: layers.tree_attention(q, k, v, parents, cu, lens, cache, cache, tables)  # noqa: E731
+    plain = call(i32([-1, 0, -1, -1, -1, 0, -1, -1, 2], gpu), i32([0, 5, 9], gpu))
+    odd = call(i32([7, 0, 2, -9, 2 ** 31 - 1, 0, 1, 2, 2], gpu), i32([0, 5, 9], gpu))
+    assert torch.equal(plain, odd)
+    assert torch.equal(plain, call(torch.tensor([-1, 0, -1, -1, -1, 0, -1, -1, 2]), torch.tensor([0, 5, 9])))  # int64, from the host
+    wild = call(None, i32([-3, 5, 4000], gpu))
+    assert torch.equal(wild, call(None, i32([0, 5, 9], gpu)))
+    x, w = rnd(1, n, 2, 128, seed=5).to(gpu), rnd(2, 3, 48, seed=6).to(gpu)
+    gates, state = torch.rand(1, n, 2, device=gpu), torch.rand(2, 2, 128, 128, device=gpu)
+    for cu in ([-3, 5, 4000], [0, 7, 3]):
+        gdn.tree_gated_delta_rule(x, x, x, -gates, gates, None, i32(cu, gpu), state)
+        layers.conv_tree(rnd(n, 48, seed=7).to(gpu), w, rnd(48, 4, seed=8).to(gpu), None, i32(cu, gpu), 48)
+        ik.slot_map(i32(cu, gpu), lens, tables, 16, n, parents=i32([0] * n, gpu))
+        ik.slot_map(i32(cu, gpu), lens, tables, 16, n)
+        free = torch.arange(6, dtype=torch.int32, device=gpu)
+        slots, _ = ik.extend_block_tables(lens, i32(cu, gpu), tables.clone(), free, i32([99], gpu), 16, n)
+    torch.cuda.synchronize()
+
+
+def test_strided_rows_and_broadcast_inputs(gpu):
+    """Columns of wider projections, single rows, expanded tensors: as their copies."""
+    wide = rnd(6, 5 * 128, seed=1).to(gpu)
+    q, k, v = wide[:, :256].view(6, 2, 128), wide[:, 256:384].view(6, 1, 128), wide[:, 512:].view(6, 1, 128)
+    cache = rnd(3, 1, 16, 128, seed=2).to(gpu)
+    args = (None, i32([0, 6], gpu), torch.tensor([40], device=gpu), cache, cache, i32([[2, 0, 1]], gpu))
+    assert torch.equal(layers.tree_attention(q, k, v, *args), layers.tree_attention(q.contiguous(), k.contiguous(), v.contiguous(), *args))
+    kx = k[:1].expand(6, 1, 128)
+    assert torch.equal(layers.tree_attention(q, kx, v, *args), layers.tree_attention(q, kx.contiguous(), v, *args))
+    odd = rnd(6, 385, seed=3).to(gpu)[:, 1:257].view(6, 2, 128)       # rows off 16-byte alignment
+    gate = rnd(2, 6, 128, seed=4).to(gpu).transpose(0, 1)            # heads outermost
+    assert torch.equal(layers.tree_attention(odd, k, v, *args, gate=gate),
+                       layers.tree_attention(odd.clone(memory_format=torch.contiguous_format), k, v, *args, gate=gate.contiguous()))
+    one = tuple(x[3:4] for x in (q, k, v))
+    single = (None, i32([0, 1], gpu), *args[2:])
+    assert torch.equal(layers.tree_attention(*one, *single), layers.tree_attention(*(x.clone() for x in one), *single))
+    proj = rnd(6, 49, seed=5).to(gpu)
+    win, w = rnd(1, 3, 24, seed=6).to(gpu), rnd(24, 4, seed=7).to(gpu)
+    assert torch.equal(layers.conv_tree(proj, win, w, *args[:2], 24), layers.conv_tree(proj[:, :24].contiguous(), win, w, *args[:2], 24))
+
+
+def _step(gpu, seed):
+    """What a speculative step holds: the trees, the caches, the states."""
+    counts = [7, 1, 20, 0, 12]
+    cu, parents = trees(counts, seed)
+    n, lengths, block, columns = cu[-1], [50, 3, 161, 90, 16], 16, 14
+    gen = torch.Generator().manual_seed(seed)
+    tables = torch.full((5, columns), -1, dtype=torch.int32)
+    order = torch.randperm(60, generator=gen).to(torch.int32)
+    at = 0
+    for r, x in enumerate(lengths):
+        m = -(-x // block)
+        tables[r, :m] = order[at:at + m]
+        at += m
+    free = torch.cat((order[at:], torch.full((at,), -1, dtype=torch.int32)))
+    d = dict(cu=i32(cu, gpu), parents=i32(parents, gpu), lengths=torch.tensor(lengths, device=gpu), tables=tables.to(gpu),
+             free=free.to(gpu), count=i32([60 - at], gpu), keys=rnd(60, 2, block, 128, seed=seed).to(gpu),
+             values=rnd(60, 2, block, 128, seed=seed + 1).to(gpu), q=rnd(n, 4, 128, seed=seed + 2).to(gpu),
+             k=rnd(n, 2, 128, seed=seed + 3).to(gpu), v=rnd(n, 2, 128, seed=seed + 4).to(gpu),
+             proj=rnd(n, 3 * 512, seed=seed + 5).to(gpu), window=rnd(5, 3, 3 * 512, seed=seed + 6).to(gpu),
+             conv_w=rnd(3 * 512, 4, seed=seed + 7, std=0.5).to(gpu), g=-torch.rand(1, n, 4, generator=gen).to(gpu),
+             beta=torch.rand(1, n, 4, generator=gen).to(gpu), state=rnd(5, 4, 128, 128, seed=seed + 8, dtype=torch.float32).to(gpu),
+             last=i32([4, -1, 13, -1, 0], gpu))
+    return d, cu, parents, lengths, block
+
+
+def _run_step(s, block):
+    n = s["q"].shape[0]
+    slots, served = ik.extend_block_tables(s["lengths"], s["cu"], s["tables"], s["free"], s["count"], block, n)
+    read = layers.tree_attention(s["q"], s["k"], s["v"], s["parents"], s["cu"], s["lengths"], s["keys"], s["values"], s["tables"])
+    x = layers.conv_tree(s["proj"], s["window"], s["conv_w"], s["parents"], s["cu"], 3 * 512, planes=3).view(3, 1, n, 4, 128)
+    o = gdn.tree_gated_delta_rule(x[0], x[1], x[2], s["g"], s["beta"], s["parents"], s["cu"], s["state"])
+    at, kept = ik.slot_map(s["cu"], s["lengths"], s["tables"], block, n, parents=s["parents"], last=s["last"])
+    layers.cache_write(s["k"], s["v"], at, s["keys"], s["values"])
+    longer = s["lengths"] + (s["cu"][1:] - s["cu"][:-1])
+    ik.trim_block_tables(longer, kept, s["tables"], s["free"], s["count"], block)
+    return slots, served, read, x, o, at, kept
+
+
+def test_a_verification_step(gpu):
+    """The operators in one step, against the decode operators run along every path, and the caches that
+    the accepted paths leave against the ones that decoding them would."""
+    s, cu, parents, lengths, block = _step(gpu, 71)
+    before = {k: v.clone() for k, v in s.items()}
+    slots, served, read, x, o, at, kept = _run_step(s, block)
+    assert served.all()
+    vmax, window = 8.0, 256                     # a ring that holds every context whole
+    size = []
+    for r, length in enumerate(lengths):
+        ids = before["tables"][r].cpu().tolist()
+        ring = [torch.zeros(1, 2, window, 128, dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+        pos = torch.full((1, 2, window), -1, dtype=torch.int32, device=gpu)
+        for p in range(length):
+            for c, name in zip(ring, ("keys", "values")):
+                c[0, :, p] = before[name][ids[p // block], :, p % block]
+        pos[0, :, :length] = torch.arange(length, dtype=torch.int32, device=gpu)
+        for i, path in enumerate(ref.paths(parents[cu[r]:cu[r + 1]], cu[r + 1] - cu[r])):
+            rows = torch.tensor([cu[r] + j for j in path], device=gpu)
+            m = len(path)
+            rk, rv, rp = ring[0].clone(), ring[1].clone(), pos.clone()
+            layers.ring_fill(s["k"][rows], s["v"][rows], i32([0, m], gpu), torch.tensor([length], device=gpu),
+                             torch.tensor([0], device=gpu), rk, rv, rp)
+            seq = im.ring_decode_attention(s["q"][rows[-1]][None, None], rk, rv, rp)[0, 0].double().cpu()
+            within(read[rows[-1]], seq, 2 * (2.0 ** -8 + 2.0 ** -12) * (seq.abs() + vmax), ("attention", r, i))
+            win = s["window"][r:r + 1].clone()
+            conv = layers.conv_prefill(s["proj"][rows].contiguous(), win, s["conv_w"], i32([0, m], gpu), 3 * 512, planes=3)
+            mine = x[:, 0, rows].reshape(3, m, 512).double().cpu()
+            within(mine, conv.double().cpu(), 2.0 ** -7 * conv.double().cpu().abs() + 2.0 ** -14, ("conv", r, i))
+            y = x[:, :, rows]
+            seq, _ = gdn.recurrent_gated_delta_rule(y[0], y[1], y[2], g=s["g"][:, rows], beta=s["beta"][:, rows],
+                                                    initial_state=s["state"][r:r + 1].clone())
+            _, terms = ref.delta_rule(*(t[0].cpu() for t in (y[0], y[1], y[2], s["g"][:, rows], s["beta"][:, rows])), None,
+                                      [0, m], s["state"][r:r + 1].cpu())
+            seq = seq[0, -1].double().cpu()
+            within(o[0, rows[-1]], seq, 2 * (2.0 ** -8 * seq.abs() + 2.0 ** -12 * terms[-1]), ("delta", r, i))
+            size.append(m)
+        last = int(s["last"][r])
+        path = ref.paths(parents[cu[r]:cu[r + 1]], cu[r + 1] - cu[r])[last] if last >= 0 else []
+        assert int(kept[r]) == length + len(path)
+        now = s["tables"][r].cpu().tolist()
+        for p in range(length + len(path)):         # the cache that decoding the accepted path would leave
+            row = s["keys"][now[p // block], :, p % block]
+            want = before["keys"][ids[p // block], :, p % block] if p < length else s["k"][cu[r] + path[p - length]]
+            assert torch.equal(row, want), (r, p)
+        assert now[-(-(length + len(path)) // block):] == [-1] * (len(now) + -(length + len(path)) // block)
+    assert max(size) > 3
+    used = sum(-(-int(x) // block) for x in kept)
+    assert int(s["count"]) == 60 - used
+    held = s["tables"][s["tables"] >= 0].tolist() + s["free"][:60 - used].tolist()
+    assert sorted(held) == list(range(60))
+
+
+def test_a_captured_step_replays(gpu):
+    """The whole step in a graph, replayed with other inputs and eager work between, against eager runs."""
+    s, _, _, _, block = _step(gpu, 81)
+    start = {k: v.clone() for k, v in s.items()}
+
+    def reset(seed):
+        for k in s:
+            s[k].copy_(start[k])
+        for j, k in enumerate(("q", "k", "v", "proj")):
+            s[k].copy_(rnd(*s[k].shape, seed=seed + j))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _run_step(s, block)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    reset(0)
+    with torch.cuda.graph(graph):
+        out = _run_step(s, block)
+    for seed in (100, 200, 300, 100):
+        reset(seed)
+        want = [t.clone() for t in _run_step(s, block)]
+        after = {k: v.clone() for k, v in s.items()}
+        reset(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+        for k in s:
+            assert torch.equal(s[k], after[k]), k
+
+
+def test_calls_on_two_streams(gpu):
+    """Two long calls that overlap, each with scratch of its own."""
+    cache = rnd(200, 2, 64, 128, seed=1).to(gpu)
+    tables = torch.arange(200, dtype=torch.int32, device=gpu).view(2, 100)
+    lens = torch.tensor([6000, 5100], device=gpu)
+    ins = [[rnd(24, h, 128, seed=s + i).to(gpu) for i, h in enumerate((8, 2, 2))] for s in (10, 20)]
+    call = lambda x: layers.tree_attention(*x, None, i32([0, 11, 24], gpu), lens, cache, cache, tables)  # noqa: E731
+    want = [call(x) for x in ins]
+    streams = [torch.cuda.Stream() for _ in ins]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for x, st in zip(ins, streams):
+            with torch.cuda.stream(st):
+                got.append(call(x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_same_bits_every_time(gpu):
+    cache = rnd(400, 2, 16, 128, seed=1).to(gpu)
+    tables = torch.arange(400, dtype=torch.int32, device=gpu).view(2, 200)
+    x = [rnd(70, h, 128, seed=i).to(gpu) for i, h in enumerate((16, 2, 2))]
+    call = lambda: layers.tree_attention(*x, None, i32([0, 64, 70], gpu), torch.tensor([3100, 2000], device=gpu), cache, cache, tables)  # noqa: E731
+    want = call()
+    assert all(torch.equal(call(), want) for _ in range(5))
