@@ -421,13 +421,15 @@ struct WriteArgs {
   int G;
 };
 
-// Bound by HBM: a token's rows are read and written once.  A thread moves a
+// Bound by HBM: a token's rows are read and written once, past the caches (65521
+// tokens x 8 heads of 128: 106 us, 5.1 TB/s; through them 115).  A thread moves a
 // 16-byte piece of the keys and of the values of kRun tokens.
-constexpr int kRun = 4;
+constexpr int kRun = 2;
 
 __global__ void __launch_bounds__(256) cache_write_kernel(WriteArgs a) {
   const int64_t n = a.N * a.pieces.d, at = static_cast<int64_t>(blockIdx.x) * (256 * kRun) + threadIdx.x;
-  uint4 x[kRun], y[kRun];
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  u4 x[kRun], y[kRun];
   int64_t to[kRun];
 #pragma unroll
   for (int u = 0; u < kRun; ++u) {
@@ -439,18 +441,18 @@ __global__ void __launch_bounds__(256) cache_write_kernel(WriteArgs a) {
     const int64_t b = slot < (1ll << 31) ? a.block.quot(in ? static_cast<uint32_t>(slot) : 0) : slot / a.block.d;
     const int64_t head = (b * a.G + g) * a.block.d + (slot - b * a.block.d);
     to[u] = in ? (head * a.row.d + (p - g * a.row.d)) * 16 : -1;
-    x[u] = y[u] = make_uint4(0, 0, 0, 0);
+    x[u] = y[u] = u4{0,0,0,0};
     if (in) {
-      x[u] = *reinterpret_cast<const uint4*>(a.k + t * a.k_ts + static_cast<int64_t>(p) * 16);
-      y[u] = *reinterpret_cast<const uint4*>(a.v + t * a.v_ts + static_cast<int64_t>(p) * 16);
+      x[u] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(a.k + t * a.k_ts + static_cast<int64_t>(p) * 16));
+      y[u] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(a.v + t * a.v_ts + static_cast<int64_t>(p) * 16));
       if (a.cache_pos && p == g * a.row.d) a.cache_pos[head] = static_cast<int32_t>(a.positions[t]);
     }
   }
 #pragma unroll
   for (int u = 0; u < kRun; ++u)
     if (to[u] >= 0) {
-      *reinterpret_cast<uint4*>(a.keys + to[u]) = x[u];
-      *reinterpret_cast<uint4*>(a.values + to[u]) = y[u];
+      __builtin_nontemporal_store(x[u], reinterpret_cast<u4*>(a.keys + to[u]));
+      __builtin_nontemporal_store(y[u], reinterpret_cast<u4*>(a.values + to[u]));
     }
 }
 
