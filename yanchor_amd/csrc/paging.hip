@@ -13,6 +13,11 @@
 // is free[count - 1 - i], and trim puts its i-th block where the next extend
 // takes it as the i-th again: the results do not depend on the order in which
 // workgroups run, and trimming takes an extension back.
+//
+// The tables move a few bytes a request and are bound by latency (128 requests:
+// extend 7.0 us, slots 3.5, trim 3.1 and 3.8), so launches are few: extend writes
+// the slots in its one launch when the tokens are few, trim takes one launch for
+// small tables.
 #include "tree.h"
 
 namespace yh {

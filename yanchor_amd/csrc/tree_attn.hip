@@ -18,6 +18,12 @@
 // kParts parts a workgroup that fits the chip): every workgroup finds its part
 // from the lengths by itself, parts of a cut item leave their unnormalised sums
 // with their maximum, and a second launch joins them in order.
+//
+// Few rows are bound by HBM, which the copies of four workgroups a CU keep at
+// 5.1 to 5.6 TB/s (128 full rings: 478 MB in 91 us; 64 block tables: 732 MB in
+// 131 us).  256 rows and more a KV head are bound by the tiles' products and
+// softmax: 516 GFLOP in 745 us, 0.69 PFLOP/s; the copies alone take 376 of them,
+// the products alone 549.
 #include <type_traits>
 
 #include "attn_tile.h"
@@ -244,8 +250,8 @@ __device__ __forceinline__ void put4(const TreeArgs& a, int64_t row, int head, i
 // With blocks of whole fours of rows (RUNS) the addresses are scalars: lane l
 // holds where the rows 4 l .. 4 l + 3 of a window of four tiles lie, from block
 // ids that come through LDS as the copies do, a window ahead (a load into
-// registers would have its wait drain the copies).  Resolved for every row of
-// every tile, they cost a step 1000 cycles, more than its products.
+// registers would have its wait drain the copies).  Resolved row by row in every
+// tile instead: 767 us for 746 at 8 long contexts.
 template <int NW>
 struct Pipe {
   static constexpr int S = NW == 8 ? 8 : NW == 4 ? 4 : 2;

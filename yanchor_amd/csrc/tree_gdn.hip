@@ -147,6 +147,11 @@ __global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
 // What is not finite in one node may reach its own descendants only, but a
 // product of a 0 in the mask with it would spread it: such elements enter the
 // products as 0 and their bits (`bad`) turn the descendants' outputs into NaN.
+//
+// Bound by the chain of a workgroup's phases (norms, products of the keys, the
+// inverses, the state's products, the tiles one after another), which three
+// workgroups a CU overlap with the read of each other's state: 421 MB in 110 us,
+// 3.8 TB/s (two a CU: 156 for 136 before the phases were shortened).
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -489,7 +494,8 @@ __global__ void __launch_bounds__(64 * W, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(G
 
 template <int ST, int V>
 void launch_mfma(const GdnArgs& a, unsigned grid, hipStream_t st) {
-  // up to 32 nodes a wave 16 columns; past them V / 4, whose registers then hold a workgroup less a CU but spill little
+  // Up to 32 nodes a wave takes 16 columns.  Past them V / 4: eight waves of four tiles each spill (128 requests of up
+  // to 64 nodes x 32 heads: 213 us for 110).
   if (a.max_nodes <= 16) hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 1, V / 16>), dim3(grid), dim3(V * 4), 0, st, a);
   else if (a.max_nodes <= 32) hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 2, V / 16>), dim3(grid), dim3(V * 4), 0, st, a);
   else hipLaunchKernelGGL((tree_gdn_mfma_kernel<ST, V, 4, 4>), dim3(grid), dim3(256), 0, st, a);
@@ -511,8 +517,8 @@ struct ConvTreeArgs {
 // y_i = silu(sum_j w_j x(3 - j steps up the path of node i)).  Bound by HBM: a
 // workgroup takes 32 VEC channels of a request, brings the window and the nodes'
 // inputs into LDS once (every row is read by up to four nodes: from L1 and L2
-// that took 73 us for 50 at 128 requests of 8 to 64 nodes x 12288 channels), and
-// each eighth of it a node at a time, a lane VEC channels.
+// that took 73 us for 50, 4.7 TB/s, at 128 requests of 8 to 64 nodes x 12288
+// channels), and each eighth of it a node at a time, a lane VEC channels.
 template <int VEC>
 __global__ void __launch_bounds__(256) conv_tree_kernel(ConvTreeArgs a) {
   using Ch = Chan<VEC>;
