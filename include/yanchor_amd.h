@@ -835,7 +835,8 @@ int64_t yh_trim_plan_bytes(int64_t n_seqs, int64_t columns);
  * columns, the call's block i is free_blocks[*free_count - 1 - i].  A request
  * takes all of its blocks or none: served[r] is 0 where its table has too few
  * columns, or the stack too few blocks for it and the requests before it.
- * wrap: a table's columns are a ring, and once all are in use no more are taken.
+ * wrap: a table's columns are a ring, and once all are in use no more are taken;
+ * of a request's tokens that share a row the last gets the slot, the others -1.
  */
 int yh_extend_block_tables(const int64_t* lengths, const int32_t* cu_seqlens, int32_t* tables,
                            const int32_t* free_blocks, int32_t* free_count, int64_t* slots, uint8_t* served,
@@ -853,8 +854,10 @@ int yh_trim_block_tables(const int64_t* lengths, const int64_t* kept, int32_t* t
 
 /*
  * Slots (int64 [total], -1: none) of the packed nodes: of all, or, with last
- * (int32 [n_seqs], each request's last accepted node, anything else none), of
- * the nodes on the path to it.  kept int64 [n_seqs]: the length of the request
+ * (int32 [n_seqs], each request's last accepted node, anything else none, but
+ * behind the end of a chain all of it), of the nodes on the path to it.  Of
+ * positions that share a row of a cache that wraps the request's last gets the
+ * slot, the others -1.  kept int64 [n_seqs]: the length of the request
  * with those nodes.  Chains (parents NULL) may be of any length.
  */
 int yh_slot_map(const int32_t* cu_seqlens, const int64_t* lengths, const int32_t* tables, const int32_t* parents,

@@ -40,8 +40,9 @@ def extend(lengths, added, tables, free, count, block, total, wrap=False):
                 tables[r][c] = free[count - 1 - taken]
                 taken += 1
         served.append(ok)
-        for p in range(length, length + a):
-            slots.append(tables[r][p // block % columns] * block + p % block if ok else -1)
+        for p in range(length, length + a):   # a ring's row goes to the last of the call that has it
+            there = ok and p + columns * block >= length + a
+            slots.append(tables[r][p // block % columns] * block + p % block if there else -1)
     return slots + [-1] * (total - len(slots)), served, count - taken
 
 
@@ -72,7 +73,8 @@ def slot_map(cu, lengths, tables, block, total, parents=None, last=None):
         kept.append(length + deep)
         for i in on:
             p = length + len(ps[i]) - 1
-            slots[a + i] = tables[r][p // block % columns] * block + p % block
+            if p + columns * block >= kept[-1]:
+                slots[a + i] = tables[r][p // block % columns] * block + p % block
     return slots, kept
 
 

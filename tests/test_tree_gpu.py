@@ -392,6 +392,46 @@ def test_extend_and_trim(gpu, n, block, columns, wrap, most):
         assert (t_dev == -1).all()       # the stack may be too small for them all; nothing is written behind it
 
 
+@pytest.mark.parametrize("n,block,columns", [(3, 4, 2), (1, 1, 1), (40, 16, 3), (1030, 8, 2)])
+def test_a_ring_takes_more_tokens_than_it_holds(gpu, n, block, columns):
+    """Of the tokens that share a row the last is written, in one launch and in several."""
+    gen = torch.Generator().manual_seed(n)
+    room = block * columns
+    lengths = torch.randint(0, 3 * room, (n,), generator=gen).tolist()
+    added = torch.randint(0, 4 * room, (n,), generator=gen).tolist()
+    tables = torch.randperm(n * columns, generator=gen).view(n, columns).to(torch.int32).tolist()
+    for r, x in enumerate(lengths):
+        tables[r][ref._used(x, block, columns, True):] = [-1] * (columns - ref._used(x, block, columns, True))
+    free = [x for x in range(n * columns) if x not in {y for t in tables for y in t}]
+    cu = torch.tensor([0] + added).cumsum(0)
+    total = int(cu[-1])
+    t_dev, f_dev, c_dev = i32(tables, gpu), i32(free + [-1], gpu), i32([len(free)], gpu)
+    len_dev = torch.tensor(lengths, device=gpu)
+    slots, served = ik.extend_block_tables(len_dev, cu.to(gpu), t_dev, f_dev, c_dev, block, total, wrap=True)
+    want, serve, _ = ref.extend(lengths, added, tables, free, len(free), block, total, True)
+    assert served.tolist() == serve == [True] * n and slots.tolist() == want and t_dev.tolist() == tables
+    again, kept = ik.slot_map(cu.to(gpu), len_dev, t_dev, block, total)
+    assert torch.equal(again, slots) and kept.tolist() == [a + b for a, b in zip(lengths, added)]
+    last = [min(room, x) - 1 for x in added]           # a part of each chain
+    got, _ = ik.slot_map(cu.to(gpu), len_dev, t_dev, block, total, last=i32(last, gpu))
+    assert got.tolist() == ref.slot_map(cu.tolist(), lengths, tables, block, total, last=last)[0]
+    short = [min(x, 64) for x in added]                # as trees
+    par, off = [i - 1 for x in short for i in range(x)], torch.tensor([0] + short).cumsum(0)
+    got, _ = ik.slot_map(off.to(gpu), len_dev, t_dev, block, len(par), parents=i32(par, gpu))
+    assert got.tolist() == ref.slot_map(off.tolist(), lengths, tables, block, len(par), par)[0]
+    k = torch.arange(total, device=gpu, dtype=torch.float32).view(-1, 1, 1).expand(total, 2, 4).contiguous()
+    keys = torch.full((n * columns, 2, block, 4), -1.0, device=gpu)
+    values = keys.clone()
+    layers.cache_write(k, -k, slots, keys, values)
+    exact = torch.full((n * columns, block), -1.0)
+    for r in range(n):                                 # one after the other
+        for i in range(added[r]):
+            p = lengths[r] + i
+            exact[tables[r][p // block % columns], p % block] = float(cu[r] + i)
+    assert torch.equal(keys.cpu(), exact[:, None, :, None].expand_as(keys))
+    assert torch.equal(values.cpu(), torch.where(exact < 0, exact, -exact)[:, None, :, None].expand_as(keys))
+
+
 @pytest.mark.parametrize("tree", [True, False])
 def test_slot_map(gpu, tree):
     counts = [5, 0, 64, 1, 17] if tree else [5, 0, 200, 1, 17]

@@ -48,6 +48,20 @@ def test_an_empty_stack_serves_no_later_request():
     assert served == [True, False, False, True] and count == 2     # the last needs no block
 
 
+@pytest.mark.parametrize("length,added", [(0, 30), (5, 8), (7, 9), (20, 17), (3, 0)])
+def test_a_ring_keeps_the_last_of_a_row(length, added):
+    block, columns = 4, 2
+    tables, free = [[-1] * columns], [7, 5]
+    ref.extend([0], [length], tables, free, 2, block, length, True)
+    used = sum(x >= 0 for x in tables[0])
+    slots, served, _ = ref.extend([length], [added], tables, free, 2 - used, block, added, True)
+    rows = [x for x in slots if x >= 0]
+    assert served == [True] and len(set(rows)) == len(rows) == min(added, block * columns)
+    assert slots[:added - len(rows)] == [-1] * (added - len(rows))
+    again, _ = ref.slot_map([0, added], [length], tables, block, added)
+    assert again == slots
+
+
 # --- refusals: nothing reaches a device ---------------------------------------
 
 def _attn(**kw):

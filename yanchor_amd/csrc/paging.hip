@@ -80,9 +80,14 @@ struct ExtendArgs {
   int R, wrap;
 };
 
-// A token's slot, given its request's share of the call (off < 0: none).
-__device__ __forceinline__ int64_t token_slot(const ExtendArgs& a, int r, int64_t length, int64_t i, int32_t off,
-                                              int32_t top) {
+// Position pos of a request that ends at `end`: a later one takes its row of a ring.
+__device__ __forceinline__ bool passed(int64_t pos, int64_t end, const Div& block, const Div& columns) {
+  return pos + static_cast<int64_t>(block.d) * columns.d < end;
+}
+
+// The slot of token i of n, given its request's share of the call (off < 0: none).
+__device__ __forceinline__ int64_t token_slot(const ExtendArgs& a, int r, int64_t length, int64_t i, int64_t n,
+                                              int32_t off, int32_t top) {
   const int64_t pos = length + i;
   if (off < 0 || pos > kMaxLength) return -1;
   const uint32_t q = a.block.quot(static_cast<uint32_t>(pos)), in = static_cast<uint32_t>(pos) - q * a.block.d;
@@ -97,7 +102,7 @@ __device__ __forceinline__ int64_t token_slot(const ExtendArgs& a, int r, int64_
   } else {
     id = row[c];
   }
-  return id < 0 ? -1 : static_cast<int64_t>(id) * a.block.d + in;
+  return id < 0 || passed(pos, length + n, a.block, a.columns) ? -1 : static_cast<int64_t>(id) * a.block.d + in;
 }
 
 // One workgroup: the requests in order, and with TOKENS (few of them) the
@@ -151,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) extend_plan_kernel(ExtendArgs a) {
       int64_t slot = -1;
       if (a.R > 0 && t >= s_cu[0] && t < s_cu[a.R]) {
         const int r = tree::request_of(s_cu, 0, a.R - 1, t);
-        slot = token_slot(a, r, s_len[r], t - s_cu[r], s_off[r], top);
+        slot = token_slot(a, r, s_len[r], t - s_cu[r], s_cu[r + 1] - s_cu[r], s_off[r], top);
       }
       a.slots[t] = slot;
     }
@@ -176,7 +181,7 @@ __global__ void __launch_bounds__(256) extend_slots_kernel(ExtendArgs a) {
     const Span s = tree::span_of(a.cu, r, a.total);
     int64_t slot = -1;
     if (t >= s.first && t < s.first + s.count)
-      slot = token_slot(a, r, clamp_length(a.lengths[r]), t - s.first, a.plan[r], top);
+      slot = token_slot(a, r, clamp_length(a.lengths[r]), t - s.first, s.count, a.plan[r], top);
     a.slots[t] = slot;
   }
 }
@@ -345,8 +350,8 @@ struct SlotArgs {
   int R;
 };
 
-__device__ __forceinline__ int64_t cache_slot(const SlotArgs& a, int64_t r, int64_t pos) {
-  if (pos > kMaxLength) return -1;
+__device__ __forceinline__ int64_t cache_slot(const SlotArgs& a, int64_t r, int64_t pos, int64_t end) {
+  if (pos > kMaxLength || passed(pos, end, a.block, a.columns)) return -1;
   const uint32_t q = a.block.quot(static_cast<uint32_t>(pos)), in = static_cast<uint32_t>(pos) - q * a.block.d;
   const uint32_t c = q - a.columns.quot(q) * a.columns.d;
   const int32_t id = a.tables[r * a.columns.d + c];
@@ -368,7 +373,9 @@ __global__ void __launch_bounds__(256) chain_slots_kernel(SlotArgs a) {
     const int r = tree::request_of(a.cu, 0, a.R - 1, t);
     const Span s = tree::span_of(a.cu, r, a.total);
     const int64_t i = t - s.first;
-    if (i >= 0 && i < s.count && (!a.last || i <= a.last[r])) slot = cache_slot(a, r, clamp_length(a.lengths[r]) + i);
+    const int64_t n = a.last && a.last[r] < s.count ? static_cast<int64_t>(a.last[r]) + 1 : s.count;
+    const int64_t length = clamp_length(a.lengths[r]);
+    if (i >= 0 && i < n) slot = cache_slot(a, r, length + i, length + n);
   }
   a.slots[t] = slot;
 }
@@ -406,7 +413,7 @@ __global__ void __launch_bounds__(256) tree_slots_kernel(SlotArgs a) {
     }
     deep = d;
   }
-  if (lane < n) a.slots[s.first + lane] = on ? cache_slot(a, r, length + __popcll(set) - 1) : -1;
+  if (lane < n) a.slots[s.first + lane] = on ? cache_slot(a, r, length + __popcll(set) - 1, length + deep) : -1;
   for (int64_t i = n + lane; i < s.count; i += kWave) a.slots[s.first + i] = -1;
   if (lane == 0) a.kept[r] = length + deep;
 }

@@ -332,7 +332,9 @@ def extend_block_tables(lengths, cu_seqlens, block_tables, free, free_count, blo
     is not served.  A request is served whole or not at all: not where its
     table has too few columns, nor where the stack holds too few blocks for it
     and the requests before it.  ``wrap``: a table's columns are a ring
-    (position p in column p // block % columns), for caches that keep a window.
+    (position p in column p // block % columns), for caches that keep a window;
+    of a request's new tokens that share a row of it the last gets the slot, the
+    others -1.
     Block i of the call, requests first, then columns, is
     ``free[free_count - 1 - i]``.  Stays on the device."""
     dev = _tree.device_of(block_tables, free, free_count)
@@ -386,7 +388,10 @@ def slot_map(cu_seqlens, lengths, block_tables, block, total, *, parents=None, l
     the last accepted node of each request, -1: none) only the nodes on the path
     to it get slots and the others -1, which ``layers.cache_write`` passes over;
     ``kept`` is the request's length with them.  Without ``last`` all nodes get
-    one, siblings the same.  Trees of more than 64 nodes: -1 for the others."""
+    one, siblings the same.  Of positions that share a row of a cache that wraps
+    the request's last gets the slot, the others -1.  Trees of more than 64
+    nodes: -1 for the others.  A ``last`` that is no node of the request: none in
+    a tree, all of a chain where it lies behind its end."""
     dev = _tree.device_of(block_tables)
     total = int(total)
     if total < 0:
