@@ -820,7 +820,8 @@ int yh_ring_fill(const void* k, int64_t k_stride, const void* v, int64_t v_strid
  * A block cache holds keys / values [blocks, G, block, D]: position p of
  * request r is row p % block of block tables[r][p / block % columns], tables
  * int32 [n_seqs, columns], entries below 0 none.  slot = id * block + row.
- * The SWA ring [rows, G, window, D] is such a cache of one column.
+ * The SWA ring [rows, G, window, D] is such a cache of one column.  Positions
+ * are below 2^31 - 4096.
  */
 
 /* Bytes of the `plan` (4-byte aligned scratch) of the two calls below; 0: none, NULL will do. */

@@ -244,6 +244,48 @@ def test_attention_empty_calls(gpu):
     assert torch.equal(out, torch.zeros_like(three))
 
 
+def test_attention_at_the_last_positions(gpu):
+    """Rings at positions near 2^31 read as at the same rows of early positions."""
+    cu, parents = trees([9, 64], 5)
+    q = rnd(cu[-1], 8, 128, seed=1).to(gpu)
+    k, v = (rnd(cu[-1], 2, 128, seed=s).to(gpu) for s in (2, 3))
+    keys, values = (rnd(2, 2, 1024, 128, seed=s).to(gpu) for s in (4, 5))
+    tables, par, off = i32([[1], [0]], gpu), i32(parents, gpu), i32(cu, gpu)
+    late = torch.tensor([2 ** 31 - 4096, 2 ** 31 - 5000], device=gpu)
+    runs = [layers.tree_attention(q, k, v, par, off, x, keys, values, tables, window=1024)
+            for x in (late, late - 1024 * (2 ** 21 - 16))]
+    assert torch.equal(*runs) and torch.isfinite(runs[0]).all()
+
+
+def test_caches_past_32_bit_offsets(gpu):
+    """Blocks, state rows and slots whose offsets pass 2^31 elements, against a small cache with the same rows."""
+    g, block, d, few = 8, 64, 128, 6
+    blocks = 2 ** 31 // (g * block * d) + few
+    big = [torch.empty(blocks, g, block, d, dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    small = [torch.empty(few, g, block, d, dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    k, v = (rnd(few * block, g, d, seed=s).to(gpu) for s in (1, 2))
+    slots = torch.arange(few * block, device=gpu)
+    layers.cache_write(k, v, slots + (blocks - few) * block, *big)
+    layers.cache_write(k, v, slots, *small)
+    assert torch.equal(big[0][-few:], small[0]) and torch.equal(big[1][-few:], small[1])
+    cu, parents = trees([7, 20], 3)
+    q = rnd(cu[-1], 32, d, seed=3).to(gpu)
+    tables = torch.tensor([[4, 0, 2], [5, 1, 3]], dtype=torch.int32, device=gpu)
+    args = (q, k[:cu[-1]], v[:cu[-1]], i32(parents, gpu), i32(cu, gpu), torch.tensor([130, 192], device=gpu))
+    assert torch.equal(layers.tree_attention(*args, *big, tables + (blocks - few)),
+                       layers.tree_attention(*args, *small, tables))
+    del big
+    rows = 2 ** 31 // (32 * 128 * 128) + 2
+    pool = torch.empty(rows, 32, 128, 128, device=gpu)
+    state = rnd(2, 32, 128, 128, seed=4, dtype=torch.float32).to(gpu)
+    pool[-2:] = state
+    qk = [rnd(1, cu[-1], 32, 128, seed=s).to(gpu) for s in (5, 6, 7)]
+    gb = [-torch.rand(1, cu[-1], 32, device=gpu), torch.rand(1, cu[-1], 32, device=gpu)]
+    for x in (qk, [t.float() for t in qk]):
+        assert torch.equal(gdn.tree_gated_delta_rule(*x, *gb, *args[3:5], pool, state_indices=i32([rows - 1, rows - 2], gpu)),
+                           gdn.tree_gated_delta_rule(*x, *gb, *args[3:5], state, state_indices=i32([1, 0], gpu)))
+
+
 # --- gated delta rule -------------------------------------------------------------
 
 def delta_case(dev, counts, *, h=2, hv=4, kd=128, vd=128, dtype=torch.bfloat16, state=torch.float32, rows=None, pad=0,

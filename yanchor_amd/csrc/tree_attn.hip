@@ -79,7 +79,7 @@ __device__ __forceinline__ Geometry geometry(const TreeArgs& a, const tree::Span
   int64_t oldest = q.length - room;
   if (a.window && q.length - a.window + 1 > oldest) oldest = q.length - a.window + 1;
   oldest = oldest < 0 ? 0 : oldest > q.length ? q.length : oldest;
-  constexpr int64_t kEnd = (1ll << 31) - 1;
+  constexpr int64_t kEnd = (1ll << 31) - 4096;   // a window of tiles past it still fits an int
   q.lo = static_cast<int>(oldest < kEnd ? oldest : kEnd);
   q.L = static_cast<int>(q.length < kEnd ? q.length : kEnd);
   q.base = q.lo & ~(attn::kTile - 1);
