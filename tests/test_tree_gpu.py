@@ -156,6 +156,18 @@ def test_attention_of_many_requests(gpu):
     attention_case(gpu, lengths, counts, h=2, g=1, seed=54, window=1200)
 
 
+@pytest.mark.parametrize("max_length", [None, 10])
+def test_attention_of_whole_items(gpu, max_length):
+    """So many heads that none is cut; a bound that is too low changes no result."""
+    gen = torch.Generator().manual_seed(2)
+    lengths = torch.randint(0, 200, (140,), generator=gen).tolist()
+    counts = torch.randint(0, 9, (140,), generator=gen).tolist()
+    attention_case(gpu, lengths, counts, h=8, g=8, d=64, block=8, window=70, gate="dense", pad=3, seed=55,
+                   max_length=max_length, max_nodes=8)
+    attention_case(gpu, lengths[:34], [min(64, 8 * x) for x in counts[:34]], h=32, g=8, d=64, block=1, columns=90,
+                   seed=56, max_length=max_length)
+
+
 def test_attention_holes_in_a_table_are_not_seen(gpu):
     attention_case(gpu, [200, 130], [8, 8], bad=[(0, 3, -1), (0, 7, 1 << 30), (1, 0, 10 ** 6), (1, 8, -5)], seed=8)
 
