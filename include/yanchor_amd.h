@@ -860,10 +860,19 @@ int yh_trim_block_tables(const int64_t* lengths, const int64_t* kept, int32_t* t
  * positions that share a row of a cache that wraps the request's last gets the
  * slot, the others -1.  kept int64 [n_seqs]: the length of the request
  * with those nodes.  Chains (parents NULL) may be of any length.
+ * The tables must hold the blocks of every request's nodes.  Where an extension
+ * may have refused some, yh_slot_map_served takes its `served` (uint8 [n_seqs],
+ * NULL: all): a request that is not served gets -1 for all of its nodes and
+ * keeps lengths[r].  So does, with wrap 0 (a table that is no ring), one whose
+ * nodes reach past its columns.
  */
 int yh_slot_map(const int32_t* cu_seqlens, const int64_t* lengths, const int32_t* tables, const int32_t* parents,
                 const int32_t* last, int64_t* slots, int64_t* kept, int64_t n_seqs, int64_t columns, int64_t total,
                 int64_t block, yh_stream_t stream);
+int yh_slot_map_served(const int32_t* cu_seqlens, const int64_t* lengths, const int32_t* tables,
+                       const int32_t* parents, const int32_t* last, const uint8_t* served, int64_t* slots,
+                       int64_t* kept, int64_t n_seqs, int64_t columns, int64_t total, int64_t block, int wrap,
+                       yh_stream_t stream);
 
 /*
  * keys / values [blocks, G, block, D] at slots[n] (int64 [N]; outside the cache:

@@ -59,7 +59,7 @@ def trim(lengths, kept, tables, free, count, block, wrap=False):
     return count + len(back)
 
 
-def slot_map(cu, lengths, tables, block, total, parents=None, last=None):
+def slot_map(cu, lengths, tables, block, total, parents=None, last=None, served=None, wrap=True):
     columns = len(tables[0])
     slots, kept = [-1] * total, []
     for r, length in enumerate(lengths):
@@ -70,6 +70,8 @@ def slot_map(cu, lengths, tables, block, total, parents=None, last=None):
         else:
             on = ps[last[r]] if 0 <= last[r] < n else []
             deep = len(on)
+        if (served is not None and not served[r]) or (not wrap and length + deep > columns * block):
+            on, deep = [], 0
         kept.append(length + deep)
         for i in on:
             p = length + len(ps[i]) - 1

@@ -729,3 +729,66 @@ def test_the_same_bits_every_time(gpu):
     call = lambda: layers.tree_attention(*x, None, i32([0, 64, 70], gpu), torch.tensor([3100, 2000], device=gpu), cache, cache, tables)  # noqa: E731
     want = call()
     assert all(torch.equal(call(), want) for _ in range(5))
+
+
+@pytest.mark.parametrize("tree", [True, False])
+@pytest.mark.parametrize("requests,columns,blocks", [(9, 6, 40), (12, 3, 200), (40, 7, 170), (1100, 5, 3600)])
+def test_a_step_that_refuses_requests(gpu, tree, requests, columns, blocks):
+    """Extend, slots, write and trim where some tables are too short and the stack runs dry: the rows of the
+    requests that were refused stay, their lengths too, and the next extension serves them from what came back."""
+    gen = torch.Generator().manual_seed(requests)
+    block = 4
+    lengths = torch.randint(0, block * columns + 1, (requests,), generator=gen).tolist()
+    while sum(ref._used(x, block, columns, False) for x in lengths) > blocks:
+        lengths[lengths.index(max(lengths))] //= 2
+    counts = torch.randint(0, 12, (requests,), generator=gen).tolist()
+    cu, parents = trees(counts, requests)
+    par = parents if tree else None
+    order = torch.randperm(blocks, generator=gen).tolist()
+    tables, free = [[-1] * columns for _ in lengths], order + [-1] * 3
+    count = ref.extend([0] * requests, lengths, tables, free, blocks, block, sum(lengths))[2]
+    last = [int(torch.randint(-1, n, (), generator=gen)) if n else -1 for n in counts]
+    total, longer = cu[-1] + 5, [x + n for x, n in zip(lengths, counts)]
+    keys = torch.zeros(blocks, 1, block, 8, device=gpu)
+    held = torch.zeros(blocks, block, dtype=torch.bool)
+    for r, x in enumerate(lengths):
+        for p in range(x):
+            held[tables[r][p // block], p % block] = True
+    t_dev, f_dev, c_dev, l_dev = i32(tables, gpu), i32(free, gpu), i32([count], gpu), torch.tensor(lengths, device=gpu)
+    par_dev = None if par is None else i32(par + [0] * 5, gpu)
+    slots, served = ik.extend_block_tables(l_dev, i32(cu, gpu), t_dev, f_dev, c_dev, block, total)
+    start = count
+    want, serve, count = ref.extend(lengths, counts, tables, free, count, block, total)
+    assert served.tolist() == serve and not all(serve) and slots.tolist() == want
+    # without `last` the deepest node decides; tables that are no rings refuse by themselves past their columns
+    for kw in (dict(served=served), dict(served=served, wrap=False), dict(wrap=False)):
+        got, kept = ik.slot_map(i32(cu, gpu), l_dev, t_dev, block, total, parents=par_dev, **kw)
+        exact = ref.slot_map(cu, lengths, tables, block, total, par, served=serve if "served" in kw else None,
+                             wrap=kw.get("wrap", True))
+        assert kept.tolist() == exact[1] and got.tolist() == [max(x, -1) for x in exact[0]]
+    at, kept = ik.slot_map(i32(cu, gpu), l_dev, t_dev, block, total, parents=par_dev, last=i32(last, gpu), served=served)
+    exact = ref.slot_map(cu, lengths, tables, block, total, par, last, serve)
+    assert at.tolist() == exact[0] and kept.tolist() == exact[1]
+    assert all(k == x for k, x, ok in zip(exact[1], lengths, serve) if not ok)
+    layers.cache_write(torch.ones(total, 1, 8, device=gpu), torch.ones(total, 1, 8, device=gpu), at, keys, keys.clone())
+    written = keys[:, 0, :, 0].cpu() > 0
+    assert not (written & held).any() and int(written.sum()) == sum(exact[1]) - sum(lengths)
+    ik.trim_block_tables(torch.tensor(longer, device=gpu), kept, t_dev, f_dev, c_dev, block)
+    count = ref.trim(longer, exact[1], tables, free, count, block)
+    assert t_dev.tolist() == tables and c_dev.item() == count <= start and f_dev[:count].tolist() == free[:count]
+    for r, k in enumerate(exact[1]):     # each request holds the blocks of its length, no more and no fewer
+        used = ref._used(k, block, columns, False)
+        assert min(tables[r][:used], default=0) >= 0 and tables[r][used:] == [-1] * (columns - used)
+    again, served = ik.extend_block_tables(kept, i32([0] + [1] * requests, gpu).cumsum(0), t_dev, f_dev, c_dev, block, requests)
+    want, serve, _ = ref.extend(exact[1], [1] * requests, tables, free, count, block, requests)
+    assert again.tolist() == want and served.tolist() == serve
+
+
+def test_served_is_checked(gpu):
+    args = (i32([0, 2], gpu), torch.tensor([1], device=gpu), i32([[0]], gpu), 4, 2)
+    for bad in (torch.ones(2, dtype=torch.bool, device=gpu), torch.ones(1, dtype=torch.int32, device=gpu)):
+        with pytest.raises(ValueError, match="served"):
+            ik.slot_map(*args, served=bad)
+    slots, kept = ik.slot_map(*args, served=torch.tensor([False]))       # from the host
+    assert slots.tolist() == [-1, -1] and kept.tolist() == [1]
+    assert ik.slot_map(*args, served=torch.tensor([True], device=gpu))[0].tolist() == [1, 2]

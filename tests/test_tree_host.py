@@ -183,3 +183,28 @@ def test_c_calls_refuse_before_device_work(lib):
     refused(lib.yh_conv_tree(p, 24, p, p, None, p, 1, 4, 24, 5, p, 1, None), b"divide")
     refused(lib.yh_conv_tree(p, 23, p, p, None, p, 1, 4, 24, 1, p, 1, None), b"bad sizes")
     refused(lib.yh_conv_tree(p, 24, p, p, None, p, 1, 4, 24, 1, p, 0, None), b"bfloat16")
+
+
+@pytest.mark.parametrize("table,free", [([5, 6], [9]), ([5, 6, -1], [])])
+def test_a_refused_request_gets_no_slots(table, free):
+    """Too few columns, or a dry stack: nothing is written, the length stays."""
+    tables = [list(table), [7] + [-1] * (len(table) - 1)]
+    slots, served, count = ref.extend([7, 1], [4, 2], tables, list(free), len(free), 4, 6)
+    assert served == [False, True] and slots == [-1] * 4 + [29, 30]
+    for par in (None, [-1, 0, 1, 2, -1, 0]):
+        for last, kept in ((None, 3), ([3, 0], 2)):
+            got = ref.slot_map([0, 4, 6], [7, 1], tables, 4, 6, par, last, served)
+            assert got == ([-1] * 4 + [29, 30 if last is None else -1], [7, kept])
+    # without `served` a table that is no ring at least does not start over
+    if len(table) == 2:
+        assert ref.slot_map([0, 4, 6], [7, 1], tables, 4, 6, wrap=False) == ([-1] * 4 + [29, 30], [7, 3])
+        assert ref.slot_map([0, 4, 6], [7, 1], tables, 4, 6)[0][:4] == [27, 20, 21, 22]      # a ring does
+
+
+def test_served_slots_refuse_before_device_work(lib):
+    p = ctypes.c_void_p(256)
+    assert lib.yh_slot_map_served(p, p, None, None, None, p, p, p, 1, 1, 4, 16, 0, None) == -1
+    assert b"null" in lib.yh_last_error()
+    assert lib.yh_slot_map_served(p, p, p, None, None, p, p, p, 1, 0, 4, 16, 0, None) == -1
+    assert b"bad sizes" in lib.yh_last_error()
+    assert lib.yh_slot_map_served(None, None, None, None, None, None, None, None, 0, 1, 0, 16, 0, None) == 0

@@ -16,8 +16,8 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libyanchor_amd.so"
 # out2_stride; 104: yh_linear_pack lays K blocks outermost; 105: yh_rmsnorm_partials takes part2;
 # 106: yh_gdn_decode_fused takes the state dtype; 107: the yh_anchor_tokens_* calls are added,
 # yh_gdn_chunk_varlen uses its workspace, yh_conv_prefill's dtype may hold a number of planes;
-# 108: the calls for drafted trees and block tables are added)
-ABI_VERSION = 108
+# 108: the calls for drafted trees and block tables are added; 109: yh_slot_map_served)
+ABI_VERSION = 109
 
 F32, BF16, F16, I32, I64, U8 = 0, 1, 2, 3, 4, 5
 DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16,
@@ -92,6 +92,7 @@ SIGNATURES: dict[str, list] = {
     "yh_extend_block_tables": [_p] * 8 + [_i64] * 5 + [_i32, _p],
     "yh_trim_block_tables": [_p] * 6 + [_i64] * 4 + [_i32, _p],
     "yh_slot_map": [_p] * 7 + [_i64] * 4 + [_p],
+    "yh_slot_map_served": [_p] * 8 + [_i64] * 4 + [_i32, _p],
     "yh_cache_write": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _p],
     "yh_tree_attention": [_p, _i64, _p, _i64, _p, _i64] + [_p] * 7 + [_i64, _i64, _p] + [_i64] * 11 + [_f32, _i32, _p, _i64, _p],
     "yh_tree_gated_delta_rule": [_p] * 8 + [_i32, _p, _p] + [_i64] * 8 + [_f32, _i32, _i32, _i32, _i32, _p],

@@ -343,12 +343,20 @@ struct SlotArgs {
   const int32_t* tables;
   const int32_t* parents;   // [total] or null: chains
   const int32_t* last;      // [R] or null: every node
+  const uint8_t* served;    // [R] or null: all
   int64_t* slots;           // [total]
   int64_t* kept;            // [R]
   int64_t total;
   Div block, columns;
-  int R;
+  int R, wrap;
 };
+
+// Whether request r, which ends at `end`, has its blocks: an extension served it, and a table that
+// is no ring reaches as far.  Otherwise none of its nodes gets a slot: a held block would take a part
+// of them, and modulo the columns they would go over the rows of its first positions.
+__device__ __forceinline__ bool placed(const SlotArgs& a, int64_t r, int64_t end) {
+  return (!a.served || a.served[r]) && (a.wrap || end <= static_cast<int64_t>(a.block.d) * a.columns.d);
+}
 
 __device__ __forceinline__ int64_t cache_slot(const SlotArgs& a, int64_t r, int64_t pos, int64_t end) {
   if (pos > kMaxLength || passed(pos, end, a.block, a.columns)) return -1;
@@ -365,7 +373,8 @@ __global__ void __launch_bounds__(256) chain_slots_kernel(SlotArgs a) {
     const Span s = tree::span_of(a.cu, t, a.total);
     int64_t n = s.count;
     if (a.last) n = a.last[t] < 0 ? 0 : a.last[t] < n ? a.last[t] + 1 : n;
-    a.kept[t] = clamp_length(a.lengths[t]) + n;
+    const int64_t length = clamp_length(a.lengths[t]);
+    a.kept[t] = placed(a, t, length + n) ? length + n : length;
   }
   if (t >= a.total) return;
   int64_t slot = -1;
@@ -375,7 +384,7 @@ __global__ void __launch_bounds__(256) chain_slots_kernel(SlotArgs a) {
     const int64_t i = t - s.first;
     const int64_t n = a.last && a.last[r] < s.count ? static_cast<int64_t>(a.last[r]) + 1 : s.count;
     const int64_t length = clamp_length(a.lengths[r]);
-    if (i >= 0 && i < n) slot = cache_slot(a, r, length + i, length + n);
+    if (i >= 0 && i < n && placed(a, r, length + n)) slot = cache_slot(a, r, length + i, length + n);
   }
   a.slots[t] = slot;
 }
@@ -412,6 +421,10 @@ __global__ void __launch_bounds__(256) tree_slots_kernel(SlotArgs a) {
       d = o > d ? o : d;
     }
     deep = d;
+  }
+  if (!placed(a, r, length + deep)) {
+    on = false;
+    deep = 0;
   }
   if (lane < n) a.slots[s.first + lane] = on ? cache_slot(a, r, length + __popcll(set) - 1, length + deep) : -1;
   for (int64_t i = n + lane; i < s.count; i += kWave) a.slots[s.first + i] = -1;
@@ -547,6 +560,14 @@ extern "C" int yh_trim_block_tables(const int64_t* lengths, const int64_t* kept,
 extern "C" int yh_slot_map(const int32_t* cu_seqlens, const int64_t* lengths, const int32_t* tables,
                            const int32_t* parents, const int32_t* last, int64_t* slots, int64_t* kept, int64_t n_seqs,
                            int64_t columns, int64_t total, int64_t block, yh_stream_t stream) {
+  return yh_slot_map_served(cu_seqlens, lengths, tables, parents, last, nullptr, slots, kept, n_seqs, columns, total,
+                            block, 1, stream);
+}
+
+extern "C" int yh_slot_map_served(const int32_t* cu_seqlens, const int64_t* lengths, const int32_t* tables,
+                                  const int32_t* parents, const int32_t* last, const uint8_t* served, int64_t* slots,
+                                  int64_t* kept, int64_t n_seqs, int64_t columns, int64_t total, int64_t block,
+                                  int wrap, yh_stream_t stream) {
   using namespace yh;
   YH_CHECK_ARG(n_seqs >= 0 && columns > 0 && total >= 0 && block > 0, "slot_map: bad sizes");
   YH_CHECK_ARG(n_seqs < (1ll << 31) && columns < (1ll << 31) && block < (1ll << 31) && total < (1ll << 31),
@@ -554,9 +575,9 @@ extern "C" int yh_slot_map(const int32_t* cu_seqlens, const int64_t* lengths, co
   if (n_seqs == 0 && total == 0) return YH_OK;
   YH_CHECK_ARG((cu_seqlens && lengths && tables && kept) || n_seqs == 0, "slot_map: null pointer");
   YH_CHECK_ARG(slots || total == 0, "slot_map: null pointer");
-  SlotArgs a{cu_seqlens, lengths, tables, parents, last, slots, kept, total,
+  SlotArgs a{cu_seqlens, lengths, tables, parents, last, served, slots, kept, total,
              tree::make_div(static_cast<uint32_t>(block)), tree::make_div(static_cast<uint32_t>(columns)),
-             static_cast<int>(n_seqs)};
+             static_cast<int>(n_seqs), wrap ? 1 : 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (parents) {
     hipLaunchKernelGGL(tree_slots_kernel, dim3(static_cast<unsigned>(n_seqs / 4 + 1)), dim3(256), 0, st, a);

@@ -380,7 +380,7 @@ def trim_block_tables(lengths, kept, block_tables, free, free_count, block, *, w
               int(bool(wrap)))
 
 
-def slot_map(cu_seqlens, lengths, block_tables, block, total, *, parents=None, last=None):
+def slot_map(cu_seqlens, lengths, block_tables, block, total, *, parents=None, last=None, served=None, wrap=True):
     """Cache slots of the packed nodes of drafted trees: (slots int64 [total],
     kept int64 [R]).  Node i of request r is at position lengths[r] + its depth
     in the tree of ``parents`` (int32 [total], each the request's own earlier
@@ -391,7 +391,14 @@ def slot_map(cu_seqlens, lengths, block_tables, block, total, *, parents=None, l
     one, siblings the same.  Of positions that share a row of a cache that wraps
     the request's last gets the slot, the others -1.  Trees of more than 64
     nodes: -1 for the others.  A ``last`` that is no node of the request: none in
-    a tree, all of a chain where it lies behind its end."""
+    a tree, all of a chain where it lies behind its end.
+
+    The tables must hold the blocks of all of the nodes.  ``served`` (bool [R],
+    as ``extend_block_tables`` returns it) names the requests whose do: the
+    nodes of the others get -1 and their ``kept`` is lengths[r].  So it is, with
+    ``wrap=False`` (tables that are no rings), for a request whose nodes reach
+    past its columns, which would otherwise be the rows of its first
+    positions."""
     dev = _tree.device_of(block_tables)
     total = int(total)
     if total < 0:
@@ -404,10 +411,15 @@ def slot_map(cu_seqlens, lengths, block_tables, block, total, *, parents=None, l
         parents = _tree.ints(parents, torch.int32, dev, "parents", total)
     if last is not None:
         last = _tree.ints(last, torch.int32, dev, "last", n)
+    if served is not None:
+        if served.dtype != torch.bool or served.shape != (n,):
+            raise ValueError(f"served must be bool [{n}]")
+        served = served.to(dev).contiguous()
     slots = torch.empty(total, dtype=torch.int64, device=dev)
     kept = torch.empty(n, dtype=torch.int64, device=dev)
     if n == 0:
         return slots.fill_(-1), kept
-    N.call_on(dev, "yh_slot_map", cu.data_ptr(), lens.data_ptr(), block_tables.data_ptr(), N.ptr(parents), N.ptr(last),
-              slots.data_ptr(), kept.data_ptr(), n, block_tables.shape[1], total, int(block))
+    N.call_on(dev, "yh_slot_map_served", cu.data_ptr(), lens.data_ptr(), block_tables.data_ptr(), N.ptr(parents),
+              N.ptr(last), N.ptr(served), slots.data_ptr(), kept.data_ptr(), n, block_tables.shape[1], total, int(block),
+              int(bool(wrap)))
     return slots, kept
