@@ -792,3 +792,29 @@ def test_served_is_checked(gpu):
     slots, kept = ik.slot_map(*args, served=torch.tensor([False]))       # from the host
     assert slots.tolist() == [-1, -1] and kept.tolist() == [1]
     assert ik.slot_map(*args, served=torch.tensor([True], device=gpu))[0].tolist() == [1, 2]
+
+
+@pytest.mark.parametrize("dtype,kd,vd,most", [(torch.bfloat16, 128, 128, None), (torch.bfloat16, 128, 64, 16),
+                                              (torch.bfloat16, 128, 128, 32), (torch.float32, 128, 128, None),
+                                              (torch.float16, 64, 64, None)])
+@pytest.mark.parametrize("chain", [True, False])
+def test_delta_rule_that_forgets(gpu, dtype, kd, vd, most, chain):
+    """Log decays of -inf, -3e4 and -200 among ordinary ones, one on a path and many: the state is gone there,
+    as it is token by token, and the decays behind them keep their bits."""
+    counts = [min(x, most or 64) for x in (64, 33, 5, 16, 1)]
+    cu, parents = trees(counts, 91, back=2)
+    par = None if chain else parents
+    n, gen = cu[-1], torch.Generator().manual_seed(92)
+    q, k = rnd(1, n, 2, kd, seed=93, dtype=dtype), rnd(1, n, 2, kd, seed=94, dtype=dtype)
+    v, s0 = rnd(1, n, 4, vd, seed=95, dtype=dtype), rnd(5, 4, kd, vd, seed=96, dtype=torch.float32, std=0.3)
+    beta = torch.rand(1, n, 4, generator=gen)
+    g = -torch.rand(1, n, 4, generator=gen)
+    kinds = torch.tensor([-float("inf"), -3e4, -200.0, -104.5, -103.0, -float("inf")])
+    for head in range(4):                      # none, one in ten, half of the nodes, all
+        at = torch.rand(n, generator=gen) < (0.0, 0.1, 0.5, 2.0)[head]
+        g[0, at, head] = kinds[torch.randint(0, 6, (int(at.sum()),), generator=gen)]
+    g[0, 0, 1] = -3e4                          # above a whole request
+    got = gdn.tree_gated_delta_rule(*(x.to(gpu) for x in (q, k, v, g, beta)), None if par is None else i32(par, gpu),
+                                    i32(cu, gpu), s0.to(gpu), max_nodes=most)
+    want, size = ref.delta_rule(q[0], k[0], v[0], g[0], beta[0], par, cu, s0)
+    within(got[0], want, half_step(dtype) * want.abs() + 2.0 ** -12 * size)

@@ -26,16 +26,16 @@ __device__ __forceinline__ Span span_of(const int32_t* cu, int64_t r, int64_t to
 // less than 2^k steps up and `up` the node 2^k steps up (-1: the context).  A
 // parent that is not an earlier node counts as the context.  The sum of `x` along
 // the path is formed with it.
-__device__ __forceinline__ uint64_t ancestors_of(int up, float* x = nullptr) {
+__device__ __forceinline__ uint64_t ancestors_of(int up, double* x = nullptr) {
   const int lane = threadIdx.x & (kWave - 1);
   if (up >= lane || up < 0) up = -1;
   uint64_t set = 1ull << lane;
-  float v = x ? *x : 0.f;
+  double v = x ? *x : 0.;
 #pragma unroll
   for (int step = 0; step < 6; ++step) {
     const int from = up < 0 ? lane : up;
     const uint64_t other = __shfl(set, from, kWave);
-    const float ov = x ? __shfl(v, from, kWave) : 0.f;
+    const double ov = x ? __shfl(v, from, kWave) : 0.;
     const int next = __shfl(up, from, kWave);
     if (up >= 0) {
       set |= other;
@@ -47,7 +47,7 @@ __device__ __forceinline__ uint64_t ancestors_of(int up, float* x = nullptr) {
   return set;
 }
 // The same for the n nodes whose parents are at `parents` (null: a chain).
-__device__ __forceinline__ uint64_t ancestors(const int32_t* parents, int n, float* x = nullptr) {
+__device__ __forceinline__ uint64_t ancestors(const int32_t* parents, int n, double* x = nullptr) {
   const int lane = threadIdx.x & (kWave - 1);
   return ancestors_of(lane >= n ? -1 : parents ? parents[lane] : lane - 1, x);
 }

@@ -10,6 +10,12 @@
 // which is the chunk form of the rule with the ancestor sets in place of the
 // causal triangle: the state is read once for all nodes and no state of a node
 // is ever formed.
+//
+// A decay between two nodes is the exponential of a difference of path sums, from
+// which one strong decay above both must cancel: the sums are held in 64 bits
+// (in 32, g = -3e4 above a node would leave its own decay of -0.2 an error of
+// 8e-4), and a g below -104, whose exponential is 0 in 32 bits, counts as -104, so
+// that -inf forgets the state as it does token by token (-inf + inf would be NaN).
 #include "conv_chan.h"
 #include "tree.h"
 
@@ -36,13 +42,16 @@ __device__ __forceinline__ void fill(void* p, int64_t from, int64_t to, int dt, 
   for (int64_t i = from + threadIdx.x; i < to; i += threads) store_any(p, i, dt, x);
 }
 
+__device__ __forceinline__ double log_decay(float g) { return g < -104.f ? -104.f : g; }   // NaN stays
+
 // Any of the types: fp32 arithmetic on the vector unit, a workgroup a request
 // and value head.
 template <int K, int V>
 __global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
   constexpr int kN = tree::kNodes;
   __shared__ float s_q[kN][K + 1], s_k[kN][K + 1], s_low[kN][kN], s_att[kN][kN], s_u[kN][V];
-  __shared__ float s_g[kN], s_beta[kN];
+  __shared__ double s_g[kN];
+  __shared__ float s_beta[kN];
   __shared__ uint64_t s_set[kN];
   const int tid = threadIdx.x, lane = tid & 63;
   if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(a.R) * a.HV) {   // rows of no request
@@ -61,7 +70,7 @@ __global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
 
   if (tid < 64) {
     const int64_t i = (span.first + (lane < n ? lane : 0)) * a.HV + hv;
-    float gate = lane < n ? load_any(a.g, i, a.g_dt) : 0.f;
+    double gate = lane < n ? log_decay(load_any(a.g, i, a.g_dt)) : 0.;
     const uint64_t set = tree::ancestors(a.parents ? a.parents + span.first : nullptr, n, &gate);
     s_set[lane] = set;
     s_g[lane] = gate;
@@ -93,7 +102,7 @@ __global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
         low = fmaf(s_k[i][c], s_k[j][c], low);
         att = fmaf(s_q[i][c], s_k[j][c], att);
       }
-      const float decay = expf(s_g[i] - s_g[j]);
+      const float decay = expf(static_cast<float>(s_g[i] - s_g[j]));
       low = i == j ? 0.f : low * decay * s_beta[i];
       att *= decay;
     }
@@ -113,7 +122,7 @@ __global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
         ks = fmaf(s_k[i][d], s[d], ks);
         qs = fmaf(s_q[i][d], s[d], qs);
       }
-      const float eg = expf(s_g[i]);
+      const float eg = expf(static_cast<float>(s_g[i]));
       const int64_t row = ((span.first + i) * a.HV + hv) * V + c;
       float u = s_beta[i] * (load_any(a.v, row, a.dt) - eg * ks), o = eg * qs;
       for (int j = 0; j < i; ++j)
@@ -206,7 +215,8 @@ __global__ void __launch_bounds__(64 * W, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(G
   auto& s_low = s_m.low;
   auto& s_att = s_m.att;
   __shared__ float s_diag[kN][20];   // -low's diagonal tiles transposed, then their inverses as split1 words
-  __shared__ float s_g[64], s_beta[64], s_rk[kN], s_rq[kN];
+  __shared__ double s_g[64];
+  __shared__ float s_beta[64], s_rk[kN], s_rq[kN];
   __shared__ uint64_t s_set[64];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n16 = lane & 15, quad = lane >> 4;
@@ -276,9 +286,9 @@ __global__ void __launch_bounds__(64 * W, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(G
       vv[t][e] = *reinterpret_cast<const vcol*>(static_cast<const uint16_t*>(a.v) + ((span.first + (i < n ? i : 0)) * a.HV + hv) * V + col);
     }
   if (w == 0) {
-    const uint64_t set = tree::ancestors_of(up, &gate);
-    s_set[lane] = set;
-    s_g[lane] = gate;
+    double sum = log_decay(gate);
+    s_set[lane] = tree::ancestors_of(up, &sum);
+    s_g[lane] = sum;
     s_beta[lane] = beta;
   }
 #pragma unroll
@@ -371,12 +381,13 @@ __global__ void __launch_bounds__(64 * W, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(G
     const int pair = W * x + w, ta = tile_a(pair), tb = pair - ta * (ta + 1) / 2;
     if (pair >= kPairs || ta >= nt) continue;
     const int j = 16 * tb + n16;
-    const float rkj = s_rk[j], gj = s_g[j];
+    const float rkj = s_rk[j];
+    const double gj = s_g[j];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = 16 * ta + 4 * quad + e;
       const bool above = (s_set[i] >> j) & 1;
-      const float f = above ? __expf(s_g[i] - gj) * rkj : 0.f;
+      const float f = above ? __expf(static_cast<float>(s_g[i] - gj)) * rkj : 0.f;
       kk[x][e] = above && i != j ? -s_beta[i] * s_rk[i] * f * kk[x][e] : 0.f;
       if (ta != tb) s_low[i][j] = split1(kk[x][e]);
       s_att[i][j] = above ? split1(s_rq[i] * f * qk[x][e]) : 0u;
@@ -417,7 +428,7 @@ __global__ void __launch_bounds__(64 * W, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(G
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = 16 * b + 4 * quad + e;
-      ge[e] = __expf(s_g[i]);
+      ge[e] = __expf(static_cast<float>(s_g[i]));
       bt[e] = s_beta[i];
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
