@@ -818,3 +818,58 @@ def test_delta_rule_that_forgets(gpu, dtype, kd, vd, most, chain):
                                     i32(cu, gpu), s0.to(gpu), max_nodes=most)
     want, size = ref.delta_rule(q[0], k[0], v[0], g[0], beta[0], par, cu, s0)
     within(got[0], want, half_step(dtype) * want.abs() + 2.0 ** -12 * size)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_the_accepted_paths_advance_states_and_windows(gpu, dtype):
+    """The second half of a step: the conv window and the recurrent state that decoding the accepted path would
+    leave, from the prefill's operators over the accepted rows; then a second draft from that state.
+
+    The states agree with float64 as the prefill's do (1e-3 of their norm), and a float16 one is rounded once
+    (2^-11).  The second draft reads such a state: its error reaches the outputs in that share of the terms."""
+    s, cu, parents, lengths, block = _step(gpu, 91)
+    s["state"] = s["state"].to(dtype)
+    start, n = s["state"].clone(), cu[-1]
+    x = layers.conv_tree(s["proj"], s["window"], s["conv_w"], s["parents"], s["cu"], 3 * 512, planes=3)
+    slots, served = ik.extend_block_tables(s["lengths"], s["cu"], s["tables"], s["free"], s["count"], block, n)
+    slots, kept = ik.slot_map(s["cu"], s["lengths"], s["tables"], block, n, parents=s["parents"], last=s["last"],
+                              served=served)
+    paths = [ref.paths(parents[a:b], b - a)[last] if last >= 0 else []
+             for a, b, last in zip(cu, cu[1:], s["last"].tolist())]
+    rows, cu_kept = (slots >= 0).nonzero()[:, 0], ik.cu_seqlens(kept - s["lengths"])
+    assert rows.tolist() == [a + j for a, p in zip(cu, paths) for j in p] and min(map(len, paths)) == 0
+    window = s["window"].clone()
+    q, k, v = layers.conv_prefill(s["proj"][rows], window, s["conv_w"], cu_kept, 3 * 512, planes=3)
+    for have, tree in zip((q, k, v), x):     # the rows that the draft saw
+        within(have, tree[rows].double().cpu(), 2.0 ** -7 * tree[rows].double().cpu().abs() + 2.0 ** -14)
+    _, new = gdn.chunk_gated_delta_rule(q.view(1, -1, 4, 128), k.view(1, -1, 4, 128), v.view(1, -1, 4, 128),
+                                        g=s["g"][:, rows], beta=s["beta"][:, rows], initial_state=s["state"].float(),
+                                        output_final_state=True, use_qk_l2norm_in_kernel=True, cu_seqlens=cu_kept)
+    s["state"].copy_(new)
+    share = 1e-3 + (2.0 ** -11 if dtype == torch.float16 else 0)
+    gates, beta = s["g"][0].double().cpu(), s["beta"][0].double().cpu()
+    q, k, v = (t.view(-1, 4, 128).double().cpu() for t in (q, k, v))
+    k = k / torch.sqrt((k * k).sum(-1, keepdim=True) + 1e-6)
+    exact, at = [], 0
+    for r, path in enumerate(paths):
+        taps = torch.cat((s["window"][r], s["proj"][[cu[r] + j for j in path]][:, :3 * 512]))[-3:]
+        assert torch.equal(window[r], taps), r
+        state = start[r].double().cpu()
+        for j in path:
+            state = state * torch.exp(gates[cu[r] + j])[:, None, None]
+            delta = beta[cu[r] + j][:, None] * (v[at] - torch.einsum("hk,hkv->hv", k[at], state))
+            state = state + k[at][:, :, None] * delta[:, None]
+            at += 1
+        exact.append(state)
+        assert (s["state"][r].double().cpu() - state).norm() <= share * state.norm(), r
+    assert at == len(rows)
+    draft = [rnd(1, 40, 4, 128, seed=i).to(gpu) for i in (1, 2, 3)]
+    gb = [-torch.rand(1, 40, 4, device=gpu), torch.rand(1, 40, 4, device=gpu)]
+    off, par = [0, 8, 16, 24, 32, 40], trees([8] * 5, 7)[1]
+    got = gdn.tree_gated_delta_rule(*draft, *gb, i32(par, gpu), i32(off, gpu), s["state"])
+    want, size = ref.delta_rule(*(t[0].cpu() for t in (*draft, *gb)), par, off, torch.stack(exact))
+    # decay and I - beta k k^T do not lengthen an error of the state, and q (norm 1, times scale) reads it
+    reach = torch.stack([x.norm(dim=(1, 2)) for x in exact]).repeat_interleave(8, 0)[..., None] * 128 ** -0.5
+    # (the bound on the state holds for all heads together: a head may have all of it)
+    reach = reach.norm(dim=1, keepdim=True)
+    within(got[0], want, share * reach + half_step(torch.bfloat16) * want.abs() + 2.0 ** -12 * size)

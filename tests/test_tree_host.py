@@ -208,3 +208,14 @@ def test_served_slots_refuse_before_device_work(lib):
     assert lib.yh_slot_map_served(p, p, p, None, None, p, p, p, 1, 0, 4, 16, 0, None) == -1
     assert b"bad sizes" in lib.yh_last_error()
     assert lib.yh_slot_map_served(None, None, None, None, None, None, None, None, 0, 1, 0, 16, 0, None) == 0
+
+
+def test_the_recurrence_refuses_packed_sequences():
+    """It has no offsets: the requests' tokens would run one after another into the first state row."""
+    x, gate = torch.zeros(1, 5, 2, 128, dtype=torch.bfloat16), torch.zeros(1, 5, 2)
+    for f in (gdn.recurrent_gated_delta_rule, gdn.fused_recurrent_gated_delta_rule):
+        with pytest.raises(ValueError, match="chunk_gated_delta_rule"):
+            f(x, x, x, g=gate, beta=gate, initial_state=torch.zeros(2, 2, 128, 128), cu_seqlens=torch.tensor([0, 3, 5]))
+        for one in (None, torch.tensor([0, 5])):       # as ever: a single sequence
+            with pytest.raises(ValueError, match="ROCm device"):
+                f(x, x, x, g=gate, beta=gate, initial_state=torch.zeros(1, 2, 128, 128), cu_seqlens=one)

@@ -32,8 +32,12 @@ def recurrent_gated_delta_rule(query, key, value, g=None, beta=None, initial_sta
     adapters.  Returns ``(o [B, T, HV, V], state)``; ``state`` is
     ``initial_state`` itself (updated in place) unless ``inplace=False``, or a
     new zero-initialised tensor when ``initial_state`` is None.  With
-    ``output_final_state=False`` the second element is None.
+    ``output_final_state=False`` the second element is None.  A batch row is one
+    sequence: packed sequences (``cu_seqlens``) are ``chunk_gated_delta_rule``'s.
     """
+    if unused.get("cu_seqlens") is not None and len(unused["cu_seqlens"]) > 2:   # would run on as one sequence
+        raise ValueError("recurrent_gated_delta_rule takes one sequence a batch row; packed sequences (cu_seqlens) "
+                         "go through chunk_gated_delta_rule")
     if g is None or beta is None:
         raise ValueError("recurrent_gated_delta_rule needs g and beta")
     if query.ndim != 4 or key.shape != query.shape or value.ndim != 4:
@@ -205,9 +209,10 @@ def tree_gated_delta_rule(query, key, value, g, beta, parents, cu_seqlens, initi
     ``initial_state`` ``[rows, HV, K, V]`` (float32 or float16): row r, or
     ``state_indices[r]`` (int ``[R]``; a row outside the state, as -1: no
     request, zeros).  Returns o ``[1, N, HV, V]``; rows behind the last request
-    are zeros.  The state is NOT updated: run the accepted path through
-    ``chunk_gated_delta_rule`` or ``recurrent_gated_delta_rule`` once it is
-    known.  ``max_nodes``: the most nodes of any request (default 64); a node
+    are zeros.  The state is NOT updated: once the accepted paths are known,
+    ``chunk_gated_delta_rule`` runs their rows, packed (its ``cu_seqlens``), from
+    the requests' states (float32: a float16 pool is widened for it) and returns
+    the states after them, which go back into the pool.  ``max_nodes``: the most nodes of any request (default 64); a node
     past it comes back as not-a-number."""
     if query.ndim != 4 or key.shape != query.shape or value.ndim != 4 or query.shape[0] != 1:
         raise ValueError("query/key must be [1, N, H, K] and value [1, N, HV, V]")
