@@ -12,11 +12,13 @@ output's type, torch.finfo(t).eps / 2):
   the products' size).
 * tables, slots and copies are exact.
 """
+from dataclasses import fields
+
 import pytest
 import torch
 
 from oracle import tree as ref
-from yanchor_amd import gdn, layers
+from yanchor_amd import gdn, layers, workloads
 from yanchor_amd import independent_memory as im
 from yanchor_amd import inference_kernels as ik
 
@@ -873,3 +875,24 @@ def test_the_accepted_paths_advance_states_and_windows(gpu, dtype):
     # (the bound on the state holds for all heads together: a head may have all of it)
     reach = reach.norm(dim=1, keepdim=True)
     within(got[0], want, share * reach + half_step(torch.bfloat16) * want.abs() + 2.0 ** -12 * size)
+
+
+@pytest.mark.parametrize("pending", [0, 40, 59, 63])
+def test_anchor_reads_of_a_draft_end_at_the_commit(gpu, pending):
+    """A drafted path's reads of the memory as it is before the step are decode's reads down to the token that
+    fills the chunk; the tokens behind it read another memory."""
+    chunk, n = 64, 12
+    memory = workloads.anchor_state(2, 2, 16, chunk, 128, seed=pending + 1, fill_pending=pending)
+    state = im.IndependentMemoryState(*(getattr(memory, f.name).to(gpu) for f in fields(memory)))
+    q = rnd(n, 1, 8, 128, seed=pending + 2).to(gpu)
+    k, v = (rnd(n, 1, 2, 128, seed=pending + s).to(gpu) for s in (3, 4))
+    draft = im.committed_gqa(q, state, i32([1] * n, gpu)).double().cpu()
+    for t in range(n):
+        read = im.committed_gqa(q[t:t + 1], state, i32([1], gpu)).double().cpu()[0]
+        off = (draft[t] - read).norm() / read.norm()
+        if t <= chunk - 1 - pending:       # two roundings to bf16, and sums in another order
+            assert off <= 2 * 2.0 ** -8, t
+        else:
+            assert off > 0.1, t
+        im.commit_decode(k[t:t + 1], v[t:t + 1], torch.full((1, 1, 2), 9.0, device=gpu), torch.tensor([True], device=gpu),
+                         chunk, state, i32([1], gpu))
