@@ -896,3 +896,43 @@ def test_anchor_reads_of_a_draft_end_at_the_commit(gpu, pending):
             assert off > 0.1, t
         im.commit_decode(k[t:t + 1], v[t:t + 1], torch.full((1, 1, 2), 9.0, device=gpu), torch.tensor([True], device=gpu),
                          chunk, state, i32([1], gpu))
+
+
+def test_offsets_past_the_rows_are_those_clamped(gpu):
+    """Offsets below 0 and past the rows give the results of the clamped ones in every operator; offsets that
+    fall give slots of the requests' own blocks or none, and take no block that is not on the stack."""
+    n, block = 9, 16
+    lens = torch.tensor([20, 30], device=gpu)
+    x, w, proj = rnd(1, n, 2, 128, seed=5).to(gpu), rnd(2, 3, 48, seed=6).to(gpu), rnd(n, 48, seed=7).to(gpu)
+    taps, g = rnd(48, 4, seed=8).to(gpu), torch.rand(1, n, 2, generator=torch.Generator().manual_seed(9)).to(gpu)
+    state = rnd(2, 2, 128, 128, seed=10, dtype=torch.float32).to(gpu)
+    par, last = i32([-1, 0, 0, 1, 2, -1, 0, 1, 1], gpu), i32([3, 2], gpu)
+
+    def run(cu):
+        cu, tables = i32(cu, gpu), i32([[0, 1, -1], [2, 3, -1]], gpu)
+        free, count = i32([7, 5, 4, -1], gpu), i32([3], gpu)
+        out = []
+        for y in (x, x.float()):
+            for most in (None, 8):
+                out.append(gdn.tree_gated_delta_rule(y, y, y, -g, g, par, cu, state, max_nodes=most))
+        for c, p in ((48, 3), (45, 1)):
+            out.append(layers.conv_tree(proj, w[..., :c].contiguous(), taps[:c], par, cu, c, planes=p))
+        for parents in (par, None):
+            for at in (None, last):
+                out += ik.slot_map(cu, lens, tables, block, n, parents=parents, last=at)
+        out += ik.extend_block_tables(lens, cu, tables, free, count, block, n)
+        return out + [tables, free, count]
+    want = run([0, 5, 9])
+    for got, exact in zip(run([-3, 5, 4000]), want):
+        assert torch.equal(got, exact)
+    out = run([0, 7, 3])
+    tables, free, count = (t.tolist() for t in out[-3:])
+    assert 0 <= count[0] <= 3 and free == [7, 5, 4, -1]
+    taken = {7, 5, 4} - set(free[:count[0]])
+    held = [{0, 1} | taken, {2, 3} | taken]
+    for row, own in zip(tables, held):
+        assert set(row) - {-1} <= own
+    for slots in (*out[6:14:2], out[14]):
+        assert slots.shape == (n,)
+        assert all(s == -1 or s // block in {0, 1, 2, 3} | taken for s in slots.tolist())
+    assert all(s == -1 or s // block in held[0] for s in out[14].tolist()[:7]) and out[14].tolist()[7:] == [-1, -1]
