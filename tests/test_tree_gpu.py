@@ -18,6 +18,7 @@ import pytest
 import torch
 
 from oracle import tree as ref
+from yanchor_amd import _native as N
 from yanchor_amd import gdn, layers, workloads
 from yanchor_amd import independent_memory as im
 from yanchor_amd import inference_kernels as ik
@@ -936,3 +937,41 @@ def test_offsets_past_the_rows_are_those_clamped(gpu):
         assert slots.shape == (n,)
         assert all(s == -1 or s // block in {0, 1, 2, 3} | taken for s in slots.tolist())
     assert all(s == -1 or s // block in held[0] for s in out[14].tolist()[:7]) and out[14].tolist()[7:] == [-1, -1]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_rows_behind_the_last_request(gpu, dtype):
+    """A step that is captured for its largest batch: most packed rows belong to no request.  They are zeros,
+    those of the requests what they are without them, whatever was in the memory."""
+    n, pad = 11, 9001
+    cu = i32([0, 4, 4, n], gpu)
+    q, k, v = (torch.nn.functional.pad(rnd(n, h, 128, seed=h + s), (0, 0, 0, 0, 0, pad), value=NAN).to(gpu)
+               for s, h in ((1, 8), (2, 2), (3, 2)))
+    cache = rnd(6, 2, 16, 128, seed=4).to(gpu)
+    args = (torch.tensor([20, 3, 32], device=gpu), cache, cache, i32([[0, 1], [2, 3], [4, 5]], gpu))
+    state, gates = rnd(3, 8, 128, 128, seed=5, dtype=torch.float32).to(gpu), torch.rand(1, n + pad, 8, device=gpu)
+    proj, window, taps = q.reshape(n + pad, 1024), rnd(3, 3, 1024, seed=6).to(gpu), rnd(1024, 4, seed=7).to(gpu)
+
+    def run(rows, cu):
+        x = q[None, :rows].to(dtype)
+        stale = [torch.full((rows, 1024), NAN, device=gpu, dtype=t) for t in (dtype, torch.bfloat16, torch.bfloat16)]
+        del stale
+        out = []
+        for most in (None, 8):
+            out.append(layers.tree_attention(q[:rows], k[:rows], v[:rows], None, cu, *args, max_nodes=most))
+            out.append(gdn.tree_gated_delta_rule(x, x, x, -gates[:, :rows], gates[:, :rows], None, cu, state, max_nodes=most)[0])
+        out.append(layers.conv_tree(proj[:rows], window, taps, None, cu, 1024))
+        return out
+    for got, want in zip(run(n + pad, cu), run(n, cu)):
+        assert torch.equal(got[:n], want) and not got[n:].any()
+    none = (torch.zeros(0, dtype=torch.int64, device=gpu), cache, cache, torch.zeros(0, 2, dtype=torch.int32, device=gpu))
+    assert not layers.tree_attention(q, k, v, None, i32([0], gpu), *none).any()
+    # outputs off 16-byte alignment, from the C call
+    store, x = torch.full((1 + (n + pad) * 1024 * 4 // dtype.itemsize,), NAN, device=gpu, dtype=dtype), q.to(dtype)
+    off = 2 if dtype == torch.bfloat16 else 1
+    N.call_on(gpu, "yh_tree_gated_delta_rule", *[x.data_ptr()] * 3, gates.data_ptr(), gates.data_ptr(), None, cu.data_ptr(),
+              state.data_ptr(), N.F32, None, store.data_ptr() + 4, 3, n + pad, 8, 8, 128, 128, 3, 64, 1.0, 1,
+              N.code(x), N.F32, N.F32)
+    rows = store[off:off + (n + pad) * 1024].view(n + pad, 1024)
+    assert rows[:n].isfinite().all() and not rows[n:].any()
+    assert store[:off].isnan().all() and store[off + (n + pad) * 1024:].isnan().all()

@@ -53,6 +53,7 @@ struct TreeArgs {
   int R, H, G, NB, max_nodes, mtiles;
   int gate8;               // gate rows keep 8-byte alignment
   float scale;
+  unsigned clear;          // workgroups at the end of the grid that clear the rows of no request
   // the cut: parts aimed at, and for requests [0, R] the first part, the first partial sum
   int target, slot_rows;   // target 0: no item is cut
   int32_t* first;          // [R + 1]
@@ -279,9 +280,9 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
   __shared__ int s_deep;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  if (blockIdx.x == gridDim.x - 1) {   // rows of no request
-    const int64_t end = a.R ? a.cu[a.R] : 0, row = static_cast<int64_t>(a.H) * D;
-    for (int64_t i = (end < 0 ? 0 : end) * row + threadIdx.x; i < a.total * row; i += NW * 64) a.out[i] = 0;
+  if (blockIdx.x >= gridDim.x - a.clear) {   // rows of no request
+    tree::clear_rows<NW * 64>(a.out, a.cu, a.R, a.total, static_cast<int64_t>(a.H) * D * 2,
+                              blockIdx.x - (gridDim.x - a.clear), a.clear);
     return;
   }
   Part part;
@@ -729,7 +730,7 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
              gate_head_stride, static_cast<uint16_t*>(out), total, window,
              tree::make_div(static_cast<uint32_t>(block)), tree::make_div(static_cast<uint32_t>(columns)),
              tree::make_div(static_cast<uint32_t>(rep)), (int)n_seqs, (int)H, (int)G, (int)blocks, (int)max_nodes,
-             (int)mtiles, gate8 ? 1 : 0, scale, (int)target, (int)(max_nodes * rep < rows ? max_nodes * rep : rows),
+             (int)mtiles, gate8 ? 1 : 0, scale, static_cast<unsigned>(tree::clearing(total, H * D * 2)), (int)target, (int)(max_nodes * rep < rows ? max_nodes * rep : rows),
              nullptr, nullptr, nullptr, nullptr};
   if (need) {
     char* sums = static_cast<char*>(workspace) + plan_bytes(n_seqs);
@@ -738,7 +739,7 @@ extern "C" int yh_tree_attention(const void* q, int64_t q_stride, const void* k,
     a.part = reinterpret_cast<float*>(sums);
     a.stat = reinterpret_cast<float2*>(sums + target * 2 * a.slot_rows * D * 4);
   }
-  const unsigned grid = static_cast<unsigned>(target + items + 1);   // the last clears the rows of no request
+  const unsigned grid = static_cast<unsigned>(target + items) + a.clear;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == YH_BF16) {
     if (D == 128) launch<YH_BF16, 128>(a, (int)rows, grid, st);

@@ -38,10 +38,6 @@ struct GdnArgs {
   float scale;
 };
 
-__device__ __forceinline__ void fill(void* p, int64_t from, int64_t to, int dt, float x, int threads) {
-  for (int64_t i = from + threadIdx.x; i < to; i += threads) store_any(p, i, dt, x);
-}
-
 __device__ __forceinline__ double log_decay(float g) { return g < -104.f ? -104.f : g; }   // NaN stays
 
 // Any of the types: fp32 arithmetic on the vector unit, a workgroup a request
@@ -54,9 +50,9 @@ __global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
   __shared__ float s_beta[kN];
   __shared__ uint64_t s_set[kN];
   const int tid = threadIdx.x, lane = tid & 63;
-  if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(a.R) * a.HV) {   // rows of no request
-    const int64_t end = a.R ? a.cu[a.R] : 0, row = static_cast<int64_t>(a.HV) * V;
-    fill(a.o, (end < 0 ? 0 : end) * row, a.total * row, a.dt, 0.f, 256);
+  if (blockIdx.x >= static_cast<unsigned>(a.R * a.HV)) {   // rows of no request
+    tree::clear_rows<256>(a.o, a.cu, a.R, a.total, static_cast<int64_t>(a.HV) * V * (a.dt == YH_F32 ? 4 : 2),
+                          blockIdx.x - a.R * a.HV, gridDim.x - a.R * a.HV);
     return;
   }
   const int hv = blockIdx.x % a.HV, r = blockIdx.x / a.HV, h = hv / (a.HV / a.H);
@@ -221,9 +217,9 @@ __global__ void __launch_bounds__(64 * W, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(G
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n16 = lane & 15, quad = lane >> 4;
   uint16_t* out = static_cast<uint16_t*>(a.o);
-  if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(a.R) * a.HV) {   // rows of no request
-    const int64_t end = a.R ? a.cu[a.R] : 0, row = static_cast<int64_t>(a.HV) * V;
-    for (int64_t i = (end < 0 ? 0 : end) * row + tid; i < a.total * row; i += TH) out[i] = 0;
+  if (blockIdx.x >= static_cast<unsigned>(a.R * a.HV)) {   // rows of no request
+    tree::clear_rows<TH>(out, a.cu, a.R, a.total, static_cast<int64_t>(a.HV) * V * 2, blockIdx.x - a.R * a.HV,
+                         gridDim.x - a.R * a.HV);
     return;
   }
   const int hv = blockIdx.x % a.HV, r = blockIdx.x / a.HV, h = hv / (a.HV / a.H);
@@ -639,7 +635,7 @@ extern "C" int yh_tree_gated_delta_rule(const void* q, const void* k, const void
                "tree_gated_delta_rule: sizes too large");
   GdnArgs a{q, k, v, g, beta, parents, cu_seqlens, state, state_indices, o, total, n_state_rows, (int)n_seqs, (int)H,
             (int)HV, (int)max_nodes, use_qk_l2norm ? 1 : 0, qkv_dtype, g_dtype, beta_dtype, state_dtype, scale};
-  const unsigned grid = static_cast<unsigned>(n_seqs * HV + 1);   // the last clears the rows of no request
+  const unsigned grid = static_cast<unsigned>(n_seqs * HV + tree::clearing(total, HV * V * (qkv_dtype == YH_F32 ? 4 : 2)));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool mfma = K == 128 && qkv_dtype == YH_BF16 && tree::aligned16(q) && tree::aligned16(k) &&
                     tree::aligned16(state) && ((reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o)) & 3) == 0;
