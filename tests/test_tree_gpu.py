@@ -975,3 +975,21 @@ def test_many_rows_behind_the_last_request(gpu, dtype):
     rows = store[off:off + (n + pad) * 1024].view(n + pad, 1024)
     assert rows[:n].isfinite().all() and not rows[n:].any()
     assert store[:off].isnan().all() and store[off + (n + pad) * 1024:].isnan().all()
+
+
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 40])
+@pytest.mark.parametrize("columns", [3, 255, 256, 257])
+def test_trim_around_one_launch(gpu, n, columns):
+    """Both forms of the trim where they meet: some requests whole, some in part, some not served, some longer
+    than what is kept."""
+    block, gen = 8, torch.Generator().manual_seed(n * columns)
+    tables = torch.randperm(n * columns, generator=gen).view(n, columns).to(torch.int32)
+    tables[torch.rand(n, columns, generator=gen) < 0.1] = -1
+    lengths = torch.randint(0, block * columns + 1, (n,), generator=gen)
+    kept = (lengths * torch.randint(0, 4, (n,), generator=gen) // 2).tolist()     # half of them as long or longer
+    lengths, want = lengths.tolist(), tables.tolist()
+    free = list(range(10 ** 6, 10 ** 6 + 5)) + [-1] * (n * columns)
+    t_dev, f_dev, c_dev = tables.to(gpu), i32(free, gpu), i32([5], gpu)
+    ik.trim_block_tables(torch.tensor(lengths, device=gpu), torch.tensor(kept, device=gpu), t_dev, f_dev, c_dev, block)
+    count = ref.trim(lengths, kept, want, free, 5, block)
+    assert t_dev.tolist() == want and c_dev.item() == count and f_dev.tolist() == free

@@ -15,9 +15,9 @@
 // workgroups run, and trimming takes an extension back.
 //
 // The tables move a few bytes a request and are bound by latency (128 requests:
-// extend 7.0 us, slots 3.5, trim 3.1 and 3.8), so launches are few: extend writes
+// extend 7.1 us, slots 3.7, trim 3.1 and 3.8), so launches are few: extend writes
 // the slots in its one launch when the tokens are few, trim takes one launch for
-// small tables.
+// few requests with short tables.
 #include "tree.h"
 
 namespace yh {
@@ -247,32 +247,27 @@ __device__ __forceinline__ void give_back(const TrimArgs& a, int32_t* row, int l
   }
 }
 
-// One workgroup, R <= kThreads: a wave a request.
+// One workgroup, R <= kWaves: a wave a request.
 __global__ void __launch_bounds__(kThreads) trim_kernel(TrimArgs a) {
-  __shared__ int32_t s_n[kThreads], s_first[kThreads];
-  const int w = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  for (int r = w; r < a.R; r += kWaves) {
-    int lo, hi;
-    trim_range(a, r, &lo, &hi);
-    const int n = count_blocks(a.tables + static_cast<int64_t>(r) * a.columns, lo, hi);
-    if (lane == 0) s_n[r] = n;
-  }
+  __shared__ int s_n[kWaves];
+  const int r = threadIdx.x / kWave;
+  int lo, hi;
+  trim_range(a, r, &lo, &hi);
+  int32_t* row = a.tables + static_cast<int64_t>(r) * a.columns;
+  const int n = count_blocks(row, lo, hi);
+  if ((threadIdx.x & (kWave - 1)) == 0) s_n[r] = n;
   const int32_t top = clamp_count(a.count, a.n_free);
   __syncthreads();
-  int64_t all = 0;
-  const int64_t off = scan(static_cast<int>(threadIdx.x) < a.R ? s_n[threadIdx.x] : 0, &all);
-  s_first[threadIdx.x] = static_cast<int32_t>(off);
-  __syncthreads();
-  for (int r = w; r < a.R; r += kWaves) {
-    if (s_n[r] == 0) continue;
-    int lo, hi;
-    trim_range(a, r, &lo, &hi);
-    give_back(a, a.tables + static_cast<int64_t>(r) * a.columns, lo, hi, s_first[r], top + all);
+  int64_t all = 0, first = 0;
+  for (int i = 0; i < a.R; ++i) {
+    first += i < r ? s_n[i] : 0;
+    all += s_n[i];
   }
+  if (n) give_back(a, row, lo, hi, first, top + all);
   if (threadIdx.x == 0) *a.count = static_cast<int32_t>(top + all < a.n_free ? top + all : a.n_free);
 }
 
-// Large tables: kSplit waves a request, a share of its columns each.  plan: the
+// More requests, or long tables: kSplit waves a request, a share of its columns each.  plan: the
 // requests' counts, the waves', and the stack's height before.
 constexpr int kSplit = 8;
 __device__ __forceinline__ void wave_range(const TrimArgs& a, int64_t r, int* lo, int* hi) {
@@ -488,9 +483,10 @@ namespace yh {
 namespace {
 // One launch where one workgroup can do it all: few tokens after the requests ...
 bool extend_in_one(int64_t n_seqs, int64_t total) { return n_seqs <= kThreads && total <= 4096; }
-// ... or tables of which one workgroup takes back all in about the second launch's time.  (128 tables
-// of 1000 columns: a few blocks each 13.9 us in one launch, 15.0 in two; all of them 86 and 21.)
-bool trim_in_one(int64_t n_seqs, int64_t columns) { return n_seqs <= kThreads && n_seqs * columns <= 16 * kThreads; }
+// ... or a wave for every request, with columns that it takes in one step.  (us in a captured step, one launch and
+// two: 1 table 5.8 and 6.6; 16 tables of 256 columns 7.6 and 7.8 with all blocks back, 6.4 and 7.5 with few; 16 of 1000
+// 13.7 and 8.3 with all; a workgroup that takes 32 requests in turn 8.1 and 7.6, 128 20 and 8, 512 68 and 9.)
+bool trim_in_one(int64_t n_seqs, int64_t columns) { return n_seqs <= kWaves && columns <= kDeep * kWave; }
 }  // namespace
 }  // namespace yh
 
@@ -547,7 +543,7 @@ extern "C" int yh_trim_block_tables(const int64_t* lengths, const int64_t* kept,
              static_cast<int>(block), static_cast<int>(columns), static_cast<int>(n_seqs), wrap ? 1 : 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (trim_in_one(n_seqs, columns)) {
-    hipLaunchKernelGGL(trim_kernel, dim3(1), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(trim_kernel, dim3(1), dim3(static_cast<unsigned>(n_seqs * kWave)), 0, st, a);
   } else {
     hipLaunchKernelGGL(trim_count_kernel, dim3(static_cast<unsigned>(n_seqs)), dim3(kSplit * kWave), 0, st, a);
     YH_CHECK_LAUNCH("trim_block_tables count");
