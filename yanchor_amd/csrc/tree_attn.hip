@@ -20,10 +20,10 @@
 // with their maximum, and a second launch joins them in order.
 //
 // Few rows are bound by HBM, which the copies of four workgroups a CU keep at
-// 5.1 to 5.6 TB/s (128 full rings: 478 MB in 91 us; 64 block tables: 732 MB in
-// 131 us).  256 rows and more a KV head are bound by the tiles' products and
-// softmax: 516 GFLOP in 745 us, 0.69 PFLOP/s; the copies alone take 376 of them,
-// the products alone 549.
+// 5.1 to 5.6 TB/s (128 rings of 1024 slots, a third of them not full: 478 MB in
+// 91 us; 64 block tables: 732 MB in 131 us).  256 rows and more a KV head are bound
+// by the tiles' products and softmax: 516 GFLOP in 724 to 771 us from run to run,
+// 0.7 PFLOP/s; the copies alone take 376 of 745, the products alone 549.
 #include <type_traits>
 
 #include "attn_tile.h"
@@ -253,6 +253,11 @@ __device__ __forceinline__ void put4(const TreeArgs& a, int64_t row, int head, i
 // ids that come through LDS as the copies do, a window ahead (a load into
 // registers would have its wait drain the copies).  Resolved row by row in every
 // tile instead: 767 us for 746 at 8 long contexts.
+//
+// Other blocks (not RUNS) load their ids into registers in every tile, whose wait
+// drains the copies in flight, and with D = 128 spill 11 to 26 vector registers:
+// 64 block tables of blocks of 15 take 430 us, of 16 142; 8 long contexts in blocks
+// of one token 1909, of 64 768.
 template <int NW>
 struct Pipe {
   static constexpr int S = NW == 8 ? 8 : NW == 4 ? 4 : 2;
@@ -471,6 +476,9 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
         const int wskip = min(max(wfrom - p0, 0), 64);
         keep = t < ctx ? (wskip > 63 ? 0 : there & (~0ull << wskip)) : wsee;
       }
+      // The weights enter the product rounded to the type's 16 bits, as in the window prefill: eps / 2 of each
+      // (sum p |v| eps / 2, as much as the output's own rounding where values have one sign).  As hi + lo pairs
+      // they take a second matrix instruction: 8 long contexts 950 us for 768, 128 rings 105 for 97.
       st.template step<false, edge.value, true>(c, stage[q % S], k2, keep);
     }
     if constexpr (!P::kEarly) issue(q + S - 1);
@@ -479,7 +487,7 @@ __global__ void __launch_bounds__(NW * 64, 2) tree_attention_kernel(TreeArgs a) 
     if ((t & 3) == 0) there_now = there_next;
   };
   // Tiles whose keys all rows see and the others take a loop each: as branches
-  // of one loop they spill (the waves' conditions may differ: both loops pass
+  // of one loop the RUNS kernels spill vector registers too (the waves' conditions may differ: both loops pass
   // two barriers a tile).
   while (t < tiles) {
 #pragma unroll 1

@@ -153,10 +153,14 @@ __global__ void __launch_bounds__(256) tree_gdn_any_kernel(GdnArgs a) {
 // product of a 0 in the mask with it would spread it: such elements enter the
 // products as 0 and their bits (`bad`) turn the descendants' outputs into NaN.
 //
-// Bound by the chain of a workgroup's phases (norms, products of the keys, the
-// inverses, the state's products, the tiles one after another), which three
-// workgroups a CU overlap with the read of each other's state: 421 MB in 110 us,
-// 3.8 TB/s (two a CU: 156 for 136 before the phases were shortened).
+// Bound by the chain of a workgroup's phases (the loads of q and k, the state's
+// read and products, the masks' products, the inverses, the tiles one after
+// another), which three workgroups a CU overlap with the read of each other's
+// state: 421 MB in 110 us, 3.8 TB/s (two a CU: 156 for 136 before the phases were
+// shortened).  Part of the chain are waits that the loads' order does not ask for:
+// a request of fewer nodes than rows zeroes q and k behind each load, which waits
+// for it, and with four tiles, V = 128 and a float32 state 5 registers spill, three
+// of them just loaded.  Of up to 16 nodes, one tile, 71 us; float16 state 105.
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -233,7 +237,7 @@ __global__ void __launch_bounds__(64 * W, T == 4 ? 3 : 4) tree_gdn_mfma_kernel(G
   if (n == 0) return;
   const int nt = (n + 15) >> 4;
 
-  // q and k rows (a thread a piece of a row), then the state, which arrives behind them
+  // q and k rows (a thread a piece of a row), then the state
   constexpr int kRows = TH / 16, kLoads = (kN + kRows - 1) / kRows;
   uint4 rq[kLoads], rk[kLoads];
 #pragma unroll
