@@ -910,7 +910,8 @@ int yh_tree_attention(const void* q, int64_t q_stride, const void* k, int64_t k_
 /*
  * The gated delta rule of the nodes: each node's state is its parent's (the
  * request's, for a node that follows the context) under yh_gdn_recurrent's
- * step; o [total, HV, V] is its output.  No state is written.
+ * step; o [total, HV, V] is its output.  No state is written.  A g below -104
+ * (e^g is 0 in float32), as -inf, forgets the state.
  *   q, k [total, H, K], v [total, HV, V] (qkv_dtype), g, beta [total, HV],
  *   state [n_state_rows, HV, K, V] (f32 or f16), state_indices NULL (row r) or
  *   int32 [n_seqs]: a row outside the state stands for no request, its nodes'

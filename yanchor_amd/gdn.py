@@ -123,7 +123,8 @@ def chunk_gated_delta_rule(query, key, value, g=None, beta=None, scale=None, ini
     kernel (chunk 64): packed ones as given, batched ones (the reference's
     own call, T > 1) as B packed sequences of T tokens.  Other shapes, or
     ``force_recurrent=True``, run the token-recurrent kernel over each
-    sequence.  ``lengths`` (host ints, one per sequence) lets the chunk
+    sequence.  The chunk kernel takes finite g; -inf, which forgets the state,
+    is the token-recurrent kernel's.  ``lengths`` (host ints, one per sequence) lets the chunk
     kernel start the longest sequences first.  Scratch memory, which only
     calls of few sequences use (25.6 KB per 64 tokens and value head, at most
     2 GiB) and do without where there is no room for it, belongs to the call,
@@ -208,12 +209,13 @@ def tree_gated_delta_rule(query, key, value, g, beta, parents, cu_seqlens, initi
     parent's state, a node that follows the context the request's row of
     ``initial_state`` ``[rows, HV, K, V]`` (float32 or float16): row r, or
     ``state_indices[r]`` (int ``[R]``; a row outside the state, as -1: no
-    request, zeros).  Returns o ``[1, N, HV, V]``; rows behind the last request
-    are zeros.  The state is NOT updated: once the accepted paths are known,
-    ``chunk_gated_delta_rule`` runs their rows, packed (its ``cu_seqlens``), from
-    the requests' states (float32: a float16 pool is widened for it) and returns
-    the states after them, which go back into the pool.  ``max_nodes``: the most nodes of any request (default 64); a node
-    past it comes back as not-a-number."""
+    request, zeros).  A g below -104, as -inf, forgets the state.  Returns o
+    ``[1, N, HV, V]``; rows behind the last request are zeros.  The state is NOT
+    updated: once the accepted paths are known, ``chunk_gated_delta_rule`` runs
+    their rows, packed (its ``cu_seqlens``), from the requests' states (float32:
+    a float16 pool is widened for it) and returns the states after them, which
+    go back into the pool.  ``max_nodes``: the most nodes of any request
+    (default 64); a node past it comes back as not-a-number."""
     if query.ndim != 4 or key.shape != query.shape or value.ndim != 4 or query.shape[0] != 1:
         raise ValueError("query/key must be [1, N, H, K] and value [1, N, HV, V]")
     _, n, h, kd = key.shape
