@@ -934,6 +934,80 @@ int yh_conv_tree(const void* proj, int64_t proj_stride, const void* window, cons
                  const int32_t* parents, const int32_t* cu_seqlens, int64_t n_seqs, int64_t total, int64_t channels,
                  int64_t planes, void* out, int dtype, yh_stream_t stream);
 
+/* ---- decoding over a quantised block cache -------------------------------------
+ *
+ * A quantised block cache keeps a row in runs of 32 values that share a power of
+ * two: value = code 2^(s - 127).  `bits` 8: e4m3 codes, keys / values [blocks, G,
+ * block, D] bytes; 4: e2m1 codes, [blocks, G, block, D / 2] bytes, the even dim in
+ * the low half; key_scales / value_scales the s, [blocks, G, D / 32, block] bytes.
+ * 16: the block cache above in bf16 or f16, its scales NULL.
+ */
+
+/*
+ * Rows into a quantised cache at slots[n] (int64 [N], distinct; outside the cache:
+ * not written): k, v rows k_stride / v_stride elements apart, [G, D] dense, 16-byte
+ * aligned, bf16 or f16.  s is the smallest byte, 16 at least, with max |x| <= M
+ * 2^(s - 127) over a run, M = 448 (8 bits) or 6 (4 bits), the code x 2^(127 - s)
+ * rounded to nearest even: nothing saturates.  A run with a NaN or an infinity
+ * gets s = 255 and reads as NaN.  D % 32 == 0.
+ */
+int yh_cache_write_quantized(const void* k, int64_t k_stride, const void* v, int64_t v_stride, const int64_t* slots,
+                             void* keys, void* values, uint8_t* key_scales, uint8_t* value_scales, int64_t N,
+                             int64_t blocks, int64_t G, int64_t D, int64_t block, int bits, int dtype,
+                             yh_stream_t stream);
+
+/*
+ * Rows of a cache (4, 8 or 16 bits) back: k, v [N, G, D] dense in dtype (bf16 or
+ * f16; that of a 16-bit cache) from slots[n]; a slot outside the cache gives zeros,
+ * a value past f16's range infinity.  D % 32 == 0 (16 bits: D % 8 == 0).
+ */
+int yh_cache_read(const int64_t* slots, const void* keys, const void* values, const uint8_t* key_scales,
+                  const uint8_t* value_scales, void* k, void* v, int64_t N, int64_t blocks, int64_t G, int64_t D,
+                  int64_t block, int bits, int dtype, yh_stream_t stream);
+
+/*
+ * Attention of one new token a request: request r has lengths[r] (int64) positions
+ * in its cache, the new one among them, and sees p from max(0, starts[r],
+ * lengths[r] - window, lengths[r] - columns * block) to lengths[r] - 1 (starts
+ * int64 [n_seqs] or NULL; window 0: none):
+ *   x_p = scale q . k_p;  softcap > 0: x_p = softcap tanh(x_p / softcap);
+ *   slopes (f32 [H]) not NULL: x_p -= slopes[h] (lengths[r] - 1 - p)
+ *   out = sum_p softmax(x)_p v_p (* sigmoid(gate)); zeros where nothing is seen
+ * q [n_seqs, H, D] rows q_stride apart, heads dense; out dense; dtype (bf16 or f16)
+ * is theirs, the gate's and a 16-bit cache's.  tables int32 [n_seqs, columns]; a
+ * position whose block is not in the cache is not seen.  H % G == 0, D 64, 128 or
+ * 256, scale > 0.  max_length: no request has more positions (< 0: unknown), which
+ * may save a launch.  workspace: 16-byte aligned, of at least
+ * yh_decode_attention_workspace_bytes bytes (0: none, NULL will do); calls that may
+ * overlap need one each.
+ */
+int64_t yh_decode_attention_workspace_bytes(int64_t n_seqs, int64_t H, int64_t G, int64_t D, int64_t block,
+                                            int64_t columns, int64_t window, int64_t max_length);
+int yh_decode_attention(const void* q, int64_t q_stride, const void* keys, const void* values,
+                        const uint8_t* key_scales, const uint8_t* value_scales, const int32_t* tables,
+                        const int64_t* lengths, const int64_t* starts, const float* slopes, const void* gate,
+                        int64_t gate_token_stride, int64_t gate_head_stride, void* out, int64_t n_seqs,
+                        int64_t blocks, int64_t columns, int64_t H, int64_t G, int64_t D, int64_t block,
+                        int64_t window, int64_t max_length, float scale, float softcap, int bits, int dtype,
+                        void* workspace, int64_t workspace_bytes, yh_stream_t stream);
+
+/*
+ * RMS norms of query and key heads and rotary positions of up to four axes:
+ *   y = x / sqrt(mean(x^2) + eps) (w + 1, or w without plus_one; q_w / k_w NULL:
+ *   no norm), then y_j, y_{j + R/2} turned by positions[axis(j)][n] freq[j], R =
+ *   rotary_dim, dims from R on as they are; float32, rounded once, the angle float64.
+ * q [N, H, D], k [N, G, D] with token and head strides (16-byte aligned heads), q_out
+ * / k_out dense, w [D], all bf16 or f16; positions int64 [axes, N]; freq f32 [R / 2];
+ * sections: HOST int64 [axes], pairs of each axis, in sum R / 2 (NULL for one axis),
+ * one behind the other, or interleaved: pair j is of axis j % axes while j < axes
+ * sections[j % axes], of axis 0 otherwise.  D 64, 128 or 256, R % 16 == 0.
+ */
+int yh_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                    int64_t k_token_stride, int64_t k_head_stride, const void* q_w, const void* k_w,
+                    const int64_t* positions, const float* freq, const int64_t* sections, int64_t axes,
+                    int interleaved, void* q_out, void* k_out, int64_t N, int64_t H, int64_t G, int64_t D,
+                    int64_t rotary_dim, float eps, int plus_one, int dtype, yh_stream_t stream);
+
 /*
  * HBM calibration stream (no counterpart in the reference: the measuring stick
  * for the HBM-bound kernels, whose roofline fractions are quoted against the

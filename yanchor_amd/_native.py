@@ -16,8 +16,9 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libyanchor_amd.so"
 # out2_stride; 104: yh_linear_pack lays K blocks outermost; 105: yh_rmsnorm_partials takes part2;
 # 106: yh_gdn_decode_fused takes the state dtype; 107: the yh_anchor_tokens_* calls are added,
 # yh_gdn_chunk_varlen uses its workspace, yh_conv_prefill's dtype may hold a number of planes;
-# 108: the calls for drafted trees and block tables are added; 109: yh_slot_map_served)
-ABI_VERSION = 109
+# 108: the calls for drafted trees and block tables are added; 109: yh_slot_map_served; 110: quantised caches, their decode
+# attention and yh_qk_norm_rope)
+ABI_VERSION = 110
 
 F32, BF16, F16, I32, I64, U8 = 0, 1, 2, 3, 4, 5
 DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16,
@@ -97,6 +98,10 @@ SIGNATURES: dict[str, list] = {
     "yh_tree_attention": [_p, _i64, _p, _i64, _p, _i64] + [_p] * 7 + [_i64, _i64, _p] + [_i64] * 11 + [_f32, _i32, _p, _i64, _p],
     "yh_tree_gated_delta_rule": [_p] * 8 + [_i32, _p, _p] + [_i64] * 8 + [_f32, _i32, _i32, _i32, _i32, _p],
     "yh_conv_tree": [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i32, _p],
+    "yh_qk_norm_rope": [_p, _i64, _i64, _p, _i64, _i64] + [_p] * 5 + [_i64, _i32, _p, _p] + [_i64] * 5 + [_f32, _i32, _i32, _p],
+    "yh_cache_write_quantized": [_p, _i64, _p, _i64] + [_p] * 5 + [_i64] * 5 + [_i32, _i32, _p],
+    "yh_cache_read": [_p] * 7 + [_i64] * 5 + [_i32, _i32, _p],
+    "yh_decode_attention": [_p, _i64] + [_p] * 9 + [_i64, _i64, _p] + [_i64] * 9 + [_f32, _f32, _i32, _i32, _p, _i64, _p],
     "yh_hbm_stream": [_i32, _i32, _p, _p, _i64, _i32, _p],
 }
 
@@ -105,6 +110,7 @@ PLAIN: dict[str, tuple] = {
     "yh_extend_plan_bytes": (_i64, [_i64, _i64]),
     "yh_trim_plan_bytes": (_i64, [_i64, _i64]),
     "yh_tree_attention_workspace_bytes": (_i64, [_i64] * 9),
+    "yh_decode_attention_workspace_bytes": (_i64, [_i64] * 8),
     "yh_topk_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "yh_linear_split": (_i32, [_i64, _i64, _i64]),
     "yh_linear_packed_split": (_i32, [_i64, _i64, _i64]),

@@ -1,0 +1,715 @@
+// Attention of one new token a request over a block cache of 16, 8 or 4 bits.
+//
+// Request r has L positions in its cache, the new token's among them (the last).
+// Query head h of KV head g = h / (H / G) sees p from max(starts, L - window, 0,
+// L - columns * block) to L - 1:
+//   x_p = q . k_p scale;  x_p = cap tanh(x_p / cap);  x_p -= slope_h (L - 1 - p)
+//   out = sum_p softmax(x)_p v_p (* sigmoid(gate)),  zeros where nothing is seen
+//
+// A wave takes 64 positions of a KV head and up to 16 of its query heads on
+// 16x16x32 MFMA:
+//   S^T = K Q^T      row i of product t is position 4 i + t of the 64, so that the
+//                    lane (head lane % 16, quarter lane / 16) ends with the scores
+//                    of the 16 positions of its quarter
+//   O^T += V^T P^T   that is how the B operand wants P: slot e of quarter c in
+//                    step s is position 16 c + 8 s + e, no lane hands one on
+// The order of a product's terms is free, so a lane loads K and V rows straight
+// into the places of the A operands, whole pieces of a row (a quarter's D / 4 dims
+// of K, D / 16 dims of V), and nothing goes through LDS.  Codes become bf16 by
+// v_cvt_scalef32, exactly; with fp16 queries, whose 11 bits bf16 does not hold,
+// queries and weights enter as two bf16 each (hi + lo).
+//
+// Requests are few or of very different lengths, so the tiles of 64 positions are
+// cut into parts of about one size, which every workgroup finds from the lengths
+// by itself; its four waves take the part's tiles in turn and join their sums in
+// LDS.  Parts of a request that was cut leave theirs, with their maximum, in the
+// workspace, and a second launch joins them in order.
+//
+// Bound by HBM.
+#include <type_traits>
+
+#include "attn_tile.h"
+#include "qcache.h"
+#include "tree.h"
+
+namespace yh {
+namespace {
+
+using namespace qcache;
+using tree::Div;
+using attn::bf16x8_t;
+using attn::f16x8_t;
+using attn::bf16x2_t;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTile = 64;        // positions a wave takes at a time
+constexpr int kCols = 16;        // query heads it takes
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kFloor = -3.0e38f;   // below every score: the maximum of nothing
+// fp16 weights are e^(x - max) 2^14, up to a quarter of the type's range: weights below 2^-14 of the largest, of which
+// a long cache may have very many, then keep their 11 bits down to 2^-28.  The denominator carries the same factor.
+constexpr float kLift = 14.f;
+
+struct DecodeArgs {
+  const uint16_t* q;       // [R, H, D], tokens q_ts apart
+  int64_t q_ts;
+  const char* keys;        // [blocks, G, block, row bytes]
+  const char* values;
+  const uint8_t* key_scales;     // [blocks, G, D / 32, block]
+  const uint8_t* value_scales;
+  const int32_t* tables;   // [R, columns]
+  const int64_t* lengths;  // [R]
+  const int64_t* starts;   // [R] or null
+  const float* slopes;     // [H] or null
+  const uint16_t* gate;    // [R, H, D] with strides, or null
+  int64_t g_ts, g_hs;
+  uint16_t* out;           // [R, H, D]
+  int64_t window;          // 0: none
+  float scale, cap;        // cap 0: none
+  Div block, columns;
+  int R, H, G, rep, mtiles, blocks, target;
+  int32_t* first;          // [R + 1] first part of each request
+  float* part;             // [parts][H][D]
+  float2* stat;            // [parts][H] maximum and denominator
+};
+
+// First and last + 1 of the positions that request r sees.
+struct Seen {
+  int lo, hi;
+};
+__device__ __forceinline__ Seen seen_of(const DecodeArgs& a, int r) {
+  const int64_t len = a.lengths[r];
+  if (len <= 0) return {0, 0};
+  int64_t lo = len - static_cast<int64_t>(a.columns.d) * a.block.d;
+  if (a.window && len - a.window > lo) lo = len - a.window;
+  if (a.starts && a.starts[r] > lo) lo = a.starts[r];
+  if (lo < 0) lo = 0;
+  if (lo >= len || len > 0x7ffff000ll) return {0, 0};
+  return {static_cast<int>(lo), static_cast<int>(len)};
+}
+__device__ __forceinline__ int tiles_of(Seen s) { return s.hi > s.lo ? (s.hi + kTile - 1) / kTile - s.lo / kTile : 0; }
+
+// Wave-inclusive sum over lanes.
+__device__ __forceinline__ int scan_wave(int x) {
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int y = __shfl_up(x, off, kWave);
+    if (lane >= off) x += y;
+  }
+  return x;
+}
+
+struct Part {
+  int r, index, count, slot;   // request, which of its parts, how many, number of the part among all
+  int tile, tiles;             // its tiles, from the request's first
+  Seen seen;
+};
+
+// Part `which` of all, found from the lengths; count 0: there is none.
+__device__ Part find_part(const DecodeArgs& a, int which) {
+  __shared__ int sums[kWaves], found[4];
+  const int t = threadIdx.x, w = t / kWave;
+  // a thread takes `each` requests in a row
+  const int each = (a.R + kThreads - 1) / kThreads, r0 = t * each, r1 = r0 + each < a.R ? r0 + each : a.R;
+  int mine = 0;
+  for (int r = r0; r < r1; ++r) mine += tiles_of(seen_of(a, r));
+  int s = scan_wave(mine);
+  if ((t & (kWave - 1)) == kWave - 1) sums[w] = s;
+  if (t == 0) found[0] = -1;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) total += sums[i];
+  __syncthreads();
+  // tiles of a part: a turn of the waves at least
+  int chunk = a.target ? (total + a.target - 1) / a.target : 0x7fffffff;
+  if (chunk < kWaves) chunk = kWaves;
+  mine = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int n = tiles_of(seen_of(a, r));
+    mine += n > chunk ? (n + chunk - 1) / chunk : 1;
+  }
+  s = scan_wave(mine);
+  if ((t & (kWave - 1)) == kWave - 1) sums[w] = s;
+  __syncthreads();
+  int at = s - mine;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) at += i < w ? sums[i] : 0;
+  if (which >= at && which < at + mine) {
+    for (int r = r0; r < r1; ++r) {
+      const int n = tiles_of(seen_of(a, r)), c = n > chunk ? (n + chunk - 1) / chunk : 1;
+      if (which < at + c) {
+        found[0] = r;
+        found[1] = which - at;
+        found[2] = c;
+        found[3] = n;
+        break;
+      }
+      at += c;
+    }
+  }
+  __syncthreads();
+  Part p;
+  p.r = found[0];
+  if (p.r < 0) {
+    p.count = 0;
+    return p;
+  }
+  p.index = found[1];
+  p.count = found[2];
+  p.slot = which;
+  const int n = found[3], each_part = n / p.count, rest = n % p.count;    // parts of a request differ by a tile
+  p.tile = p.index * each_part + (p.index < rest ? p.index : rest);
+  p.tiles = each_part + (p.index < rest ? 1 : 0);
+  p.seen = seen_of(a, p.r);
+  return p;
+}
+
+// Two dims of one position's codes to bf16, `half` the pair within a dword.
+template <int FMT>
+struct Codes;
+template <>
+struct Codes<kFp8> {
+  static constexpr int kBits = 8;
+  template <int PAIR>
+  static __device__ __forceinline__ uint32_t two(const uint32_t* w, float s) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[PAIR / 2], s, PAIR % 2 == 1));
+  }
+};
+template <>
+struct Codes<kFp4> {
+  static constexpr int kBits = 4;
+  template <int PAIR>
+  static __device__ __forceinline__ uint32_t two(const uint32_t* w, float s) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[PAIR / 4], s, PAIR % 4));
+  }
+};
+template <>
+struct Codes<k16> {
+  static constexpr int kBits = 16;
+  template <int PAIR>
+  static __device__ __forceinline__ uint32_t two(const uint32_t* w, float) {
+    return w[PAIR];
+  }
+};
+
+// BYTES bytes (2 to 64) into dwords.
+template <int BYTES>
+__device__ __forceinline__ void load_bytes(uint32_t* w, const char* p) {
+  if constexpr (BYTES == 2) {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else if constexpr (BYTES == 4) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (BYTES == 8) {
+    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+    w[0] = x[0];
+    w[1] = x[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(p + 16 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
+    }
+  }
+}
+
+template <int I, int N, class F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<I + 1, N>(f);
+  }
+}
+
+// The product's type: the queries' for a 16-bit cache, bf16 for codes.
+template <int MT>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (MT == YH_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+// The compiler puts no wait where a matrix result is first read behind branches that meet.
+template <int N>
+__device__ __forceinline__ void settle(f32x4 (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
+  asm volatile("s_nop 7\n\ts_nop 7" : "+v"(x[0]));
+#pragma unroll
+  for (int i = 1; i < N; ++i) asm volatile("" : "+v"(x[i]));
+}
+
+template <int DT, int FMT, int D, bool RUNS>
+__global__ void __launch_bounds__(kThreads) decode_attention_kernel(DecodeArgs a) {
+  using C = Codes<FMT>;
+  constexpr int MT = FMT == k16 ? DT : YH_BF16;
+  constexpr bool kPair = FMT != k16 && DT == YH_F16;    // queries and weights as hi + lo
+  constexpr int kRow = D * C::kBits / 8;                // bytes of a row
+  constexpr int kKd = D / 4, kVd = D / 16;              // dims of a lane: K, V
+  constexpr int kKb = kRow / 4, kVb = kRow / 16;        // and their bytes
+  constexpr int kKw = (kKb + 3) / 4, kVw = (kVb + 3) / 4;
+  constexpr int kKs = kKd > kRun ? kKd / kRun : 1;      // scales of a lane's K dims
+  constexpr int kSteps = D / 32;                        // products over the dims
+  using M = attn::Mfma<DT>;
+  __shared__ float2 wave_stat[kWaves][kCols];
+  __shared__ float wave_acc[kWaves][kCols][D + 4];
+
+  const int g = blockIdx.x % a.G, mt = blockIdx.x / a.G % a.mtiles;
+  const Part part = find_part(a, blockIdx.x / a.G / a.mtiles);
+  if (part.count == 0) return;
+  const int r = part.r;
+  if (a.first && part.index == 0 && g == 0 && mt == 0 && threadIdx.x == 0) {
+    a.first[r] = part.slot;
+    if (r == a.R - 1) a.first[a.R] = part.slot + part.count;
+  }
+
+  const int lane = threadIdx.x & (kWave - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int col = lane & 15, quarter = lane >> 4;
+  const int cols = a.rep - mt * kCols < kCols ? a.rep - mt * kCols : kCols;
+  const int head = g * a.rep + mt * kCols + (col < cols ? col : 0);
+
+  // the queries as the B operand: column `col`, dims as the K rows have them
+  u32x4 qh[kSteps], ql[kPair ? kSteps : 1];
+#pragma unroll
+  for (int c = 0; c < kSteps; ++c) {
+    const int dim = FMT == k16 ? 32 * c + 8 * quarter : kKd * quarter + 8 * c;
+    u32x4 x = *reinterpret_cast<const u32x4*>(a.q + r * a.q_ts + static_cast<int64_t>(head) * D + dim);
+    if (col >= cols) x = u32x4{0, 0, 0, 0};
+    if constexpr (kPair) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x0 = f16_to_f32(x[i] & 0xffff), x1 = f16_to_f32(x[i] >> 16);
+        const uint16_t h0 = f32_to_bf16(x0), h1 = f32_to_bf16(x1);
+        qh[c][i] = attn::pack2(h0, h1);
+        ql[c][i] = attn::pack2(f32_to_bf16(x0 - bf16_to_f32(h0)), f32_to_bf16(x1 - bf16_to_f32(h1)));
+      }
+    } else {
+      qh[c] = x;
+    }
+  }
+  // scores in powers of two
+  const float mul = a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : kLog2e * a.scale;
+  const float cap2 = a.cap * kLog2e, slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+
+  float top = kFloor, den = 0.f;
+  f32x4 acc[kVd];
+#pragma unroll
+  for (int n = 0; n < kVd; ++n) acc[n] = f32x4{0, 0, 0, 0};
+
+  const int32_t* table = a.tables + static_cast<int64_t>(r) * a.columns.d;
+  // the row (of all rows of all heads) of position p, < 0 where the table holds no block
+  auto row_of = [&](int p) -> int64_t {
+    const uint32_t b = a.block.quot(p), c = b - a.columns.quot(b) * a.columns.d;
+    const int id = table[c];
+    return id < 0 || id >= a.blocks ? -1 : (static_cast<int64_t>(id) * a.G + g) * a.block.d + (p - b * a.block.d);
+  };
+  // of its scale, run `run` of the dims
+  auto scale_at = [&](int64_t row, int p, int run) -> int64_t {
+    const uint32_t in = p - a.block.quot(p) * a.block.d;
+    return (row - in) * (D / kRun) + static_cast<int64_t>(run) * a.block.d + in;
+  };
+  const int first_tile = part.seen.lo / kTile + part.tile;
+
+  for (int i = w; i < part.tiles; i += kWaves) {
+    const int base = (first_tile + i) * kTile;
+    const int pk = base + 4 * col, pv = base + 16 * quarter;      // the lane's positions: 4 of K, 16 of V
+    uint32_t kw[4][kKw], vw[16][kVw];
+    uint32_t ksc[kKs], vsc[4];      // scale bytes of 4 and 16 positions
+    uint32_t khole = 0, vhole = 0;  // positions without a block
+    if constexpr (RUNS) {
+      const int64_t krow = row_of(pk), vrow = row_of(pv);
+      if (krow < 0) {
+        khole = 15;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < kKw; ++e) kw[t][e] = 0;
+#pragma unroll
+        for (int e = 0; e < kKs; ++e) ksc[e] = 0x7f7f7f7fu;
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const char* p = a.keys + (krow + t) * kRow;
+          if constexpr (FMT == k16) {
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c) load_bytes<16>(kw[t] + 4 * c, p + (32 * c + 8 * quarter) * 2);
+          } else {
+            load_bytes<kKb>(kw[t], p + quarter * kKb);
+          }
+        }
+        if constexpr (FMT != k16) {
+#pragma unroll
+          for (int e = 0; e < kKs; ++e)
+            ksc[e] = *reinterpret_cast<const uint32_t*>(a.key_scales + scale_at(krow, pk, quarter * kKd / kRun + e));
+        }
+      }
+      if (vrow < 0) {
+        vhole = 0xffff;
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+#pragma unroll
+          for (int e = 0; e < kVw; ++e) vw[u][e] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vsc[e] = 0x7f7f7f7fu;
+      } else {
+#pragma unroll
+        for (int u = 0; u < 16; ++u) load_bytes<kVb>(vw[u], a.values + (vrow + u) * kRow + col * kVb);
+        if constexpr (FMT != k16) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(a.value_scales + scale_at(vrow, pv, col * kVd / kRun));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vsc[e] = x[e];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kKs; ++e) ksc[e] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vsc[e] = 0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int64_t row = row_of(pk + t);
+        if (row < 0) {
+          khole |= 1u << t;
+#pragma unroll
+          for (int e = 0; e < kKw; ++e) kw[t][e] = 0;
+          continue;
+        }
+        const char* p = a.keys + row * kRow;
+        if constexpr (FMT == k16) {
+#pragma unroll
+          for (int c = 0; c < kSteps; ++c) load_bytes<16>(kw[t] + 4 * c, p + (32 * c + 8 * quarter) * 2);
+        } else {
+          load_bytes<kKb>(kw[t], p + quarter * kKb);
+#pragma unroll
+          for (int e = 0; e < kKs; ++e)
+            ksc[e] |= static_cast<uint32_t>(a.key_scales[scale_at(row, pk + t, quarter * kKd / kRun + e)]) << (8 * t);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const int64_t row = row_of(pv + u);
+        if (row < 0) {
+          vhole |= 1u << u;
+#pragma unroll
+          for (int e = 0; e < kVw; ++e) vw[u][e] = 0;
+          continue;
+        }
+        load_bytes<kVb>(vw[u], a.values + row * kRow + col * kVb);
+        if constexpr (FMT != k16)
+          vsc[u / 4] |= static_cast<uint32_t>(a.value_scales[scale_at(row, pv + u, col * kVd / kRun)]) << (8 * (u % 4));
+      }
+    }
+
+    // S^T, product t: positions 4 i + t
+    f32x4 s[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      s[t] = f32x4{0, 0, 0, 0};
+      each<0, kSteps>([&](auto step) {
+        constexpr int ST = decltype(step)::value;
+        u32x4 x;
+        const float sc = FMT == k16 ? 1.f : scale_value((ksc[ST * 8 / kRun] >> (8 * t)) & 0xff);
+        each<0, 4>([&](auto pair) { x[decltype(pair)::value] = C::template two<4 * ST + decltype(pair)::value>(kw[t], sc); });
+        s[t] = mfma<MT>(x, qh[ST], s[t]);
+        if constexpr (kPair) s[t] = mfma<MT>(x, ql[ST], s[t]);
+      });
+    }
+    settle(s);
+
+    // what of the 16 positions of this quarter is seen; value u = 4 j + t is s[t][j]
+    uint32_t dead = vhole;
+    const bool inside = base >= part.seen.lo && base + kTile <= part.seen.hi;
+    if (!inside) {
+#pragma unroll
+      for (int u = 0; u < 16; ++u) dead |= pv + u < part.seen.lo || pv + u >= part.seen.hi ? 1u << u : 0u;
+    }
+    const bool masked = __ballot(dead != 0) != 0;
+    float x[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      float y = s[u % 4][u / 4] * mul;
+      if (a.cap > 0.f) y = cap2 * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y) + 1.f));
+      x[u] = a.slopes ? y - slope * static_cast<float>(part.seen.hi - 1 - pv - u) : y;
+    }
+    if (masked) {
+      // what is not seen may be anything: its values are cleared too
+#pragma unroll
+      for (int u = 0; u < 16; ++u)
+        if (dead >> u & 1) {
+          x[u] = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < kVw; ++e) vw[u][e] = 0;
+          vsc[u / 4] = (vsc[u / 4] & ~(0xffu << (8 * (u % 4)))) | 0x7fu << (8 * (u % 4));
+        }
+    }
+    float m = x[0];
+#pragma unroll
+    for (int u = 1; u < 16; ++u) m = fmaxf(m, x[u]);
+    m = fmaxf(m, __shfl_xor(m, 16, kWave));
+    m = fmaxf(m, __shfl_xor(m, 32, kWave));
+    if (__ballot(m > top)) {
+      const float next = fmaxf(top, m), f = __builtin_amdgcn_exp2f(top - next);
+      top = next;
+      den *= f;
+#pragma unroll
+      for (int n = 0; n < kVd; ++n) acc[n] *= f;
+    }
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      x[u] = __builtin_amdgcn_exp2f(x[u] - (MT == YH_F16 ? top - kLift : top));
+      den += x[u];
+    }
+    // P^T as the B operand, step st: positions 8 st + e of the quarter
+    u32x4 ph[2], pl[2];
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x0 = x[8 * st + 2 * e], x1 = x[8 * st + 2 * e + 1];
+        ph[st][e] = attn::Mfma<MT>::round2(x0, x1);
+        if constexpr (kPair)
+          pl[st][e] = attn::Mfma<MT>::round2(x0 - __uint_as_float(ph[st][e] << 16),
+                                             x1 - __uint_as_float(ph[st][e] & 0xffff0000u));
+      }
+    // O^T: product n takes dim n of each lane's kVd
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      float sc[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        sc[e] = FMT == k16 ? 1.f : scale_value((vsc[2 * st + e / 4] >> (8 * (e % 4))) & 0xff);
+      each<0, kVd / 2>([&](auto pair) {
+        constexpr int P = decltype(pair)::value;
+        u32x4 lo, hi;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t y0 = C::template two<P>(vw[8 * st + 2 * e], sc[2 * e]);
+          const uint32_t y1 = C::template two<P>(vw[8 * st + 2 * e + 1], sc[2 * e + 1]);
+          lo[e] = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
+          hi[e] = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
+        }
+        acc[2 * P] = mfma<MT>(lo, ph[st], acc[2 * P]);
+        acc[2 * P + 1] = mfma<MT>(hi, ph[st], acc[2 * P + 1]);
+        if constexpr (kPair) {
+          acc[2 * P] = mfma<MT>(lo, pl[st], acc[2 * P]);
+          acc[2 * P + 1] = mfma<MT>(hi, pl[st], acc[2 * P + 1]);
+        }
+      });
+    }
+    settle(acc);
+  }
+
+  // the waves' sums: lane (col, quarter) has dims (4 quarter + j) kVd + n of column col in acc[n][j]
+  den += __shfl_xor(den, 16, kWave);
+  den += __shfl_xor(den, 32, kWave);
+  if (quarter == 0) wave_stat[w][col] = make_float2(top, den);
+  if (col < cols) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int n = 0; n < kVd; ++n) wave_acc[w][col][(4 * quarter + j) * kVd + n] = acc[n][j];
+  }
+  __syncthreads();
+  for (int at = threadIdx.x; at < cols * (D / 4); at += kThreads) {
+    const int c = at / (D / 4), dim = at % (D / 4) * 4;
+    float m = kFloor;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) m = fmaxf(m, wave_stat[i][c].x);
+    float dn = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      const float f = __builtin_amdgcn_exp2f(wave_stat[i][c].x - m);
+      dn = fmaf(wave_stat[i][c].y, f, dn);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(wave_acc[i][c][dim + e], f, o[e]);
+    }
+    const int hd = g * a.rep + mt * kCols + c;
+    if (part.count > 1) {
+      const int64_t slot = static_cast<int64_t>(part.slot) * a.H + hd;
+      *reinterpret_cast<float4*>(a.part + slot * D + dim) = make_float4(o[0], o[1], o[2], o[3]);
+      if (dim == 0) a.stat[slot] = make_float2(m, dn);
+    } else {
+      const float inv = dn > 0.f || dn != dn ? 1.f / dn : 0.f;     // nothing seen: zeros
+      const int64_t to = (static_cast<int64_t>(r) * a.H + hd) * D + dim;
+      uint16_t y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float z = o[e] * inv;
+        if (a.gate) z *= 1.f / (1.f + __expf(-M::widen(a.gate[r * a.g_ts + hd * a.g_hs + dim + e])));
+        y[e] = M::round(z);
+      }
+      *reinterpret_cast<u32x2*>(a.out + to) = u32x2{attn::pack2(y[0], y[1]), attn::pack2(y[2], y[3])};
+    }
+  }
+}
+
+// The parts of the cut requests joined in order, D / 4 lanes a head.
+template <int DT, int D>
+__global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
+  using M = attn::Mfma<DT>;
+  constexpr int kLanes = D / 4, kHeads = kThreads / kLanes;
+  const int r = blockIdx.x, hd = blockIdx.y * kHeads + threadIdx.x / kLanes, dim = threadIdx.x % kLanes * 4;
+  const int first = a.first[r], count = a.first[r + 1] - first;
+  if (count <= 1 || hd >= a.H) return;
+  const int64_t slot = static_cast<int64_t>(first) * a.H + hd;
+  float m = kFloor;
+  for (int j = 0; j < count; ++j) m = fmaxf(m, a.stat[slot + static_cast<int64_t>(j) * a.H].x);
+  float dn = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < count; ++j) {
+    const int64_t s = slot + static_cast<int64_t>(j) * a.H;
+    const float2 st = a.stat[s];
+    const float4 x = *reinterpret_cast<const float4*>(a.part + s * D + dim);
+    const float f = __builtin_amdgcn_exp2f(st.x - m);
+    dn = fmaf(st.y, f, dn);
+    o[0] = fmaf(x.x, f, o[0]);
+    o[1] = fmaf(x.y, f, o[1]);
+    o[2] = fmaf(x.z, f, o[2]);
+    o[3] = fmaf(x.w, f, o[3]);
+  }
+  const float inv = dn > 0.f || dn != dn ? 1.f / dn : 0.f;
+  const int64_t to = (static_cast<int64_t>(r) * a.H + hd) * D + dim;
+  uint16_t y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float z = o[e] * inv;
+    if (a.gate) z *= 1.f / (1.f + __expf(-M::widen(a.gate[r * a.g_ts + hd * a.g_hs + dim + e])));
+    y[e] = M::round(z);
+  }
+  *reinterpret_cast<u32x2*>(a.out + to) = u32x2{attn::pack2(y[0], y[1]), attn::pack2(y[2], y[3])};
+}
+
+constexpr int kWorkgroups = 1024;     // parts aimed at, over all heads: four workgroups a CU
+
+// Parts aimed at for each KV head, 0 where no request is cut.
+int64_t target_for(int64_t R, int64_t H, int64_t G, int64_t block, int64_t columns, int64_t window, int64_t max_length) {
+  int64_t most = columns * block;
+  if (window && window < most) most = window;
+  if (max_length >= 0 && max_length < most) most = max_length;
+  if (most + kTile - 1 <= kWaves * kTile) return 0;     // a turn of the waves at most
+  const int64_t each = G * ((H / G + kCols - 1) / kCols), n = (kWorkgroups + each - 1) / each;
+  return n < 1 ? 1 : n;
+}
+int64_t plan_bytes(int64_t R) { return ((R + 1) * 4 + 255) / 256 * 256; }
+
+template <int DT, int FMT, int D>
+void launch(const DecodeArgs& a, unsigned grid, hipStream_t st) {
+  if (a.block.d % 16 == 0)
+    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, true>), dim3(grid), dim3(kThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, false>), dim3(grid), dim3(kThreads), 0, st, a);
+  if (a.target) {
+    constexpr int kHeads = kThreads / (D / 4);
+    hipLaunchKernelGGL((decode_join_kernel<DT, D>), dim3(a.R, (a.H + kHeads - 1) / kHeads), dim3(kThreads), 0, st, a);
+  }
+}
+template <int DT, int FMT>
+void launch_dim(const DecodeArgs& a, int64_t D, unsigned grid, hipStream_t st) {
+  if (D == 64) launch<DT, FMT, 64>(a, grid, st);
+  else if (D == 128) launch<DT, FMT, 128>(a, grid, st);
+  else launch<DT, FMT, 256>(a, grid, st);
+}
+template <int DT>
+void launch_bits(const DecodeArgs& a, int bits, int64_t D, unsigned grid, hipStream_t st) {
+  if (bits == 16) launch_dim<DT, k16>(a, D, grid, st);
+  else if (bits == 8) launch_dim<DT, kFp8>(a, D, grid, st);
+  else launch_dim<DT, kFp4>(a, D, grid, st);
+}
+
+}  // namespace
+}  // namespace yh
+
+extern "C" int64_t yh_decode_attention_workspace_bytes(int64_t n_seqs, int64_t H, int64_t G, int64_t D, int64_t block,
+                                                       int64_t columns, int64_t window, int64_t max_length) {
+  using namespace yh;
+  if (n_seqs <= 0 || G <= 0 || H < G || D <= 0 || block <= 0 || columns <= 0 || columns >= (1ll << 31) ||
+      block >= (1ll << 31))
+    return 0;
+  const int64_t target = target_for(n_seqs, H, G, block, columns, window, max_length);
+  return target ? plan_bytes(n_seqs) + (n_seqs + target) * H * (D * 4 + 8) : 0;
+}
+
+extern "C" int yh_decode_attention(const void* q, int64_t q_stride, const void* keys, const void* values,
+                                   const uint8_t* key_scales, const uint8_t* value_scales, const int32_t* tables,
+                                   const int64_t* lengths, const int64_t* starts, const float* slopes,
+                                   const void* gate, int64_t gate_token_stride, int64_t gate_head_stride, void* out,
+                                   int64_t n_seqs, int64_t blocks, int64_t columns, int64_t H, int64_t G, int64_t D,
+                                   int64_t block, int64_t window, int64_t max_length, float scale, float softcap,
+                                   int bits, int dtype, void* workspace, int64_t workspace_bytes, yh_stream_t stream) {
+  using namespace yh;
+  YH_CHECK_ARG(n_seqs >= 0 && blocks >= 0 && columns > 0 && H > 0 && G > 0 && H % G == 0 && block > 0 && window >= 0,
+               "decode_attention: bad sizes");
+  YH_CHECK_ARG(D == 64 || D == 128 || D == 256, "decode_attention: head dim must be 64, 128 or 256");
+  YH_CHECK_ARG(bits == 4 || bits == 8 || bits == 16, "decode_attention: a cache holds 4, 8 or 16 bits a value");
+  YH_CHECK_ARG(scale > 0.f && scale < INFINITY, "decode_attention: scale must be positive");
+  YH_CHECK_ARG(softcap >= 0.f && softcap < INFINITY, "decode_attention: softcap must be positive, or 0 for none");
+  if (dtype != YH_BF16 && dtype != YH_F16) {
+    set_error("decode_attention: dtype must be bf16 or fp16");
+    return YH_ERR_UNSUPPORTED;
+  }
+  if (n_seqs == 0) return YH_OK;
+  YH_CHECK_ARG(q && out && lengths && tables && ((keys && values) || blocks == 0), "decode_attention: null pointer");
+  YH_CHECK_ARG(bits == 16 || blocks == 0 || (key_scales && value_scales), "decode_attention: a quantised cache needs its scales");
+  YH_CHECK_ARG(tree::aligned16(q) && tree::aligned16(out) && tree::aligned16(keys) && tree::aligned16(values) &&
+                   (block % 16 || (tree::aligned16(key_scales) && tree::aligned16(value_scales))),
+               "decode_attention: tensors must be 16-byte aligned");
+  YH_CHECK_ARG(q_stride % 8 == 0 && q_stride >= H * D, "decode_attention: the token stride must hold whole heads and keep 16-byte rows");
+  YH_CHECK_ARG(!gate || (gate_head_stride >= D && gate_token_stride >= H * gate_head_stride),
+               "decode_attention: bad gate strides");
+  const int64_t each = G * ((H / G + kCols - 1) / kCols);
+  YH_CHECK_ARG(n_seqs < (1ll << 20) && columns < (1ll << 31) && block < (1ll << 31) && H < (1ll << 16) &&
+                   blocks < (1ll << 31) && blocks * block < (1ll << 40),
+               "decode_attention: sizes too large");
+  const int64_t target = target_for(n_seqs, H, G, block, columns, window, max_length);
+  int64_t most = columns * block;
+  if (window && window < most) most = window;
+  YH_CHECK_ARG(n_seqs * (most / kTile + 2) < (1ll << 31), "decode_attention: sizes too large");
+  const int64_t grid = (n_seqs + target) * each;
+  YH_CHECK_ARG(grid < (1ll << 24), "decode_attention: sizes too large");
+  const int64_t need = yh_decode_attention_workspace_bytes(n_seqs, H, G, D, block, columns, window, max_length);
+  YH_CHECK_ARG(need == 0 || (workspace && tree::aligned16(workspace) && workspace_bytes >= need),
+               "decode_attention: workspace too small");
+  DecodeArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_ts = q_stride;
+  a.keys = static_cast<const char*>(keys);
+  a.values = static_cast<const char*>(values);
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
+  a.tables = tables;
+  a.lengths = lengths;
+  a.starts = starts;
+  a.slopes = slopes;
+  a.gate = static_cast<const uint16_t*>(gate);
+  a.g_ts = gate_token_stride;
+  a.g_hs = gate_head_stride;
+  a.out = static_cast<uint16_t*>(out);
+  a.window = window;
+  a.scale = scale;
+  a.cap = softcap;
+  a.block = tree::make_div(static_cast<uint32_t>(block));
+  a.columns = tree::make_div(static_cast<uint32_t>(columns));
+  a.R = static_cast<int>(n_seqs);
+  a.H = static_cast<int>(H);
+  a.G = static_cast<int>(G);
+  a.rep = static_cast<int>(H / G);
+  a.mtiles = (a.rep + kCols - 1) / kCols;
+  a.blocks = static_cast<int>(blocks);
+  a.target = static_cast<int>(target);
+  if (need) {
+    a.first = static_cast<int32_t*>(workspace);
+    char* sums = static_cast<char*>(workspace) + plan_bytes(n_seqs);
+    a.part = reinterpret_cast<float*>(sums);
+    a.stat = reinterpret_cast<float2*>(sums + (n_seqs + target) * H * D * 4);
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == YH_BF16) launch_bits<YH_BF16>(a, bits, D, static_cast<unsigned>(grid), st);
+  else launch_bits<YH_F16>(a, bits, D, static_cast<unsigned>(grid), st);
+  YH_CHECK_LAUNCH("decode_attention");
+  return YH_OK;
+}

@@ -767,3 +767,232 @@ def conv_tree(proj, window, conv_w, parents, cu_seqlens, channels, planes=1):
     N.call_on(dev, "yh_conv_tree", proj.data_ptr(), max(proj.stride(0), channels), window.data_ptr(),
               conv_w.data_ptr(), N.ptr(parents), cu.data_ptr(), r, n, channels, planes, out.data_ptr(), N.BF16)
     return out
+
+
+# ---------------------------------------------------------------------------
+# Decoding over a quantised block cache: rows in runs of 32 values that share a
+# power of two, 2^(s - 127), as e4m3 codes (8 bits) or e2m1 codes (4 bits).
+# Nothing is read back to the host, so these calls can be captured.
+
+def quantized_cache(blocks, groups, block, dim, *, bits=8, device=None):
+    """An empty quantised block cache (keys, values, key_scales, value_scales):
+    8 bits: keys / values [blocks, G, block, D] float8_e4m3fn; 4 bits: [blocks, G,
+    block, D / 2] uint8, two e2m1 codes a byte, the even dim in the low half;
+    scales uint8 [blocks, G, D / 32, block].  D is a multiple of 32."""
+    if bits not in (4, 8):
+        raise ValueError("a quantised cache holds 4 or 8 bits a value")
+    if dim % 32 or dim < 32 or blocks < 0 or groups < 1 or block < 1:
+        raise ValueError("a quantised cache needs a head dim that is a multiple of 32")
+    device = torch.device("cuda" if device is None else device)
+    data = [torch.zeros(blocks, groups, block, dim * bits // 8, dtype=torch.uint8, device=device) for _ in range(2)]
+    if bits == 8:
+        data = [x.view(torch.float8_e4m3fn) for x in data]
+    return (*data, *(torch.zeros(blocks, groups, dim // 32, block, dtype=torch.uint8, device=device) for _ in range(2)))
+
+
+def _any_cache(keys, values, key_scales, value_scales, g, d, dtype):
+    """Bits a value of a block cache of [*, G, *, D] rows, whose form is checked;
+    ``dtype`` that of a 16-bit one."""
+    if keys.ndim != 4 or values.shape != keys.shape or values.dtype != keys.dtype or not keys.is_contiguous() or \
+            not values.is_contiguous():
+        raise ValueError("keys and values must be contiguous [blocks, G, block, D] of one type")
+    if keys.dtype in (torch.bfloat16, torch.float16):
+        if key_scales is not None or value_scales is not None:
+            raise ValueError("a 16-bit cache has no scales")
+        if keys.dtype != dtype:
+            raise ValueError(f"a 16-bit cache must be in {dtype}")
+        bits, width = 16, d
+    elif keys.dtype == torch.float8_e4m3fn:
+        bits, width = 8, d
+    elif keys.dtype == torch.uint8:
+        bits, width = 4, d // 2
+    else:
+        raise ValueError("a cache is bf16, fp16, float8_e4m3fn (8 bits) or uint8 (4 bits, two a byte)")
+    if keys.shape[1] != g or keys.shape[3] != width or keys.shape[2] < 1:
+        raise ValueError(f"a {bits}-bit cache of these heads is [blocks, {g}, block, {width}]")
+    if bits < 16:
+        if d % 32:
+            raise ValueError("the head dim of a quantised cache must be a multiple of 32")
+        shape = (keys.shape[0], g, d // 32, keys.shape[2])
+        for s in (key_scales, value_scales):
+            if s is None or s.shape != shape or s.dtype != torch.uint8 or not s.is_contiguous():
+                raise ValueError(f"a quantised cache needs contiguous uint8 scales {list(shape)}")
+    return bits
+
+
+def cache_write_quantized(k, v, slots, keys, values, key_scales, value_scales):
+    """Key and value rows into a quantised block cache (``quantized_cache``) IN
+    PLACE: slot ``slots[n]`` = block id * block + row takes k[n], v[n] [N, G, D]
+    (bf16 / fp16, any token stride); a slot below 0 or past the cache is passed
+    over, the others must be distinct.  A run of 32 values gets the smallest power
+    of two (2^-111 at least) at which none is past the largest code, so nothing
+    saturates and what is read back is off by half a step of the code: 2^-4 of an
+    e4m3 value, a quarter of the leading power of two of an e2m1 one (in both,
+    half of the smallest code near zero).  A run that holds a NaN or an infinity
+    reads back as NaN."""
+    if k.ndim != 3 or v.shape != k.shape or k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("cache_write_quantized takes bf16 / fp16 k and v [N, G, D]")
+    n, g, d = k.shape
+    bits = _any_cache(keys, values, key_scales, value_scales, g, d, None)
+    dev = _tree.device_of(k, v, keys, values, key_scales, value_scales)
+    slots = _tree.ints(slots, torch.int64, dev, "slots", n)
+    (k, ks), (v, vs) = _heads(k), _heads(v)
+    N.call_on(dev, "yh_cache_write_quantized", k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(), keys.data_ptr(),
+              values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), n, keys.shape[0], g, d,
+              keys.shape[2], bits, N.code(k))
+
+
+def cache_read(slots, keys, values, key_scales=None, value_scales=None, *, dtype=None):
+    """Rows of a block cache of 4, 8 or 16 bits back as (k, v) [N, G, D] in
+    ``dtype`` (bf16 / fp16; default bf16, or that of a 16-bit cache), from slots
+    int [N] as ``slot_map`` gives them (``slot_map(cu_seqlens, zeros, ...)`` those
+    of whole prefixes): what a prefill that continues a request reads.  A slot
+    outside the cache gives zeros."""
+    if keys.ndim != 4:
+        raise ValueError("keys and values must be contiguous [blocks, G, block, D] of one type")
+    half = keys.dtype in (torch.bfloat16, torch.float16)
+    dtype = dtype or (keys.dtype if half else torch.bfloat16)
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("cache_read gives bf16 or fp16 rows")
+    g, d = keys.shape[1], keys.shape[3] * (2 if keys.dtype == torch.uint8 else 1)
+    bits = _any_cache(keys, values, key_scales, value_scales, g, d, dtype)
+    if d % 8 or not d or not g:
+        raise ValueError("a head's row must be a multiple of 16 bytes")
+    dev = _tree.device_of(keys, values, key_scales, value_scales)
+    slots = _tree.ints(slots, torch.int64, dev, "slots")
+    n = slots.shape[0]
+    k, v = (torch.empty(n, g, d, dtype=dtype, device=dev) for _ in range(2))
+    N.call_on(dev, "yh_cache_read", slots.data_ptr(), keys.data_ptr(), values.data_ptr(), N.ptr(key_scales),
+              N.ptr(value_scales), k.data_ptr(), v.data_ptr(), n, keys.shape[0], g, d, keys.shape[2], bits,
+              N.DTYPE_CODE[dtype])
+    return k, v
+
+
+def decode_attention(q, keys, values, block_tables, lengths, *, key_scales=None, value_scales=None, starts=None,
+                     window=None, softcap=None, slopes=None, gate=None, scale=None, max_length=None):
+    """Attention of one new token a request over a block cache of 4, 8 or 16 bits
+    that holds it already.  Request r has ``lengths[r]`` cached positions; its token
+    is the last of them and sees those that lie less than ``window`` before it
+    (None: all), not before ``starts[r]`` (int [R], where its document begins) and
+    among the last columns * block of the table.  q [R, H, D] (bf16 / fp16, any
+    token stride; D 64, 128 or 256); keys / values [blocks, G, block, D] in q's
+    dtype, or a ``quantized_cache`` with its scales; position p is row p % block of
+    block ``block_tables[r, p // block % columns]`` (int32 [R, columns]), and is not
+    seen where that is no block of the cache.  Scores are scale q . k (default
+    D ** -0.5), then ``softcap`` tanh(score / softcap), then less ``slopes[h]``
+    (float32 [H]) times the distance.  gate None or [R, H, D] (unit last stride):
+    the result is read * sigmoid(gate).  Returns [R, H, D]; a row that sees nothing
+    (a length of 0 in a captured batch) is zeros.  ``max_length``: no request has
+    more positions (a call of short ones then takes one launch)."""
+    if q.dtype not in (torch.bfloat16, torch.float16) or q.ndim != 3:
+        raise ValueError("decode_attention takes bf16 / fp16 q [R, H, D]")
+    r, h, d = q.shape
+    if d not in (64, 128, 256):
+        raise ValueError("head dim must be 64, 128 or 256")
+    if keys.ndim != 4 or keys.shape[1] < 1 or h < 1 or h % keys.shape[1]:
+        raise ValueError("decode_attention needs keys [blocks, G, block, D] with G dividing the query heads")
+    g = keys.shape[1]
+    bits = _any_cache(keys, values, key_scales, value_scales, g, d, q.dtype)
+    dev = _tree.device_of(q, keys, values, block_tables, key_scales, value_scales, gate, slopes)
+    lens = _tree.ints(lengths, torch.int64, dev, "lengths", r)
+    if starts is not None:
+        starts = _tree.ints(starts, torch.int64, dev, "starts", r)
+    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.shape[0] != r or \
+            block_tables.shape[1] < 1:
+        raise ValueError("block_tables must be int32 [R, columns]")
+    tables = block_tables if block_tables.is_contiguous() else block_tables.contiguous()
+    if window is not None and int(window) < 1:
+        raise ValueError("window must be at least 1")
+    sc = float(d ** -0.5 if scale is None else scale)
+    if not 0 < sc < float("inf"):
+        raise ValueError("scale must be positive")
+    cap = 0.0 if softcap is None else float(softcap)
+    if softcap is not None and not 0 < cap < float("inf"):
+        raise ValueError("softcap must be positive")
+    if slopes is not None:
+        if slopes.dtype != torch.float32 or slopes.shape != (h,):
+            raise ValueError("slopes must be float32 [H]")
+        slopes = slopes.contiguous()
+    q, qs = _heads(q)
+    gp, gts, ghs = None, 0, 0
+    if gate is not None:
+        if gate.shape != (r, h, d) or gate.dtype != q.dtype:
+            raise ValueError("gate must be [R, H, D] in the query dtype")
+        if gate.stride(2) != 1 or gate.stride(1) < d or gate.stride(0) < h * gate.stride(1):   # not rows of heads
+            gate = gate.contiguous()
+        gp = gate.data_ptr()
+        gts, ghs = (h * d, d) if gate.is_contiguous() else (gate.stride(0), gate.stride(1))
+    out = torch.empty(r, h, d, dtype=q.dtype, device=dev)
+    block, columns, win = keys.shape[2], tables.shape[1], 0 if window is None else int(window)
+    longest = -1 if max_length is None else int(max_length)
+    # scratch of the call: concurrent calls on different streams are independent
+    need = N.lib().yh_decode_attention_workspace_bytes(r, h, g, d, block, columns, win, longest)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    N.call_on(dev, "yh_decode_attention", q.data_ptr(), qs, keys.data_ptr(), values.data_ptr(), N.ptr(key_scales),
+              N.ptr(value_scales), tables.data_ptr(), lens.data_ptr(), N.ptr(starts), N.ptr(slopes), gp, gts, ghs,
+              out.data_ptr(), r, keys.shape[0], columns, h, g, d, block, win, longest, sc, cap, bits, N.code(q),
+              N.ptr(ws), need)
+    return out
+
+
+def _head_rows(x):
+    """(x, token stride, head stride) of x [N, heads, D] with 16-byte aligned
+    heads (a column view of a projection qualifies), of a copy otherwise."""
+    n, h, d = x.shape
+    if x.numel() and (x.stride(2) != 1 or (n > 1 and x.stride(0) % 8) or (h > 1 and x.stride(1) % 8) or
+                      x.data_ptr() % 16):
+        x = x.clone(memory_format=torch.contiguous_format)
+    if x.is_contiguous():   # a stride of a single row says nothing
+        return x, h * d, d
+    return x, x.stride(0) if n > 1 else 0, x.stride(1) if h > 1 else 0
+
+
+def qk_norm_rope(q, k, q_w, k_w, positions, inv_freq, eps, *, sections=None, interleaved=False, plus_one=True):
+    """RMSNorm of every query and key head (x / rms(x) * (1 + w), or * w without
+    ``plus_one``; a weight of None: no norm), then rotate-half RoPE of the first
+    2 * len(inv_freq) dims, of both in one launch: q [N, H, D], k [N, G, D] (bf16 /
+    fp16, any token and head strides, D 64, 128 or 256) -> new dense (q, k).
+    positions int [N], or [axes, N] (1 to 4: time, height, width of images and
+    video) with ``sections``, the pairs of each axis: one section behind the other,
+    or ``interleaved``, pair j of axis j % axes while that has pairs left and of
+    axis 0 otherwise.  inv_freq float32, a multiple of 8 of them.  float32
+    throughout and rounded once; the angle in float64, so positions of millions
+    keep theirs (``head_norm_rope`` takes tables, of one axis, and rounds the norm)."""
+    if q.ndim != 3 or k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or \
+            q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype:
+        raise ValueError("qk_norm_rope takes bf16 / fp16 q [N, H, D] and k [N, G, D] of one dtype")
+    (n, h, d), g = q.shape, k.shape[1]
+    if d not in (64, 128, 256):
+        raise ValueError("head dim must be 64, 128 or 256")
+    for w in (q_w, k_w):
+        if w is not None and (w.shape != (d,) or w.dtype != q.dtype):
+            raise ValueError("norm weights must be [D] in the dtype of q and k")
+    if inv_freq.ndim != 1 or inv_freq.dtype != torch.float32 or inv_freq.shape[0] % 8 or 2 * inv_freq.shape[0] > d:
+        raise ValueError("inv_freq must be float32, a multiple of 8 and at most D / 2 of them")
+    if not 0 <= float(eps) < float("inf"):
+        raise ValueError("eps must not be negative")
+    half = inv_freq.shape[0]
+    axes = 1 if positions.ndim == 1 else positions.shape[0] if positions.ndim == 2 else 0
+    if not 1 <= axes <= 4 or positions.shape[-1] != n or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError("positions must be integers [N] or [axes, N] of 1 to 4 axes")
+    if sections is None:
+        if axes > 1:
+            raise ValueError("positions of several axes need their sections")
+        sections = [half]
+    sections = [int(x) for x in sections]
+    if len(sections) != axes or min(sections) < 0 or sum(sections) != half:
+        raise ValueError("sections must hold one count an axis that add up to len(inv_freq)")
+    if interleaved and any(x and i + axes * (x - 1) >= half for i, x in enumerate(sections) if i):
+        raise ValueError("an interleaved section reaches past the pairs")
+    dev = _tree.device_of(q, k, q_w, k_w, inv_freq)
+    pos = positions.to(device=dev, dtype=torch.int64).contiguous()
+    (q, qts, qhs), (k, kts, khs) = _head_rows(q), _head_rows(k)
+    q_w, k_w = (w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else w.clone(
+        memory_format=torch.contiguous_format) for w in (q_w, k_w))
+    freq = inv_freq.contiguous()
+    qo, ko = torch.empty(n, h, d, dtype=q.dtype, device=dev), torch.empty(n, g, d, dtype=q.dtype, device=dev)
+    counts = (ctypes.c_int64 * axes)(*sections)
+    N.call_on(dev, "yh_qk_norm_rope", q.data_ptr(), qts, qhs, k.data_ptr(), kts, khs, N.ptr(q_w), N.ptr(k_w),
+              pos.data_ptr(), freq.data_ptr(), counts, axes, int(bool(interleaved)), qo.data_ptr(), ko.data_ptr(), n, h,
+              g, d, 2 * half, float(eps), int(bool(plus_one)), N.code(q))
+    return qo, ko
