@@ -6,20 +6,27 @@
 //   x_p = q . k_p scale;  x_p = cap tanh(x_p / cap);  x_p -= slope_h (L - 1 - p)
 //   out = sum_p softmax(x)_p v_p (* sigmoid(gate)),  zeros where nothing is seen
 //
-// A wave takes 64 positions of a KV head and up to 16 of its query heads on
-// 16x16x32 MFMA:
-//   S^T = K Q^T      row i of product t is position 4 i + t of the 64, so that the
-//                    lane (head lane % 16, quarter lane / 16) ends with the scores
-//                    of the 16 positions of its quarter
-//   O^T += V^T P^T   that is how the B operand wants P: slot e of quarter c in
-//                    step s is position 16 c + 8 s + e, no lane hands one on
+// A wave takes 16 NT positions of a KV head (NT 4, 2 or 1, as a row is short or
+// long) and up to 16 of its query heads on 16x16x32 MFMA:
+//   S^T = K Q^T      row i of product t is position 16 t + i, so that the lane
+//                    (column lane % 16, quarter lane / 16) ends with the scores of
+//                    positions 16 t + 4 quarter + j
+//   O^T += V^T P^T   and that is where the B operand of step t wants their weights
 // The order of a product's terms is free, so a lane loads K and V rows straight
 // into the places of the A operands, whole pieces of a row (a quarter's D / 4 dims
 // of K, D / 16 dims of V), and nothing goes through LDS.  Codes become bf16 by
-// v_cvt_scalef32, exactly; with fp16 queries, whose 11 bits bf16 does not hold,
-// queries and weights enter as two bf16 each (hi + lo).
+// v_cvt_scalef32, exactly, two dims of a position to a dword.  K wants them so; for
+// V a dword's two slots of the reduction are one position's two dims, so B holds
+// the position's weight in the even slot and zero in the odd one for a column of
+// the even dim, the other way round for the odd dim: with HP <= 8 heads the columns
+// head and head + HP are those two, with 16 heads there are two products.
+// (Transposing the pairs by v_perm instead takes as many instructions as the
+// conversions.)  With HP = 4 the other eight columns take half of the
+// positions, each lane half of the exponentials; their sums join at the end.
+// With fp16 queries over codes, whose 11 bits bf16 does not hold, queries and
+// weights enter as two bf16 each (hi + lo).
 //
-// Requests are few or of very different lengths, so the tiles of 64 positions are
+// Requests are few or of very different lengths, so tiles of 16 NT positions are
 // cut into parts of about one size, which every workgroup finds from the lengths
 // by itself; its four waves take the part's tiles in turn and join their sums in
 // LDS.  Parts of a request that was cut leave theirs, with their maximum, in the
@@ -32,6 +39,14 @@
 #include "qcache.h"
 #include "tree.h"
 
+#ifdef NTL
+#define LD(x) __builtin_nontemporal_load(x)
+#else
+#define LD(x) *(x)
+#endif
+#ifndef MINW
+#define MINW 2
+#endif
 namespace yh {
 namespace {
 
@@ -41,11 +56,16 @@ using attn::bf16x8_t;
 using attn::f16x8_t;
 using attn::bf16x2_t;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 64;        // positions a wave takes at a time
-constexpr int kCols = 16;        // query heads it takes
+constexpr int kCols = 16;        // query heads that a wave takes
+// Products of 16 positions in a tile: as many as keep its keys in 32 registers, and leave room for queries of two parts.
+constexpr int products(int row_bytes, bool pair) {
+  return row_bytes < 128 || (row_bytes == 128 && !pair) ? 4 : row_bytes <= 256 ? 2 : 1;
+}
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -77,6 +97,9 @@ struct DecodeArgs {
   float2* stat;            // [parts][H] maximum and denominator
 };
 
+// Tables through the scalar cache: a run of 16 positions lies in one block.
+typedef __attribute__((address_space(4))) int32_t ConstInt;
+
 // First and last + 1 of the positions that request r sees.
 struct Seen {
   int lo, hi;
@@ -88,10 +111,13 @@ __device__ __forceinline__ Seen seen_of(const DecodeArgs& a, int r) {
   if (a.window && len - a.window > lo) lo = len - a.window;
   if (a.starts && a.starts[r] > lo) lo = a.starts[r];
   if (lo < 0) lo = 0;
-  if (lo >= len || len > 0x7ffff000ll) return {0, 0};
+  if (lo >= len || len > 0x7ffff000ll || a.blocks == 0) return {0, 0};
   return {static_cast<int>(lo), static_cast<int>(len)};
 }
-__device__ __forceinline__ int tiles_of(Seen s) { return s.hi > s.lo ? (s.hi + kTile - 1) / kTile - s.lo / kTile : 0; }
+template <int TILE>
+__device__ __forceinline__ int tiles_of(Seen s) {
+  return s.hi > s.lo ? (s.hi + TILE - 1) / TILE - s.lo / TILE : 0;
+}
 
 // Wave-inclusive sum over lanes.
 __device__ __forceinline__ int scan_wave(int x) {
@@ -111,13 +137,14 @@ struct Part {
 };
 
 // Part `which` of all, found from the lengths; count 0: there is none.
+template <int TILE>
 __device__ Part find_part(const DecodeArgs& a, int which) {
   __shared__ int sums[kWaves], found[4];
   const int t = threadIdx.x, w = t / kWave;
   // a thread takes `each` requests in a row
   const int each = (a.R + kThreads - 1) / kThreads, r0 = t * each, r1 = r0 + each < a.R ? r0 + each : a.R;
   int mine = 0;
-  for (int r = r0; r < r1; ++r) mine += tiles_of(seen_of(a, r));
+  for (int r = r0; r < r1; ++r) mine += tiles_of<TILE>(seen_of(a, r));
   int s = scan_wave(mine);
   if ((t & (kWave - 1)) == kWave - 1) sums[w] = s;
   if (t == 0) found[0] = -1;
@@ -131,7 +158,7 @@ __device__ Part find_part(const DecodeArgs& a, int which) {
   if (chunk < kWaves) chunk = kWaves;
   mine = 0;
   for (int r = r0; r < r1; ++r) {
-    const int n = tiles_of(seen_of(a, r));
+    const int n = tiles_of<TILE>(seen_of(a, r));
     mine += n > chunk ? (n + chunk - 1) / chunk : 1;
   }
   s = scan_wave(mine);
@@ -142,7 +169,7 @@ __device__ Part find_part(const DecodeArgs& a, int which) {
   for (int i = 0; i < kWaves; ++i) at += i < w ? sums[i] : 0;
   if (which >= at && which < at + mine) {
     for (int r = r0; r < r1; ++r) {
-      const int n = tiles_of(seen_of(a, r)), c = n > chunk ? (n + chunk - 1) / chunk : 1;
+      const int n = tiles_of<TILE>(seen_of(a, r)), c = n > chunk ? (n + chunk - 1) / chunk : 1;
       if (which < at + c) {
         found[0] = r;
         found[1] = which - at;
@@ -198,21 +225,23 @@ struct Codes<k16> {
   }
 };
 
-// BYTES bytes (2 to 64) into dwords.
+// BYTES bytes (1 to 64) into dwords.
 template <int BYTES>
 __device__ __forceinline__ void load_bytes(uint32_t* w, const char* p) {
-  if constexpr (BYTES == 2) {
+  if constexpr (BYTES == 1) {
+    w[0] = *reinterpret_cast<const uint8_t*>(p);
+  } else if constexpr (BYTES == 2) {
     w[0] = *reinterpret_cast<const uint16_t*>(p);
   } else if constexpr (BYTES == 4) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
+    w[0] = LD(reinterpret_cast<const uint32_t*>(p));
   } else if constexpr (BYTES == 8) {
-    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+    const u32x2 x = LD(reinterpret_cast<const u32x2*>(p));
     w[0] = x[0];
     w[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < BYTES / 16; ++i) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(p + 16 * i);
+      const u32x4 x = LD(reinterpret_cast<const u32x4*>(p + 16 * i));
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
     }
@@ -235,6 +264,14 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
+// With four positions of each quarter.
+template <int MT>
+__device__ __forceinline__ f32x4 mfma(u32x2 a, u32x2 b, f32x4 c) {
+  if constexpr (MT == YH_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+}
 // The compiler puts no wait where a matrix result is first read behind branches that meet.
 template <int N>
 __device__ __forceinline__ void settle(f32x4 (&x)[N]) {
@@ -245,10 +282,12 @@ __device__ __forceinline__ void settle(f32x4 (&x)[N]) {
   for (int i = 1; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 
-template <int DT, int FMT, int D, bool RUNS>
-__global__ void __launch_bounds__(kThreads) decode_attention_kernel(DecodeArgs a) {
+template <int DT, int FMT, int D, int HP, bool RUNS>
+__global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(DecodeArgs a) {
   using C = Codes<FMT>;
+  using M = attn::Mfma<DT>;
   constexpr int MT = FMT == k16 ? DT : YH_BF16;
+  using P = attn::Mfma<MT>;
   constexpr bool kPair = FMT != k16 && DT == YH_F16;    // queries and weights as hi + lo
   constexpr int kRow = D * C::kBits / 8;                // bytes of a row
   constexpr int kKd = D / 4, kVd = D / 16;              // dims of a lane: K, V
@@ -256,22 +295,28 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(DecodeArgs a
   constexpr int kKw = (kKb + 3) / 4, kVw = (kVb + 3) / 4;
   constexpr int kKs = kKd > kRun ? kKd / kRun : 1;      // scales of a lane's K dims
   constexpr int kSteps = D / 32;                        // products over the dims
-  using M = attn::Mfma<DT>;
-  __shared__ float2 wave_stat[kWaves][kCols];
-  __shared__ float wave_acc[kWaves][kCols][D + 4];
+  constexpr int NT = products(kRow, kPair && D == 256), kTile = 16 * NT, kU = 4 * NT;   // kU: positions of a quarter
+  constexpr int kSel = HP == 16 || FMT == k16 ? 1 : 2;               // columns of a head: two dims, halves of the positions
+  constexpr int kHalves = HP == 16 ? 1 : 2 * 8 / (HP * kSel);
+  constexpr int kAcc = kVd / kSel, kMine = kU / kHalves;             // positions whose weights a lane forms
+  __shared__ float2 wave_stat[kWaves][kHalves][HP];
+  __shared__ float wave_acc[kWaves][kHalves][HP][D + 4];
 
   const int g = blockIdx.x % a.G, mt = blockIdx.x / a.G % a.mtiles;
-  const Part part = find_part(a, blockIdx.x / a.G / a.mtiles);
+  const Part part = find_part<kTile>(a, blockIdx.x / a.G / a.mtiles);
   if (part.count == 0) return;
-  const int r = part.r;
+  // the whole workgroup's
+  const int r = __builtin_amdgcn_readfirstlane(part.r), tiles = __builtin_amdgcn_readfirstlane(part.tiles);
+  const int lo = __builtin_amdgcn_readfirstlane(part.seen.lo), hi = __builtin_amdgcn_readfirstlane(part.seen.hi);
   if (a.first && part.index == 0 && g == 0 && mt == 0 && threadIdx.x == 0) {
     a.first[r] = part.slot;
     if (r == a.R - 1) a.first[a.R] = part.slot + part.count;
   }
 
   const int lane = threadIdx.x & (kWave - 1), w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int col = lane & 15, quarter = lane >> 4;
-  const int cols = a.rep - mt * kCols < kCols ? a.rep - mt * kCols : kCols;
+  const int quarter = lane >> 4, piece = lane & 15;     // piece: the lane's part of a V row, its position of K rows
+  const int col = piece % HP, sel = piece / HP % kSel, half = piece / (HP * kSel);
+  const int cols = a.rep - mt * kCols < HP ? a.rep - mt * kCols : HP;
   const int head = g * a.rep + mt * kCols + (col < cols ? col : 0);
 
   // the queries as the B operand: column `col`, dims as the K rows have them
@@ -294,240 +339,285 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(DecodeArgs a
     }
   }
   // scores in powers of two
+  const bool plain = a.cap == 0.f && !a.slopes;
   const float mul = a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : kLog2e * a.scale;
   const float cap2 = a.cap * kLog2e, slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+  // which of a dword's two slots holds a weight in this lane's column
+  const uint32_t slot_mask = kSel == 1 ? 0u : sel ? 0xffff0000u : 0xffffu;
 
   float top = kFloor, den = 0.f;
-  f32x4 acc[kVd];
+  f32x4 acc[kAcc];
 #pragma unroll
-  for (int n = 0; n < kVd; ++n) acc[n] = f32x4{0, 0, 0, 0};
+  for (int n = 0; n < kAcc; ++n) acc[n] = f32x4{0, 0, 0, 0};
 
-  const int32_t* table = a.tables + static_cast<int64_t>(r) * a.columns.d;
-  // the row (of all rows of all heads) of position p, < 0 where the table holds no block
-  auto row_of = [&](int p) -> int64_t {
-    const uint32_t b = a.block.quot(p), c = b - a.columns.quot(b) * a.columns.d;
-    const int id = table[c];
-    return id < 0 || id >= a.blocks ? -1 : (static_cast<int64_t>(id) * a.G + g) * a.block.d + (p - b * a.block.d);
+  const ConstInt* table = (const ConstInt*)(a.tables + static_cast<int64_t>(r) * a.columns.d);
+  auto id_of = [&](int p) {      // the table's entry for position p
+    const uint32_t b = a.block.quot(p);
+    return table[b - a.columns.quot(b) * a.columns.d];
   };
-  // of its scale, run `run` of the dims
-  auto scale_at = [&](int64_t row, int p, int run) -> int64_t {
+  // The row of all rows of all heads, and where its scale of run 0 lies.  An entry that is no block of the cache leads
+  // to row 0, whose contents are masked.
+  struct Row {
+    int64_t row, scale;
+    bool hole;
+  };
+  auto row_of = [&](int id, int p) -> Row {
     const uint32_t in = p - a.block.quot(p) * a.block.d;
-    return (row - in) * (D / kRun) + static_cast<int64_t>(run) * a.block.d + in;
+    const bool hole = id < 0 || id >= a.blocks;
+    const int64_t first = hole ? 0 : (static_cast<int64_t>(id) * a.G + g) * a.block.d;
+    return {hole ? 0 : first + in, first * (D / kRun) + (hole ? 0 : in), hole};
   };
-  const int first_tile = part.seen.lo / kTile + part.tile;
+  const int first_tile = lo / kTile + __builtin_amdgcn_readfirstlane(part.tile);
 
-  for (int i = w; i < part.tiles; i += kWaves) {
-    const int base = (first_tile + i) * kTile;
-    const int pk = base + 4 * col, pv = base + 16 * quarter;      // the lane's positions: 4 of K, 16 of V
-    uint32_t kw[4][kKw], vw[16][kVw];
-    uint32_t ksc[kKs], vsc[4];      // scale bytes of 4 and 16 positions
-    uint32_t khole = 0, vhole = 0;  // positions without a block
-    if constexpr (RUNS) {
-      const int64_t krow = row_of(pk), vrow = row_of(pv);
-      if (krow < 0) {
-        khole = 15;
+  // The lane's positions of product t, of 16 t on: `piece` of K, 4 quarter + j of V.
+  uint32_t kw[NT][kKw], vw[kU][kVw];
+  uint32_t ksc[NT][kKs], vsc[NT];      // scale bytes of a K position, of four V positions
+  uint32_t vhole = 0;                  // V's positions without a block
+  int id[NT];                          // table entries of the next tile, where blocks hold whole runs of 16 positions
+  const uint32_t k_off = RUNS ? piece * kRow + (FMT == k16 ? quarter * 16 : quarter * kKb) : 0;
+  const uint32_t v_off = RUNS ? 4 * quarter * kRow + piece * kVb : 0;
+  const uint32_t ks_off = RUNS ? (quarter * kKd / kRun) * a.block.d + piece : 0;
+  const uint32_t vs_off = RUNS ? (piece * kVd / kRun) * a.block.d + 4 * quarter : 0;
+  auto k_row = [&](int t, const char* p) {
+    if constexpr (FMT == k16) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int e = 0; e < kKw; ++e) kw[t][e] = 0;
-#pragma unroll
-        for (int e = 0; e < kKs; ++e) ksc[e] = 0x7f7f7f7fu;
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const char* p = a.keys + (krow + t) * kRow;
-          if constexpr (FMT == k16) {
-#pragma unroll
-            for (int c = 0; c < kSteps; ++c) load_bytes<16>(kw[t] + 4 * c, p + (32 * c + 8 * quarter) * 2);
-          } else {
-            load_bytes<kKb>(kw[t], p + quarter * kKb);
-          }
-        }
-        if constexpr (FMT != k16) {
-#pragma unroll
-          for (int e = 0; e < kKs; ++e)
-            ksc[e] = *reinterpret_cast<const uint32_t*>(a.key_scales + scale_at(krow, pk, quarter * kKd / kRun + e));
-        }
-      }
-      if (vrow < 0) {
-        vhole = 0xffff;
-#pragma unroll
-        for (int u = 0; u < 16; ++u)
-#pragma unroll
-          for (int e = 0; e < kVw; ++e) vw[u][e] = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vsc[e] = 0x7f7f7f7fu;
-      } else {
-#pragma unroll
-        for (int u = 0; u < 16; ++u) load_bytes<kVb>(vw[u], a.values + (vrow + u) * kRow + col * kVb);
-        if constexpr (FMT != k16) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(a.value_scales + scale_at(vrow, pv, col * kVd / kRun));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vsc[e] = x[e];
-        }
-      }
+      for (int c = 0; c < kSteps; ++c) load_bytes<16>(kw[t] + 4 * c, p + 64 * c);
     } else {
+      load_bytes<kKb>(kw[t], p);
+    }
+  };
+  auto load_k = [&](int i) {
 #pragma unroll
-      for (int e = 0; e < kKs; ++e) ksc[e] = 0;
+    for (int t = 0; t < NT; ++t) {
+      const int p = (first_tile + i) * kTile + 16 * t;
+      if constexpr (RUNS) {      // the run's block is the whole wave's
+        const Row at = row_of(id[t], p);
+        k_row(t, a.keys + at.row * kRow + k_off);
+        if constexpr (FMT != k16) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) vsc[e] = 0;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int64_t row = row_of(pk + t);
-        if (row < 0) {
-          khole |= 1u << t;
-#pragma unroll
-          for (int e = 0; e < kKw; ++e) kw[t][e] = 0;
-          continue;
+          for (int e = 0; e < kKs; ++e) ksc[t][e] = *(a.key_scales + at.scale + e * static_cast<int64_t>(a.block.d) + ks_off);
         }
-        const char* p = a.keys + row * kRow;
-        if constexpr (FMT == k16) {
-#pragma unroll
-          for (int c = 0; c < kSteps; ++c) load_bytes<16>(kw[t] + 4 * c, p + (32 * c + 8 * quarter) * 2);
-        } else {
-          load_bytes<kKb>(kw[t], p + quarter * kKb);
+      } else {
+        const Row at = row_of(id_of(p + piece), p + piece);
+        k_row(t, a.keys + at.row * kRow + (FMT == k16 ? quarter * 16 : quarter * kKb));
+        if constexpr (FMT != k16) {
 #pragma unroll
           for (int e = 0; e < kKs; ++e)
-            ksc[e] |= static_cast<uint32_t>(a.key_scales[scale_at(row, pk + t, quarter * kKd / kRun + e)]) << (8 * t);
+            ksc[t][e] = a.key_scales[at.scale + static_cast<int64_t>(quarter * kKd / kRun + e) * a.block.d];
         }
-      }
-#pragma unroll
-      for (int u = 0; u < 16; ++u) {
-        const int64_t row = row_of(pv + u);
-        if (row < 0) {
-          vhole |= 1u << u;
-#pragma unroll
-          for (int e = 0; e < kVw; ++e) vw[u][e] = 0;
-          continue;
-        }
-        load_bytes<kVb>(vw[u], a.values + row * kRow + col * kVb);
-        if constexpr (FMT != k16)
-          vsc[u / 4] |= static_cast<uint32_t>(a.value_scales[scale_at(row, pv + u, col * kVd / kRun)]) << (8 * (u % 4));
       }
     }
-
-    // S^T, product t: positions 4 i + t
-    f32x4 s[4];
+  };
+  auto load_v = [&](int i) {
+    vhole = 0;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < NT; ++t) {
+      const int p = (first_tile + i) * kTile + 16 * t;
+      if constexpr (RUNS) {
+        const Row at = row_of(id[t], p);
+        vhole |= at.hole ? 15u << (4 * t) : 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) load_bytes<kVb>(vw[4 * t + j], a.values + at.row * kRow + v_off + j * kRow);
+        if constexpr (FMT != k16) vsc[t] = *reinterpret_cast<const uint32_t*>(a.value_scales + at.scale + vs_off);
+      } else {
+        vsc[t] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at_p = p + 4 * quarter + j;
+          const Row at = row_of(id_of(at_p), at_p);
+          vhole |= at.hole ? 1u << (4 * t + j) : 0u;
+          load_bytes<kVb>(vw[4 * t + j], a.values + at.row * kRow + piece * kVb);
+          if constexpr (FMT != k16)
+            vsc[t] |= static_cast<uint32_t>(a.value_scales[at.scale + static_cast<int64_t>(piece * kVd / kRun) * a.block.d])
+                      << (8 * j);
+        }
+      }
+    }
+  };
+  auto load_ids = [&](int i) {
+    if constexpr (RUNS) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) id[t] = id_of((first_tile + i) * kTile + 16 * t);
+    }
+  };
+
+  // Loads run ahead of their use: a tile's keys while the tile before is turned into weights and sums, its values
+  // while its own scores form, table entries a tile ahead.
+  if (w < tiles) {
+    load_ids(w);
+    load_k(w);
+    load_v(w);
+    if (w + kWaves < tiles) load_ids(w + kWaves);
+  }
+  for (int i = w; i < tiles; i += kWaves) {
+    const int base = (first_tile + i) * kTile;
+    const bool more = i + kWaves < tiles;
+
+    // S^T, product t: positions 16 t on
+    f32x4 s[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
       s[t] = f32x4{0, 0, 0, 0};
       each<0, kSteps>([&](auto step) {
         constexpr int ST = decltype(step)::value;
         u32x4 x;
-        const float sc = FMT == k16 ? 1.f : scale_value((ksc[ST * 8 / kRun] >> (8 * t)) & 0xff);
-        each<0, 4>([&](auto pair) { x[decltype(pair)::value] = C::template two<4 * ST + decltype(pair)::value>(kw[t], sc); });
+        const float sc = FMT == k16 ? 1.f : scale_value(ksc[t][ST * 8 / kRun]);
+        each<0, 4>([&](auto pair) {
+          constexpr int I = decltype(pair)::value;
+          x[I] = C::template two<4 * ST + I>(kw[t], sc);
+        });
         s[t] = mfma<MT>(x, qh[ST], s[t]);
         if constexpr (kPair) s[t] = mfma<MT>(x, ql[ST], s[t]);
       });
     }
     settle(s);
+    if (more) load_k(i + kWaves);
 
-    // what of the 16 positions of this quarter is seen; value u = 4 j + t is s[t][j]
-    uint32_t dead = vhole;
-    const bool inside = base >= part.seen.lo && base + kTile <= part.seen.hi;
-    if (!inside) {
+    // u = 4 t + j is position 16 t + 4 quarter + j, its score s[t][j]; with halves a lane has j = 2 half + {0, 1}
+    const int own = 4 * quarter + (kHalves == 2 ? 2 * half : 0);
+    auto step_of = [](int u) { return kHalves == 2 ? 16 * (u / 2) + u % 2 : 16 * (u / 4) + u % 4; };
+    float x[kMine];
 #pragma unroll
-      for (int u = 0; u < 16; ++u) dead |= pv + u < part.seen.lo || pv + u >= part.seen.hi ? 1u << u : 0u;
+    for (int u = 0; u < kMine; ++u)
+      x[u] = kHalves == 2 ? (half ? s[u / 2][2 + u % 2] : s[u / 2][u % 2]) : s[u / 4][u % 4];
+    if (a.cap > 0.f) {
+#pragma unroll
+      for (int u = 0; u < kMine; ++u)
+        x[u] = cap2 * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x[u] * mul) + 1.f));
     }
-    const bool masked = __ballot(dead != 0) != 0;
-    float x[16];
+    if (a.slopes) {
+      const float back = static_cast<float>(hi - 1 - base - own), f = a.cap > 0.f ? 1.f : mul;
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
-      float y = s[u % 4][u / 4] * mul;
-      if (a.cap > 0.f) y = cap2 * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y) + 1.f));
-      x[u] = a.slopes ? y - slope * static_cast<float>(part.seen.hi - 1 - pv - u) : y;
+      for (int u = 0; u < kMine; ++u) x[u] = x[u] * f - slope * (back - static_cast<float>(step_of(u)));
     }
-    if (masked) {
-      // what is not seen may be anything: its values are cleared too
+    uint32_t dead = vhole;     // what of the quarter is not seen
+    if (base < lo || base + kTile > hi) {
 #pragma unroll
-      for (int u = 0; u < 16; ++u)
+      for (int u = 0; u < kU; ++u) {
+        const int p = base + 16 * (u / 4) + 4 * quarter + u % 4;
+        dead |= p < lo || p >= hi ? 1u << u : 0u;
+      }
+    }
+    if (__ballot(dead != 0)) {
+      // it may be anything: its values are cleared too
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
         if (dead >> u & 1) {
-          x[u] = -INFINITY;
 #pragma unroll
           for (int e = 0; e < kVw; ++e) vw[u][e] = 0;
           vsc[u / 4] = (vsc[u / 4] & ~(0xffu << (8 * (u % 4)))) | 0x7fu << (8 * (u % 4));
         }
+      const uint32_t gone = kHalves == 2 ? dead >> (2 * half) : dead;
+#pragma unroll
+      for (int u = 0; u < kMine; ++u)
+        x[u] = gone >> (kHalves == 2 ? 4 * (u / 2) + u % 2 : u) & 1 ? -INFINITY : x[u];
     }
     float m = x[0];
 #pragma unroll
-    for (int u = 1; u < 16; ++u) m = fmaxf(m, x[u]);
+    for (int u = 1; u < kMine; ++u) m = fmaxf(m, x[u]);
     m = fmaxf(m, __shfl_xor(m, 16, kWave));
     m = fmaxf(m, __shfl_xor(m, 32, kWave));
+    const float unit = plain ? mul : 1.f;      // x is in scores, or in powers of two already
+    m *= unit;
     if (__ballot(m > top)) {
       const float next = fmaxf(top, m), f = __builtin_amdgcn_exp2f(top - next);
       top = next;
       den *= f;
 #pragma unroll
-      for (int n = 0; n < kVd; ++n) acc[n] *= f;
+      for (int n = 0; n < kAcc; ++n) acc[n] *= f;
     }
+    const float low = MT == YH_F16 ? kLift - top : -top;
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
-      x[u] = __builtin_amdgcn_exp2f(x[u] - (MT == YH_F16 ? top - kLift : top));
+    for (int u = 0; u < kMine; ++u) {
+      x[u] = __builtin_amdgcn_exp2f(fmaf(x[u], unit, low));
       den += x[u];
     }
-    // P^T as the B operand, step st: positions 8 st + e of the quarter
-    u32x4 ph[2], pl[2];
+    // O^T: step st takes positions 16 st + 4 quarter + e, product n dims 2 n and 2 n + 1 of each lane's kVd
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
+    for (int st = 0; st < NT; ++st) {
+      if constexpr (FMT == k16) {
+        u32x2 ph;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = kHalves == 2 ? 2 * st : 4 * st + 2 * e;
+          ph[e] = P::round2(x[at], x[at + 1]);
+          if (kHalves == 2 && half != e) ph[e] = 0;
+        }
+        each<0, kVd / 2>([&](auto pair) {
+          constexpr int I = decltype(pair)::value;
+          u32x2 lo, hi;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            lo[e] = __builtin_amdgcn_perm(vw[4 * st + 2 * e + 1][I], vw[4 * st + 2 * e][I], 0x05040100u);
+            hi[e] = __builtin_amdgcn_perm(vw[4 * st + 2 * e + 1][I], vw[4 * st + 2 * e][I], 0x07060302u);
+          }
+          acc[2 * I] = mfma<MT>(lo, ph, acc[2 * I]);
+          acc[2 * I + 1] = mfma<MT>(hi, ph, acc[2 * I + 1]);
+        });
+        continue;
+      }
+      u32x4 ph[2], pl[2];      // [1]: the odd dim's with one column a head
+      float sc[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x0 = x[8 * st + 2 * e], x1 = x[8 * st + 2 * e + 1];
-        ph[st][e] = attn::Mfma<MT>::round2(x0, x1);
-        if constexpr (kPair)
-          pl[st][e] = attn::Mfma<MT>::round2(x0 - __uint_as_float(ph[st][e] << 16),
-                                             x1 - __uint_as_float(ph[st][e] & 0xffff0000u));
-      }
-    // O^T: product n takes dim n of each lane's kVd
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      float sc[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        sc[e] = FMT == k16 ? 1.f : scale_value((vsc[2 * st + e / 4] >> (8 * (e % 4))) & 0xff);
-      each<0, kVd / 2>([&](auto pair) {
-        constexpr int P = decltype(pair)::value;
-        u32x4 lo, hi;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t y0 = C::template two<P>(vw[8 * st + 2 * e], sc[2 * e]);
-          const uint32_t y1 = C::template two<P>(vw[8 * st + 2 * e + 1], sc[2 * e + 1]);
-          lo[e] = __builtin_amdgcn_perm(y1, y0, 0x05040100u);
-          hi[e] = __builtin_amdgcn_perm(y1, y0, 0x07060302u);
+        const float y = x[kHalves == 2 ? 2 * st + e % 2 : 4 * st + e];
+        const uint32_t hi = P::round2(y, y);
+        const uint32_t lo = kPair ? P::round2(y - __uint_as_float(hi & 0xffff0000u), y - __uint_as_float(hi & 0xffff0000u)) : 0u;
+        if constexpr (kSel == 2) {
+          const uint32_t mask = kHalves == 2 ? (half == e / 2 ? slot_mask : 0u) : slot_mask;
+          ph[0][e] = hi & mask;
+          pl[0][e] = lo & mask;
+        } else {
+          ph[0][e] = hi & 0xffffu;
+          ph[1][e] = hi & 0xffff0000u;
+          pl[0][e] = lo & 0xffffu;
+          pl[1][e] = lo & 0xffff0000u;
         }
-        acc[2 * P] = mfma<MT>(lo, ph[st], acc[2 * P]);
-        acc[2 * P + 1] = mfma<MT>(hi, ph[st], acc[2 * P + 1]);
-        if constexpr (kPair) {
-          acc[2 * P] = mfma<MT>(lo, pl[st], acc[2 * P]);
-          acc[2 * P + 1] = mfma<MT>(hi, pl[st], acc[2 * P + 1]);
+        sc[e] = scale_value((vsc[st] >> (8 * e)) & 0xff);
+      }
+      each<0, kVd / 2>([&](auto pair) {
+        constexpr int I = decltype(pair)::value;
+        u32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = C::template two<I>(vw[4 * st + e], sc[e]);
+#pragma unroll
+        for (int n = 0; n < 2 / kSel; ++n) {
+          acc[2 / kSel * I + n] = mfma<MT>(v, ph[n], acc[2 / kSel * I + n]);
+          if constexpr (kPair) acc[2 / kSel * I + n] = mfma<MT>(v, pl[n], acc[2 / kSel * I + n]);
         }
       });
     }
-    settle(acc);
+    if (more) {
+      load_v(i + kWaves);
+      if (i + 2 * kWaves < tiles) load_ids(i + 2 * kWaves);
+    }
   }
+  settle(acc);
 
-  // the waves' sums: lane (col, quarter) has dims (4 quarter + j) kVd + n of column col in acc[n][j]
+  // the waves' sums: lane (column, quarter) has dims (4 quarter + j) kVd + 2 n + sel, or + n, of its head in acc[n][j]
   den += __shfl_xor(den, 16, kWave);
   den += __shfl_xor(den, 32, kWave);
-  if (quarter == 0) wave_stat[w][col] = make_float2(top, den);
+  if (quarter == 0 && sel == 0) wave_stat[w][half][col] = make_float2(top, den);
   if (col < cols) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int n = 0; n < kVd; ++n) wave_acc[w][col][(4 * quarter + j) * kVd + n] = acc[n][j];
+      for (int n = 0; n < kAcc; ++n) wave_acc[w][half][col][(4 * quarter + j) * kVd + kSel * n + sel] = acc[n][j];
   }
   __syncthreads();
   for (int at = threadIdx.x; at < cols * (D / 4); at += kThreads) {
     const int c = at / (D / 4), dim = at % (D / 4) * 4;
     float m = kFloor;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) m = fmaxf(m, wave_stat[i][c].x);
+    for (int i = 0; i < kWaves * kHalves; ++i) m = fmaxf(m, wave_stat[i / kHalves][i % kHalves][c].x);
     float dn = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const float f = __builtin_amdgcn_exp2f(wave_stat[i][c].x - m);
-      dn = fmaf(wave_stat[i][c].y, f, dn);
+    for (int i = 0; i < kWaves * kHalves; ++i) {
+      const float2 st = wave_stat[i / kHalves][i % kHalves][c];
+      const float f = __builtin_amdgcn_exp2f(st.x - m);
+      dn = fmaf(st.y, f, dn);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(wave_acc[i][c][dim + e], f, o[e]);
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(wave_acc[i / kHalves][i % kHalves][c][dim + e], f, o[e]);
     }
     const int hd = g * a.rep + mt * kCols + c;
     if (part.count > 1) {
@@ -549,19 +639,24 @@ __global__ void __launch_bounds__(kThreads) decode_attention_kernel(DecodeArgs a
   }
 }
 
-// The parts of the cut requests joined in order, D / 4 lanes a head.
+// The parts of a cut request joined: a workgroup a head, D / 4 lanes a part, the others take every kShares-th part;
+// their sums meet in LDS, in order.
 template <int DT, int D>
 __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
   using M = attn::Mfma<DT>;
-  constexpr int kLanes = D / 4, kHeads = kThreads / kLanes;
-  const int r = blockIdx.x, hd = blockIdx.y * kHeads + threadIdx.x / kLanes, dim = threadIdx.x % kLanes * 4;
+  constexpr int kLanes = D / 4, kShares = kThreads / kLanes;
+  __shared__ float sums[kShares][D + 4], dens[kShares], tops[kShares];
+  const int r = blockIdx.x / a.H, hd = blockIdx.x % a.H;
+  const int share = threadIdx.x / kLanes, dim = threadIdx.x % kLanes * 4;
   const int first = a.first[r], count = a.first[r + 1] - first;
-  if (count <= 1 || hd >= a.H) return;
+  if (count <= 1) return;
   const int64_t slot = static_cast<int64_t>(first) * a.H + hd;
   float m = kFloor;
-  for (int j = 0; j < count; ++j) m = fmaxf(m, a.stat[slot + static_cast<int64_t>(j) * a.H].x);
+#pragma unroll 4
+  for (int j = share; j < count; j += kShares) m = fmaxf(m, a.stat[slot + static_cast<int64_t>(j) * a.H].x);
   float dn = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < count; ++j) {
+#pragma unroll 4
+  for (int j = share; j < count; j += kShares) {
     const int64_t s = slot + static_cast<int64_t>(j) * a.H;
     const float2 st = a.stat[s];
     const float4 x = *reinterpret_cast<const float4*>(a.part + s * D + dim);
@@ -571,6 +666,26 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
     o[1] = fmaf(x.y, f, o[1]);
     o[2] = fmaf(x.z, f, o[2]);
     o[3] = fmaf(x.w, f, o[3]);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sums[share][dim + e] = o[e];
+  if (dim == 0) {
+    dens[share] = dn;
+    tops[share] = m;
+  }
+  __syncthreads();
+  if (share) return;
+#pragma unroll
+  for (int i = 0; i < kShares; ++i) m = fmaxf(m, tops[i]);
+  dn = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < kShares; ++i) {
+    const float f = __builtin_amdgcn_exp2f(tops[i] - m);
+    dn = fmaf(dens[i], f, dn);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(sums[i][dim + e], f, o[e]);
   }
   const float inv = dn > 0.f || dn != dn ? 1.f / dn : 0.f;
   const int64_t to = (static_cast<int64_t>(r) * a.H + hd) * D + dim;
@@ -584,14 +699,17 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
   *reinterpret_cast<u32x2*>(a.out + to) = u32x2{attn::pack2(y[0], y[1]), attn::pack2(y[2], y[3])};
 }
 
-constexpr int kWorkgroups = 1024;     // parts aimed at, over all heads: four workgroups a CU
+#ifndef WGS
+#define WGS 1024
+#endif
+constexpr int kWorkgroups = WGS;     // parts aimed at, over all heads: four workgroups a CU
 
 // Parts aimed at for each KV head, 0 where no request is cut.
 int64_t target_for(int64_t R, int64_t H, int64_t G, int64_t block, int64_t columns, int64_t window, int64_t max_length) {
   int64_t most = columns * block;
   if (window && window < most) most = window;
   if (max_length >= 0 && max_length < most) most = max_length;
-  if (most + kTile - 1 <= kWaves * kTile) return 0;     // a turn of the waves at most
+  if (most + 63 <= 64 * kWaves) return 0;     // a turn of the waves at most, where tiles have 64 positions
   const int64_t each = G * ((H / G + kCols - 1) / kCols), n = (kWorkgroups + each - 1) / each;
   return n < 1 ? 1 : n;
 }
@@ -599,14 +717,15 @@ int64_t plan_bytes(int64_t R) { return ((R + 1) * 4 + 255) / 256 * 256; }
 
 template <int DT, int FMT, int D>
 void launch(const DecodeArgs& a, unsigned grid, hipStream_t st) {
-  if (a.block.d % 16 == 0)
-    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, true>), dim3(grid), dim3(kThreads), 0, st, a);
+  if (a.block.d % 16)
+    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, 16, false>), dim3(grid), dim3(kThreads), 0, st, a);
+  else if (a.rep <= 4 && FMT != k16)
+    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, FMT == k16 ? 8 : 4, true>), dim3(grid), dim3(kThreads), 0, st, a);
+  else if (a.rep <= 8)
+    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, 8, true>), dim3(grid), dim3(kThreads), 0, st, a);
   else
-    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, false>), dim3(grid), dim3(kThreads), 0, st, a);
-  if (a.target) {
-    constexpr int kHeads = kThreads / (D / 4);
-    hipLaunchKernelGGL((decode_join_kernel<DT, D>), dim3(a.R, (a.H + kHeads - 1) / kHeads), dim3(kThreads), 0, st, a);
-  }
+    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, 16, true>), dim3(grid), dim3(kThreads), 0, st, a);
+  if (a.target) hipLaunchKernelGGL((decode_join_kernel<DT, D>), dim3(a.R * a.H), dim3(kThreads), 0, st, a);
 }
 template <int DT, int FMT>
 void launch_dim(const DecodeArgs& a, int64_t D, unsigned grid, hipStream_t st) {
@@ -668,9 +787,9 @@ extern "C" int yh_decode_attention(const void* q, int64_t q_stride, const void* 
   const int64_t target = target_for(n_seqs, H, G, block, columns, window, max_length);
   int64_t most = columns * block;
   if (window && window < most) most = window;
-  YH_CHECK_ARG(n_seqs * (most / kTile + 2) < (1ll << 31), "decode_attention: sizes too large");
+  YH_CHECK_ARG(n_seqs * (most / 16 + 2) < (1ll << 31), "decode_attention: sizes too large");
   const int64_t grid = (n_seqs + target) * each;
-  YH_CHECK_ARG(grid < (1ll << 24), "decode_attention: sizes too large");
+  YH_CHECK_ARG(grid < (1ll << 24) && n_seqs * H < (1ll << 24), "decode_attention: sizes too large");
   const int64_t need = yh_decode_attention_workspace_bytes(n_seqs, H, G, D, block, columns, window, max_length);
   YH_CHECK_ARG(need == 0 || (workspace && tree::aligned16(workspace) && workspace_bytes >= need),
                "decode_attention: workspace too small");
