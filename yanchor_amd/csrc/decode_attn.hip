@@ -39,14 +39,6 @@
 #include "qcache.h"
 #include "tree.h"
 
-#ifdef NTL
-#define LD(x) __builtin_nontemporal_load(x)
-#else
-#define LD(x) *(x)
-#endif
-#ifndef MINW
-#define MINW 2
-#endif
 namespace yh {
 namespace {
 
@@ -197,7 +189,9 @@ __device__ Part find_part(const DecodeArgs& a, int which) {
   return p;
 }
 
-// Two dims of one position's codes to bf16, `half` the pair within a dword.
+// Two dims of one position's codes to bf16 under the scale 2^(s - 127), given as a float whose exponent s is: the
+// conversion takes no more of it, and makes NaN of any code under s = 255.
+__device__ __forceinline__ float exponent(uint32_t s) { return __uint_as_float(s << 23); }
 template <int FMT>
 struct Codes;
 template <>
@@ -233,15 +227,15 @@ __device__ __forceinline__ void load_bytes(uint32_t* w, const char* p) {
   } else if constexpr (BYTES == 2) {
     w[0] = *reinterpret_cast<const uint16_t*>(p);
   } else if constexpr (BYTES == 4) {
-    w[0] = LD(reinterpret_cast<const uint32_t*>(p));
+    w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
   } else if constexpr (BYTES == 8) {
-    const u32x2 x = LD(reinterpret_cast<const u32x2*>(p));
+    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
     w[0] = x[0];
     w[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < BYTES / 16; ++i) {
-      const u32x4 x = LD(reinterpret_cast<const u32x4*>(p + 16 * i));
+      const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 16 * i));
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
     }
@@ -283,7 +277,7 @@ __device__ __forceinline__ void settle(f32x4 (&x)[N]) {
 }
 
 template <int DT, int FMT, int D, int HP, bool RUNS>
-__global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) decode_attention_kernel(DecodeArgs a) {
   using C = Codes<FMT>;
   using M = attn::Mfma<DT>;
   constexpr int MT = FMT == k16 ? DT : YH_BF16;
@@ -356,24 +350,23 @@ __global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(Decode
     return table[b - a.columns.quot(b) * a.columns.d];
   };
   // The row of all rows of all heads, and where its scale of run 0 lies.  An entry that is no block of the cache leads
-  // to row 0, whose contents are masked.
+  // to block 0, whose contents are masked.
   struct Row {
     int64_t row, scale;
-    bool hole;
   };
+  auto is_block = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.blocks); };
   auto row_of = [&](int id, int p) -> Row {
     const uint32_t in = p - a.block.quot(p) * a.block.d;
-    const bool hole = id < 0 || id >= a.blocks;
-    const int64_t first = hole ? 0 : (static_cast<int64_t>(id) * a.G + g) * a.block.d;
-    return {hole ? 0 : first + in, first * (D / kRun) + (hole ? 0 : in), hole};
+    const int64_t first = (static_cast<int64_t>(is_block(id) ? id : 0) * a.G + g) * a.block.d;
+    return {first + in, first * (D / kRun) + in};
   };
   const int first_tile = lo / kTile + __builtin_amdgcn_readfirstlane(part.tile);
 
   // The lane's positions of product t, of 16 t on: `piece` of K, 4 quarter + j of V.
   uint32_t kw[NT][kKw], vw[kU][kVw];
   uint32_t ksc[NT][kKs], vsc[NT];      // scale bytes of a K position, of four V positions
-  uint32_t vhole = 0;                  // V's positions without a block
-  int id[NT];                          // table entries of the next tile, where blocks hold whole runs of 16 positions
+  Row rows[NT];                        // of the next tile's products, where blocks hold whole runs of 16 positions
+  uint32_t holes = 0, vhole = 0;       // V's positions without a block: of the next tile, of this one
   const uint32_t k_off = RUNS ? piece * kRow + (FMT == k16 ? quarter * 16 : quarter * kKb) : 0;
   const uint32_t v_off = RUNS ? 4 * quarter * kRow + piece * kVb : 0;
   const uint32_t ks_off = RUNS ? (quarter * kKd / kRun) * a.block.d + piece : 0;
@@ -391,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(Decode
     for (int t = 0; t < NT; ++t) {
       const int p = (first_tile + i) * kTile + 16 * t;
       if constexpr (RUNS) {      // the run's block is the whole wave's
-        const Row at = row_of(id[t], p);
+        const Row at = rows[t];
         k_row(t, a.keys + at.row * kRow + k_off);
         if constexpr (FMT != k16) {
 #pragma unroll
@@ -409,13 +402,12 @@ __global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(Decode
     }
   };
   auto load_v = [&](int i) {
-    vhole = 0;
+    vhole = RUNS ? holes : 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int p = (first_tile + i) * kTile + 16 * t;
       if constexpr (RUNS) {
-        const Row at = row_of(id[t], p);
-        vhole |= at.hole ? 15u << (4 * t) : 0u;
+        const Row at = rows[t];
 #pragma unroll
         for (int j = 0; j < 4; ++j) load_bytes<kVb>(vw[4 * t + j], a.values + at.row * kRow + v_off + j * kRow);
         if constexpr (FMT != k16) vsc[t] = *reinterpret_cast<const uint32_t*>(a.value_scales + at.scale + vs_off);
@@ -424,8 +416,9 @@ __global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(Decode
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int at_p = p + 4 * quarter + j;
-          const Row at = row_of(id_of(at_p), at_p);
-          vhole |= at.hole ? 1u << (4 * t + j) : 0u;
+          const int id = id_of(at_p);
+          const Row at = row_of(id, at_p);
+          vhole |= is_block(id) ? 0u : 1u << (4 * t + j);
           load_bytes<kVb>(vw[4 * t + j], a.values + at.row * kRow + piece * kVb);
           if constexpr (FMT != k16)
             vsc[t] |= static_cast<uint32_t>(a.value_scales[at.scale + static_cast<int64_t>(piece * kVd / kRun) * a.block.d])
@@ -434,10 +427,21 @@ __global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(Decode
       }
     }
   };
+  int ids[NT];
   auto load_ids = [&](int i) {
     if constexpr (RUNS) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) id[t] = id_of((first_tile + i) * kTile + 16 * t);
+      for (int t = 0; t < NT; ++t) ids[t] = id_of((first_tile + i) * kTile + 16 * t);
+    }
+  };
+  auto find_rows = [&](int i) {
+    if constexpr (RUNS) {
+      holes = 0;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        rows[t] = row_of(ids[t], (first_tile + i) * kTile + 16 * t);
+        holes |= is_block(ids[t]) ? 0u : 15u << (4 * t);
+      }
     }
   };
 
@@ -445,6 +449,7 @@ __global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(Decode
   // while its own scores form, table entries a tile ahead.
   if (w < tiles) {
     load_ids(w);
+    find_rows(w);
     load_k(w);
     load_v(w);
     if (w + kWaves < tiles) load_ids(w + kWaves);
@@ -461,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(Decode
       each<0, kSteps>([&](auto step) {
         constexpr int ST = decltype(step)::value;
         u32x4 x;
-        const float sc = FMT == k16 ? 1.f : scale_value(ksc[t][ST * 8 / kRun]);
+        const float sc = FMT == k16 ? 1.f : exponent(ksc[t][ST * 8 / kRun]);
         each<0, 4>([&](auto pair) {
           constexpr int I = decltype(pair)::value;
           x[I] = C::template two<4 * ST + I>(kw[t], sc);
@@ -471,7 +476,10 @@ __global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(Decode
       });
     }
     settle(s);
-    if (more) load_k(i + kWaves);
+    if (more) {
+      find_rows(i + kWaves);
+      load_k(i + kWaves);
+    }
 
     // u = 4 t + j is position 16 t + 4 quarter + j, its score s[t][j]; with halves a lane has j = 2 half + {0, 1}
     const int own = 4 * quarter + (kHalves == 2 ? 2 * half : 0);
@@ -573,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, MINW) decode_attention_kernel(Decode
           pl[0][e] = lo & 0xffffu;
           pl[1][e] = lo & 0xffff0000u;
         }
-        sc[e] = scale_value((vsc[st] >> (8 * e)) & 0xff);
+        sc[e] = exponent((vsc[st] >> (8 * e)) & 0xff);
       }
       each<0, kVd / 2>([&](auto pair) {
         constexpr int I = decltype(pair)::value;
@@ -699,10 +707,7 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
   *reinterpret_cast<u32x2*>(a.out + to) = u32x2{attn::pack2(y[0], y[1]), attn::pack2(y[2], y[3])};
 }
 
-#ifndef WGS
-#define WGS 1024
-#endif
-constexpr int kWorkgroups = WGS;     // parts aimed at, over all heads: four workgroups a CU
+constexpr int kWorkgroups = 2048;     // parts aimed at, over all heads: four workgroups a CU
 
 // Parts aimed at for each KV head, 0 where no request is cut.
 int64_t target_for(int64_t R, int64_t H, int64_t G, int64_t block, int64_t columns, int64_t window, int64_t max_length) {
