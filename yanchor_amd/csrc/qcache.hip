@@ -14,6 +14,8 @@ namespace {
 
 using namespace qcache;
 using tree::Div;
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 struct Args {
   const uint16_t* k;       // write: rows in, tokens ks / vs apart
@@ -27,32 +29,39 @@ struct Args {
   uint8_t* key_scales;
   uint8_t* value_scales;
   int64_t N, n_slots;      // n_slots = blocks * block
-  Div block, pieces, row;  // a row's pieces of eight values; a head's
+  Div block, per, row;     // per: a token's pieces of eight values, kThreads at most; row: a head's
+  uint32_t pieces;         // all of a token's
+  uint32_t tokens;         // that a workgroup takes at a time
   int G;
 };
 
-// Where piece p of token t lies: its slot, head and dim, or slot < 0.
-struct Place {
-  int64_t token, head;     // head: (block id * G + g) * block rows + row, in rows
-  int64_t run;             // of its scale byte
-  uint32_t p, dim;
+constexpr int kThreads = 256;
+// Tokens that a thread takes in a row where there are many (U = 1 for few): what lies where in a row is found once.
+constexpr int kMany = 4;
+
+// Piece p of a token's row: its bytes from the block's begin on, of FMT, and its scale's.
+template <int FMT>
+struct Piece {
+  uint32_t code, scale, row;   // row: bytes of a head's row
+  __device__ __forceinline__ Piece(const Args& a, uint32_t p) {
+    const uint32_t g = a.row.quot(p), dim = (p - g * a.row.d) * 8;
+    row = FMT == k16 ? a.row.d * 16 : FMT == kFp8 ? a.row.d * 8 : a.row.d * 4;
+    code = g * a.block.d * row + (FMT == k16 ? dim * 2 : FMT == kFp8 ? dim : dim / 2);
+    scale = (g * (a.row.d / 4) + dim / kRun) * a.block.d;
+  }
+};
+// Where the row of slot s begins, or that it is none.
+struct Slot {
+  int64_t block;
+  uint32_t row;
   bool in;
 };
-__device__ __forceinline__ Place place(const Args& a, int64_t i, int64_t n) {
-  Place w;
-  const int64_t j = i < n ? i : n - 1;
-  w.token = j < (1ll << 31) ? a.pieces.quot(static_cast<uint32_t>(j)) : j / a.pieces.d;
-  const int64_t slot = a.slots[w.token];
-  w.in = i < n && slot >= 0 && slot < a.n_slots;
-  w.p = static_cast<uint32_t>(j - w.token * a.pieces.d);
-  const uint32_t g = a.row.quot(w.p);
-  w.dim = (w.p - g * a.row.d) * 8;
-  const int64_t sl = w.in ? slot : 0;
-  const int64_t b = sl < (1ll << 31) ? a.block.quot(static_cast<uint32_t>(sl)) : sl / a.block.d;
-  const int64_t row = sl - b * a.block.d;
-  w.head = (b * a.G + g) * a.block.d + row;
-  w.run = ((b * a.G + g) * (a.row.d / 4) + w.dim / kRun) * a.block.d + row;
-  return w;
+__device__ __forceinline__ Slot slot_of(const Args& a, int64_t t) {
+  const int64_t s = t < a.N ? a.slots[t] : -1;
+  const bool in = s >= 0 && s < a.n_slots;
+  const int64_t x = in ? s : 0;
+  const int64_t b = x < (1ll << 31) ? a.block.quot(static_cast<uint32_t>(x)) : x / a.block.d;
+  return {b, static_cast<uint32_t>(x - b * a.block.d), in};
 }
 
 template <int DT>
@@ -67,76 +76,118 @@ __device__ __forceinline__ void widen8(uint4 x, float* y) {
 
 // Eight values into their codes and, by the first of a run's four lanes, its scale.
 template <int DT, int FMT>
-__device__ __forceinline__ void put8(const Args& a, const Place& w, uint4 x, char* codes, uint8_t* scales) {
-  float y[8], top = 0.f;
+__device__ __forceinline__ void put8(uint4 x, bool in, bool first, char* codes, uint8_t* scale) {
+  float y[8];
   widen8<DT>(x, y);
+  uint32_t top = 0;      // of the magnitudes, as bits: a NaN's are the largest
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // a NaN has the largest bit pattern of all magnitudes
-    const float m = __uint_as_float(__float_as_uint(y[i]) & 0x7fffffffu);
-    top = __float_as_uint(m) > __float_as_uint(top) ? m : top;
-  }
-#pragma unroll
-  for (int off = 1; off < 4; off <<= 1) {
-    const uint32_t other = __shfl_xor(__float_as_uint(top), off, kWave);
-    top = other > __float_as_uint(top) ? __uint_as_float(other) : top;
-  }
-  const int s = scale_of<FMT>(top);
-  const float inv = s == kNotANumber ? 0.f : scale_inverse(s);   // such a run reads back as NaN by its scale
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1, kWave)));
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2, kWave)));
+  const int s = scale_of<FMT>(__uint_as_float(top));
+  const float inv = scale_inverse(s);
+  // a run that is not finite reads back as NaN by its scale
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = s == kNotANumber ? 0.f : y[i] * inv;
-  if (!w.in) return;
+  if (!in) return;
   if constexpr (FMT == kFp8) {
-    uint2 c;
-    c.x = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-    c.x = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c.x, true);
-    c.y = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
-    c.y = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], c.y, true);
-    *reinterpret_cast<uint2*>(codes + w.head * (a.row.d * 8) + w.dim) = c;
+    u2 c;
+    c[0] = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    c[0] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c[0], true);
+    c[1] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
+    c[1] = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], c[1], true);
+    *reinterpret_cast<u2*>(codes) = c;
   } else {
     uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], 1.f, 0);
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[2], y[3], 1.f, 1);
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[4], y[5], 1.f, 2);
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[6], y[7], 1.f, 3);
-    *reinterpret_cast<uint32_t*>(codes + w.head * (a.row.d * 4) + w.dim / 2) = c;
+    *reinterpret_cast<uint32_t*>(codes) = c;
   }
-  if (w.dim % kRun == 0) scales[w.run] = static_cast<uint8_t>(s);
+  if (first) *scale = static_cast<uint8_t>(s);
 }
 
-// Bound by HBM.  A thread takes eight values of the keys and of the values.
-template <int DT, int FMT>
-__global__ void __launch_bounds__(256) write_kernel(Args a) {
-  const int64_t n = a.N * a.pieces.d, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const Place w = place(a, i, n);
-  uint4 x = make_uint4(0, 0, 0, 0), y = x;
-  if (w.in) {
-    x = *reinterpret_cast<const uint4*>(a.k + w.token * a.ks + w.p * 8);
-    y = *reinterpret_cast<const uint4*>(a.v + w.token * a.vs + w.p * 8);
-  }
-  put8<DT, FMT>(a, w, x, a.keys, a.key_scales);
-  put8<DT, FMT>(a, w, y, a.values, a.value_scales);
+__device__ __forceinline__ uint4 stream_load(const void* p) {
+  const u4 x = __builtin_nontemporal_load(static_cast<const u4*>(p));
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void stream_store(void* p, uint4 x) {
+  __builtin_nontemporal_store(u4{x.x, x.y, x.z, x.w}, static_cast<u4*>(p));
 }
 
-template <int DT, int FMT>
-__device__ __forceinline__ uint4 get8(const Args& a, const Place& w, const char* codes, const uint8_t* scales) {
-  if (!w.in) return make_uint4(0, 0, 0, 0);
+// Both kernels: thread (token of the workgroup's, piece), U tokens a thread, and more pieces where a row has more than
+// the workgroup has threads.
+template <int DT, int FMT, int U>
+__global__ void __launch_bounds__(kThreads) write_kernel(Args a) {
+  const uint32_t sub = a.per.quot(threadIdx.x), p0 = threadIdx.x - sub * a.per.d;
+  if (sub >= a.tokens) return;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (U * a.tokens) + sub;
+  const int64_t block_codes = static_cast<int64_t>(a.G) * a.block.d * (a.row.d * (FMT == kFp8 ? 8 : 4));
+  const int64_t block_scales = static_cast<int64_t>(a.G) * a.block.d * (a.row.d / 4);
+  Slot slot[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) slot[u] = slot_of(a, t0 + u * a.tokens);
+  for (uint32_t p = p0; p < a.pieces; p += kThreads) {
+    const Piece<FMT> at(a, p);
+    uint4 x[U], y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u] = y[u] = make_uint4(0, 0, 0, 0);
+      if (slot[u].in) {
+        x[u] = stream_load(a.k + (t0 + u * a.tokens) * a.ks + p * 8);
+        y[u] = stream_load(a.v + (t0 + u * a.tokens) * a.vs + p * 8);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t code = slot[u].block * block_codes + at.code + static_cast<uint64_t>(slot[u].row) * at.row;
+      const int64_t scale = slot[u].block * block_scales + at.scale + slot[u].row;
+      put8<DT, FMT>(x[u], slot[u].in, p % 4 == 0, a.keys + code, a.key_scales + scale);
+      put8<DT, FMT>(y[u], slot[u].in, p % 4 == 0, a.values + code, a.value_scales + scale);
+    }
+  }
+}
+
+// Eight values as they are stored, and their scale.
+struct Raw {
+  uint4 codes;
+  uint32_t scale;
+};
+template <int FMT>
+__device__ __forceinline__ Raw fetch8(bool in, const char* codes, const uint8_t* scale) {
+  Raw r{};
+  if (!in) return r;
   if constexpr (FMT == k16) {
-    return *reinterpret_cast<const uint4*>(codes + (w.head * (a.row.d * 8) + w.dim) * 2);
+    r.codes = stream_load(codes);
   } else {
-    const float s = scale_value(scales[w.run]);
+    r.scale = *scale;
+    if constexpr (FMT == kFp8) {
+      const u2 c = __builtin_nontemporal_load(reinterpret_cast<const u2*>(codes));
+      r.codes.x = c[0];
+      r.codes.y = c[1];
+    } else {
+      r.codes.x = *reinterpret_cast<const uint32_t*>(codes);
+    }
+  }
+  return r;
+}
+template <int DT, int FMT>
+__device__ __forceinline__ uint4 decode8(Raw r) {
+  if constexpr (FMT == k16) {
+    return r.codes;
+  } else {
+    const float s = scale_value(r.scale);
     float y[8];
     if constexpr (FMT == kFp8) {
-      const uint2 c = *reinterpret_cast<const uint2*>(codes + w.head * (a.row.d * 8) + w.dim);
-      const auto p0 = __builtin_amdgcn_cvt_pk_f32_fp8(c.x, false), p1 = __builtin_amdgcn_cvt_pk_f32_fp8(c.x, true);
-      const auto p2 = __builtin_amdgcn_cvt_pk_f32_fp8(c.y, false), p3 = __builtin_amdgcn_cvt_pk_f32_fp8(c.y, true);
+      const auto p0 = __builtin_amdgcn_cvt_pk_f32_fp8(r.codes.x, false), p1 = __builtin_amdgcn_cvt_pk_f32_fp8(r.codes.x, true);
+      const auto p2 = __builtin_amdgcn_cvt_pk_f32_fp8(r.codes.y, false), p3 = __builtin_amdgcn_cvt_pk_f32_fp8(r.codes.y, true);
       y[0] = p0[0]; y[1] = p0[1]; y[2] = p1[0]; y[3] = p1[1];
       y[4] = p2[0]; y[5] = p2[1]; y[6] = p3[0]; y[7] = p3[1];
     } else {
-      const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + w.head * (a.row.d * 4) + w.dim / 2);
-      const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0);
-      const auto p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1);
-      const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2);
-      const auto p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3);
+      const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r.codes.x, 1.f, 0);
+      const auto p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r.codes.x, 1.f, 1);
+      const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r.codes.x, 1.f, 2);
+      const auto p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r.codes.x, 1.f, 3);
       y[0] = p0[0]; y[1] = p0[1]; y[2] = p1[0]; y[3] = p1[1];
       y[4] = p2[0]; y[5] = p2[1]; y[6] = p3[0]; y[7] = p3[1];
     }
@@ -151,14 +202,34 @@ __device__ __forceinline__ uint4 get8(const Args& a, const Place& w, const char*
   }
 }
 
-template <int DT, int FMT>
-__global__ void __launch_bounds__(256) read_kernel(Args a) {
-  const int64_t n = a.N * a.pieces.d, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const Place w = place(a, i, n);
-  const uint4 x = get8<DT, FMT>(a, w, a.keys, a.key_scales), y = get8<DT, FMT>(a, w, a.values, a.value_scales);
-  if (i >= n) return;
-  *reinterpret_cast<uint4*>(a.k_out + i * 8) = x;
-  *reinterpret_cast<uint4*>(a.v_out + i * 8) = y;
+template <int DT, int FMT, int U>
+__global__ void __launch_bounds__(kThreads) read_kernel(Args a) {
+  const uint32_t sub = a.per.quot(threadIdx.x), p0 = threadIdx.x - sub * a.per.d;
+  if (sub >= a.tokens) return;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (U * a.tokens) + sub;
+  const int64_t block_codes = static_cast<int64_t>(a.G) * a.block.d * (a.row.d * (FMT == k16 ? 16 : FMT == kFp8 ? 8 : 4));
+  const int64_t block_scales = static_cast<int64_t>(a.G) * a.block.d * (a.row.d / 4);
+  Slot slot[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) slot[u] = slot_of(a, t0 + u * a.tokens);
+  for (uint32_t p = p0; p < a.pieces; p += kThreads) {
+    const Piece<FMT> at(a, p);
+    Raw x[U], y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t code = slot[u].block * block_codes + at.code + static_cast<uint64_t>(slot[u].row) * at.row;
+      const int64_t scale = slot[u].block * block_scales + at.scale + slot[u].row;
+      x[u] = fetch8<FMT>(slot[u].in, a.keys + code, a.key_scales + scale);
+      y[u] = fetch8<FMT>(slot[u].in, a.values + code, a.value_scales + scale);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = t0 + u * a.tokens;
+      if (t >= a.N) break;
+      stream_store(a.k_out + (t * a.pieces + p) * 8, decode8<DT, FMT>(x[u]));
+      stream_store(a.v_out + (t * a.pieces + p) * 8, decode8<DT, FMT>(y[u]));
+    }
+  }
 }
 
 int check_cache(const char* what, const void* keys, const void* values, const uint8_t* key_scales,
@@ -170,7 +241,7 @@ int check_cache(const char* what, const void* keys, const void* values, const ui
   YH_CHECK_ARG(N < (1ll << 31) && blocks < (1ll << 31) && block < (1ll << 31) && G < (1ll << 31) && D < (1ll << 31) &&
                    G * D < (1ll << 31) && blocks * block < (1ll << 40),
                "%s: sizes too large", what);
-  YH_CHECK_ARG((N * (G * D / 8) + 255) / 256 < (1ll << 24), "%s: sizes too large", what);
+  YH_CHECK_ARG(G * block * D * 2 < (1ll << 32) && N * (G * D / 8) < (1ll << 32), "%s: sizes too large", what);
   if (N == 0) return YH_OK;
   YH_CHECK_ARG(slots && ((keys && values && (bits == 16 || (key_scales && value_scales))) || blocks == 0),
                "%s: null pointer", what);
@@ -189,10 +260,29 @@ Args args_of(const int64_t* slots, const void* keys, const void* values, const u
   a.N = N;
   a.n_slots = blocks * block;
   a.block = tree::make_div(static_cast<uint32_t>(block));
-  a.pieces = tree::make_div(static_cast<uint32_t>(G * D / 8));
+  a.pieces = static_cast<uint32_t>(G * D / 8);
+  a.per = tree::make_div(a.pieces < kThreads ? a.pieces : kThreads);
+  a.tokens = kThreads / a.per.d;
   a.row = tree::make_div(static_cast<uint32_t>(D / 8));
   a.G = static_cast<int>(G);
   return a;
+}
+
+// Whether each thread takes several tokens: where that still leaves four workgroups a CU.
+bool many(const Args& a) { return a.N >= static_cast<int64_t>(1024) * kMany * a.tokens; }
+unsigned grid_of(const Args& a) {
+  const int64_t each = (many(a) ? kMany : 1) * static_cast<int64_t>(a.tokens);
+  return static_cast<unsigned>((a.N + each - 1) / each);
+}
+template <int DT, int FMT>
+void launch_write(const Args& a, hipStream_t st) {
+  if (many(a)) hipLaunchKernelGGL((write_kernel<DT, FMT, kMany>), dim3(grid_of(a)), dim3(kThreads), 0, st, a);
+  else hipLaunchKernelGGL((write_kernel<DT, FMT, 1>), dim3(grid_of(a)), dim3(kThreads), 0, st, a);
+}
+template <int DT, int FMT>
+void launch_read(const Args& a, hipStream_t st) {
+  if (many(a)) hipLaunchKernelGGL((read_kernel<DT, FMT, kMany>), dim3(grid_of(a)), dim3(kThreads), 0, st, a);
+  else hipLaunchKernelGGL((read_kernel<DT, FMT, 1>), dim3(grid_of(a)), dim3(kThreads), 0, st, a);
 }
 
 }  // namespace
@@ -217,14 +307,13 @@ extern "C" int yh_cache_write_quantized(const void* k, int64_t k_stride, const v
   a.v = static_cast<const uint16_t*>(v);
   a.ks = k_stride;
   a.vs = v_stride;
-  const dim3 grid(static_cast<unsigned>((N * a.pieces.d + 255) / 256));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == YH_BF16) {
-    if (bits == 8) hipLaunchKernelGGL((write_kernel<YH_BF16, kFp8>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((write_kernel<YH_BF16, kFp4>), grid, dim3(256), 0, st, a);
+    if (bits == 8) launch_write<YH_BF16, kFp8>(a, st);
+    else launch_write<YH_BF16, kFp4>(a, st);
   } else {
-    if (bits == 8) hipLaunchKernelGGL((write_kernel<YH_F16, kFp8>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((write_kernel<YH_F16, kFp4>), grid, dim3(256), 0, st, a);
+    if (bits == 8) launch_write<YH_F16, kFp8>(a, st);
+    else launch_write<YH_F16, kFp4>(a, st);
   }
   YH_CHECK_LAUNCH("cache_write_quantized");
   return YH_OK;
@@ -242,16 +331,15 @@ extern "C" int yh_cache_read(const int64_t* slots, const void* keys, const void*
   Args a = args_of(slots, keys, values, key_scales, value_scales, N, blocks, G, D, block);
   a.k_out = static_cast<uint16_t*>(k);
   a.v_out = static_cast<uint16_t*>(v);
-  const dim3 grid(static_cast<unsigned>((N * a.pieces.d + 255) / 256));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (bits == 16) {
-    hipLaunchKernelGGL((read_kernel<YH_BF16, k16>), grid, dim3(256), 0, st, a);   // 16 bits move as they are
+    launch_read<YH_BF16, k16>(a, st);   // 16 bits move as they are
   } else if (dtype == YH_BF16) {
-    if (bits == 8) hipLaunchKernelGGL((read_kernel<YH_BF16, kFp8>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((read_kernel<YH_BF16, kFp4>), grid, dim3(256), 0, st, a);
+    if (bits == 8) launch_read<YH_BF16, kFp8>(a, st);
+    else launch_read<YH_BF16, kFp4>(a, st);
   } else {
-    if (bits == 8) hipLaunchKernelGGL((read_kernel<YH_F16, kFp8>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((read_kernel<YH_F16, kFp4>), grid, dim3(256), 0, st, a);
+    if (bits == 8) launch_read<YH_F16, kFp8>(a, st);
+    else launch_read<YH_F16, kFp4>(a, st);
   }
   YH_CHECK_LAUNCH("cache_read");
   return YH_OK;
