@@ -128,9 +128,34 @@ struct Part {
   Seen seen;
 };
 
-// Part `which` of all, found from the lengths; count 0: there is none.
+// Tiles of a part: a turn of the waves at least.
+__device__ __forceinline__ int chunk_of(const DecodeArgs& a, int total) {
+  const int chunk = a.target ? (total + a.target - 1) / a.target : 0x7fffffff;
+  return chunk < kWaves ? kWaves : chunk;
+}
+__device__ __forceinline__ int parts_of(int tiles, int chunk) { return tiles > chunk ? (tiles + chunk - 1) / chunk : 1; }
+// Part `index` of `count` of a request of n tiles; they differ by a tile.
+__device__ __forceinline__ Part part_of(int r, int index, int count, int slot, int n, Seen seen) {
+  const int each = n / count, rest = n % count;
+  return {r, index, count, slot, index * each + (index < rest ? index : rest), each + (index < rest ? 1 : 0), seen};
+}
+
+// Part `which` of all, found from the lengths; count 0: there is none.  Every wave finds it by itself where it has a
+// lane for each request (a call for one request: X us of Y with the workgroup's scan).
 template <int TILE>
 __device__ Part find_part(const DecodeArgs& a, int which) {
+  if (a.R <= kWave) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const Seen seen = lane < a.R ? seen_of(a, lane) : Seen{0, 0};
+    const int n = tiles_of<TILE>(seen);
+    const int chunk = chunk_of(a, __shfl(scan_wave(n), kWave - 1, kWave));
+    const int c = lane < a.R ? parts_of(n, chunk) : 0, end = scan_wave(c);
+    const uint64_t behind = __ballot(end > which);
+    if (behind == 0) return {0, 0, 0, 0, 0, 0, {0, 0}};
+    const int r = __ffsll(static_cast<unsigned long long>(behind)) - 1;
+    const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, r); };
+    return part_of(r, which - (of(end) - of(c)), of(c), which, of(n), {of(seen.lo), of(seen.hi)});
+  }
   __shared__ int sums[kWaves], found[4];
   const int t = threadIdx.x, w = t / kWave;
   // a thread takes `each` requests in a row
@@ -145,13 +170,10 @@ __device__ Part find_part(const DecodeArgs& a, int which) {
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) total += sums[i];
   __syncthreads();
-  // tiles of a part: a turn of the waves at least
-  int chunk = a.target ? (total + a.target - 1) / a.target : 0x7fffffff;
-  if (chunk < kWaves) chunk = kWaves;
+  const int chunk = chunk_of(a, total);
   mine = 0;
   for (int r = r0; r < r1; ++r) {
-    const int n = tiles_of<TILE>(seen_of(a, r));
-    mine += n > chunk ? (n + chunk - 1) / chunk : 1;
+    mine += parts_of(tiles_of<TILE>(seen_of(a, r)), chunk);
   }
   s = scan_wave(mine);
   if ((t & (kWave - 1)) == kWave - 1) sums[w] = s;
@@ -161,7 +183,7 @@ __device__ Part find_part(const DecodeArgs& a, int which) {
   for (int i = 0; i < kWaves; ++i) at += i < w ? sums[i] : 0;
   if (which >= at && which < at + mine) {
     for (int r = r0; r < r1; ++r) {
-      const int n = tiles_of<TILE>(seen_of(a, r)), c = n > chunk ? (n + chunk - 1) / chunk : 1;
+      const int n = tiles_of<TILE>(seen_of(a, r)), c = parts_of(n, chunk);
       if (which < at + c) {
         found[0] = r;
         found[1] = which - at;
@@ -173,20 +195,8 @@ __device__ Part find_part(const DecodeArgs& a, int which) {
     }
   }
   __syncthreads();
-  Part p;
-  p.r = found[0];
-  if (p.r < 0) {
-    p.count = 0;
-    return p;
-  }
-  p.index = found[1];
-  p.count = found[2];
-  p.slot = which;
-  const int n = found[3], each_part = n / p.count, rest = n % p.count;    // parts of a request differ by a tile
-  p.tile = p.index * each_part + (p.index < rest ? p.index : rest);
-  p.tiles = each_part + (p.index < rest ? 1 : 0);
-  p.seen = seen_of(a, p.r);
-  return p;
+  if (found[0] < 0) return {0, 0, 0, 0, 0, 0, {0, 0}};
+  return part_of(found[0], found[1], found[2], which, found[3], seen_of(a, found[0]));
 }
 
 // Two dims of one position's codes to bf16 under the scale 2^(s - 127), given as a float whose exponent s is: the
@@ -659,21 +669,19 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
   const int first = a.first[r], count = a.first[r + 1] - first;
   if (count <= 1) return;
   const int64_t slot = static_cast<int64_t>(first) * a.H + hd;
-  float m = kFloor;
-#pragma unroll 4
-  for (int j = share; j < count; j += kShares) m = fmaxf(m, a.stat[slot + static_cast<int64_t>(j) * a.H].x);
-  float dn = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  float m = kFloor, dn = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int j = share; j < count; j += kShares) {
     const int64_t s = slot + static_cast<int64_t>(j) * a.H;
     const float2 st = a.stat[s];
     const float4 x = *reinterpret_cast<const float4*>(a.part + s * D + dim);
-    const float f = __builtin_amdgcn_exp2f(st.x - m);
-    dn = fmaf(st.y, f, dn);
-    o[0] = fmaf(x.x, f, o[0]);
-    o[1] = fmaf(x.y, f, o[1]);
-    o[2] = fmaf(x.z, f, o[2]);
-    o[3] = fmaf(x.w, f, o[3]);
+    const float next = fmaxf(m, st.x), f = __builtin_amdgcn_exp2f(m - next), h = __builtin_amdgcn_exp2f(st.x - next);
+    m = next;
+    dn = fmaf(dn, f, st.y * h);
+    o[0] = fmaf(o[0], f, x.x * h);
+    o[1] = fmaf(o[1], f, x.y * h);
+    o[2] = fmaf(o[2], f, x.z * h);
+    o[3] = fmaf(o[3], f, x.w * h);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) sums[share][dim + e] = o[e];

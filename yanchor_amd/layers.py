@@ -774,6 +774,9 @@ def conv_tree(proj, window, conv_w, parents, cu_seqlens, channels, planes=1):
 # power of two, 2^(s - 127), as e4m3 codes (8 bits) or e2m1 codes (4 bits).
 # Nothing is read back to the host, so these calls can be captured.
 
+_INF = float("inf")
+
+
 def quantized_cache(blocks, groups, block, dim, *, bits=8, device=None):
     """An empty quantised block cache (keys, values, key_scales, value_scales):
     8 bits: keys / values [blocks, G, block, D] float8_e4m3fn; 4 bits: [blocks, G,
@@ -791,32 +794,33 @@ def quantized_cache(blocks, groups, block, dim, *, bits=8, device=None):
 
 
 def _any_cache(keys, values, key_scales, value_scales, g, d, dtype):
-    """Bits a value of a block cache of [*, G, *, D] rows, whose form is checked;
-    ``dtype`` that of a 16-bit one."""
-    if keys.ndim != 4 or values.shape != keys.shape or values.dtype != keys.dtype or not keys.is_contiguous() or \
+    """Bits a value of a block cache of [*, G, *, D] rows, whose form is checked
+    (``dtype``: of a 16-bit one)."""
+    shape, kind = keys.shape, keys.dtype
+    if len(shape) != 4 or values.shape != shape or values.dtype != kind or not keys.is_contiguous() or \
             not values.is_contiguous():
         raise ValueError("keys and values must be contiguous [blocks, G, block, D] of one type")
-    if keys.dtype in (torch.bfloat16, torch.float16):
+    if kind == torch.float8_e4m3fn:
+        bits, width = 8, d
+    elif kind == torch.uint8:
+        bits, width = 4, d // 2
+    elif kind in (torch.bfloat16, torch.float16):
         if key_scales is not None or value_scales is not None:
             raise ValueError("a 16-bit cache has no scales")
-        if keys.dtype != dtype:
+        if kind != dtype:
             raise ValueError(f"a 16-bit cache must be in {dtype}")
         bits, width = 16, d
-    elif keys.dtype == torch.float8_e4m3fn:
-        bits, width = 8, d
-    elif keys.dtype == torch.uint8:
-        bits, width = 4, d // 2
     else:
         raise ValueError("a cache is bf16, fp16, float8_e4m3fn (8 bits) or uint8 (4 bits, two a byte)")
-    if keys.shape[1] != g or keys.shape[3] != width or keys.shape[2] < 1:
+    if shape[1] != g or shape[3] != width or shape[2] < 1:
         raise ValueError(f"a {bits}-bit cache of these heads is [blocks, {g}, block, {width}]")
     if bits < 16:
         if d % 32:
             raise ValueError("the head dim of a quantised cache must be a multiple of 32")
-        shape = (keys.shape[0], g, d // 32, keys.shape[2])
+        want = (shape[0], g, d // 32, shape[2])
         for s in (key_scales, value_scales):
-            if s is None or s.shape != shape or s.dtype != torch.uint8 or not s.is_contiguous():
-                raise ValueError(f"a quantised cache needs contiguous uint8 scales {list(shape)}")
+            if s is None or s.shape != want or s.dtype != torch.uint8 or not s.is_contiguous():
+                raise ValueError(f"a quantised cache needs contiguous uint8 scales {list(want)}")
     return bits
 
 
@@ -904,10 +908,10 @@ def decode_attention(q, keys, values, block_tables, lengths, *, key_scales=None,
     if window is not None and int(window) < 1:
         raise ValueError("window must be at least 1")
     sc = float(d ** -0.5 if scale is None else scale)
-    if not 0 < sc < float("inf"):
+    if not 0 < sc < _INF:
         raise ValueError("scale must be positive")
     cap = 0.0 if softcap is None else float(softcap)
-    if softcap is not None and not 0 < cap < float("inf"):
+    if softcap is not None and not 0 < cap < _INF:
         raise ValueError("softcap must be positive")
     if slopes is not None:
         if slopes.dtype != torch.float32 or slopes.shape != (h,):
@@ -939,12 +943,16 @@ def _head_rows(x):
     """(x, token stride, head stride) of x [N, heads, D] with 16-byte aligned
     heads (a column view of a projection qualifies), of a copy otherwise."""
     n, h, d = x.shape
-    if x.numel() and (x.stride(2) != 1 or (n > 1 and x.stride(0) % 8) or (h > 1 and x.stride(1) % 8) or
-                      x.data_ptr() % 16):
-        x = x.clone(memory_format=torch.contiguous_format)
-    if x.is_contiguous():   # a stride of a single row says nothing
-        return x, h * d, d
-    return x, x.stride(0) if n > 1 else 0, x.stride(1) if h > 1 else 0
+    a, b, c = x.stride()
+    if (c != 1 or a % 8 and n > 1 or b % 8 and h > 1 or x.data_ptr() % 16) and x.numel():
+        x, a, b = x.clone(memory_format=torch.contiguous_format), h * d, d
+    return x, a if n > 1 else 0, b if h > 1 else 0     # a stride of a single row says nothing
+
+
+def _weight(w):
+    if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0):
+        return w
+    return w.clone(memory_format=torch.contiguous_format)
 
 
 def qk_norm_rope(q, k, q_w, k_w, positions, inv_freq, eps, *, sections=None, interleaved=False, plus_one=True):
@@ -969,30 +977,32 @@ def qk_norm_rope(q, k, q_w, k_w, positions, inv_freq, eps, *, sections=None, int
             raise ValueError("norm weights must be [D] in the dtype of q and k")
     if inv_freq.ndim != 1 or inv_freq.dtype != torch.float32 or inv_freq.shape[0] % 8 or 2 * inv_freq.shape[0] > d:
         raise ValueError("inv_freq must be float32, a multiple of 8 and at most D / 2 of them")
-    if not 0 <= float(eps) < float("inf"):
+    eps = float(eps)
+    if not 0 <= eps < _INF:
         raise ValueError("eps must not be negative")
     half = inv_freq.shape[0]
     axes = 1 if positions.ndim == 1 else positions.shape[0] if positions.ndim == 2 else 0
     if not 1 <= axes <= 4 or positions.shape[-1] != n or positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be integers [N] or [axes, N] of 1 to 4 axes")
-    if sections is None:
-        if axes > 1:
-            raise ValueError("positions of several axes need their sections")
-        sections = [half]
-    sections = [int(x) for x in sections]
-    if len(sections) != axes or min(sections) < 0 or sum(sections) != half:
-        raise ValueError("sections must hold one count an axis that add up to len(inv_freq)")
-    if interleaved and any(x and i + axes * (x - 1) >= half for i, x in enumerate(sections) if i):
-        raise ValueError("an interleaved section reaches past the pairs")
+    counts = None
+    if sections is not None:
+        sections = [int(x) for x in sections]
+        if len(sections) != axes or min(sections) < 0 or sum(sections) != half:
+            raise ValueError("sections must hold one count an axis that add up to len(inv_freq)")
+        if interleaved and any(x and i + axes * (x - 1) >= half for i, x in enumerate(sections) if i):
+            raise ValueError("an interleaved section reaches past the pairs")
+        counts = (ctypes.c_int64 * axes)(*sections)
+    elif axes > 1:
+        raise ValueError("positions of several axes need their sections")
     dev = _tree.device_of(q, k, q_w, k_w, inv_freq)
-    pos = positions.to(device=dev, dtype=torch.int64).contiguous()
+    if positions.dtype != torch.int64 or positions.device != dev or not positions.is_contiguous():
+        positions = positions.to(device=dev, dtype=torch.int64).contiguous()
     (q, qts, qhs), (k, kts, khs) = _head_rows(q), _head_rows(k)
-    q_w, k_w = (w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else w.clone(
-        memory_format=torch.contiguous_format) for w in (q_w, k_w))
-    freq = inv_freq.contiguous()
+    q_w, k_w = _weight(q_w), _weight(k_w)
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
     qo, ko = torch.empty(n, h, d, dtype=q.dtype, device=dev), torch.empty(n, g, d, dtype=q.dtype, device=dev)
-    counts = (ctypes.c_int64 * axes)(*sections)
     N.call_on(dev, "yh_qk_norm_rope", q.data_ptr(), qts, qhs, k.data_ptr(), kts, khs, N.ptr(q_w), N.ptr(k_w),
-              pos.data_ptr(), freq.data_ptr(), counts, axes, int(bool(interleaved)), qo.data_ptr(), ko.data_ptr(), n, h,
-              g, d, 2 * half, float(eps), int(bool(plus_one)), N.code(q))
+              positions.data_ptr(), inv_freq.data_ptr(), counts, axes, 1 if interleaved else 0, qo.data_ptr(),
+              ko.data_ptr(), n, h, g, d, 2 * half, eps, 1 if plus_one else 0, N.code(q))
     return qo, ko
