@@ -141,7 +141,8 @@ __device__ __forceinline__ Part part_of(int r, int index, int count, int slot, i
 }
 
 // Part `which` of all, found from the lengths; count 0: there is none.  Every wave finds it by itself where it has a
-// lane for each request (a call for one request: X us of Y with the workgroup's scan).
+// lane for each request (one request: 7.6 us for 9.8 with the workgroup's scan; four
+// requests a lane: 8.3, and nothing gained for 133).
 template <int TILE>
 __device__ Part find_part(const DecodeArgs& a, int which) {
   if (a.R <= kWave) {
@@ -286,8 +287,13 @@ __device__ __forceinline__ void settle(f32x4 (&x)[N]) {
   for (int i = 1; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 
+// Waves a SIMD that the registers are held to, where none spills for it.
+constexpr int waves_for(int DT, int FMT, int D, int HP) {
+  return D == 64 ? 3 : D == 256 || (FMT != k16 && (HP == 16 || (FMT == kFp8 && DT == YH_F16))) ? 2 : 3;
+}
+
 template <int DT, int FMT, int D, int HP, bool RUNS>
-__global__ void __launch_bounds__(kThreads, 2) decode_attention_kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP)) decode_attention_kernel(DecodeArgs a) {
   using C = Codes<FMT>;
   using M = attn::Mfma<DT>;
   constexpr int MT = FMT == k16 ? DT : YH_BF16;
@@ -297,7 +303,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attention_kernel(DecodeArg
   constexpr int kKd = D / 4, kVd = D / 16;              // dims of a lane: K, V
   constexpr int kKb = kRow / 4, kVb = kRow / 16;        // and their bytes
   constexpr int kKw = (kKb + 3) / 4, kVw = (kVb + 3) / 4;
-  constexpr int kKs = kKd > kRun ? kKd / kRun : 1;      // scales of a lane's K dims
+  // A lane's K dims come in pieces of 16 bytes, piece c of quarter q at byte 64 c + 16 q, so that a load takes whole
+  // 64 bytes of each row (D / 4 dims in a row a lane: 513 us for 400 with 8 bits, D = 256 and 2.4 GB).
+  constexpr int kPb = kKb < 16 ? kKb : 16, kPd = kPb * 8 / C::kBits, kPieces = kKb / kPb;
   constexpr int kSteps = D / 32;                        // products over the dims
   constexpr int NT = products(kRow, kPair && D == 256), kTile = 16 * NT, kU = 4 * NT;   // kU: positions of a quarter
   constexpr int kSel = HP == 16 || FMT == k16 ? 1 : 2;               // columns of a head: two dims, halves of the positions
@@ -327,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attention_kernel(DecodeArg
   u32x4 qh[kSteps], ql[kPair ? kSteps : 1];
 #pragma unroll
   for (int c = 0; c < kSteps; ++c) {
-    const int dim = FMT == k16 ? 32 * c + 8 * quarter : kKd * quarter + 8 * c;
+    const int dim = 8 * c / kPd * (4 * kPd) + kPd * quarter + 8 * c % kPd;
     u32x4 x = *reinterpret_cast<const u32x4*>(a.q + r * a.q_ts + static_cast<int64_t>(head) * D + dim);
     if (col >= cols) x = u32x4{0, 0, 0, 0};
     if constexpr (kPair) {
@@ -374,19 +382,22 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attention_kernel(DecodeArg
 
   // The lane's positions of product t, of 16 t on: `piece` of K, 4 quarter + j of V.
   uint32_t kw[NT][kKw], vw[kU][kVw];
-  uint32_t ksc[NT][kKs], vsc[NT];      // scale bytes of a K position, of four V positions
+  uint32_t ksc[NT][kPieces], vsc[NT];      // scale bytes of a K position, of four V positions
   Row rows[NT];                        // of the next tile's products, where blocks hold whole runs of 16 positions
   uint32_t holes = 0, vhole = 0;       // V's positions without a block: of the next tile, of this one
-  const uint32_t k_off = RUNS ? piece * kRow + (FMT == k16 ? quarter * 16 : quarter * kKb) : 0;
+  const uint32_t k_off = (RUNS ? piece * kRow : 0) + quarter * kPb;
   const uint32_t v_off = RUNS ? 4 * quarter * kRow + piece * kVb : 0;
-  const uint32_t ks_off = RUNS ? (quarter * kKd / kRun) * a.block.d + piece : 0;
+  const uint32_t ks_off = (quarter * kPd / kRun) * a.block.d + (RUNS ? piece : 0);
   const uint32_t vs_off = RUNS ? (piece * kVd / kRun) * a.block.d + 4 * quarter : 0;
   auto k_row = [&](int t, const char* p) {
-    if constexpr (FMT == k16) {
 #pragma unroll
-      for (int c = 0; c < kSteps; ++c) load_bytes<16>(kw[t] + 4 * c, p + 64 * c);
-    } else {
-      load_bytes<kKb>(kw[t], p);
+    for (int c = 0; c < kPieces; ++c) load_bytes<kPb>(kw[t] + kPb / 4 * c, p + 64 * c);
+  };
+  auto k_scale = [&](int t, int64_t at) {
+    if constexpr (FMT != k16) {
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c)
+        ksc[t][c] = *(a.key_scales + at + static_cast<int64_t>(c * (4 * kPd / kRun)) * a.block.d + ks_off);
     }
   };
   auto load_k = [&](int i) {
@@ -396,18 +407,11 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attention_kernel(DecodeArg
       if constexpr (RUNS) {      // the run's block is the whole wave's
         const Row at = rows[t];
         k_row(t, a.keys + at.row * kRow + k_off);
-        if constexpr (FMT != k16) {
-#pragma unroll
-          for (int e = 0; e < kKs; ++e) ksc[t][e] = *(a.key_scales + at.scale + e * static_cast<int64_t>(a.block.d) + ks_off);
-        }
+        k_scale(t, at.scale);
       } else {
         const Row at = row_of(id_of(p + piece), p + piece);
-        k_row(t, a.keys + at.row * kRow + (FMT == k16 ? quarter * 16 : quarter * kKb));
-        if constexpr (FMT != k16) {
-#pragma unroll
-          for (int e = 0; e < kKs; ++e)
-            ksc[t][e] = a.key_scales[at.scale + static_cast<int64_t>(quarter * kKd / kRun + e) * a.block.d];
-        }
+        k_row(t, a.keys + at.row * kRow + k_off);
+        k_scale(t, at.scale);
       }
     }
   };
@@ -476,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_attention_kernel(DecodeArg
       each<0, kSteps>([&](auto step) {
         constexpr int ST = decltype(step)::value;
         u32x4 x;
-        const float sc = FMT == k16 ? 1.f : exponent(ksc[t][ST * 8 / kRun]);
+        const float sc = FMT == k16 ? 1.f : exponent(ksc[t][ST * 8 / kPd]);
         each<0, 4>([&](auto pair) {
           constexpr int I = decltype(pair)::value;
           x[I] = C::template two<4 * ST + I>(kw[t], sc);
