@@ -292,7 +292,16 @@ def test_attention_caps_biases_and_gates(gpu, bits, dtype):
 
 
 def test_attention_slopes_of_both_signs_and_none(gpu):
-    attention_case(gpu, [70, 300], slopes=[-0.01, 0.0, 0.5, -0.0, 1.0, 3.0, 0.001, 0.25], seed=11)
+    slopes = [-0.01, 0.0, 0.5, -0.0, 1.0, 3.0, 0.001, -20.0]
+    attention_case(gpu, [70, 300], slopes=slopes, seed=11)
+    # biases of up to 10^5 over the length: only those near the end that has the least count
+    attention_case(gpu, [5000, 4000], slopes=slopes, starts=[0, 1500], window=3900, softcap=20.0, d=64, seed=11)
+
+
+@pytest.mark.parametrize("cap", [0.01, 1.0, 3e4, 1e8])
+def test_attention_caps_of_any_size(gpu, cap):
+    """Scores far past the cap, and a cap far past the scores, which then are what they were."""
+    attention_case(gpu, [300, 40], softcap=cap, seed=21)
 
 
 @pytest.mark.parametrize("bits,dtype", FORMS)

@@ -261,6 +261,15 @@ __device__ __forceinline__ void each(F f) {
   }
 }
 
+// 1 - 2 / (e^2x + 1), which is off by some 2^-24: below 0.3 the series to x^9 (2^-24 of its value there), since a cap
+// far above the scores makes all of them small.
+__device__ __forceinline__ float tanh_of(float x) {
+  const float y = x * x;
+  const float p = fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+  const float e = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.f * kLog2e * x) + 1.f);
+  return y < 0.09f ? x * p : e;
+}
+
 // The product's type: the queries' for a 16-bit cache, bf16 for codes.
 template <int MT>
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -350,10 +359,12 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP)) decode_at
       qh[c] = x;
     }
   }
-  // scores in powers of two
+  // scores in powers of two, of a cap in caps
   const bool plain = a.cap == 0.f && !a.slopes;
-  const float mul = a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : kLog2e * a.scale;
+  const float mul = a.cap > 0.f ? a.scale / a.cap : kLog2e * a.scale;
   const float cap2 = a.cap * kLog2e, slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+  // Biases count from the end that has the least: the sum of a large one and a score would lose the score.
+  const int origin = slope < 0.f ? lo : hi - 1;
   // which of a dword's two slots holds a weight in this lane's column
   const uint32_t slot_mask = kSel == 1 ? 0u : sel ? 0xffff0000u : 0xffffu;
 
@@ -504,11 +515,10 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP)) decode_at
       x[u] = kHalves == 2 ? (half ? s[u / 2][2 + u % 2] : s[u / 2][u % 2]) : s[u / 4][u % 4];
     if (a.cap > 0.f) {
 #pragma unroll
-      for (int u = 0; u < kMine; ++u)
-        x[u] = cap2 * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x[u] * mul) + 1.f));
+      for (int u = 0; u < kMine; ++u) x[u] = cap2 * tanh_of(x[u] * mul);
     }
     if (a.slopes) {
-      const float back = static_cast<float>(hi - 1 - base - own), f = a.cap > 0.f ? 1.f : mul;
+      const float back = static_cast<float>(origin - base - own), f = a.cap > 0.f ? 1.f : mul;
 #pragma unroll
       for (int u = 0; u < kMine; ++u) x[u] = x[u] * f - slope * (back - static_cast<float>(step_of(u)));
     }
@@ -783,7 +793,8 @@ extern "C" int yh_decode_attention(const void* q, int64_t q_stride, const void* 
   YH_CHECK_ARG(D == 64 || D == 128 || D == 256, "decode_attention: head dim must be 64, 128 or 256");
   YH_CHECK_ARG(bits == 4 || bits == 8 || bits == 16, "decode_attention: a cache holds 4, 8 or 16 bits a value");
   YH_CHECK_ARG(scale > 0.f && scale < INFINITY, "decode_attention: scale must be positive");
-  YH_CHECK_ARG(softcap >= 0.f && softcap < INFINITY, "decode_attention: softcap must be positive, or 0 for none");
+  YH_CHECK_ARG(softcap == 0.f || (softcap >= 1e-30f && softcap <= 1e30f),
+               "decode_attention: softcap must be 1e-30 to 1e30, or 0 for none");
   if (dtype != YH_BF16 && dtype != YH_F16) {
     set_error("decode_attention: dtype must be bf16 or fp16");
     return YH_ERR_UNSUPPORTED;

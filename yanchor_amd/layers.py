@@ -911,8 +911,8 @@ def decode_attention(q, keys, values, block_tables, lengths, *, key_scales=None,
     if not 0 < sc < _INF:
         raise ValueError("scale must be positive")
     cap = 0.0 if softcap is None else float(softcap)
-    if softcap is not None and not 0 < cap < _INF:
-        raise ValueError("softcap must be positive")
+    if softcap is not None and not 1e-30 <= cap <= 1e30:     # the scores in caps, and back, are float32
+        raise ValueError("softcap must be positive, 1e-30 to 1e30")
     if slopes is not None:
         if slopes.dtype != torch.float32 or slopes.shape != (h,):
             raise ValueError("slopes must be float32 [H]")
