@@ -394,7 +394,14 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP)) decode_at
   // The lane's positions of product t, of 16 t on: `piece` of K, 4 quarter + j of V.
   uint32_t kw[NT][kKw], vw[kU][kVw];
   uint32_t ksc[NT][kPieces], vsc[NT];      // scale bytes of a K position, of four V positions
-  Row rows[NT];                        // of the next tile's products, where blocks hold whole runs of 16 positions
+  // Table entries of the next tile's products, the whole wave's where blocks hold whole runs of 16 positions, of the
+  // lane's K positions elsewhere, and their rows, or the entries of the tile whose V is loaded.
+  int ids[NT], own_ids[NT];
+  Row rows[NT];
+  auto load_ids = [&](int i) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) ids[t] = id_of((first_tile + i) * kTile + 16 * t + (RUNS ? 0 : piece));
+  };
   uint32_t holes = 0, vhole = 0;       // V's positions without a block: of the next tile, of this one
   const uint32_t k_off = (RUNS ? piece * kRow : 0) + quarter * kPb;
   const uint32_t v_off = RUNS ? 4 * quarter * kRow + piece * kVb : 0;
@@ -420,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP)) decode_at
         k_row(t, a.keys + at.row * kRow + k_off);
         k_scale(t, at.scale);
       } else {
-        const Row at = row_of(id_of(p + piece), p + piece);
+        const Row at = row_of(ids[t], p + piece);
         k_row(t, a.keys + at.row * kRow + k_off);
         k_scale(t, at.scale);
       }
@@ -440,8 +447,8 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP)) decode_at
         vsc[t] = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int at_p = p + 4 * quarter + j;
-          const int id = id_of(at_p);
+          // that of the lane which has the position for K
+          const int at_p = p + 4 * quarter + j, id = __shfl(own_ids[t], 4 * quarter + j, kWave);
           const Row at = row_of(id, at_p);
           vhole |= is_block(id) ? 0u : 1u << (4 * t + j);
           load_bytes<kVb>(vw[4 * t + j], a.values + at.row * kRow + piece * kVb);
@@ -452,13 +459,6 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP)) decode_at
       }
     }
   };
-  int ids[NT];
-  auto load_ids = [&](int i) {
-    if constexpr (RUNS) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) ids[t] = id_of((first_tile + i) * kTile + 16 * t);
-    }
-  };
   auto find_rows = [&](int i) {
     if constexpr (RUNS) {
       holes = 0;
@@ -467,6 +467,9 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP)) decode_at
         rows[t] = row_of(ids[t], (first_tile + i) * kTile + 16 * t);
         holes |= is_block(ids[t]) ? 0u : 15u << (4 * t);
       }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) own_ids[t] = ids[t];
     }
   };
 
