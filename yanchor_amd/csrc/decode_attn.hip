@@ -297,12 +297,12 @@ __device__ __forceinline__ void settle(f32x4 (&x)[N]) {
 }
 
 // Waves a SIMD that the registers are held to, where none spills for it.
-constexpr int waves_for(int DT, int FMT, int D, int HP) {
-  return D == 64 ? 3 : D == 256 || (FMT != k16 && (HP == 16 || (FMT == kFp8 && DT == YH_F16))) ? 2 : 3;
+constexpr int waves_for(int DT, int FMT, int D, int HP, bool RUNS) {
+  return D == 64 ? 3 : D == 256 || (FMT != k16 && (HP == 16 || !RUNS || (FMT == kFp8 && DT == YH_F16))) ? 2 : 3;
 }
 
 template <int DT, int FMT, int D, int HP, bool RUNS>
-__global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP)) decode_attention_kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) decode_attention_kernel(DecodeArgs a) {
   using C = Codes<FMT>;
   using M = attn::Mfma<DT>;
   constexpr int MT = FMT == k16 ? DT : YH_BF16;
@@ -745,16 +745,19 @@ int64_t target_for(int64_t R, int64_t H, int64_t G, int64_t block, int64_t colum
 }
 int64_t plan_bytes(int64_t R) { return ((R + 1) * 4 + 255) / 256 * 256; }
 
+template <int DT, int FMT, int D, int HP>
+void launch_heads(const DecodeArgs& a, bool runs, unsigned grid, hipStream_t st) {
+  // blocks that runs of 16 positions straddle: four columns or sixteen are enough kernels for a form off the main path
+  constexpr int kOdd = HP == 4 ? 4 : 16;
+  if (runs) hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, HP, true>), dim3(grid), dim3(kThreads), 0, st, a);
+  else hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, kOdd, false>), dim3(grid), dim3(kThreads), 0, st, a);
+}
 template <int DT, int FMT, int D>
 void launch(const DecodeArgs& a, unsigned grid, hipStream_t st) {
-  if (a.block.d % 16)
-    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, 16, false>), dim3(grid), dim3(kThreads), 0, st, a);
-  else if (a.rep <= 4 && FMT != k16)
-    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, FMT == k16 ? 8 : 4, true>), dim3(grid), dim3(kThreads), 0, st, a);
-  else if (a.rep <= 8)
-    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, 8, true>), dim3(grid), dim3(kThreads), 0, st, a);
-  else
-    hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, 16, true>), dim3(grid), dim3(kThreads), 0, st, a);
+  const bool runs = a.block.d % 16 == 0;
+  if (a.rep <= 4 && FMT != k16) launch_heads<DT, FMT, D, FMT == k16 ? 8 : 4>(a, runs, grid, st);
+  else if (a.rep <= 8) launch_heads<DT, FMT, D, 8>(a, runs, grid, st);
+  else launch_heads<DT, FMT, D, 16>(a, runs, grid, st);
   if (a.target) hipLaunchKernelGGL((decode_join_kernel<DT, D>), dim3(a.R * a.H), dim3(kThreads), 0, st, a);
 }
 template <int DT, int FMT>
