@@ -169,7 +169,7 @@ def call_on(device: torch.device, name: str, *args) -> None:
     """``call`` on the device's current stream (the last argument), with the
     device current, as a launch on its streams needs."""
     stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         call(name, *args, stream)
     else:
         with torch.cuda.device(device):

@@ -8,15 +8,15 @@ MAX_NODES = 64
 
 def device_of(first, *rest):
     """The ROCm device that all of the tensors (or None) share."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise ValueError(f"yanchor_amd kernels take ROCm device tensors (got a tensor on {dev})")
+    at = first.get_device()      # cheaper than comparing devices
+    if at < 0:
+        raise ValueError(f"yanchor_amd kernels take ROCm device tensors (got a tensor on {first.device})")
     for t in rest:
-        if t is not None and t.device != dev:
-            if t.device.type != "cuda":
+        if t is not None and t.get_device() != at:
+            if t.get_device() < 0:
                 raise ValueError(f"yanchor_amd kernels take ROCm device tensors (got a tensor on {t.device})")
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-    return dev
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    return first.device
 
 
 def ints(t, dtype, device, name, size=None):
