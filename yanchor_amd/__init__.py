@@ -8,7 +8,8 @@ Modules mirror the reference's call sites:
 * ``yanchor_amd.inference_kernels``   counter sampling, presence penalty, slot
                                       bookkeeping, packing and compaction, block tables
 * ``yanchor_amd.layers``              the steps between them: projections, norms,
-                                      prefill, attention over drafted trees
+                                      prefill, attention over drafted trees, quantised
+                                      caches and the decode attention over them
 
 All compute runs in hand-written HIP kernels from ``lib/libyanchor_amd.so``
 (built by ``python -m yanchor_amd.build``); there is no CPU fallback.

@@ -20,9 +20,12 @@
 // the position's weight in the even slot and zero in the odd one for a column of
 // the even dim, the other way round for the odd dim: with HP <= 8 heads the columns
 // head and head + HP are those two, with 16 heads there are two products.
-// (Transposing the pairs by v_perm instead takes as many instructions as the
-// conversions.)  With HP = 4 the other eight columns take half of the
-// positions, each lane half of the exponentials; their sums join at the end.
+// With HP = 4 the other eight columns take half of the positions, each lane half of
+// the exponentials; their sums join at the end.  (Pairs transposed by v_perm, as many
+// as there are conversions, and all exponentials in every column: 156 us for 135 with
+// 64 requests over 4 bits.)  In 16 bits, where a pair's other dim may hold an
+// infinity that zero would not hide, the pairs are transposed: there are no
+// conversions beside it.
 // With fp16 queries over codes, whose 11 bits bf16 does not hold, queries and
 // weights enter as two bf16 each (hi + lo).
 //
@@ -32,7 +35,13 @@
 // LDS.  Parts of a request that was cut leave theirs, with their maximum, in the
 // workspace, and a second launch joins them in order.
 //
-// Bound by HBM.
+// Bound by HBM: 133 ragged requests over 8 bits 214 us (1.18 GB, 5.5 TB/s), 8 long
+// contexts 193 (6.2), 64 requests over 4 bits 117 (5.4), heads of 256 in 16 bits 154
+// (5.4), where a large copy reaches 6.2 and a read alone 7.0.  Nontemporal loads,
+// since nothing is read twice but by up to four waves for 64 heads and more: the
+// long contexts 201 us for 217.  Blocks that runs of 16 positions straddle (block %
+// 16) have their table entries and rows a lane: 224 us for the long contexts with
+// blocks of 24, 368 with blocks of 1.
 #include <type_traits>
 
 #include "attn_tile.h"
@@ -732,14 +741,17 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
   *reinterpret_cast<u32x2*>(a.out + to) = u32x2{attn::pack2(y[0], y[1]), attn::pack2(y[2], y[3])};
 }
 
-constexpr int kWorkgroups = 2048;     // parts aimed at, over all heads: four workgroups a CU
+// Parts aimed at, over all heads, so that the last of those that fit the chip (two or three workgroups a CU) end at
+// about one time.  us of 133 requests over 8 bits, 64 over 4 bits and 8 long contexts: 1024 parts 236, 160, 236; 2048 229,
+// 156, 219; 4096 239, 145, 230.
+constexpr int kWorkgroups = 2048;
 
 // Parts aimed at for each KV head, 0 where no request is cut.
 int64_t target_for(int64_t R, int64_t H, int64_t G, int64_t block, int64_t columns, int64_t window, int64_t max_length) {
   int64_t most = columns * block;
   if (window && window < most) most = window;
   if (max_length >= 0 && max_length < most) most = max_length;
-  if (most + 63 <= 64 * kWaves) return 0;     // a turn of the waves at most, where tiles have 64 positions
+  if (most + 63 <= 64 * kWaves) return 0;     // a turn of the waves at most, where tiles have 64 positions: no second launch
   const int64_t each = G * ((H / G + kCols - 1) / kCols), n = (kWorkgroups + each - 1) / each;
   return n < 1 ? 1 : n;
 }
@@ -821,6 +833,7 @@ extern "C" int yh_decode_attention(const void* q, int64_t q_stride, const void* 
   const int64_t target = target_for(n_seqs, H, G, block, columns, window, max_length);
   int64_t most = columns * block;
   if (window && window < most) most = window;
+  if (most > (1ll << 31)) most = 1ll << 31;      // positions are below
   YH_CHECK_ARG(n_seqs * (most / 16 + 2) < (1ll << 31), "decode_attention: sizes too large");
   const int64_t grid = (n_seqs + target) * each;
   YH_CHECK_ARG(grid < (1ll << 24) && n_seqs * H < (1ll << 24), "decode_attention: sizes too large");

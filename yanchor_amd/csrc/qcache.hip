@@ -6,6 +6,13 @@
 // is read back are exact but for that one rounding (half a step: 2^-4 of an e4m3
 // value, 1/4 of the code's power of two of an e2m1 value).
 // Read: value = code 2^(s - 127), rounded to the output's type.
+//
+// Bound by HBM and, where slots are scattered, by its granules: 65521 tokens of 8
+// heads of 128 into scattered rows of 4 bits 92 us for 340 MB, of which the scale
+// bytes, each in a granule of its own, take 23 and the 64-byte rows 14 (the input
+// alone streams in 43); back 79; 146000 tokens in order of 8 bits back 177 us, 5.1
+// TB/s.  Rows in and out pass the caches (101 and 91 us through them); codes of 4 bits
+// do not, as two rows share a granule (79 us for 91).
 #include "qcache.h"
 #include "tree.h"
 
@@ -36,7 +43,8 @@ struct Args {
 };
 
 constexpr int kThreads = 256;
-// Tokens that a thread takes in a row where there are many (U = 1 for few): what lies where in a row is found once.
+// Tokens that a thread takes where there are many (U = 1 for few), so that what lies where in a row is found once.
+// (us of the prefixes in order back: one 187, two 184, four 177, eight 174, but eight write in 100 for 92.)
 constexpr int kMany = 4;
 
 // Piece p of a token's row: its bytes from the block's begin on, of FMT, and its scale's.
@@ -241,7 +249,7 @@ int check_cache(const char* what, const void* keys, const void* values, const ui
   YH_CHECK_ARG(N < (1ll << 31) && blocks < (1ll << 31) && block < (1ll << 31) && G < (1ll << 31) && D < (1ll << 31) &&
                    G * D < (1ll << 31) && blocks * block < (1ll << 40),
                "%s: sizes too large", what);
-  YH_CHECK_ARG(G * block * D * 2 < (1ll << 32) && N * (G * D / 8) < (1ll << 32), "%s: sizes too large", what);
+  YH_CHECK_ARG(G * D * block * 2 < (1ll << 32) && N * (G * D / 8) < (1ll << 32), "%s: sizes too large", what);
   if (N == 0) return YH_OK;
   YH_CHECK_ARG(slots && ((keys && values && (bits == 16 || (key_scales && value_scales))) || blocks == 0),
                "%s: null pointer", what);

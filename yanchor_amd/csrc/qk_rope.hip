@@ -11,8 +11,12 @@
 // and its reduction to one turn are float64, and sine and cosine take the turn's
 // rest in float32 (2^-25 of a turn).
 //
-// Bound by HBM: heads are read and written once.  A wave takes heads of one token,
-// eight elements a lane; its lanes form the token's angles, one or two each, once.
+// Bound by HBM, heads are read and written once: 65521 tokens of 40 heads of 128 in
+// 231 us, 5.8 TB/s.  A wave takes heads of one token, eight elements a lane; its lanes
+// form the token's angles, one or two each, once, and exchange them through LDS.
+// (296 us with a square root and a division a head, weights and angles applied one
+// after the other, sums by LDS shuffles and one load ahead: 210 instructions for four
+// heads, of which the memory leaves time for about 150.)
 #include "attn_tile.h"
 #include "tree.h"
 
