@@ -657,3 +657,63 @@ def test_unchanged_inputs_and_repeated_calls(gpu):
     assert torch.equal(first, call()) and math.isfinite(first.float().sum().item())
     after = [t.view(torch.uint8) for t in (*c, q.view(torch.uint8), tables.view(torch.uint8), lens.view(torch.uint8))]
     assert all(torch.equal(a, b) for a, b in zip(before, after))
+
+
+def test_odd_arguments(gpu):
+    """Vectors from the host or in int32, layers of one pool, broadcast gates, rows that are no rows, tables with room."""
+    g, block, d, h, blocks = 2, 24, 64, 6, 10
+    pool = [torch.zeros(3, *t.shape, dtype=torch.uint8, device=gpu) for t in layers.quantized_cache(blocks, g, block, d, device="cpu")]
+    layer = [pool[0][1].view(torch.float8_e4m3fn), pool[1][1].view(torch.float8_e4m3fn), pool[2][1], pool[3][1]]
+    n = 100
+    k, v = (rnd(n, g, d, seed=s).to(gpu) for s in (1, 2))
+    slots = torch.randperm(blocks * block, generator=torch.Generator().manual_seed(3))[:n]
+    layers.cache_write_quantized(k, v, slots.to(torch.int32), *layer)                       # from the host
+    assert not any(t[0].any() or t[2].any() for t in pool)
+    spread = torch.zeros(n, 2, g, d, dtype=B, device=gpu)[:, 0]                             # rows of twice the width
+    spread.copy_(k)
+    again = [t.clone() for t in layer]
+    layers.cache_write_quantized(spread, k.transpose(1, 2).contiguous().transpose(1, 2).copy_(v), slots.to(gpu), *again)
+    for a, b in zip(layer, again):
+        same = torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        assert same
+    back = layers.cache_read(slots.to(torch.int32), *layer)
+    for x, y in zip((k, v), back):
+        same = torch.equal(y.cpu(), ref.quantise(x.cpu(), 8)[0].to(B))
+        assert same
+    q = rnd(2, h, d, seed=4).to(gpu)
+    tables = i32([[3, 1, 0, 7], [9, 4, 5, 2]], gpu)
+    gate = rnd(1, h, d, seed=5).to(gpu)
+    lens = torch.tensor([70, 41])
+    call = lambda q, tables, lens, gate, **kw: layers.decode_attention(  # noqa: E731
+        q, layer[0], layer[1], tables, lens, key_scales=layer[2], value_scales=layer[3], gate=gate, **kw)
+    plain = call(q, tables, lens.to(gpu), gate.expand(2, h, d).contiguous(), starts=torch.tensor([5, 0], device=gpu))
+    wide = i32([[3, 1, 0, 7, -1, 50], [9, 4, 5, 2, 6, 8]], gpu)
+    for got in (call(q, tables, lens, gate.expand(2, h, d), starts=torch.tensor([5, 0], dtype=torch.int32)),
+                call(q.transpose(0, 1).contiguous().transpose(0, 1), wide[:, :4], lens.to(torch.int32), gate.expand(2, h, d),
+                     starts=torch.tensor([5, 0])),
+                call(q.repeat_interleave(2, 2)[..., ::2], wide, lens, gate.expand(2, h, d), starts=torch.tensor([5, 0]))):
+        assert torch.equal(got, plain)
+    one = call(q[:1], tables[:1], lens[:1], gate, starts=torch.tensor([5]))                 # a single row's strides say nothing
+    assert torch.equal(one, plain[:1])
+    x, pos = rnd(7, 3, 128, seed=6).to(gpu), torch.arange(21).view(7, 3).T
+    freq = torch.rand(32, generator=torch.Generator().manual_seed(7))
+    a = layers.qk_norm_rope(x, x, None, None, pos, freq[::2].to(gpu), 1e-6, sections=[6, 5, 5])
+    b = layers.qk_norm_rope(x.expand(7, 3, 128), x[:, :1].expand(7, 3, 128), None, None, pos.to(gpu), freq[::2].contiguous().to(gpu),
+                            1e-6, sections=(6, 5, 5))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1][:, :1].expand(7, 3, 128), b[1])
+
+
+def test_other_cuda_streams_own_scratch(gpu):
+    """Inputs made on one stream, used on another that waits for it; scratch is the using stream's."""
+    side = torch.cuda.Stream()
+    x, y = (rnd(200, 1, 16, 128, seed=s) for s in (1, 2))
+    c = [t.to(gpu) for t in cache_of(x, y, 4)]
+    q, tables, lens = rnd(1, 4, 128, seed=3).to(gpu), i32([list(range(200))], gpu), torch.tensor([3200], device=gpu)
+    want = layers.decode_attention(q, c[0], c[1], tables, lens, key_scales=c[2], value_scales=c[3])
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = layers.decode_attention(q, c[0], c[1], tables, lens, key_scales=c[2], value_scales=c[3])
+        rows = layers.cache_read(torch.arange(40, device=gpu), *c)
+    torch.cuda.current_stream().wait_stream(side)
+    noise = [torch.full((1 << 20,), NAN, device=gpu) for _ in range(4)]
+    assert torch.equal(got, want) and rows[0].shape == (40, 1, 128) and len(noise) == 4
