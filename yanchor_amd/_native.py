@@ -159,7 +159,7 @@ def lib() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Invoke entry point ``name``; raise NativeError with the library's message on failure."""
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != 0:
         msg = lib().yh_last_error().decode(errors="replace")
         raise NativeError(f"{name} failed ({rc}): {msg}")

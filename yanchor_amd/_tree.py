@@ -21,10 +21,11 @@ def device_of(first, *rest):
 
 def ints(t, dtype, device, name, size=None):
     """``t`` as a contiguous 1-D integer tensor of ``dtype`` on the device."""
-    if t.ndim != 1 or (t.dtype != dtype and t.dtype not in (torch.int32, torch.int64)):
+    shape = t.shape
+    if len(shape) != 1 or (t.dtype != dtype and t.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"{name} must be a 1-D integer tensor")
-    if size is not None and t.shape[0] != size:
-        raise ValueError(f"{name} must hold {size} entries, got {t.shape[0]}")
+    if size is not None and shape[0] != size:
+        raise ValueError(f"{name} must hold {size} entries, got {shape[0]}")
     if t.dtype != dtype or t.device != device:
         t = t.to(device=device, dtype=dtype)
     return t if t.is_contiguous() else t.contiguous()

@@ -775,6 +775,7 @@ def conv_tree(proj, window, conv_w, parents, cu_seqlens, channels, planes=1):
 # Nothing is read back to the host, so these calls can be captured.
 
 _INF = float("inf")
+_HALF = (torch.bfloat16, torch.float16)
 
 
 def quantized_cache(blocks, groups, block, dim, *, bits=8, device=None):
@@ -800,24 +801,25 @@ def _any_cache(keys, values, key_scales, value_scales, g, d, dtype):
     if len(shape) != 4 or values.shape != shape or values.dtype != kind or not keys.is_contiguous() or \
             not values.is_contiguous():
         raise ValueError("keys and values must be contiguous [blocks, G, block, D] of one type")
+    blocks, groups, block, width = shape
     if kind == torch.float8_e4m3fn:
-        bits, width = 8, d
+        bits = 8
     elif kind == torch.uint8:
-        bits, width = 4, d // 2
-    elif kind in (torch.bfloat16, torch.float16):
+        bits, width = 4, 2 * width
+    elif kind in _HALF:
         if key_scales is not None or value_scales is not None:
             raise ValueError("a 16-bit cache has no scales")
         if kind != dtype:
             raise ValueError(f"a 16-bit cache must be in {dtype}")
-        bits, width = 16, d
+        bits = 16
     else:
         raise ValueError("a cache is bf16, fp16, float8_e4m3fn (8 bits) or uint8 (4 bits, two a byte)")
-    if shape[1] != g or shape[3] != width or shape[2] < 1:
-        raise ValueError(f"a {bits}-bit cache of these heads is [blocks, {g}, block, {width}]")
+    if groups != g or width != d or block < 1:
+        raise ValueError(f"a {bits}-bit cache of these heads is [blocks, {g}, block, {d // 2 if bits == 4 else d}]")
     if bits < 16:
         if d % 32:
             raise ValueError("the head dim of a quantised cache must be a multiple of 32")
-        want = (shape[0], g, d // 32, shape[2])
+        want = (blocks, g, d // 32, block)
         for s in (key_scales, value_scales):
             if s is None or s.shape != want or s.dtype != torch.uint8 or not s.is_contiguous():
                 raise ValueError(f"a quantised cache needs contiguous uint8 scales {list(want)}")
@@ -834,16 +836,18 @@ def cache_write_quantized(k, v, slots, keys, values, key_scales, value_scales):
     e4m3 value, a quarter of the leading power of two of an e2m1 one (in both,
     half of the smallest code near zero).  A run that holds a NaN or an infinity
     reads back as NaN."""
-    if k.ndim != 3 or v.shape != k.shape or k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16):
+    kind, shape = k.dtype, k.shape
+    if len(shape) != 3 or v.shape != shape or v.dtype != kind or kind not in _HALF:
         raise ValueError("cache_write_quantized takes bf16 / fp16 k and v [N, G, D]")
-    n, g, d = k.shape
+    n, g, d = shape
     bits = _any_cache(keys, values, key_scales, value_scales, g, d, None)
     dev = _tree.device_of(k, v, keys, values, key_scales, value_scales)
     slots = _tree.ints(slots, torch.int64, dev, "slots", n)
     (k, ks), (v, vs) = _heads(k), _heads(v)
+    blocks, _, block, _ = keys.shape
     N.call_on(dev, "yh_cache_write_quantized", k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(), keys.data_ptr(),
-              values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), n, keys.shape[0], g, d,
-              keys.shape[2], bits, N.code(k))
+              values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), n, blocks, g, d, block, bits,
+              N.DTYPE_CODE[kind])
 
 
 def cache_read(slots, keys, values, key_scales=None, value_scales=None, *, dtype=None):
@@ -854,21 +858,23 @@ def cache_read(slots, keys, values, key_scales=None, value_scales=None, *, dtype
     outside the cache gives zeros."""
     if keys.ndim != 4:
         raise ValueError("keys and values must be contiguous [blocks, G, block, D] of one type")
-    half = keys.dtype in (torch.bfloat16, torch.float16)
-    dtype = dtype or (keys.dtype if half else torch.bfloat16)
-    if dtype not in (torch.bfloat16, torch.float16):
+    kind = keys.dtype
+    dtype = dtype or (kind if kind in _HALF else torch.bfloat16)
+    if dtype not in _HALF:
         raise ValueError("cache_read gives bf16 or fp16 rows")
-    g, d = keys.shape[1], keys.shape[3] * (2 if keys.dtype == torch.uint8 else 1)
+    blocks, g, block, d = keys.shape
+    if kind == torch.uint8:
+        d *= 2
     bits = _any_cache(keys, values, key_scales, value_scales, g, d, dtype)
     if d % 8 or not d or not g:
         raise ValueError("a head's row must be a multiple of 16 bytes")
     dev = _tree.device_of(keys, values, key_scales, value_scales)
     slots = _tree.ints(slots, torch.int64, dev, "slots")
     n = slots.shape[0]
-    k, v = (torch.empty(n, g, d, dtype=dtype, device=dev) for _ in range(2))
+    k = torch.empty((n, g, d), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     N.call_on(dev, "yh_cache_read", slots.data_ptr(), keys.data_ptr(), values.data_ptr(), N.ptr(key_scales),
-              N.ptr(value_scales), k.data_ptr(), v.data_ptr(), n, keys.shape[0], g, d, keys.shape[2], bits,
-              N.DTYPE_CODE[dtype])
+              N.ptr(value_scales), k.data_ptr(), v.data_ptr(), n, blocks, g, d, block, bits, N.DTYPE_CODE[dtype])
     return k, v
 
 
@@ -888,31 +894,40 @@ def decode_attention(q, keys, values, block_tables, lengths, *, key_scales=None,
     the result is read * sigmoid(gate).  Returns [R, H, D]; a row that sees nothing
     (a length of 0 in a captured batch) is zeros.  ``max_length``: no request has
     more positions (a call of short ones then takes one launch)."""
-    if q.dtype not in (torch.bfloat16, torch.float16) or q.ndim != 3:
+    kind, shape = q.dtype, q.shape
+    if kind not in _HALF or len(shape) != 3:
         raise ValueError("decode_attention takes bf16 / fp16 q [R, H, D]")
-    r, h, d = q.shape
+    r, h, d = shape
     if d not in (64, 128, 256):
         raise ValueError("head dim must be 64, 128 or 256")
-    if keys.ndim != 4 or keys.shape[1] < 1 or h < 1 or h % keys.shape[1]:
+    if keys.ndim != 4:
         raise ValueError("decode_attention needs keys [blocks, G, block, D] with G dividing the query heads")
-    g = keys.shape[1]
-    bits = _any_cache(keys, values, key_scales, value_scales, g, d, q.dtype)
+    blocks, g, block, _ = keys.shape
+    if g < 1 or h < 1 or h % g:
+        raise ValueError("decode_attention needs keys [blocks, G, block, D] with G dividing the query heads")
+    bits = _any_cache(keys, values, key_scales, value_scales, g, d, kind)
     dev = _tree.device_of(q, keys, values, block_tables, key_scales, value_scales, gate, slopes)
-    lens = _tree.ints(lengths, torch.int64, dev, "lengths", r)
+    lengths = _tree.ints(lengths, torch.int64, dev, "lengths", r)
     if starts is not None:
         starts = _tree.ints(starts, torch.int64, dev, "starts", r)
-    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.shape[0] != r or \
-            block_tables.shape[1] < 1:
+    shape = block_tables.shape
+    if block_tables.dtype != torch.int32 or len(shape) != 2 or shape[0] != r or shape[1] < 1:
         raise ValueError("block_tables must be int32 [R, columns]")
+    columns = shape[1]
     tables = block_tables if block_tables.is_contiguous() else block_tables.contiguous()
-    if window is not None and int(window) < 1:
-        raise ValueError("window must be at least 1")
-    sc = float(d ** -0.5 if scale is None else scale)
-    if not 0 < sc < _INF:
+    win = 0
+    if window is not None:
+        win = int(window)
+        if win < 1:
+            raise ValueError("window must be at least 1")
+    scale = float(d ** -0.5 if scale is None else scale)
+    if not 0 < scale < _INF:
         raise ValueError("scale must be positive")
-    cap = 0.0 if softcap is None else float(softcap)
-    if softcap is not None and not 1e-30 <= cap <= 1e30:     # the scores in caps, and back, are float32
-        raise ValueError("softcap must be positive, 1e-30 to 1e30")
+    cap = 0.0
+    if softcap is not None:
+        cap = float(softcap)
+        if not 1e-30 <= cap <= 1e30:     # the scores in caps, and back, are float32
+            raise ValueError("softcap must be positive, 1e-30 to 1e30")
     if slopes is not None:
         if slopes.dtype != torch.float32 or slopes.shape != (h,):
             raise ValueError("slopes must be float32 [H]")
@@ -920,39 +935,41 @@ def decode_attention(q, keys, values, block_tables, lengths, *, key_scales=None,
     q, qs = _heads(q)
     gp, gts, ghs = None, 0, 0
     if gate is not None:
-        if gate.shape != (r, h, d) or gate.dtype != q.dtype:
+        if gate.shape != (r, h, d) or gate.dtype != kind:
             raise ValueError("gate must be [R, H, D] in the query dtype")
-        if gate.stride(2) != 1 or gate.stride(1) < d or gate.stride(0) < h * gate.stride(1):   # not rows of heads
-            gate = gate.contiguous()
+        gts, ghs, unit = gate.stride()
+        if unit != 1 or ghs < d or gts < h * ghs:       # not rows of heads, or of a single head or row
+            if not gate.is_contiguous():
+                gate = gate.contiguous()
+            gts, ghs = h * d, d
         gp = gate.data_ptr()
-        gts, ghs = (h * d, d) if gate.is_contiguous() else (gate.stride(0), gate.stride(1))
-    out = torch.empty(r, h, d, dtype=q.dtype, device=dev)
-    block, columns, win = keys.shape[2], tables.shape[1], 0 if window is None else int(window)
+    out = torch.empty((r, h, d), dtype=kind, device=dev)
     longest = -1 if max_length is None else int(max_length)
     # scratch of the call: concurrent calls on different streams are independent
     need = N.lib().yh_decode_attention_workspace_bytes(r, h, g, d, block, columns, win, longest)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
     N.call_on(dev, "yh_decode_attention", q.data_ptr(), qs, keys.data_ptr(), values.data_ptr(), N.ptr(key_scales),
-              N.ptr(value_scales), tables.data_ptr(), lens.data_ptr(), N.ptr(starts), N.ptr(slopes), gp, gts, ghs,
-              out.data_ptr(), r, keys.shape[0], columns, h, g, d, block, win, longest, sc, cap, bits, N.code(q),
+              N.ptr(value_scales), tables.data_ptr(), lengths.data_ptr(), N.ptr(starts), N.ptr(slopes), gp, gts, ghs,
+              out.data_ptr(), r, blocks, columns, h, g, d, block, win, longest, scale, cap, bits, N.DTYPE_CODE[kind],
               N.ptr(ws), need)
     return out
 
 
-def _head_rows(x):
+def _head_rows(x, n, h, d):
     """(x, token stride, head stride) of x [N, heads, D] with 16-byte aligned
     heads (a column view of a projection qualifies), of a copy otherwise."""
-    n, h, d = x.shape
     a, b, c = x.stride()
-    if (c != 1 or a % 8 and n > 1 or b % 8 and h > 1 or x.data_ptr() % 16) and x.numel():
+    if (c != 1 or a % 8 and n > 1 or b % 8 and h > 1 or x.data_ptr() % 16) and n and h:
         x, a, b = x.clone(memory_format=torch.contiguous_format), h * d, d
     return x, a if n > 1 else 0, b if h > 1 else 0     # a stride of a single row says nothing
 
 
-def _weight(w):
-    if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0):
-        return w
-    return w.clone(memory_format=torch.contiguous_format)
+def _weight(w, d, dtype):
+    if w is None:
+        return None
+    if w.shape != (d,) or w.dtype != dtype:
+        raise ValueError("norm weights must be [D] in the dtype of q and k")
+    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
 
 
 def qk_norm_rope(q, k, q_w, k_w, positions, inv_freq, eps, *, sections=None, interleaved=False, plus_one=True):
@@ -966,23 +983,23 @@ def qk_norm_rope(q, k, q_w, k_w, positions, inv_freq, eps, *, sections=None, int
     axis 0 otherwise.  inv_freq float32, a multiple of 8 of them.  float32
     throughout and rounded once; the angle in float64, so positions of millions
     keep theirs (``head_norm_rope`` takes tables, of one axis, and rounds the norm)."""
-    if q.ndim != 3 or k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or \
-            q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype:
+    kind, shape, other = q.dtype, q.shape, k.shape
+    if len(shape) != 3 or len(other) != 3 or other[0] != shape[0] or other[2] != shape[2] or kind not in _HALF or \
+            k.dtype != kind:
         raise ValueError("qk_norm_rope takes bf16 / fp16 q [N, H, D] and k [N, G, D] of one dtype")
-    (n, h, d), g = q.shape, k.shape[1]
+    (n, h, d), g = shape, other[1]
     if d not in (64, 128, 256):
         raise ValueError("head dim must be 64, 128 or 256")
-    for w in (q_w, k_w):
-        if w is not None and (w.shape != (d,) or w.dtype != q.dtype):
-            raise ValueError("norm weights must be [D] in the dtype of q and k")
-    if inv_freq.ndim != 1 or inv_freq.dtype != torch.float32 or inv_freq.shape[0] % 8 or 2 * inv_freq.shape[0] > d:
+    q_w, k_w = _weight(q_w, d, kind), _weight(k_w, d, kind)
+    shape = inv_freq.shape
+    if len(shape) != 1 or inv_freq.dtype != torch.float32 or shape[0] % 8 or 2 * shape[0] > d:
         raise ValueError("inv_freq must be float32, a multiple of 8 and at most D / 2 of them")
-    eps = float(eps)
+    half, eps = shape[0], float(eps)
     if not 0 <= eps < _INF:
         raise ValueError("eps must not be negative")
-    half = inv_freq.shape[0]
-    axes = 1 if positions.ndim == 1 else positions.shape[0] if positions.ndim == 2 else 0
-    if not 1 <= axes <= 4 or positions.shape[-1] != n or positions.dtype not in (torch.int32, torch.int64):
+    shape = positions.shape
+    axes = 1 if len(shape) == 1 else shape[0] if len(shape) == 2 else 0
+    if not 1 <= axes <= 4 or shape[-1] != n or positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be integers [N] or [axes, N] of 1 to 4 axes")
     counts = None
     if sections is not None:
@@ -997,12 +1014,11 @@ def qk_norm_rope(q, k, q_w, k_w, positions, inv_freq, eps, *, sections=None, int
     dev = _tree.device_of(q, k, q_w, k_w, inv_freq)
     if positions.dtype != torch.int64 or positions.device != dev or not positions.is_contiguous():
         positions = positions.to(device=dev, dtype=torch.int64).contiguous()
-    (q, qts, qhs), (k, kts, khs) = _head_rows(q), _head_rows(k)
-    q_w, k_w = _weight(q_w), _weight(k_w)
+    (q, qts, qhs), (k, kts, khs) = _head_rows(q, n, h, d), _head_rows(k, n, g, d)
     if not inv_freq.is_contiguous():
         inv_freq = inv_freq.contiguous()
-    qo, ko = torch.empty(n, h, d, dtype=q.dtype, device=dev), torch.empty(n, g, d, dtype=q.dtype, device=dev)
+    qo, ko = (torch.empty((n, x, d), dtype=kind, device=dev) for x in (h, g))
     N.call_on(dev, "yh_qk_norm_rope", q.data_ptr(), qts, qhs, k.data_ptr(), kts, khs, N.ptr(q_w), N.ptr(k_w),
               positions.data_ptr(), inv_freq.data_ptr(), counts, axes, 1 if interleaved else 0, qo.data_ptr(),
-              ko.data_ptr(), n, h, g, d, 2 * half, eps, 1 if plus_one else 0, N.code(q))
+              ko.data_ptr(), n, h, g, d, 2 * half, eps, 1 if plus_one else 0, N.DTYPE_CODE[kind])
     return qo, ko
