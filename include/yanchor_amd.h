@@ -983,7 +983,7 @@ int yh_cache_read(const int64_t* slots, const void* keys, const void* values, co
  * overlap need one each.
  */
 int64_t yh_decode_attention_workspace_bytes(int64_t n_seqs, int64_t H, int64_t G, int64_t D, int64_t block,
-                                            int64_t columns, int64_t window, int64_t max_length);
+                                            int64_t columns, int64_t window, int64_t max_length, int bits, int dtype);
 int yh_decode_attention(const void* q, int64_t q_stride, const void* keys, const void* values,
                         const uint8_t* key_scales, const uint8_t* value_scales, const int32_t* tables,
                         const int64_t* lengths, const int64_t* starts, const float* slopes, const void* gate,

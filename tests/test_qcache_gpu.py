@@ -323,6 +323,16 @@ def test_attention_of_many_requests(gpu):
     attention_case(gpu, lengths, h=2, g=1, d=64, block=32, seed=16)
 
 
+@pytest.mark.parametrize("requests,h,g", [(130, 2, 1), (40, 8, 8), (64, 20, 1), (65, 4, 4)])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_attention_of_many_requests_in_parts(gpu, bits, requests, h, g):
+    """Some cut and some not, found by a wave (64 requests) and by a workgroup (65), parts of several turns."""
+    gen = torch.Generator().manual_seed(requests)
+    lengths = torch.randint(0, 900, (requests,), generator=gen).tolist()
+    lengths[2], lengths[-1], lengths[requests // 2] = 3300, 2500, 0
+    attention_case(gpu, lengths, bits=bits, h=h, g=g, d=64, block=48, seed=22)
+
+
 @pytest.mark.parametrize("max_length", [None, 10, 250, 5000])
 def test_attention_bounds_change_nothing(gpu, max_length):
     """A bound that is too low changes no result."""

@@ -195,8 +195,8 @@ def test_c_calls_refuse_before_device_work(lib):
     refused(attn(gate=p, ghs=64), b"gate strides")
     refused(attn(n=1 << 20), b"too large")
     refused(attn(n=1 << 15, columns=1 << 26), b"too large")
-    need = lib.yh_decode_attention_workspace_bytes(1, 8, 2, 128, 16, 900, 0, -1)
-    assert need > 0 and lib.yh_decode_attention_workspace_bytes(1, 8, 2, 128, 16, 900, 100, -1) == 0
+    need = lib.yh_decode_attention_workspace_bytes(1, 8, 2, 128, 16, 900, 0, -1, 8, 1)
+    assert need > 0 and lib.yh_decode_attention_workspace_bytes(1, 8, 2, 128, 16, 900, 100, -1, 8, 1) == 0
     refused(attn(columns=900, ws=need - 1), b"workspace")
     assert attn(dtype=0) == -3 and attn(n=0) == 0
 

@@ -110,7 +110,7 @@ PLAIN: dict[str, tuple] = {
     "yh_extend_plan_bytes": (_i64, [_i64, _i64]),
     "yh_trim_plan_bytes": (_i64, [_i64, _i64]),
     "yh_tree_attention_workspace_bytes": (_i64, [_i64] * 9),
-    "yh_decode_attention_workspace_bytes": (_i64, [_i64] * 8),
+    "yh_decode_attention_workspace_bytes": (_i64, [_i64] * 8 + [_i32] * 2),
     "yh_topk_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "yh_linear_split": (_i32, [_i64, _i64, _i64]),
     "yh_linear_packed_split": (_i32, [_i64, _i64, _i64]),

@@ -137,10 +137,18 @@ struct Part {
   Seen seen;
 };
 
-// Tiles of a part: a turn of the waves at least.
+// Tiles of a part, of `total` of each KV head: as many as leave `target` parts, and a turn of the waves at least; up to
+// four turns (eight of 16 positions) where there are more than two parts a CU, since each begins with a chain of loads.
+// (us of captured calls, 8 KV heads of 128 in 8 bits, with a turn at least: 64 requests of 900 positions 27 for 37, 200
+// of 1800 157 for 169; heads of 256 in 16 bits, eight turns and four: 93 and 98 with 64 requests of 900.)
+template <int TILE>
 __device__ __forceinline__ int chunk_of(const DecodeArgs& a, int total) {
-  const int chunk = a.target ? (total + a.target - 1) / a.target : 0x7fffffff;
-  return chunk < kWaves ? kWaves : chunk;
+  if (a.target == 0) return 0x7fffffff;
+  constexpr int kMost = (TILE == 16 ? 8 : 4) * kWaves;
+  const int fine = (total + a.target - 1) / a.target;
+  const int64_t room = static_cast<int64_t>(total) * (a.G * a.mtiles) / 512;
+  const int turns = room < kWaves ? kWaves : room > kMost ? kMost : static_cast<int>(room);
+  return fine > turns ? fine : turns;
 }
 __device__ __forceinline__ int parts_of(int tiles, int chunk) { return tiles > chunk ? (tiles + chunk - 1) / chunk : 1; }
 // Part `index` of `count` of a request of n tiles; they differ by a tile.
@@ -158,7 +166,7 @@ __device__ Part find_part(const DecodeArgs& a, int which) {
     const int lane = threadIdx.x & (kWave - 1);
     const Seen seen = lane < a.R ? seen_of(a, lane) : Seen{0, 0};
     const int n = tiles_of<TILE>(seen);
-    const int chunk = chunk_of(a, __shfl(scan_wave(n), kWave - 1, kWave));
+    const int chunk = chunk_of<TILE>(a, __shfl(scan_wave(n), kWave - 1, kWave));
     const int c = lane < a.R ? parts_of(n, chunk) : 0, end = scan_wave(c);
     const uint64_t behind = __ballot(end > which);
     if (behind == 0) return {0, 0, 0, 0, 0, 0, {0, 0}};
@@ -180,7 +188,7 @@ __device__ Part find_part(const DecodeArgs& a, int which) {
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) total += sums[i];
   __syncthreads();
-  const int chunk = chunk_of(a, total);
+  const int chunk = chunk_of<TILE>(a, total);
   mine = 0;
   for (int r = r0; r < r1; ++r) {
     mine += parts_of(tiles_of<TILE>(seen_of(a, r)), chunk);
@@ -746,13 +754,21 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
 // 156, 219; 4096 239, 145, 230.
 constexpr int kWorkgroups = 2048;
 
-// Parts aimed at for each KV head, 0 where no request is cut.
-int64_t target_for(int64_t R, int64_t H, int64_t G, int64_t block, int64_t columns, int64_t window, int64_t max_length) {
+// Positions of a tile.
+int64_t tile_of(int bits, int64_t D, int dtype) {
+  return 16 * products(static_cast<int>(D * bits / 8), bits != 16 && dtype == YH_F16 && D == 256);
+}
+// Parts aimed at for each KV head, 0 where no request is cut and the second launch is not made: up to two turns of the
+// waves, or eight where there are heads enough.  (400 positions: one request 7.7 us captured and 13 called for 8.9 and
+// 18, 64 requests 15 for 22, 200 47 for 61.)
+int64_t target_for(int64_t R, int64_t H, int64_t G, int64_t D, int64_t block, int64_t columns, int64_t window,
+                   int64_t max_length, int bits, int dtype) {
   int64_t most = columns * block;
   if (window && window < most) most = window;
   if (max_length >= 0 && max_length < most) most = max_length;
-  if (most + 63 <= 64 * kWaves) return 0;     // a turn of the waves at most, where tiles have 64 positions: no second launch
-  const int64_t each = G * ((H / G + kCols - 1) / kCols), n = (kWorkgroups + each - 1) / each;
+  const int64_t each = G * ((H / G + kCols - 1) / kCols), tile = tile_of(bits, D, dtype), tiles = (most + tile - 1) / tile;
+  if (tiles <= 2 * kWaves || (R * each >= 512 && tiles <= 8 * kWaves)) return 0;
+  const int64_t n = (kWorkgroups + each - 1) / each;
   return n < 1 ? 1 : n;
 }
 int64_t plan_bytes(int64_t R) { return ((R + 1) * 4 + 255) / 256 * 256; }
@@ -789,12 +805,13 @@ void launch_bits(const DecodeArgs& a, int bits, int64_t D, unsigned grid, hipStr
 }  // namespace yh
 
 extern "C" int64_t yh_decode_attention_workspace_bytes(int64_t n_seqs, int64_t H, int64_t G, int64_t D, int64_t block,
-                                                       int64_t columns, int64_t window, int64_t max_length) {
+                                                       int64_t columns, int64_t window, int64_t max_length, int bits,
+                                                       int dtype) {
   using namespace yh;
   if (n_seqs <= 0 || G <= 0 || H < G || D <= 0 || block <= 0 || columns <= 0 || columns >= (1ll << 31) ||
-      block >= (1ll << 31))
+      block >= (1ll << 31) || (bits != 4 && bits != 8 && bits != 16))
     return 0;
-  const int64_t target = target_for(n_seqs, H, G, block, columns, window, max_length);
+  const int64_t target = target_for(n_seqs, H, G, D, block, columns, window, max_length, bits, dtype);
   return target ? plan_bytes(n_seqs) + (n_seqs + target) * H * (D * 4 + 8) : 0;
 }
 
@@ -830,14 +847,15 @@ extern "C" int yh_decode_attention(const void* q, int64_t q_stride, const void* 
   YH_CHECK_ARG(n_seqs < (1ll << 20) && columns < (1ll << 31) && block < (1ll << 31) && H < (1ll << 16) &&
                    blocks < (1ll << 31) && blocks * block < (1ll << 40),
                "decode_attention: sizes too large");
-  const int64_t target = target_for(n_seqs, H, G, block, columns, window, max_length);
+  const int64_t target = target_for(n_seqs, H, G, D, block, columns, window, max_length, bits, dtype);
   int64_t most = columns * block;
   if (window && window < most) most = window;
   if (most > (1ll << 31)) most = 1ll << 31;      // positions are below
   YH_CHECK_ARG(n_seqs * (most / 16 + 2) < (1ll << 31), "decode_attention: sizes too large");
   const int64_t grid = (n_seqs + target) * each;
   YH_CHECK_ARG(grid < (1ll << 24) && n_seqs * H < (1ll << 24), "decode_attention: sizes too large");
-  const int64_t need = yh_decode_attention_workspace_bytes(n_seqs, H, G, D, block, columns, window, max_length);
+  const int64_t need = yh_decode_attention_workspace_bytes(n_seqs, H, G, D, block, columns, window, max_length,
+                                                            bits, dtype);
   YH_CHECK_ARG(need == 0 || (workspace && tree::aligned16(workspace) && workspace_bytes >= need),
                "decode_attention: workspace too small");
   DecodeArgs a{};

@@ -946,11 +946,12 @@ def decode_attention(q, keys, values, block_tables, lengths, *, key_scales=None,
     out = torch.empty((r, h, d), dtype=kind, device=dev)
     longest = -1 if max_length is None else int(max_length)
     # scratch of the call: concurrent calls on different streams are independent
-    need = N.lib().yh_decode_attention_workspace_bytes(r, h, g, d, block, columns, win, longest)
+    code = N.DTYPE_CODE[kind]
+    need = N.lib().yh_decode_attention_workspace_bytes(r, h, g, d, block, columns, win, longest, bits, code)
     ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
     N.call_on(dev, "yh_decode_attention", q.data_ptr(), qs, keys.data_ptr(), values.data_ptr(), N.ptr(key_scales),
               N.ptr(value_scales), tables.data_ptr(), lengths.data_ptr(), N.ptr(starts), N.ptr(slopes), gp, gts, ghs,
-              out.data_ptr(), r, blocks, columns, h, g, d, block, win, longest, scale, cap, bits, N.DTYPE_CODE[kind],
+              out.data_ptr(), r, blocks, columns, h, g, d, block, win, longest, scale, cap, bits, code,
               N.ptr(ws), need)
     return out
 
