@@ -979,8 +979,9 @@ int yh_cache_read(const int64_t* slots, const void* keys, const void* values, co
  * 256, scale > 0, softcap 0 (none) or 1e-30 to 1e30.  max_length: no request has more
  * positions (< 0: unknown), which
  * may save a launch.  workspace: 16-byte aligned, of at least
- * yh_decode_attention_workspace_bytes bytes (0: none, NULL will do); calls that may
- * overlap need one each.
+ * yh_decode_attention_workspace_bytes bytes, asked with the call's own arguments (0:
+ * none, NULL will do); calls that may overlap need one each.  Positions are below
+ * 2^31 - 4096; a request that has more sees nothing.
  */
 int64_t yh_decode_attention_workspace_bytes(int64_t n_seqs, int64_t H, int64_t G, int64_t D, int64_t block,
                                             int64_t columns, int64_t window, int64_t max_length, int bits, int dtype);

@@ -35,13 +35,13 @@
 // LDS.  Parts of a request that was cut leave theirs, with their maximum, in the
 // workspace, and a second launch joins them in order.
 //
-// Bound by HBM: 133 ragged requests over 8 bits 214 us (1.18 GB, 5.5 TB/s), 8 long
-// contexts 193 (6.2), 64 requests over 4 bits 117 (5.4), heads of 256 in 16 bits 154
-// (5.4), where a large copy reaches 6.2 and a read alone 7.0.  Nontemporal loads,
+// Bound by HBM: 133 ragged requests over 8 bits 215 us (1.18 GB, 5.5 TB/s), 8 long
+// contexts 194 (6.1), 64 requests over 4 bits 118 (5.4), heads of 256 in 16 bits 151
+// (5.6), where a large copy reaches 6.2 and a read alone 7.0.  Nontemporal loads,
 // since nothing is read twice but by up to four waves for 64 heads and more: the
 // long contexts 201 us for 217.  Blocks that runs of 16 positions straddle (block %
-// 16) have their table entries and rows a lane: 224 us for the long contexts with
-// blocks of 24, 368 with blocks of 1.
+// 16) have their table entries and rows a lane: 219 us for the long contexts with
+// blocks of 24, 369 with blocks of 1.
 #include <type_traits>
 
 #include "attn_tile.h"
@@ -55,7 +55,6 @@ using namespace qcache;
 using tree::Div;
 using attn::bf16x8_t;
 using attn::f16x8_t;
-using attn::bf16x2_t;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -158,8 +157,8 @@ __device__ __forceinline__ Part part_of(int r, int index, int count, int slot, i
 }
 
 // Part `which` of all, found from the lengths; count 0: there is none.  Every wave finds it by itself where it has a
-// lane for each request (one request: 7.6 us for 9.8 with the workgroup's scan; four
-// requests a lane: 8.3, and nothing gained for 133).
+// lane for each request (one request: 7.6 us for 9.8 with the workgroup's scan; four requests a lane: 8.3, and nothing
+// gained for 133).
 template <int TILE>
 __device__ Part find_part(const DecodeArgs& a, int which) {
   if (a.R <= kWave) {
@@ -190,9 +189,7 @@ __device__ Part find_part(const DecodeArgs& a, int which) {
   __syncthreads();
   const int chunk = chunk_of<TILE>(a, total);
   mine = 0;
-  for (int r = r0; r < r1; ++r) {
-    mine += parts_of(tiles_of<TILE>(seen_of(a, r)), chunk);
-  }
+  for (int r = r0; r < r1; ++r) mine += parts_of(tiles_of<TILE>(seen_of(a, r)), chunk);
   s = scan_wave(mine);
   if ((t & (kWave - 1)) == kWave - 1) sums[w] = s;
   __syncthreads();
@@ -247,12 +244,10 @@ struct Codes<k16> {
   }
 };
 
-// BYTES bytes (1 to 64) into dwords.
+// BYTES bytes (2 to 32) into dwords.
 template <int BYTES>
 __device__ __forceinline__ void load_bytes(uint32_t* w, const char* p) {
-  if constexpr (BYTES == 1) {
-    w[0] = *reinterpret_cast<const uint8_t*>(p);
-  } else if constexpr (BYTES == 2) {
+  if constexpr (BYTES == 2) {
     w[0] = *reinterpret_cast<const uint16_t*>(p);
   } else if constexpr (BYTES == 4) {
     w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
