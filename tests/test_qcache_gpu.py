@@ -713,6 +713,23 @@ def test_odd_arguments(gpu):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1][:, :1].expand(7, 3, 128), b[1])
 
 
+@pytest.mark.parametrize("bits,dtype", FORMS)
+def test_idle_rows_may_hold_anything(gpu, bits, dtype):
+    """Rows of a captured batch that no request has: queries, gates and tables of anything, zeros out; the others as ever."""
+    x, y = (rnd(40, 2, 16, 64, seed=s, dtype=dtype) for s in (1, 2))
+    c = [None if t is None else t.to(gpu) for t in (cache_of(x, y, bits) if bits < 16 else (x, y, None, None))]
+    q, gate = rnd(4, 8, 64, seed=3, dtype=dtype).to(gpu), rnd(4, 8, 64, seed=4, dtype=dtype).to(gpu)
+    tables, lens = torch.arange(160, dtype=torch.int32, device=gpu).view(4, 40) % 40, torch.tensor([600, 0, 30, 0], device=gpu)
+    starts = torch.tensor([0, 0, 30, 5], device=gpu)
+    call = lambda: layers.decode_attention(q, c[0], c[1], tables, lens, key_scales=c[2], value_scales=c[3], starts=starts, gate=gate)  # noqa: E731
+    clean = call()
+    q[1:] = NAN
+    gate[1:] = torch.tensor([NAN, INF, -INF], device=gpu, dtype=dtype).view(3, 1, 1)
+    tables[1:] = 1 << 30
+    got = call()
+    assert torch.equal(got[0], clean[0]) and not got[1:].any() and not clean[1:].any() and torch.isfinite(got).all()
+
+
 def test_other_cuda_streams_own_scratch(gpu):
     """Inputs made on one stream, used on another that waits for it; scratch is the using stream's."""
     side = torch.cuda.Stream()

@@ -308,6 +308,23 @@ __device__ __forceinline__ void settle(f32x4 (&x)[N]) {
   for (int i = 1; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 
+// Four dims of a head's output: o / den, gated.  Where nothing was seen they are zeros, whatever the gate of an idle row
+// holds.
+template <int DT>
+__device__ __forceinline__ void put4(const DecodeArgs& a, int r, int head, int dim, int D, const float* o, float den) {
+  using M = attn::Mfma<DT>;
+  const float inv = 1.f / den;
+  uint16_t y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float z = o[e] * inv;
+    if (a.gate) z *= 1.f / (1.f + __expf(-M::widen(a.gate[r * a.g_ts + head * a.g_hs + dim + e])));
+    y[e] = den == 0.f ? 0 : M::round(z);
+  }
+  const int64_t to = (static_cast<int64_t>(r) * a.H + head) * D + dim;
+  *reinterpret_cast<u32x2*>(a.out + to) = u32x2{attn::pack2(y[0], y[1]), attn::pack2(y[2], y[3])};
+}
+
 // Waves a SIMD that the registers are held to, where none spills for it.
 constexpr int waves_for(int DT, int FMT, int D, int HP, bool RUNS) {
   return D == 64 ? 3 : D == 256 || (FMT != k16 && (HP == 16 || !RUNS || (FMT == kFp8 && DT == YH_F16))) ? 2 : 3;
@@ -316,7 +333,6 @@ constexpr int waves_for(int DT, int FMT, int D, int HP, bool RUNS) {
 template <int DT, int FMT, int D, int HP, bool RUNS>
 __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) decode_attention_kernel(DecodeArgs a) {
   using C = Codes<FMT>;
-  using M = attn::Mfma<DT>;
   constexpr int MT = FMT == k16 ? DT : YH_BF16;
   using P = attn::Mfma<MT>;
   constexpr bool kPair = FMT != k16 && DT == YH_F16;    // queries and weights as hi + lo
@@ -672,16 +688,7 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
       *reinterpret_cast<float4*>(a.part + slot * D + dim) = make_float4(o[0], o[1], o[2], o[3]);
       if (dim == 0) a.stat[slot] = make_float2(m, dn);
     } else {
-      const float inv = dn > 0.f || dn != dn ? 1.f / dn : 0.f;     // nothing seen: zeros
-      const int64_t to = (static_cast<int64_t>(r) * a.H + hd) * D + dim;
-      uint16_t y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float z = o[e] * inv;
-        if (a.gate) z *= 1.f / (1.f + __expf(-M::widen(a.gate[r * a.g_ts + hd * a.g_hs + dim + e])));
-        y[e] = M::round(z);
-      }
-      *reinterpret_cast<u32x2*>(a.out + to) = u32x2{attn::pack2(y[0], y[1]), attn::pack2(y[2], y[3])};
+      put4<DT>(a, r, hd, dim, D, o, dn);
     }
   }
 }
@@ -690,7 +697,6 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
 // their sums meet in LDS, in order.
 template <int DT, int D>
 __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
-  using M = attn::Mfma<DT>;
   constexpr int kLanes = D / 4, kShares = kThreads / kLanes;
   __shared__ float sums[kShares][D + 4], dens[kShares], tops[kShares];
   const int r = blockIdx.x / a.H, hd = blockIdx.x % a.H;
@@ -732,16 +738,7 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(sums[i][dim + e], f, o[e]);
   }
-  const float inv = dn > 0.f || dn != dn ? 1.f / dn : 0.f;
-  const int64_t to = (static_cast<int64_t>(r) * a.H + hd) * D + dim;
-  uint16_t y[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float z = o[e] * inv;
-    if (a.gate) z *= 1.f / (1.f + __expf(-M::widen(a.gate[r * a.g_ts + hd * a.g_hs + dim + e])));
-    y[e] = M::round(z);
-  }
-  *reinterpret_cast<u32x2*>(a.out + to) = u32x2{attn::pack2(y[0], y[1]), attn::pack2(y[2], y[3])};
+  put4<DT>(a, r, hd, dim, D, o, dn);
 }
 
 // Parts aimed at, over all heads, so that the last of those that fit the chip (two or three workgroups a CU) end at
