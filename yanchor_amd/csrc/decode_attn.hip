@@ -767,7 +767,7 @@ int64_t plan_bytes(int64_t R) { return ((R + 1) * 4 + 255) / 256 * 256; }
 
 template <int DT, int FMT, int D, int HP>
 void launch_heads(const DecodeArgs& a, bool runs, unsigned grid, hipStream_t st) {
-  // blocks that runs of 16 positions straddle: four columns or sixteen are enough kernels for a form off the main path
+  // for blocks that runs of 16 positions straddle, a form off the main path, four heads or sixteen are kernels enough
   constexpr int kOdd = HP == 4 ? 4 : 16;
   if (runs) hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, HP, true>), dim3(grid), dim3(kThreads), 0, st, a);
   else hipLaunchKernelGGL((decode_attention_kernel<DT, FMT, D, kOdd, false>), dim3(grid), dim3(kThreads), 0, st, a);

@@ -9,8 +9,8 @@
 //
 // Bound by HBM and, where slots are scattered, by its granules: 65521 tokens of 8
 // heads of 128 into scattered rows of 4 bits 92 us for 340 MB, of which the scale
-// bytes, each in a granule of its own, take 23 and the 64-byte rows 14 (the input
-// alone streams in 43); back 79; 146000 tokens in order of 8 bits back 177 us, 5.1
+// bytes, each in a granule of its own, take 23 and the 64-byte rows 14 (the input is
+// 43 at a copy's rate); back 79; 154000 tokens in order of 8 bits back 177 us, 5.4
 // TB/s.  Rows in and out pass the caches (101 and 91 us through them); codes of 4 bits
 // do not, as two rows share a granule (79 us for 91).
 #include "qcache.h"
