@@ -959,7 +959,7 @@ int yh_cache_write_quantized(const void* k, int64_t k_stride, const void* v, int
 /*
  * Rows of a cache (4, 8 or 16 bits) back: k, v [N, G, D] dense in dtype (bf16 or
  * f16; that of a 16-bit cache) from slots[n]; a slot outside the cache gives zeros,
- * a value past f16's range infinity.  D % 32 == 0 (16 bits: D % 8 == 0).
+ * a value past dtype's range infinity.  D % 32 == 0 (16 bits: D % 8 == 0).
  */
 int yh_cache_read(const int64_t* slots, const void* keys, const void* values, const uint8_t* key_scales,
                   const uint8_t* value_scales, void* k, void* v, int64_t N, int64_t blocks, int64_t G, int64_t D,

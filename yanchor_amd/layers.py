@@ -855,7 +855,8 @@ def cache_read(slots, keys, values, key_scales=None, value_scales=None, *, dtype
     ``dtype`` (bf16 / fp16; default bf16, or that of a 16-bit cache), from slots
     int [N] as ``slot_map`` gives them (``slot_map(cu_seqlens, zeros, ...)`` those
     of whole prefixes): what a prefill that continues a request reads.  A slot
-    outside the cache gives zeros."""
+    outside the cache gives zeros; a value whose code rounds past the dtype's range
+    (65504 in 8 bits reads as 65536) infinity."""
     if keys.ndim != 4:
         raise ValueError("keys and values must be contiguous [blocks, G, block, D] of one type")
     kind = keys.dtype
