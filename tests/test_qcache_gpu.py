@@ -744,3 +744,118 @@ def test_other_cuda_streams_own_scratch(gpu):
     torch.cuda.current_stream().wait_stream(side)
     noise = [torch.full((1 << 20,), NAN, device=gpu) for _ in range(4)]
     assert torch.equal(got, want) and rows[0].shape == (40, 1, 128) and len(noise) == 4
+
+
+# --- what is not finite, in each value ------------------------------------------------
+
+def same_or_within(got, want, bound, what=""):
+    """As ``within`` where want is finite; elsewhere the same infinity, or NaN for NaN."""
+    least = torch.finfo(got.dtype).smallest_normal * half_step(got.dtype) + 1e-30
+    got, fine = got.detach().double().cpu(), want.isfinite()
+    assert torch.equal(got[~fine].nan_to_num(7.0), want[~fine].nan_to_num(7.0)), (what, got[~fine], want[~fine])
+    got[~fine] = 0
+    zero = torch.zeros_like(want)
+    bad = ~((got - torch.where(fine, want, zero)).abs() <= torch.where(fine, bound, zero) + least)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, first at {bad.nonzero()[0].tolist()}"
+
+
+def spoiled_case(dev, cache, lengths, h, dtype, d, block, seed, mark=None, **kw):
+    """The case's output against the oracle over the cache as its product takes it (codes past bf16's range: infinities)."""
+    r, blocks = len(lengths), cache[0].shape[0]
+    columns = blocks // r
+    tables = torch.randperm(blocks, generator=torch.Generator().manual_seed(seed))[:r * columns].to(torch.int32).view(r, columns)
+    cache = [None if t is None else t.clone() for t in cache]
+    mark(cache, lambda i, p: (int(tables[i, p // block]), p % block))
+    q = rnd(r, h, d, seed=seed + 3, dtype=dtype)
+    full = [ref.cache_values(cache[i], cache[2 + i]) for i in range(2)]
+    full = [t.to(B).double() if cache[2] is not None else t for t in full]
+    on = [None if t is None else t.to(dev) for t in cache]
+    got = layers.decode_attention(q.to(dev), on[0], on[1], tables.to(dev), torch.tensor(lengths, device=dev),
+                                  key_scales=on[2], value_scales=on[3], **kw)
+    want, _ = ref.attention(q, *full, tables, lengths, **kw)
+    full[1] = full[1].nan_to_num(0.0, 0.0, 0.0)
+    _, size = ref.attention(q, *full, tables, lengths, **kw)
+    p_step = 2.0 ** -16 if dtype == H16 and cache[2] is not None else half_step(dtype)
+    same_or_within(got, want, half_step(dtype) * want.abs() + (p_step + 2.0 ** -12) * size, (dtype, d, h, block))
+    return got.cpu(), want
+
+
+@pytest.mark.parametrize("dtype", [B, H16])
+@pytest.mark.parametrize("d,h,block", [(64, 3, 16), (128, 4, 16), (128, 7, 16), (256, 4, 16), (128, 16, 16), (128, 20, 16),
+                                       (256, 16, 24), (128, 4, 24), (64, 2, 1)])
+def test_attention_nan_codes_stay_in_their_dim(gpu, dtype, d, h, block):
+    """An e4m3 NaN in one value's dim is that dim's only, whatever lies beside it in a dword or a tile."""
+    columns = -(-2100 // block)
+    x, y = (rnd(3 * columns, 1, block, d, seed=s) for s in (1, 2))
+    c = cache_of(x, y, 8)
+
+    def mark(cache, at):
+        for i, p, dim in ((0, 9, 3), (0, 30, 6), (1, 2000, d - 1), (1, 0, 8)):
+            b, row = at(i, p)
+            cache[1].view(torch.uint8)[b, 0, row, dim] = 0xff if dim == 3 else 0x7f
+    got, _ = spoiled_case(gpu, c, [100, 2050, 700], h, dtype, d, block, 5, mark)
+    assert got[0].isnan().sum() == 2 * h and got[1].isnan().sum() == 2 * h and got[2].isfinite().all()
+
+
+@pytest.mark.parametrize("bits,huge", [(4, 3.0e38), (8, 3.31e38)])
+@pytest.mark.parametrize("d,h,block", [(128, 4, 16), (64, 8, 16), (128, 16, 16), (256, 4, 24)])
+def test_attention_values_that_round_past_bf16(gpu, bits, huge, d, h, block):
+    """Rows whose largest value becomes 2^128: an infinity for its dim, and finite values beside it in the run."""
+    columns = -(-200 // block)
+    k, v = (rnd(200, 1, d, seed=s) for s in (1, 2))
+    v[50, 0, 34], v[50, 0, 35], v[50, 0, 36] = huge, 9.0e37, -9.0e37
+    v[70, 0, 9], v[70, 0, 8] = -huge, 9.0e37
+    cache = layers.quantized_cache(2 * columns, 1, block, d, bits=bits, device=gpu)
+    tables = torch.randperm(2 * columns, generator=torch.Generator().manual_seed(3)).to(torch.int32).view(2, columns)
+    slots = torch.tensor([int(tables[0, p // block]) * block + p % block for p in range(200)])
+    layers.cache_write_quantized(k.to(gpu), v.to(gpu), slots.to(gpu), *cache)
+    val, s = ref.quantise(v, bits)
+    assert s.max() == (253 if bits == 4 else 247) and val.max() == 2.0 ** 128
+    q = rnd(2, h, d, seed=4)
+    got = layers.decode_attention(q.to(gpu), cache[0], cache[1], tables.to(gpu), torch.tensor([200, 0], device=gpu),
+                                  key_scales=cache[2], value_scales=cache[3])
+    keys, values = (ref.quantise(t, bits)[0].transpose(0, 1)[None] for t in (k, v))
+    values = values.to(B).double()
+    one = torch.zeros(1, 1, dtype=torch.int32)
+    want, _ = ref.attention(q[:1], keys, values, one, [200])
+    _, size = ref.attention(q[:1], keys, values.nan_to_num(0.0, 0.0, 0.0), one, [200])
+    assert want.isinf().sum() == 2 * h
+    same_or_within(got[:1], want, half_step(B) * want.abs() + (half_step(B) + 2.0 ** -12) * size)
+    assert not got[1].any()
+
+
+@pytest.mark.parametrize("dtype", [B, H16])
+@pytest.mark.parametrize("d,h,block", [(128, 4, 16), (64, 8, 16), (128, 7, 48), (256, 5, 16), (128, 16, 16), (64, 20, 16),
+                                       (256, 3, 24), (128, 2, 1)])
+def test_attention_infinite_values_are_infinite(gpu, dtype, d, h, block):
+    """16-bit caches: an infinity gives an infinity, both signs NaN, in their dims alone, wherever they lie in a tile."""
+    columns = -(-2100 // block)
+    x, y = (rnd(3 * columns, 1, block, d, seed=s, dtype=dtype) for s in (1, 2))
+
+    def mark(cache, at):
+        for i, p, dim, z in ((0, 9, 3, INF), (0, 10, 5, -INF), (0, 20, 7, INF), (0, 22, 7, -INF), (0, 31, 9, NAN),
+                             (0, 99, 10, INF), (1, 2049, 0, -INF), (1, 1, 1, INF), (1, 1000, 1, -INF)):
+            b, row = at(i, p)
+            cache[1][b, 0, row, dim] = z
+    _, want = spoiled_case(gpu, [x, y, None, None], [100, 2050, 700], h, dtype, d, block, 5, mark)
+    assert want[0].isinf().sum() == 3 * h and want[0].isnan().sum() == 2 * h and want[2].isfinite().all()
+    _, want = spoiled_case(gpu, [x, y, None, None], [100, 2050, 700], h, dtype, d, block, 6, mark, window=60, softcap=9.0)
+    assert want[0].isinf().sum() == h
+
+
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("n", [300, 6000])
+def test_attention_infinite_values_of_far_lower_scores(gpu, first, n):
+    """An infinity whose weight float32 holds as zero beside the largest is still one, within a part and between parts."""
+    d, h = 128, 4
+    x, y = torch.zeros(n // 16 + 1, 1, 16, d, dtype=B), rnd(n // 16 + 1, 1, 16, d, seed=2)
+    high, low = (n - 7, 3) if first else (3, n - 7)
+    x[high // 16, 0, high % 16] = 5.0            # a score of 128 5 / sqrt(128) 4 = 226 over the others' zero
+    y[low // 16, 0, low % 16, 17], y[low // 16, 0, low % 16, 18] = INF, -INF
+    tables = torch.arange(n // 16 + 1, dtype=torch.int32)[None]
+    q = torch.full((1, h, d), 4.0, dtype=B)
+    got = layers.decode_attention(q.to(gpu), x.to(gpu), y.to(gpu), tables.to(gpu), torch.tensor([n], device=gpu))
+    want, _ = ref.attention(q, x.double(), y.double(), tables, [n])
+    _, size = ref.attention(q, x.double(), y.double().nan_to_num(0.0, 0.0, 0.0), tables, [n])
+    assert want.isinf().sum() == 2 * h
+    same_or_within(got, want, half_step(B) * want.abs() + (half_step(B) + 2.0 ** -12) * size)

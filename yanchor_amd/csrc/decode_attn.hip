@@ -23,9 +23,11 @@
 // With HP = 4 the other eight columns take half of the positions, each lane half of
 // the exponentials; their sums join at the end.  (Pairs transposed by v_perm, as many
 // as there are conversions, and all exponentials in every column: 156 us for 135 with
-// 64 requests over 4 bits.)  In 16 bits, where a pair's other dim may hold an
-// infinity that zero would not hide, the pairs are transposed: there are no
-// conversions beside it.
+// 64 requests over 4 bits.)  In 16 bits, where there are no conversions beside it, the
+// pairs are transposed.
+// A weight of zero does not take out a value that is not finite (NaN codes, 16-bit
+// infinities, codes of 2^128 and more, which bf16 holds as infinities), so a part's
+// sums that are not finite are formed again by dims.
 // With fp16 queries over codes, whose 11 bits bf16 does not hold, queries and
 // weights enter as two bf16 each (hi + lo).
 //
@@ -99,6 +101,34 @@ struct DecodeArgs {
 
 // Tables through the scalar cache: a run of 16 positions lies in one block.
 typedef __attribute__((address_space(4))) int32_t ConstInt;
+
+// The table's entry for position p of request r.
+__device__ __forceinline__ int table_entry(const DecodeArgs& a, int r, int p) {
+  const uint32_t b = a.block.quot(p);
+  return ((const ConstInt*)(a.tables + static_cast<int64_t>(r) * a.columns.d))[b - a.columns.quot(b) * a.columns.d];
+}
+__device__ __forceinline__ bool block_there(const DecodeArgs& a, int id) {
+  return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.blocks);
+}
+// The row of all rows of all heads, and where its scale of run 0 lies.  An entry that is no block of the cache leads
+// to block 0, whose contents are masked.
+struct Row {
+  int64_t row, scale;
+};
+template <int D>
+__device__ __forceinline__ Row row_at(const DecodeArgs& a, int g, int id, int p) {
+  const uint32_t in = p - a.block.quot(p) * a.block.d;
+  const int64_t first = (static_cast<int64_t>(block_there(a, id) ? id : 0) * a.G + g) * a.block.d;
+  return {first + in, first * (D / kRun) + in};
+}
+
+// The kernel's arguments, loaded where this stands: kept over a loop before it they would take the loop's scalar registers.
+__device__ __forceinline__ const DecodeArgs& arguments_again() {
+  typedef __attribute__((address_space(4))) DecodeArgs Const;
+  Const* p = (Const*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const DecodeArgs*)p;
+}
 
 // First and last + 1 of the positions that request r sees.
 struct Seen {
@@ -265,6 +295,23 @@ __device__ __forceinline__ void load_bytes(uint32_t* w, const char* p) {
   }
 }
 
+// Value `dim` of the row at `row` of all rows, its scale of run 0 at `scale`, runs `run` apart.
+template <int DT, int FMT, int D>
+__device__ __forceinline__ float value_of(const char* data, const uint8_t* scales, int64_t row, int64_t scale, uint32_t run,
+                                          int dim) {
+  if constexpr (FMT == k16) {
+    return attn::Mfma<DT>::widen(reinterpret_cast<const uint16_t*>(data)[row * D + dim]);
+  } else {
+    const float s = scale_value(scales[scale + static_cast<int64_t>(dim / kRun) * run]);
+    if constexpr (FMT == kFp8) {
+      return __builtin_amdgcn_cvt_f32_fp8(static_cast<uint8_t>(data[row * D + dim]), 0) * s;
+    } else {
+      const auto two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(static_cast<uint8_t>(data[(row * D + dim) / 2]), 1.f, 0);
+      return (dim & 1 ? two[1] : two[0]) * s;
+    }
+  }
+}
+
 template <int I, int N, class F>
 __device__ __forceinline__ void each(F f) {
   if constexpr (I < N) {
@@ -350,6 +397,10 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
   constexpr int kAcc = kVd / kSel, kMine = kU / kHalves;             // positions whose weights a lane forms
   __shared__ float2 wave_stat[kWaves][kHalves][HP];
   __shared__ float wave_acc[kWaves][kHalves][HP][D + 4];
+  // columns whose sums are not finite, and what forms them again
+  __shared__ uint32_t spoiled;
+  __shared__ float redo_weight[kThreads], redo_sum[kThreads / (D / 4)][D];
+  __shared__ int redo_id[kThreads];
 
   const int g = blockIdx.x % a.G, mt = blockIdx.x / a.G % a.mtiles;
   const Part part = find_part<kTile>(a, blockIdx.x / a.G / a.mtiles);
@@ -401,22 +452,9 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
 #pragma unroll
   for (int n = 0; n < kAcc; ++n) acc[n] = f32x4{0, 0, 0, 0};
 
-  const ConstInt* table = (const ConstInt*)(a.tables + static_cast<int64_t>(r) * a.columns.d);
-  auto id_of = [&](int p) {      // the table's entry for position p
-    const uint32_t b = a.block.quot(p);
-    return table[b - a.columns.quot(b) * a.columns.d];
-  };
-  // The row of all rows of all heads, and where its scale of run 0 lies.  An entry that is no block of the cache leads
-  // to block 0, whose contents are masked.
-  struct Row {
-    int64_t row, scale;
-  };
-  auto is_block = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.blocks); };
-  auto row_of = [&](int id, int p) -> Row {
-    const uint32_t in = p - a.block.quot(p) * a.block.d;
-    const int64_t first = (static_cast<int64_t>(is_block(id) ? id : 0) * a.G + g) * a.block.d;
-    return {first + in, first * (D / kRun) + in};
-  };
+  auto id_of = [&](int p) { return table_entry(a, r, p); };
+  auto is_block = [&](int id) { return block_there(a, id); };
+  auto row_of = [&](int id, int p) { return row_at<D>(a, g, id, p); };
   const int first_tile = lo / kTile + __builtin_amdgcn_readfirstlane(part.tile);
 
   // The lane's positions of product t, of 16 t on: `piece` of K, 4 quarter + j of V.
@@ -657,6 +695,8 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
   }
   settle(acc);
 
+  const DecodeArgs& b = arguments_again();
+
   // the waves' sums: lane (column, quarter) has dims (4 quarter + j) kVd + 2 n + sel, or + n, of its head in acc[n][j]
   den += __shfl_xor(den, 16, kWave);
   den += __shfl_xor(den, 32, kWave);
@@ -667,13 +707,16 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
 #pragma unroll
       for (int n = 0; n < kAcc; ++n) wave_acc[w][half][col][(4 * quarter + j) * kVd + kSel * n + sel] = acc[n][j];
   }
+  if (threadIdx.x == 0) spoiled = 0;
   __syncthreads();
-  for (int at = threadIdx.x; at < cols * (D / 4); at += kThreads) {
-    const int c = at / (D / 4), dim = at % (D / 4) * 4;
-    float m = kFloor;
+  // Four dims of a column: the largest score, the denominator and the sums of all waves.
+  auto join = [&](int c, int dim, float& m, float& dn, float* o) {
+    m = kFloor;
 #pragma unroll
     for (int i = 0; i < kWaves * kHalves; ++i) m = fmaxf(m, wave_stat[i / kHalves][i % kHalves][c].x);
-    float dn = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    dn = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < kWaves * kHalves; ++i) {
       const float2 st = wave_stat[i / kHalves][i % kHalves][c];
@@ -682,16 +725,89 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(wave_acc[i / kHalves][i % kHalves][c][dim + e], f, o[e]);
     }
-    const int hd = g * a.rep + mt * kCols + c;
+  };
+  auto put = [&](int c, int dim, float m, float dn, const float* o) {
+    const int hd = g * b.rep + mt * kCols + c;
     if (part.count > 1) {
-      const int64_t slot = static_cast<int64_t>(part.slot) * a.H + hd;
-      *reinterpret_cast<float4*>(a.part + slot * D + dim) = make_float4(o[0], o[1], o[2], o[3]);
-      if (dim == 0) a.stat[slot] = make_float2(m, dn);
+      const int64_t slot = static_cast<int64_t>(part.slot) * b.H + hd;
+      *reinterpret_cast<float4*>(b.part + slot * D + dim) = make_float4(o[0], o[1], o[2], o[3]);
+      if (dim == 0) b.stat[slot] = make_float2(m, dn);
     } else {
-      put4<DT>(a, r, hd, dim, D, o, dn);
+      put4<DT>(b, r, hd, dim, D, o, dn);
+    }
+  };
+  // Where the denominator is no number, no dim is one; elsewhere a sum that is none says nothing of its own dim.
+  auto finite = [](float dn, const float* o) {
+    return dn != dn || fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < INFINITY;
+  };
+  for (int at = threadIdx.x; at < cols * (D / 4); at += kThreads) {
+    const int c = at / (D / 4), dim = at % (D / 4) * 4;
+    float m, dn, o[4];
+    join(c, dim, m, dn, o);
+    if (finite(dn, o)) put(c, dim, m, dn, o);
+    else atomicOr(&spoiled, 1u << c);
+  }
+  __syncthreads();
+  // Values that are not finite reach, through weights of 0, the other dim of their dword and the other half of the
+  // positions.  Sums that are not finite are formed again without such products, for the columns that have any: a lane
+  // a position for the weights, four dims a lane for the sums.
+#pragma unroll 1
+  for (uint32_t left = spoiled; left; left &= left - 1) {
+    constexpr int kLanes = D / 4, kShares = kThreads / kLanes;
+    const int c = __builtin_ctz(left), share = threadIdx.x / kLanes, dim = threadIdx.x % kLanes * 4;
+    const int hd = g * b.rep + mt * kCols + c;
+    const uint16_t* qr = b.q + r * b.q_ts + static_cast<int64_t>(hd) * D;
+    const float steep = b.slopes ? b.slopes[hd] * kLog2e : 0.f;
+    const int end = (first_tile + tiles) * kTile < hi ? (first_tile + tiles) * kTile : hi;
+    float m, dn, o[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+    join(c, dim, m, dn, o);
+#pragma unroll 1
+    for (int p0 = first_tile * kTile < lo ? lo : first_tile * kTile; p0 < end; p0 += kThreads) {
+      const int p = p0 + static_cast<int>(threadIdx.x);
+      const int id = p < end ? table_entry(b, r, p) : -1;
+      float wt = -1.f;
+      if (block_there(b, id)) {
+        const Row at = row_at<D>(b, g, id, p);
+        float x = 0.f;
+#pragma unroll 8
+        for (int d = 0; d < D; ++d)
+          x = fmaf(attn::Mfma<DT>::widen(qr[d]), value_of<DT, FMT, D>(b.keys, b.key_scales, at.row, at.scale, b.block.d, d), x);
+        x = b.cap > 0.f ? b.cap * kLog2e * tanh_of(x * (b.scale / b.cap)) : x * (kLog2e * b.scale);
+        if (b.slopes) x -= steep * static_cast<float>((steep < 0.f ? lo : hi - 1) - p);
+        wt = __builtin_amdgcn_exp2f(x + (MT == YH_F16 ? kLift - m : -m));
+      }
+      __syncthreads();      // the positions before are summed
+      redo_weight[threadIdx.x] = wt;
+      redo_id[threadIdx.x] = id;
+      __syncthreads();
+      for (int j = share; j < kThreads && p0 + j < end; j += kShares) {
+        const float wj = redo_weight[j];
+        if (wj < 0.f) continue;
+        const Row at = row_at<D>(b, g, redo_id[j], p0 + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = value_of<DT, FMT, D>(b.values, b.value_scales, at.row, at.scale, b.block.d, dim + e);
+          sum[e] = fabsf(v) < INFINITY ? fmaf(wj, v, sum[e]) : sum[e] + v;      // however small the weight
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) redo_sum[share][dim + e] = sum[e];
+    __syncthreads();
+    if (share == 0 && !finite(dn, o)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (fabsf(o[e]) < INFINITY) continue;
+        o[e] = 0.f;
+        for (int i = 0; i < kShares; ++i) o[e] += redo_sum[i][dim + e];
+      }
+      put(c, dim, m, dn, o);
     }
   }
 }
+
+// A sum at a factor of at most 1: an infinite one stays, where float32 holds the factor as 0.
+__device__ __forceinline__ float scaled(float x, float f) { return fabsf(x) == INFINITY ? x : x * f; }
 
 // The parts of a cut request joined: a workgroup a head, D / 4 lanes a part, the others take every kShares-th part;
 // their sums meet in LDS, in order.
@@ -713,10 +829,10 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
     const float next = fmaxf(m, st.x), f = __builtin_amdgcn_exp2f(m - next), h = __builtin_amdgcn_exp2f(st.x - next);
     m = next;
     dn = fmaf(dn, f, st.y * h);
-    o[0] = fmaf(o[0], f, x.x * h);
-    o[1] = fmaf(o[1], f, x.y * h);
-    o[2] = fmaf(o[2], f, x.z * h);
-    o[3] = fmaf(o[3], f, x.w * h);
+    o[0] = scaled(o[0], f) + scaled(x.x, h);
+    o[1] = scaled(o[1], f) + scaled(x.y, h);
+    o[2] = scaled(o[2], f) + scaled(x.z, h);
+    o[3] = scaled(o[3], f) + scaled(x.w, h);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) sums[share][dim + e] = o[e];
@@ -736,7 +852,7 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
     const float f = __builtin_amdgcn_exp2f(tops[i] - m);
     dn = fmaf(dens[i], f, dn);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(sums[i][dim + e], f, o[e]);
+    for (int e = 0; e < 4; ++e) o[e] += scaled(sums[i][dim + e], f);
   }
   put4<DT>(a, r, hd, dim, D, o, dn);
 }
