@@ -4,10 +4,10 @@ Tolerances, from the roundings that each kernel makes (e = half a step of a type
 torch.finfo(t).eps / 2):
 * quantised rows are exact: the scales are powers of two and the codes are
   rounded from exact quotients.
-* attention: the output is rounded once (e |o|).  Weights enter the value
-  product once rounded to the type of the product, e sum p |v|: bf16 for bf16
-  queries, fp16 for a 16-bit fp16 cache, and a pair of bf16 (2^-16) for fp16
-  queries over codes.  Scores, exponentials and sums are float32: the error of a
+* attention: the output is rounded once (e |o|).  Weights that enter the value
+  product rounded once to its type are off by e sum p |v|, as a pair by 2^-16: the
+  kernel takes pairs, most bounds here allow the one rounding (bf16 for bf16
+  queries, fp16 for a 16-bit fp16 cache), and the tests of equal weights do not.  Scores, exponentials and sums are float32: the error of a
   score (256 terms, 2^-24 each, of scores up to some tens, a capped one 2^-22 of
   its cap, a bias 2^-24 of its size) leaves 2^-12 sum p |v|.
 * norms and rotations: the output once (e |o|); the norm (2^-22), the angle
@@ -859,3 +859,29 @@ def test_attention_infinite_values_of_far_lower_scores(gpu, first, n):
     _, size = ref.attention(q, x.double(), y.double().nan_to_num(0.0, 0.0, 0.0), tables, [n])
     assert want.isinf().sum() == 2 * h
     same_or_within(got, want, half_step(B) * want.abs() + (half_step(B) + 2.0 ** -12) * size)
+
+
+@pytest.mark.parametrize("score,scale", [(2, 1), (13, 1024)])
+@pytest.mark.parametrize("bits,dtype", FORMS)
+def test_attention_of_equal_weights_beside_larger_ones(gpu, bits, dtype, score, scale):
+    """Every 16th key has a score of 2 (13; 12 in 4 bits) and a value of 0, the others' weights are e^-2 (e^-13) of its,
+    which a 16-bit type would round all the same way: by 2^-8.4 in bf16, 2^-11.7 in fp16 (2^-8.9, 2^-11.3).  The output
+    is within half a step of its own binade and 2^-14 of sum p |v|: weights of two parts 2^-16, scores (exact, times
+    log2(e) / 8 and less the largest: 2^-24 of 19 each) 2^-19, sums of at most 64 positions a lane and 100 parts 2^-17
+    in numerator and denominator."""
+    d, h, lengths = 64, 4, [18, 23, 29, 47, 64, 101, 333, 5000]
+    blocks = 5008 // 16
+    x, y = torch.zeros(blocks, 1, 16, d, dtype=dtype), torch.ones(blocks, 1, 16, d, dtype=dtype)
+    x[:, 0, 3] = score / 8
+    y[:] = (1 + torch.arange(d) / 64) * scale
+    y[:, 0, 3] = 0
+    cache = list(cache_of(x, y, bits)) if bits < 16 else [x, y, None, None]
+    full = [ref.cache_values(cache[i], cache[2 + i]) for i in range(2)]
+    tables = torch.arange(blocks, dtype=torch.int32).repeat(len(lengths), 1)
+    q = torch.ones(len(lengths), h, d, dtype=dtype)
+    on = [None if t is None else t.to(gpu) for t in cache]
+    got = layers.decode_attention(q.to(gpu), on[0], on[1], tables.to(gpu), torch.tensor(lengths, device=gpu),
+                                  key_scales=on[2], value_scales=on[3])
+    want, size = ref.attention(q, *full, tables, lengths)
+    step = torch.exp2(torch.floor(torch.log2(want * (1 + 2.0 ** -14)))) * half_step(dtype)
+    within(got, want, step + 2.0 ** -14 * size, (bits, dtype))

@@ -28,8 +28,10 @@
 // A weight of zero does not take out a value that is not finite (NaN codes, 16-bit
 // infinities, codes of 2^128 and more, which bf16 holds as infinities), so a part's
 // sums that are not finite are formed again by dims.
-// With fp16 queries over codes, whose 11 bits bf16 does not hold, queries and
-// weights enter as two bf16 each (hi + lo).
+// Weights enter as two values of the product's type each (hi + lo, 16 bits at
+// least), since the denominator sums them as they are: rounded once, equal weights
+// would all be off the same way.  With fp16 queries over codes, whose 11 bits bf16
+// does not hold, the queries do too.
 //
 // Requests are few or of very different lengths, so tiles of 16 NT positions are
 // cut into parts of about one size, which every workgroup finds from the lengths
@@ -73,7 +75,8 @@ constexpr int kThreads = kWaves * kWave;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kFloor = -3.0e38f;   // below every score: the maximum of nothing
 // fp16 weights are e^(x - max) 2^14, up to a quarter of the type's range: weights below 2^-14 of the largest, of which
-// a long cache may have very many, then keep their 11 bits down to 2^-28.  The denominator carries the same factor.
+// a long cache may have very many, then keep 22 bits down to 2^-17 and 11 down to 2^-28.  The denominator carries the
+// same factor.
 constexpr float kLift = 14.f;
 
 struct DecodeArgs {
@@ -345,6 +348,13 @@ __device__ __forceinline__ f32x4 mfma(u32x2 a, u32x2 b, f32x4 c) {
   else
     return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
 }
+// Two weights as hi + lo, each rounded to the product's type.
+template <int MT>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  using P = attn::Mfma<MT>;
+  hi = P::round2(x, y);
+  lo = P::round2(x - P::widen(hi & 0xffff), y - P::widen(hi >> 16));
+}
 // The compiler puts no wait where a matrix result is first read behind branches that meet.
 template <int N>
 __device__ __forceinline__ void settle(f32x4 (&x)[N]) {
@@ -372,9 +382,13 @@ __device__ __forceinline__ void put4(const DecodeArgs& a, int r, int head, int d
   *reinterpret_cast<u32x2*>(a.out + to) = u32x2{attn::pack2(y[0], y[1]), attn::pack2(y[2], y[3])};
 }
 
-// Waves a SIMD that the registers are held to, where none spills for it.
+// Waves a SIMD that the registers are held to: as many as fit without spilling, but
+// for fp16 queries over 8 bits with sixteen columns of heads of 256, which spill up to 9 registers (us of the long contexts
+// with 128 heads, blocks of 64 and 24: 462 and 549, with one wave a SIMD 524 and 582).
 constexpr int waves_for(int DT, int FMT, int D, int HP, bool RUNS) {
-  return D == 64 ? 3 : D == 256 || (FMT != k16 && (HP == 16 || !RUNS || (FMT == kFp8 && DT == YH_F16))) ? 2 : 3;
+  if (D == 64) return 3;
+  if (D == 128 && FMT == kFp4 && DT == YH_BF16 && HP == 4 && RUNS) return 4;
+  return D == 256 || (FMT != k16 && (HP == 16 || !RUNS || (FMT == kFp8 && DT == YH_F16))) ? 2 : 3;
 }
 
 template <int DT, int FMT, int D, int HP, bool RUNS>
@@ -382,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
   using C = Codes<FMT>;
   constexpr int MT = FMT == k16 ? DT : YH_BF16;
   using P = attn::Mfma<MT>;
-  constexpr bool kPair = FMT != k16 && DT == YH_F16;    // queries and weights as hi + lo
+  constexpr bool kPair = FMT != k16 && DT == YH_F16;    // queries as hi + lo
   constexpr int kRow = D * C::kBits / 8;                // bytes of a row
   constexpr int kKd = D / 4, kVd = D / 16;              // dims of a lane: K, V
   constexpr int kKb = kRow / 4, kVb = kRow / 16;        // and their bytes
@@ -637,12 +651,14 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
 #pragma unroll
     for (int st = 0; st < NT; ++st) {
       if constexpr (FMT == k16) {
-        u32x2 ph;
+        u32x2 ph, pl;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int at = kHalves == 2 ? 2 * st : 4 * st + 2 * e;
-          ph[e] = P::round2(x[at], x[at + 1]);
-          if (kHalves == 2 && half != e) ph[e] = 0;
+          uint32_t hi, lo;
+          split2<MT>(x[at], x[at + 1], hi, lo);
+          ph[e] = kHalves == 2 && half != e ? 0u : hi;
+          pl[e] = kHalves == 2 && half != e ? 0u : lo;
         }
         each<0, kVd / 2>([&](auto pair) {
           constexpr int I = decltype(pair)::value;
@@ -654,16 +670,22 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
           }
           acc[2 * I] = mfma<MT>(lo, ph, acc[2 * I]);
           acc[2 * I + 1] = mfma<MT>(hi, ph, acc[2 * I + 1]);
+          acc[2 * I] = mfma<MT>(lo, pl, acc[2 * I]);
+          acc[2 * I + 1] = mfma<MT>(hi, pl, acc[2 * I + 1]);
         });
         continue;
       }
+      // a step's weights are split in the step: all steps' at once spill with eight heads over 8 bits (248 us for 206
+      // with 64 heads and the long contexts)
+      __builtin_amdgcn_sched_barrier(0);
       u32x4 ph[2], pl[2];      // [1]: the odd dim's with one column a head
       float sc[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float y = x[kHalves == 2 ? 2 * st + e % 2 : 4 * st + e];
         const uint32_t hi = P::round2(y, y);
-        const uint32_t lo = kPair ? P::round2(y - __uint_as_float(hi & 0xffff0000u), y - __uint_as_float(hi & 0xffff0000u)) : 0u;
+        const float rest = y - __uint_as_float(hi & 0xffff0000u);
+        const uint32_t lo = P::round2(rest, rest);
         if constexpr (kSel == 2) {
           const uint32_t mask = kHalves == 2 ? (half == e / 2 ? slot_mask : 0u) : slot_mask;
           ph[0][e] = hi & mask;
@@ -684,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
 #pragma unroll
         for (int n = 0; n < 2 / kSel; ++n) {
           acc[2 / kSel * I + n] = mfma<MT>(v, ph[n], acc[2 / kSel * I + n]);
-          if constexpr (kPair) acc[2 / kSel * I + n] = mfma<MT>(v, pl[n], acc[2 / kSel * I + n]);
+          acc[2 / kSel * I + n] = mfma<MT>(v, pl[n], acc[2 / kSel * I + n]);
         }
       });
     }
