@@ -977,10 +977,9 @@ int yh_cache_read(const int64_t* slots, const void* keys, const void* values, co
  * is theirs, the gate's and a 16-bit cache's.  tables int32 [n_seqs, columns]; a
  * position whose block is not in the cache is not seen.  Values that are not finite
  * reach their own dim of the heads that see them; codes that stand for 2^128 and more
- * are infinities.  H % G == 0, D 64, 128 or
- * 256, scale > 0, softcap 0 (none) or 1e-30 to 1e30.  max_length: no request has more
- * positions (< 0: unknown), which
- * may save a launch.  workspace: 16-byte aligned, of at least
+ * are infinities.  H % G == 0, D 64, 128 or 256, scale > 0, softcap 0 (none) or 1e-30
+ * to 1e30, over codes D / 32 * block < 2^32.  max_length: no request has more positions
+ * (< 0: unknown), which may save a launch.  workspace: 16-byte aligned, of at least
  * yh_decode_attention_workspace_bytes bytes, asked with the call's own arguments (0:
  * none, NULL will do); calls that may overlap need one each.  Positions are below
  * 2^31 - 4096; a request that has more sees nothing.

@@ -218,3 +218,13 @@ def test_c_calls_refuse_before_device_work(lib):
     refused(rope(qts=12), b"aligned")
     refused(rope(eps=math.nan), b"eps")
     assert rope(dtype=0) == -3 and rope(n=0) == 0
+
+
+@pytest.mark.parametrize("d,block", [(128, 1 << 30), (256, 1 << 29), (256, 613566757), (256, (1 << 31) - 16)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_attention_refuses_blocks_whose_scales_pass_32_bits(lib, d, block, bits):
+    """A block's scales of one head are D / 32 runs of ``block`` bytes, which the kernel counts in 32 bits."""
+    p = ctypes.c_void_p(256)
+    rc = lib.yh_decode_attention(p, 8 * d, p, p, p, p, p, p, None, None, None, 0, 0, p, 1, 1, 1, 8, 2, d, block, 0, -1, 1.0, 0.0,
+                                 bits, 1, p, 1 << 40, None)
+    assert rc == -1 and b"too large" in lib.yh_last_error(), (rc, lib.yh_last_error())

@@ -975,7 +975,7 @@ extern "C" int yh_decode_attention(const void* q, int64_t q_stride, const void* 
                "decode_attention: bad gate strides");
   const int64_t each = G * ((H / G + kCols - 1) / kCols);
   YH_CHECK_ARG(n_seqs < (1ll << 20) && columns < (1ll << 31) && block < (1ll << 31) && H < (1ll << 16) &&
-                   blocks < (1ll << 31) && blocks * block < (1ll << 40),
+                   blocks < (1ll << 31) && blocks * block < (1ll << 40) && (bits == 16 || D / kRun * block < (1ll << 32)),
                "decode_attention: sizes too large");
   const int64_t target = target_for(n_seqs, H, G, D, block, columns, window, max_length, bits, dtype);
   int64_t most = columns * block;
