@@ -885,3 +885,19 @@ def test_attention_of_equal_weights_beside_larger_ones(gpu, bits, dtype, score, 
     want, size = ref.attention(q, *full, tables, lengths)
     step = torch.exp2(torch.floor(torch.log2(want * (1 + 2.0 ** -14)))) * half_step(dtype)
     within(got, want, step + 2.0 ** -14 * size, (bits, dtype))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_read_every_scale_byte(gpu, bits):
+    """All codes under each of the 256 scale bytes, those included that the write never makes."""
+    codes = torch.arange(256).to(torch.uint8)
+    d = 32 * len(codes.view(-1, 32 if bits == 8 else 16))
+    keys = codes.view(1, 1, 1, -1).expand(256, 1, 1, -1).contiguous()
+    s = torch.arange(256).to(torch.uint8).view(256, 1, 1, 1).expand(256, 1, d // 32, 1).contiguous()
+    keys = keys.view(torch.float8_e4m3fn) if bits == 8 else keys
+    for dtype in (B, H16):
+        got = layers.cache_read(torch.arange(256, device=gpu), keys.to(gpu), keys.to(gpu), s.to(gpu), s.to(gpu), dtype=dtype)
+        want = ref.cache_values(keys, s)[:, :, 0].to(dtype)
+        for x in got:
+            same = x.cpu() == want
+            assert (same | (x.cpu().isnan() & want.isnan())).all(), (~same).nonzero()[:5].tolist()

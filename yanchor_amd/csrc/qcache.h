@@ -31,11 +31,11 @@ __device__ __forceinline__ int scale_of(float top) {
                             : static_cast<int>((bits + 0x3fffffu) >> 23) - 2;
   return s < kLeast ? kLeast : s;
 }
-// 2^(s - 127), a NaN for 255.
+// 2^(s - 127), a NaN for 255; of 0, which the write does not make, the subnormal 2^-127.
 __device__ __forceinline__ float scale_value(int s) {
-  return s == kNotANumber ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(s) << 23);
+  return s == kNotANumber ? __uint_as_float(0x7fc00000u) : __uint_as_float(s == 0 ? 1u << 22 : static_cast<uint32_t>(s) << 23);
 }
-// 2^(127 - s) for s in [kLeast, 246], the inverse of a finite run's scale; of another, NaN.
+// 2^(127 - s) for s in [kLeast, 253], the inverse of a finite run's scale (up to 247 in 8 bits, 253 in 4); of 255, NaN.
 __device__ __forceinline__ float scale_inverse(int s) {
   return s == kNotANumber ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(254 - s) << 23);
 }
