@@ -24,6 +24,7 @@ import torch
 
 from oracle import qcache as ref
 from yanchor_amd import inference_kernels as ik
+from yanchor_amd import _native as N
 from yanchor_amd import layers
 
 pytestmark = pytest.mark.gpu
@@ -901,3 +902,60 @@ def test_read_every_scale_byte(gpu, bits):
         for x in got:
             same = x.cpu() == want
             assert (same | (x.cpu().isnan() & want.isnan())).all(), (~same).nonzero()[:5].tolist()
+
+
+# --- scratch that is used -----------------------------------------------------------
+
+def scratch_case(dev, seed, lengths=(3200, 7)):
+    """A call over 4 bits that needs its workspace, and the workspace's size."""
+    r, g, block, d, h, columns = len(lengths), 2, 16, 128, 8, 200
+    x, y = (rnd(r * columns, g, block, d, seed=seed + s) for s in (1, 2))
+    c = [t.to(dev) for t in cache_of(x, y, 4)]
+    q = rnd(r, h, d, seed=seed + 3).to(dev)
+    tables = torch.arange(r * columns, dtype=torch.int32, device=dev).view(r, columns)
+    lens = torch.tensor(lengths, device=dev)
+    need = N.lib().yh_decode_attention_workspace_bytes(r, h, g, d, block, columns, 0, -1, 4, N.BF16)
+    assert need > 0
+    call = lambda: layers.decode_attention(q, c[0], c[1], tables, lens, key_scales=c[2], value_scales=c[3])  # noqa: E731
+    return call, need, c
+
+
+def test_scratch_of_earlier_calls_does_not_matter(gpu):
+    """The memory that a call's scratch comes from is filled with NaN and with ones between calls: the same bits."""
+    call, need, _ = scratch_case(gpu, 40)
+    first = call()
+    assert torch.isfinite(first).all() and first.any()
+    for byte in (0xff, 0x00, 0x3f):
+        torch.cuda.synchronize()
+        dirt = [torch.full((need,), byte, dtype=torch.uint8, device=gpu) for _ in range(8)]
+        where = {t.data_ptr() for t in dirt}
+        del dirt
+        again = torch.empty((need,), dtype=torch.uint8, device=gpu)
+        assert again.data_ptr() in where       # the allocator gives what was just filled
+        del again
+        assert torch.equal(first, call())
+
+
+def test_side_stream_work_beside_the_main_stream(gpu):
+    """Calls queued on a side stream while the main stream allocates and fills memory of the scratch's size: each is right,
+    as are rows read there."""
+    call, need, c = scratch_case(gpu, 50)
+    want, slots = call(), torch.arange(300, device=gpu)
+    rows = layers.cache_read(slots, *c)
+    for x, which in zip(rows, (0, 1)):
+        full = ref.cache_values(c[which].cpu(), c[2 + which].cpu()).transpose(1, 2).reshape(-1, 2, 128)[:300]
+        assert torch.equal(x.cpu(), full.to(B))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    busy = torch.randn(4096, 4096, device=gpu)
+    outs, noise = [], []
+    for _ in range(10):
+        with torch.cuda.stream(side):
+            busy @ busy                        # what follows is still queued when the noise starts
+            outs.append((call(), layers.cache_read(slots, *c)))
+        noise += [torch.full((need,), 0xff, dtype=torch.uint8, device=gpu) for _ in range(4)]
+    assert not side.query()                    # there was work to run beside
+    torch.cuda.current_stream().wait_stream(side)
+    for got, back in outs:
+        same = torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(back, rows))
+        assert same
