@@ -228,3 +228,11 @@ def test_attention_refuses_blocks_whose_scales_pass_32_bits(lib, d, block, bits)
     rc = lib.yh_decode_attention(p, 8 * d, p, p, p, p, p, p, None, None, None, 0, 0, p, 1, 1, 1, 8, 2, d, block, 0, -1, 1.0, 0.0,
                                  bits, 1, p, 1 << 40, None)
     assert rc == -1 and b"too large" in lib.yh_last_error(), (rc, lib.yh_last_error())
+
+
+def test_write_of_a_16_bit_cache_names_what_it_takes():
+    half, x = torch.zeros(2, 2, 16, 128, dtype=B), torch.zeros(3, 2, 128, dtype=B)
+    scales = cache8()[2:]
+    for args in ((half, half, None, None), (half, half, *scales)):
+        with pytest.raises(ValueError, match="4 or 8 bits"):
+            layers.cache_write_quantized(x, x, torch.zeros(3, dtype=torch.int64), *args)

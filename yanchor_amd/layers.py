@@ -840,6 +840,8 @@ def cache_write_quantized(k, v, slots, keys, values, key_scales, value_scales):
     if len(shape) != 3 or v.shape != shape or v.dtype != kind or kind not in _HALF:
         raise ValueError("cache_write_quantized takes bf16 / fp16 k and v [N, G, D]")
     n, g, d = shape
+    if keys.dtype in _HALF:
+        raise ValueError("cache_write_quantized takes a cache of 4 or 8 bits a value")
     bits = _any_cache(keys, values, key_scales, value_scales, g, d, None)
     dev = _tree.device_of(k, v, keys, values, key_scales, value_scales)
     slots = _tree.ints(slots, torch.int64, dev, "slots", n)
