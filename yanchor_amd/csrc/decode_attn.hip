@@ -382,6 +382,12 @@ __device__ __forceinline__ void put4(const DecodeArgs& a, int r, int head, int d
   *reinterpret_cast<u32x2*>(a.out + to) = u32x2{attn::pack2(y[0], y[1]), attn::pack2(y[2], y[3])};
 }
 
+// Whether four dims' sums can be taken as they are.  Where the denominator is no number, no dim is one; elsewhere a sum
+// that is not finite says nothing of its own dim.
+__device__ __forceinline__ bool all_finite(float den, const float* o) {
+  return den != den || fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < INFINITY;
+}
+
 // Waves a SIMD that the registers are held to: as many as fit without spilling, but
 // for fp16 queries over 8 bits with sixteen columns of heads of 256, which spill up to 9 registers (us of the long contexts
 // with 128 heads, blocks of 64 and 24: 462 and 549, with one wave a SIMD 524 and 582).
@@ -758,15 +764,11 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
       put4<DT>(b, r, hd, dim, D, o, dn);
     }
   };
-  // Where the denominator is no number, no dim is one; elsewhere a sum that is none says nothing of its own dim.
-  auto finite = [](float dn, const float* o) {
-    return dn != dn || fabsf(o[0]) + fabsf(o[1]) + fabsf(o[2]) + fabsf(o[3]) < INFINITY;
-  };
   for (int at = threadIdx.x; at < cols * (D / 4); at += kThreads) {
     const int c = at / (D / 4), dim = at % (D / 4) * 4;
     float m, dn, o[4];
     join(c, dim, m, dn, o);
-    if (finite(dn, o)) put(c, dim, m, dn, o);
+    if (all_finite(dn, o)) put(c, dim, m, dn, o);
     else atomicOr(&spoiled, 1u << c);
   }
   __syncthreads();
@@ -816,7 +818,7 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
 #pragma unroll
     for (int e = 0; e < 4; ++e) redo_sum[share][dim + e] = sum[e];
     __syncthreads();
-    if (share == 0 && !finite(dn, o)) {
+    if (share == 0 && !all_finite(dn, o)) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (fabsf(o[e]) < INFINITY) continue;
@@ -827,9 +829,6 @@ __global__ void __launch_bounds__(kThreads, waves_for(DT, FMT, D, HP, RUNS)) dec
     }
   }
 }
-
-// A sum at a factor of at most 1: an infinite one stays, where float32 holds the factor as 0.
-__device__ __forceinline__ float scaled(float x, float f) { return fabsf(x) == INFINITY ? x : x * f; }
 
 // The parts of a cut request joined: a workgroup a head, D / 4 lanes a part, the others take every kShares-th part;
 // their sums meet in LDS, in order.
@@ -851,10 +850,10 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
     const float next = fmaxf(m, st.x), f = __builtin_amdgcn_exp2f(m - next), h = __builtin_amdgcn_exp2f(st.x - next);
     m = next;
     dn = fmaf(dn, f, st.y * h);
-    o[0] = scaled(o[0], f) + scaled(x.x, h);
-    o[1] = scaled(o[1], f) + scaled(x.y, h);
-    o[2] = scaled(o[2], f) + scaled(x.z, h);
-    o[3] = scaled(o[3], f) + scaled(x.w, h);
+    o[0] = fmaf(o[0], f, x.x * h);
+    o[1] = fmaf(o[1], f, x.y * h);
+    o[2] = fmaf(o[2], f, x.z * h);
+    o[3] = fmaf(o[3], f, x.w * h);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) sums[share][dim + e] = o[e];
@@ -874,7 +873,23 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(DecodeArgs a) {
     const float f = __builtin_amdgcn_exp2f(tops[i] - m);
     dn = fmaf(dens[i], f, dn);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += scaled(sums[i][dim + e], f);
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(sums[i][dim + e], f, o[e]);
+  }
+  if (!all_finite(dn, o)) {
+    // a part's infinity stays one, where float32 holds its factor as 0
+    auto scaled = [](float x, float f) { return fabsf(x) == INFINITY ? x : x * f; };
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < count; ++j) {
+      const int64_t s = slot + static_cast<int64_t>(j) * a.H;
+      const float4 x = *reinterpret_cast<const float4*>(a.part + s * D + dim);
+      const float f = __builtin_amdgcn_exp2f(a.stat[s].x - m);
+      o[0] += scaled(x.x, f);
+      o[1] += scaled(x.y, f);
+      o[2] += scaled(x.z, f);
+      o[3] += scaled(x.w, f);
+    }
   }
   put4<DT>(a, r, hd, dim, D, o, dn);
 }
