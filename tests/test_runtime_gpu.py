@@ -112,3 +112,39 @@ def test_tail_compaction_keeps_every_sequence(gpu):
     for i, c in enumerate(caps):
         assert len(o0[i]) == len(o1[i]) == c, i
         assert o0[i] == o1[i], i
+
+
+def test_decode_step_on_the_side_stream_itself(gpu):
+    """Streams come from a pool that goes round, so the stream that a step runs on, or is captured on, may be the one
+    that the model took for its memory path: the two paths' split-K partials then must not meet in one workspace."""
+    cfg = small_cfg()
+    m = rt.Model(cfg, batch=4, device=gpu, seed=3)
+    prompts = torch.randint(0, cfg.vocab, (4, 16), generator=torch.Generator().manual_seed(4)).to(gpu)
+    _, caches = m.prefill(prompts)
+    start = [c.clone() for c in caches]
+    tokens, pos = prompts[:, 0].contiguous(), torch.full((4,), 16, dtype=torch.long, device=gpu)
+    valid = torch.ones(4, dtype=torch.bool, device=gpu)
+
+    def step():
+        for dst, src in zip(m.cache_tensors(), start):
+            dst.copy_(src)
+        return m.decode_step(tokens, pos, valid)
+    want = step().clone()
+    torch.cuda.synchronize()
+    side = m._side_stream(prompts)
+    assert side is not None
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    m._side = side
+    with torch.cuda.graph(graph, stream=side):
+        out = m.decode_step(tokens, pos, valid)
+    for _ in range(3):
+        for dst, src in zip(m.cache_tensors(), start):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

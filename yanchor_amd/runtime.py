@@ -783,7 +783,10 @@ class Model:
     def _side_stream(self, x):
         if not (getattr(self, "overlap", False) and x.is_cuda):
             return None
-        if getattr(self, "_side", None) is None:
+        # Never the stream of the call itself: streams come from a pool that goes round, and the paths' split-K
+        # partials lie in a workspace a stream.
+        main = torch.cuda.current_stream(x.device).cuda_stream
+        while getattr(self, "_side", None) is None or self._side.cuda_stream == main:
             self._side = torch.cuda.Stream(device=x.device)   # default priority
         return self._side
 
