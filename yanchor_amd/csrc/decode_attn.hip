@@ -39,13 +39,14 @@
 // LDS.  Parts of a request that was cut leave theirs, with their maximum, in the
 // workspace, and a second launch joins them in order.
 //
-// Bound by HBM: 133 ragged requests over 8 bits 215 us (1.18 GB, 5.5 TB/s), 8 long
-// contexts 194 (6.1), 64 requests over 4 bits 118 (5.4), heads of 256 in 16 bits 151
+// Bound by HBM: 133 ragged requests over 8 bits 216 us (1.18 GB, 5.5 TB/s), 8 long
+// contexts 194 (6.1), 64 requests over 4 bits 120 (5.3), heads of 256 in 16 bits 151
 // (5.6), where a large copy reaches 6.2 and a read alone 7.0.  Nontemporal loads,
-// since nothing is read twice but by up to four waves for 64 heads and more: the
-// long contexts 201 us for 217.  Blocks that runs of 16 positions straddle (block %
-// 16) have their table entries and rows a lane: 219 us for the long contexts with
-// blocks of 24, 369 with blocks of 1.
+// since up to 16 query heads of a KV head share one read of its rows: the long
+// contexts 201 us for 217.  (Every 16 heads more are a workgroup of their own that
+// reads them once more.)  Blocks that runs of 16 positions straddle (block % 16) have
+// their table entries and rows a lane: 220 us for the long contexts with blocks of 24,
+// 367 with blocks of 1.
 #include <type_traits>
 
 #include "attn_tile.h"
@@ -904,7 +905,7 @@ int64_t tile_of(int bits, int64_t D, int dtype) {
   return 16 * products(static_cast<int>(D * bits / 8), bits != 16 && dtype == YH_F16 && D == 256);
 }
 // Parts aimed at for each KV head, 0 where no request is cut and the second launch is not made: up to two turns of the
-// waves, or eight where there are heads enough.  (400 positions: one request 7.7 us captured and 13 called for 8.9 and
+// waves, or eight where there are heads enough.  (400 positions, before the weights' second product: one request 7.7 us captured and 13 called for 8.9 and
 // 18, 64 requests 15 for 22, 200 47 for 61.)
 int64_t target_for(int64_t R, int64_t H, int64_t G, int64_t D, int64_t block, int64_t columns, int64_t window,
                    int64_t max_length, int bits, int dtype) {

@@ -856,7 +856,8 @@ def cache_read(slots, keys, values, key_scales=None, value_scales=None, *, dtype
     """Rows of a block cache of 4, 8 or 16 bits back as (k, v) [N, G, D] in
     ``dtype`` (bf16 / fp16; default bf16, or that of a 16-bit cache), from slots
     int [N] as ``slot_map`` gives them (``slot_map(cu_seqlens, zeros, ...)`` those
-    of whole prefixes): what a prefill that continues a request reads.  A slot
+    of whole prefixes), for a caller that attends to a cached prefix by its own
+    means (no call here takes such rows).  A slot
     outside the cache gives zeros; a value whose code rounds past the dtype's range
     (65504 in 8 bits reads as 65536) infinity."""
     if keys.ndim != 4:
