@@ -959,3 +959,62 @@ def test_side_stream_work_beside_the_main_stream(gpu):
     for got, back in outs:
         same = torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(back, rows))
         assert same
+
+
+@pytest.mark.parametrize("bits,dtype", FORMS)
+@pytest.mark.parametrize("block", [16, 24])
+def test_attention_values_not_finite_beside_masks_biases_and_gates(gpu, bits, dtype, block):
+    """Infinities (NaN codes over quantised caches) in seen positions, before starts, and in blocks taken out of the table,
+    with caps, biases of both signs and gates; whole and in parts; replayed as a graph beside calls without such values."""
+    d, g, h, lengths, starts = 128, 2, 8, [2100, 90, 300], [1000, 0, 40]
+    columns = -(-2100 // block)
+    x, y = (rnd(3 * columns, g, block, d, seed=s, dtype=dtype) for s in (1, 2))
+    tables = torch.randperm(3 * columns, generator=torch.Generator().manual_seed(3)).to(torch.int32).view(3, columns)
+    cache = list(cache_of(x, y, bits)) if bits < 16 else [x, y, None, None]
+    clean = [None if t is None else t.clone() for t in cache]
+    for i, p, dim in ((0, 999, 2), (0, 1000, 5), (0, 2099, 40), (1, 47, 7), (1, 89, 100), (2, 39, 1), (2, 200, 66)):
+        b, row = int(tables[i, p // block]), p % block
+        if bits == 16:
+            cache[1][b, 1, row, dim] = -INF if dim == 5 else INF
+        elif bits == 8:
+            cache[1].view(torch.uint8)[b, 1, row, dim] = 0x7f
+        else:
+            cache[3][b, 1, dim // 32, row] = 255
+    tables[1, 47 // block] = -1               # request 1 does not see position 47
+    tables[2, 0] = 1 << 30
+    q, gate = rnd(3, h, d, seed=4, dtype=dtype), rnd(3, h, d, seed=5, dtype=dtype)
+    slopes = torch.tensor([0.01 * (i - 3) for i in range(h)])
+    kw = dict(softcap=12.0, scale=0.1)
+    full = [ref.cache_values(cache[i], cache[2 + i]) for i in range(2)]
+    want, _ = ref.attention(q, *full, tables, lengths, starts=starts, slopes=slopes, gate=gate, **kw)
+    full[1] = full[1].nan_to_num(0.0, 0.0, 0.0)
+    _, size = ref.attention(q, *full, tables, lengths, starts=starts, slopes=slopes, gate=gate, **kw)
+    assert want[:, :4].isfinite().all()       # those of the other KV head
+    lost = 32 if bits == 4 else 1             # a scale is its run's
+    assert [int((~want[i, 4:].isfinite()).sum()) for i in range(3)] == [4 * 2 * lost, 4 * lost, 4 * lost]
+    on = [None if t is None else t.to(gpu) for t in cache]
+    dq, dt, dl, ds = q.to(gpu), tables.to(gpu), torch.tensor(lengths, device=gpu), torch.tensor(starts, device=gpu)
+    sl, dg = slopes.to(gpu), gate.to(gpu)
+    call = lambda: layers.decode_attention(dq, on[0], on[1], dt, dl, key_scales=on[2], value_scales=on[3], starts=ds,  # noqa: E731
+                                           slopes=sl, gate=dg, **kw)
+    got = call()
+    same_or_within(got, want, half_step(dtype) * want.abs() + (2.0 ** -16 + 2.0 ** -12) * size, (bits, dtype, block))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    spoiled = [None if t is None else t.clone() for t in on]
+    for turn in range(3):
+        for t, s, c in zip(on, spoiled, clean):
+            if t is not None:
+                t.view(torch.uint8).copy_((c.to(gpu) if turn == 1 else s).view(torch.uint8))
+        eager = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), eager.view(torch.int16))
+        assert torch.equal(eager.view(torch.int16), got.view(torch.int16)) == (turn != 1)
+        assert eager.isfinite().all() == (turn == 1)
